@@ -434,6 +434,69 @@ int tx_rope_kv_cache_prefill_split(uint64_t qkv_handle, const void *partials, in
                                    const float *cos_table, const float *sin_table, int heads, int kv_heads, int head_dim,
                                    void *q_out, void *k_cache, void *v_cache, int64_t max_context, void *stream);
 
+/* ---- Serving several sequences (no reference counterpart: the reference leaves attention and caches to
+ * Hugging Face's modules) ----
+ * Types: TX_DTYPE_BF16 or TX_DTYPE_F16 for all rows of a call. Strides are in elements. `device` is the GPU that holds
+ * the arrays and `stream`; it need not be the current one. Lengths, block tables and cu arrays are int32 in device memory
+ * and read by the kernels alone, so a captured call serves whatever they hold when it is replayed. */
+
+/* Causal attention of packed sequences: sequence s has the queries cu_q[s] .. cu_q[s + 1] - 1 of q [total_q][heads]
+ * [head_dim] and the keys and values cu_k[s] .. cu_k[s + 1] - 1 of k and v [total_k][kv_heads][head_dim]; its last query
+ * sees its last key: query i sees the keys j <= i + (keys - queries), so keys of earlier turns come first. A query
+ * that sees no key gets zeros. Rows of out [total_q][heads][head_dim] that belong to no sequence are left as they are.
+ * head_dim 64 or 128; heads a multiple of kv_heads; rows of q, k and v 16-byte aligned, of out 8-byte. out must not
+ * overlap the inputs. fp32 scores, softmax statistics and sums; the probabilities are rounded to the rows' type before
+ * they meet the values. */
+int tx_packed_attention(const void *q, int64_t q_token, int64_t q_head, const void *k, int64_t k_token, int64_t k_head,
+                        const void *v, int64_t v_token, int64_t v_head, int dtype, int heads, int kv_heads, int head_dim,
+                        const int *cu_q, const int *cu_k, int sequences, int64_t total_q, int64_t total_k, float scale,
+                        void *out, int64_t out_token, int64_t out_head, int device, void *stream);
+
+/* The paged 4-bit KV cache. A pool is num_pages pages of page_size positions (a power of two, 16 to 1024): uint8
+ * [num_pages][kv_heads][2 (keys, values)][page_size * head_dim * 17 / 32], 16-byte aligned; each of these halves holds
+ * packed E2M1 codes [page_size][head_dim / 2] (even element in the low nibble), then E8M0 scales
+ * [page_size][head_dim / 32], one for 32 elements. head_dim 64 or 128. Position p of sequence s lies at offset
+ * p % page_size of page block_table[s][p / page_size] (rows of max_pages entries, table_stride apart). lengths[s]: the positions
+ * in use, those that a call appends included; above max_pages * page_size they count as that, below 0 as 0. A page id outside the
+ * pool is allowed: its positions are skipped.
+ *
+ * tx_kv4_append: token rows k and v [tokens][kv_heads][head_dim] into the cache. cu [sequences + 1]: the tokens
+ * cu[s] .. cu[s + 1] - 1 become the last ones of sequence s's lengths[s] positions; NULL: one token for each sequence.
+ * Tokens outside cu, and positions below 0, are skipped. A group of 32 elements is stored with the scale
+ * 2^(floor(log2(amax)) - 2) (at least 2^-127), each element as the nearest E2M1 value of v / scale, ties to the even
+ * code, saturated at 6; a group with an infinity or a NaN is stored as NaN. A page that receives tokens must be one
+ * sequence's alone (two tokens of a call at one place: either may end there, or parts of both).
+ *
+ * tx_kv4_read: the same rows back, value times scale rounded to k's and v's type. Rows that name no position of the
+ * cache are left as they are. */
+int tx_kv4_append(const void *k, int64_t k_token, int64_t k_head, const void *v, int64_t v_token, int64_t v_head, int dtype,
+                  int64_t tokens, const int *cu, void *pages, int64_t num_pages, int kv_heads, int head_dim, int page_size,
+                  const int *block_table, int64_t table_stride, int max_pages, const int *lengths, int sequences,
+                  int device, void *stream);
+int tx_kv4_read(void *k, int64_t k_token, int64_t k_head, void *v, int64_t v_token, int64_t v_head, int dtype, int64_t tokens,
+                const int *cu, const void *pages, int64_t num_pages, int kv_heads, int head_dim, int page_size,
+                const int *block_table, int64_t table_stride, int max_pages, const int *lengths, int sequences, int device,
+                void *stream);
+
+/* One query token per sequence over the cache: q [sequences][heads][head_dim] against the lengths[s] positions of its
+ * sequence; out the same shape, zeros for an empty sequence. heads a multiple of kv_heads; every query 16-byte
+ * aligned, every output row 8-byte. workspace: at least tx_kv4_attention_workspace bytes, 16-byte aligned, not shared
+ * with a call that may run at the same time; it need not be cleared. fp32 scores, statistics and sums; probabilities rounded
+ * to q's type. In fp16, cached values beyond 65504 (a cache written from bf16) read as infinities. */
+int tx_kv4_attention_workspace(int sequences, int heads, int kv_heads, int head_dim, int page_size, int max_pages, int device,
+                               int64_t *bytes);
+int tx_kv4_attention(const void *q, int64_t q_sequence, int64_t q_head, int dtype, int heads, const void *pages,
+                     int64_t num_pages, int kv_heads, int head_dim, int page_size, const int *block_table,
+                     int64_t table_stride, int max_pages, const int *lengths, int sequences, float scale, void *workspace,
+                     int64_t workspace_bytes, void *out, int64_t out_sequence, int64_t out_head, int device, void *stream);
+
+/* Copies page src[i] to page dst[i], i < count, in each of `layers` pools [layers][num_pages][page_bytes] (page_bytes a
+ * multiple of 16): a fork copies the last, partly filled page, a compaction moves pages. src and dst are host arrays, read
+ * before the call returns. All copies happen at once: a page that is copied to twice, or that is both copied from and copied to, is
+ * refused, with nothing copied. */
+int tx_kv4_copy_pages(void *pages, int layers, int64_t num_pages, int64_t page_bytes, const int64_t *src, const int64_t *dst,
+                      int64_t count, int device, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

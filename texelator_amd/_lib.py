@@ -85,6 +85,16 @@ SIGNATURES = {
     "tx_prefill_split": (_I32, [_U64, _P, _I64, _P, _I64, ctypes.POINTER(ctypes.c_int), _P]),
     "tx_add_rmsnorm_prefill_split": (_I32, [_P, _U64, _P, _I64, _P, ctypes.c_float, _P, _I64, _P]),
     "tx_rope_kv_cache_prefill_split": (_I32, [_U64, _P, _I64, _P, _P, _P, _I32, _I32, _I32, _P, _P, _P, _I64, _P]),
+    "tx_packed_attention": (_I32, [_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I32, _I32, _I32, _I32, _P, _P, _I32, _I64,
+                                   _I64, ctypes.c_float, _P, _I64, _I64, _I32, _P]),
+    "tx_kv4_append": (_I32, [_P, _I64, _I64, _P, _I64, _I64, _I32, _I64, _P, _P, _I64, _I32, _I32, _I32, _P, _I64, _I32, _P,
+                             _I32, _I32, _P]),
+    "tx_kv4_read": (_I32, [_P, _I64, _I64, _P, _I64, _I64, _I32, _I64, _P, _P, _I64, _I32, _I32, _I32, _P, _I64, _I32, _P,
+                           _I32, _I32, _P]),
+    "tx_kv4_attention_workspace": (_I32, [_I32, _I32, _I32, _I32, _I32, _I32, _I32, ctypes.POINTER(_I64)]),
+    "tx_kv4_attention": (_I32, [_P, _I64, _I64, _I32, _I32, _P, _I64, _I32, _I32, _I32, _P, _I64, _I32, _P, _I32,
+                                ctypes.c_float, _P, _I64, _P, _I64, _I64, _I32, _P]),
+    "tx_kv4_copy_pages": (_I32, [_P, _I32, _I64, _I64, _P, _P, _I64, _I32, _P]),
 }
 
 _LIB = None

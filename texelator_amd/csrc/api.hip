@@ -16,6 +16,7 @@
 #include "bc4_device.h"
 #include "elementwise.h"
 #include "kernels.h"
+#include "kv4.h"
 
 // Static scratch of tx_linear_noalloc: split-K partial sums for callers that cannot allocate.
 // File-scope device memory: every GPU the library runs on holds its own copy from the first use
@@ -1404,6 +1405,219 @@ int tx_rope_rotate_half(const void *q, const void *k, int64_t tokens, int heads,
                                      kv_heads, head_dim, static_cast<const uint16_t *>(cos),
                                      static_cast<const uint16_t *>(sin), static_cast<uint16_t *>(q_out),
                                      static_cast<uint16_t *>(k_out), reinterpret_cast<hipStream_t>(stream)));
+  return TX_OK;
+}
+
+namespace {
+
+// CUs of a device, cheaply enough to ask at every call.
+int multiprocessors(int device) {
+  int cus = 0;
+  if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, device) != hipSuccess || cus <= 0) cus = 256;
+  return cus;
+}
+
+// The cache of a call as the kernels take it; a message where the arguments do not describe one.
+const char *kv4_pool(tx::Kv4Pool &pool, const void *pages, int64_t num_pages, int kv_heads, int head_dim, int page_size,
+                     const int *block_table, int64_t table_stride, int max_pages, const int *lengths, int sequences) {
+  if (!pages || !block_table || !lengths) return "null pointer";
+  if (head_dim != 64 && head_dim != 128) return "head_dim must be 64 or 128";
+  if (page_size < 16 || page_size > 1024 || (page_size & (page_size - 1))) return "page_size must be a power of two from 16 to 1024";
+  if (num_pages <= 0 || num_pages > 0x7FFFFFFF || kv_heads <= 0 || kv_heads > 1024) return "bad pool shape";
+  if (sequences < 0 || sequences > 65535 || max_pages <= 0 || table_stride < 0) return "bad block table shape";
+  if ((int64_t)max_pages * page_size > (int64_t)1 << 30) return "a sequence holds at most 2^30 positions";
+  if (reinterpret_cast<uintptr_t>(pages) % 16 || reinterpret_cast<uintptr_t>(block_table) % 4 || reinterpret_cast<uintptr_t>(lengths) % 4)
+    return "pages must be 16-byte aligned, the block table and the lengths 4-byte";
+  int shift = 4;
+  while (1 << shift < page_size) ++shift;
+  pool.pages = static_cast<uint8_t *>(const_cast<void *>(pages));
+  pool.num_pages = num_pages;
+  pool.page_shift = shift;
+  pool.kv_heads = kv_heads;
+  pool.table = block_table;
+  pool.table_stride = table_stride;
+  pool.max_pages = max_pages;
+  pool.lengths = lengths;
+  pool.sequences = sequences;
+  return nullptr;
+}
+
+const char *kv4_rows(const void *k, int64_t k_token, int64_t k_head, const void *v, int64_t v_token, int64_t v_head,
+                     int dtype, int64_t tokens, const int *cu, int sequences) {
+  if (!k || !v) return "null pointer";
+  if (dtype != TX_DTYPE_F16 && dtype != TX_DTYPE_BF16) return "rows must be FP16 or BF16";
+  if (tokens < 0 || tokens > 0x7FFFFFFF / 2) return "bad token count";
+  if (!cu && tokens != sequences) return "without cu there is one token per sequence";
+  if ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) % 16 || (k_token | k_head | v_token | v_head) % 8)
+    return "every row must be 16-byte aligned";
+  if (reinterpret_cast<uintptr_t>(cu) % 4) return "cu must be 4-byte aligned";
+  return nullptr;
+}
+
+}  // namespace
+
+int tx_kv4_append(const void *k, int64_t k_token, int64_t k_head, const void *v, int64_t v_token, int64_t v_head, int dtype,
+                  int64_t tokens, const int *cu, void *pages, int64_t num_pages, int kv_heads, int head_dim, int page_size,
+                  const int *block_table, int64_t table_stride, int max_pages, const int *lengths, int sequences,
+                  int device, void *stream) {
+  g_last_error.clear();
+  tx::Kv4Pool pool;
+  const char *bad = kv4_pool(pool, pages, num_pages, kv_heads, head_dim, page_size, block_table, table_stride, max_pages,
+                             lengths, sequences);
+  if (!bad) bad = kv4_rows(k, k_token, k_head, v, v_token, v_head, dtype, tokens, cu, sequences);
+  if (bad) return fail(TX_ERR_INVALID, std::string("kv4_append: ") + bad);
+  if (tokens == 0 || sequences == 0) return TX_OK;
+  DeviceGuard guard(device);
+  TX_HIP(tx::launch_kv4_append(static_cast<const uint16_t *>(k), k_token, k_head, static_cast<const uint16_t *>(v), v_token,
+                               v_head, (int)tokens, dtype == TX_DTYPE_F16, head_dim, cu, pool,
+                               reinterpret_cast<hipStream_t>(stream)));
+  return TX_OK;
+}
+
+int tx_kv4_read(void *k, int64_t k_token, int64_t k_head, void *v, int64_t v_token, int64_t v_head, int dtype, int64_t tokens,
+                const int *cu, const void *pages, int64_t num_pages, int kv_heads, int head_dim, int page_size,
+                const int *block_table, int64_t table_stride, int max_pages, const int *lengths, int sequences, int device,
+                void *stream) {
+  g_last_error.clear();
+  tx::Kv4Pool pool;
+  const char *bad = kv4_pool(pool, pages, num_pages, kv_heads, head_dim, page_size, block_table, table_stride, max_pages,
+                             lengths, sequences);
+  if (!bad) bad = kv4_rows(k, k_token, k_head, v, v_token, v_head, dtype, tokens, cu, sequences);
+  if (bad) return fail(TX_ERR_INVALID, std::string("kv4_read: ") + bad);
+  if (tokens == 0 || sequences == 0) return TX_OK;
+  DeviceGuard guard(device);
+  TX_HIP(tx::launch_kv4_read(static_cast<uint16_t *>(k), k_token, k_head, static_cast<uint16_t *>(v), v_token, v_head,
+                             (int)tokens, dtype == TX_DTYPE_F16, head_dim, cu, pool, reinterpret_cast<hipStream_t>(stream)));
+  return TX_OK;
+}
+
+int tx_kv4_attention_workspace(int sequences, int heads, int kv_heads, int head_dim, int page_size, int max_pages, int device,
+                               int64_t *bytes) {
+  g_last_error.clear();
+  if (!bytes) return fail(TX_ERR_INVALID, "kv4_attention_workspace: null pointer");
+  static int dummy;
+  tx::Kv4Attention a = {};
+  const char *bad = kv4_pool(a.pool, reinterpret_cast<void *>(16), 1, kv_heads, head_dim, page_size, &dummy, max_pages, max_pages,
+                             &dummy, sequences);
+  if (!bad && (heads <= 0 || heads % kv_heads || heads / kv_heads > 65535)) bad = "heads must be a multiple of kv_heads";
+  if (!bad && !tx::kv4_attention_fits(a.pool)) bad = "sequences x kv_heads x positions too large";
+  if (bad) return fail(TX_ERR_INVALID, std::string("kv4_attention_workspace: ") + bad);
+  a.group = heads / kv_heads;
+  tx::kv4_attention_plan(a, head_dim, multiprocessors(device));
+  *bytes = a.piece_bytes;
+  return TX_OK;
+}
+
+int tx_kv4_attention(const void *q, int64_t q_sequence, int64_t q_head, int dtype, int heads, const void *pages,
+                     int64_t num_pages, int kv_heads, int head_dim, int page_size, const int *block_table,
+                     int64_t table_stride, int max_pages, const int *lengths, int sequences, float scale, void *workspace,
+                     int64_t workspace_bytes, void *out, int64_t out_sequence, int64_t out_head, int device, void *stream) {
+  g_last_error.clear();
+  tx::Kv4Attention a = {};
+  const char *bad = kv4_pool(a.pool, pages, num_pages, kv_heads, head_dim, page_size, block_table, table_stride, max_pages,
+                             lengths, sequences);
+  if (!bad && (!q || !out || !workspace)) bad = "null pointer";
+  if (!bad && dtype != TX_DTYPE_F16 && dtype != TX_DTYPE_BF16) bad = "q must be FP16 or BF16";
+  if (!bad && (heads <= 0 || heads % kv_heads || heads / kv_heads > 65535)) bad = "heads must be a multiple of kv_heads";
+  if (!bad && (reinterpret_cast<uintptr_t>(q) % 16 || (q_sequence | q_head) % 8)) bad = "every query must be 16-byte aligned";
+  if (!bad && (reinterpret_cast<uintptr_t>(out) % 8 || (out_sequence | out_head) % 4)) bad = "every output row must be 8-byte aligned";
+  if (!bad && reinterpret_cast<uintptr_t>(workspace) % 16) bad = "the workspace must be 16-byte aligned";
+  if (!bad && !tx::kv4_attention_fits(a.pool)) bad = "sequences x kv_heads x positions too large";
+  if (bad) return fail(TX_ERR_INVALID, std::string("kv4_attention: ") + bad);
+  if (sequences == 0) return TX_OK;
+  a.q = static_cast<const uint16_t *>(q);
+  a.q_sequence = q_sequence;
+  a.q_head = q_head;
+  a.out = static_cast<uint16_t *>(out);
+  a.out_sequence = out_sequence;
+  a.out_head = out_head;
+  a.group = heads / kv_heads;
+  a.scale = scale;
+  a.pieces = static_cast<float *>(workspace);
+  tx::kv4_attention_plan(a, head_dim, multiprocessors(device));
+  if (workspace_bytes < a.piece_bytes) return fail(TX_ERR_INVALID, "kv4_attention: workspace too small (tx_kv4_attention_workspace)");
+  DeviceGuard guard(device);
+  TX_HIP(tx::launch_kv4_attention(a, dtype == TX_DTYPE_F16, head_dim, reinterpret_cast<hipStream_t>(stream)));
+  return TX_OK;
+}
+
+int tx_kv4_copy_pages(void *pages, int layers, int64_t num_pages, int64_t page_bytes, const int64_t *src, const int64_t *dst,
+                      int64_t count, int device, void *stream) {
+  g_last_error.clear();
+  if (!pages || (count > 0 && (!src || !dst))) return fail(TX_ERR_INVALID, "kv4_copy_pages: null pointer");
+  if (layers <= 0 || layers > 65535 || num_pages <= 0 || num_pages > 0x7FFFFFFF || page_bytes <= 0 || page_bytes % 16 ||
+      page_bytes > (int64_t)1 << 32 || reinterpret_cast<uintptr_t>(pages) % 16)
+    return fail(TX_ERR_INVALID, "kv4_copy_pages: pages must be 16-byte aligned and hold a multiple of 16 bytes");
+  if (count < 0 || count > num_pages) return fail(TX_ERR_INVALID, "kv4_copy_pages: more copies than pages");
+  try {
+    // Pages are copied all at once: a page is written once, and no page that is read is written.
+    std::vector<int64_t> targets(dst, dst + count);
+    std::sort(targets.begin(), targets.end());
+    if (count && (targets.front() < 0 || targets.back() >= num_pages)) return fail(TX_ERR_INVALID, "kv4_copy_pages: page id outside the pool");
+    if (std::adjacent_find(targets.begin(), targets.end()) != targets.end())
+      return fail(TX_ERR_INVALID, "kv4_copy_pages: a page is copied to twice");
+    for (int64_t i = 0; i < count; ++i) {
+      if (src[i] < 0 || src[i] >= num_pages) return fail(TX_ERR_INVALID, "kv4_copy_pages: page id outside the pool");
+      if (std::binary_search(targets.begin(), targets.end(), src[i]))
+        return fail(TX_ERR_INVALID, "kv4_copy_pages: a page is both copied from and copied to");
+    }
+  } catch (const std::bad_alloc &) {
+    return fail(TX_ERR_INVALID, "kv4_copy_pages: out of host memory");
+  }
+  if (count == 0) return TX_OK;
+  DeviceGuard guard(device);
+  TX_HIP(tx::launch_kv4_copy_pages(static_cast<uint8_t *>(pages), layers, num_pages * page_bytes, page_bytes, src, dst, count,
+                                   reinterpret_cast<hipStream_t>(stream)));
+  return TX_OK;
+}
+
+int tx_packed_attention(const void *q, int64_t q_token, int64_t q_head, const void *k, int64_t k_token, int64_t k_head,
+                        const void *v, int64_t v_token, int64_t v_head, int dtype, int heads, int kv_heads, int head_dim,
+                        const int *cu_q, const int *cu_k, int sequences, int64_t total_q, int64_t total_k, float scale,
+                        void *out, int64_t out_token, int64_t out_head, int device, void *stream) {
+  g_last_error.clear();
+  const char *bad = nullptr;
+  auto row = [](int64_t stride) { return stride >= 0 && stride <= (1 << 24) && stride % 8 == 0; };
+  if (!q || !out || !cu_q || !cu_k || (total_k > 0 && (!k || !v))) bad = "null pointer";
+  else if (dtype != TX_DTYPE_F16 && dtype != TX_DTYPE_BF16) bad = "q, k and v must be FP16 or BF16";
+  else if (head_dim != 64 && head_dim != 128) bad = "head_dim must be 64 or 128";
+  else if (kv_heads <= 0 || heads <= 0 || heads > 65535 || heads % kv_heads) bad = "heads must be a multiple of kv_heads";
+  else if (sequences < 0 || sequences > 65535 || total_q < 0 || total_k < 0 || total_q > 1 << 28 || total_k > 1 << 28)
+    bad = "bad sequence or token count";
+  else if ((total_q / 32 + sequences) * heads > 0x7FFFFFFF) bad = "the grid exceeds the launch limit";
+  else if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) % 16 || !row(q_token) ||
+           !row(q_head) || !row(k_token) || !row(k_head) || !row(v_token) || !row(v_head))
+    bad = "every row of q, k and v must be 16-byte aligned";
+  // A row past the last one must lie past the end of its block's descriptor.
+  else if (total_k > 1 && (k_token < head_dim || v_token < head_dim)) bad = "rows of k and v must not overlap";
+  else if (reinterpret_cast<uintptr_t>(out) % 8 || (out_token | out_head) % 4) bad = "every output row must be 8-byte aligned";
+  else if ((reinterpret_cast<uintptr_t>(cu_q) | reinterpret_cast<uintptr_t>(cu_k)) % 4) bad = "cu must be 4-byte aligned";
+  if (bad) return fail(TX_ERR_INVALID, std::string("packed_attention: ") + bad);
+  if (sequences == 0 || total_q == 0) return TX_OK;
+  tx::PackedAttention a = {};
+  a.q = static_cast<const uint16_t *>(q);
+  a.k = static_cast<const uint16_t *>(k);
+  a.v = static_cast<const uint16_t *>(v);
+  a.out = static_cast<uint16_t *>(out);
+  a.q_token = q_token;
+  a.q_head = q_head;
+  a.k_token = k_token;
+  a.k_head = k_head;
+  a.v_token = v_token;
+  a.v_head = v_head;
+  a.out_token = out_token;
+  a.out_head = out_head;
+  a.cu_q = cu_q;
+  a.cu_k = cu_k;
+  a.sequences = sequences;
+  a.total_q = (int)total_q;
+  a.total_k = (int)total_k;
+  a.heads = heads;
+  a.group = heads / kv_heads;
+  a.scale = scale;
+  DeviceGuard guard(device);
+  TX_HIP(tx::launch_packed_attention(a, dtype == TX_DTYPE_F16, head_dim, multiprocessors(device),
+                                     reinterpret_cast<hipStream_t>(stream)));
   return TX_OK;
 }
 

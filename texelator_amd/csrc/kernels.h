@@ -236,4 +236,34 @@ int64_t lm_head_argmax_workspace();
 hipError_t launch_lm_head_argmax(const uint16_t *weight, int64_t vocab, int hidden, const uint16_t *x, uint16_t *logits,
                                  void *workspace, int64_t *token, hipStream_t stream);
 
+
+// The paged 4-bit KV cache (kv4.hip, kv4_attention.hip; layout in kv4.h).
+struct Kv4Pool;
+// Token rows [tokens][kv_heads][dim] (strides in elements, rows 16-byte aligned) into and out of the cache; cu as in
+// the header's tx_kv4_append.
+hipError_t launch_kv4_append(const uint16_t *k, int64_t k_token, int64_t k_head, const uint16_t *v, int64_t v_token,
+                             int64_t v_head, int tokens, bool f16, int dim, const int *cu, const Kv4Pool &pool,
+                             hipStream_t stream);
+hipError_t launch_kv4_read(uint16_t *k, int64_t k_token, int64_t k_head, uint16_t *v, int64_t v_token, int64_t v_head,
+                           int tokens, bool f16, int dim, const int *cu, const Kv4Pool &pool, hipStream_t stream);
+constexpr int kKv4Pairs = 448;  // page pairs of one copy launch: 3.5 KiB of kernel arguments
+hipError_t launch_kv4_copy_pages(uint8_t *pool, int layers, int64_t layer_bytes, int64_t page_bytes, const int64_t *src,
+                                 const int64_t *dst, int64_t count, hipStream_t stream);
+struct Kv4Attention;
+bool kv4_attention_fits(const Kv4Pool &pool);
+// Fills in workgroups, least_units and piece_bytes (the workspace's size).
+void kv4_attention_plan(Kv4Attention &a, int dim, int cus);
+hipError_t launch_kv4_attention(const Kv4Attention &a, bool f16, int dim, hipStream_t stream);
+
+// Causal attention of packed sequences (packed_attention.hip). Strides in elements.
+struct PackedAttention {
+  const uint16_t *q, *k, *v;
+  uint16_t *out;
+  int64_t q_token, q_head, k_token, k_head, v_token, v_head, out_token, out_head;
+  const int *cu_q, *cu_k;  // [sequences + 1] first rows
+  int sequences, total_q, total_k, heads, group;
+  float scale;
+};
+hipError_t launch_packed_attention(const PackedAttention &a, bool f16, int dim, int cus, hipStream_t stream);
+
 }  // namespace tx

@@ -540,3 +540,200 @@ def swiglu(gate_up: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tens
         out = torch.empty((rows, width // 2), dtype=torch.bfloat16, device=gate_up.device)
     check(_lib.load().tx_swiglu(_ptr(gate_up), rows, width // 2, _ptr(out), _stream(gate_up)))
     return out
+
+
+# ---------------------------------------------------------------------------------------------
+# Several sequences at once
+
+_ROW_CODE = {torch.float16: _lib.TX_DTYPE_F16, torch.bfloat16: _lib.TX_DTYPE_BF16}
+
+
+def _expect_rows(name: str, t: torch.Tensor, like: torch.Tensor, heads: int, head_dim: int) -> None:
+    _expect(t.dim() == 3 and t.dtype == like.dtype and t.device == like.device and t.shape[1] == heads
+            and t.shape[2] == head_dim and t.stride(2) == 1, f"{name} must be {like.dtype} [rows, {heads}, {head_dim}] on one device, "
+            "the last dimension contiguous")
+
+
+def _expect_ints(name: str, t: torch.Tensor, count: int, device: torch.device) -> None:
+    _expect(t.dtype == torch.int32 and t.dim() == 1 and t.shape[0] == count and t.device == device and t.is_contiguous(),
+            f"{name} must be a contiguous int32 [{count}] on the same device")
+
+
+def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor, scale: float,
+                     cu_k: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal attention of several sequences packed one behind the other: ``q`` ``[tokens, heads, dim]`` against
+    ``k``/``v`` ``[keys, kv_heads, dim]`` (bf16 or fp16, dim 64 or 128, every row 16-byte aligned: views of one
+    ``[q | k | v]`` projection will do). Sequence ``s`` has the queries ``cu_q[s] .. cu_q[s + 1] - 1`` and the keys
+    ``cu_k[s] .. cu_k[s + 1] - 1`` (int32 on the device; ``cu_k`` defaults to ``cu_q``); its last query sees its last key,
+    so keys of earlier turns come first. A query that sees no key gets zeros; rows of ``out`` that belong to no
+    sequence are left as they are (uninitialised where ``out`` is not given). Returns ``[tokens, heads, dim]``."""
+    _expect(q.is_cuda and q.dim() == 3 and q.dtype in _ROW_CODE and q.stride(2) == 1,
+            "q must be CUDA bf16 or fp16 [tokens, heads, dim], the last dimension contiguous")
+    total, heads, dim = q.shape
+    kv_heads = k.shape[1] if k.dim() == 3 else 0
+    _expect_rows("k", k, q, kv_heads, dim)
+    _expect_rows("v", v, q, kv_heads, dim)
+    _expect(kv_heads > 0 and v.shape[0] == k.shape[0], "k and v must have as many rows and at least one head")
+    _expect(cu_q.dim() == 1 and cu_q.shape[0] > 0, "cu_q must be int32 [sequences + 1]")
+    if cu_k is None:
+        _expect(k.shape[0] == total, "without cu_k there is a key for each query")
+        cu_k = cu_q
+    _expect_ints("cu_q", cu_q, cu_q.shape[0], q.device)
+    _expect_ints("cu_k", cu_k, cu_q.shape[0], q.device)
+    if out is None:
+        out = torch.empty((total, heads, dim), dtype=q.dtype, device=q.device)
+    else:
+        _expect_rows("out", out, q, heads, dim)
+        _expect(out.shape[0] == total, "out must be shaped like q")
+    if total == 0:
+        return out
+    check(_lib.load().tx_packed_attention(
+        q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
+        _ROW_CODE[q.dtype], heads, kv_heads, dim, cu_q.data_ptr(), cu_k.data_ptr(), cu_q.shape[0] - 1, total, k.shape[0],
+        float(scale), out.data_ptr(), out.stride(0), out.stride(1), q.device.index, _stream(q)))
+    return out
+
+
+def kv4_pages(num_pages: int, kv_heads: int, head_dim: int, page_size: int = 64, layers: int | None = None,
+              device: torch.device | str = "cuda") -> torch.Tensor:
+    """An empty pool of a paged 4-bit KV cache: uint8 ``[num_pages, kv_heads, 2, page_size * head_dim * 17 / 32]``, behind
+    ``layers`` where given (``pages[i]`` is layer i's pool, and one block table serves them all). A key or value takes
+    ``head_dim * 17 / 32`` bytes: E2M1 codes and an E8M0 scale for 32 elements. ``page_size``: positions of a page, a
+    power of two from 16 to 1024; ``head_dim`` 64 or 128."""
+    _expect(head_dim in (64, 128), "head_dim must be 64 or 128")
+    _expect(16 <= page_size <= 1024 and page_size & (page_size - 1) == 0, "page_size must be a power of two from 16 to 1024")
+    _expect(num_pages > 0 and kv_heads > 0 and (layers is None or layers > 0), "bad pool shape")
+    shape = (num_pages, kv_heads, 2, page_size * head_dim * 17 // 32)
+    return torch.zeros(shape if layers is None else (layers, *shape), dtype=torch.uint8, device=device)
+
+
+def _kv4_args(pages: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor, head_dim: int) -> tuple:
+    """The cache's arguments of a C call, from pages to sequences."""
+    _expect(head_dim in (64, 128), "head_dim must be 64 or 128")
+    _expect(pages.is_cuda and pages.dtype == torch.uint8 and pages.dim() == 4 and pages.shape[2] == 2 and pages.is_contiguous(),
+            "pages must be contiguous CUDA uint8 [num_pages, kv_heads, 2, page bytes]")
+    num_pages, kv_heads, _, half = pages.shape
+    row = head_dim * 17 // 32
+    _expect(half % row == 0, "pages were made for another head_dim")
+    _expect(block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.device == pages.device
+            and (block_table.stride(1) == 1 or block_table.shape[1] == 1),
+            "block_table must be int32 [sequences, pages] on the same device, rows contiguous")
+    sequences, max_pages = block_table.shape
+    _expect_ints("lengths", lengths, sequences, pages.device)
+    return (pages.data_ptr(), num_pages, kv_heads, head_dim, half // row, block_table.data_ptr(), block_table.stride(0),
+            max_pages, lengths.data_ptr(), sequences)
+
+
+def kv4_append(k: torch.Tensor, v: torch.Tensor, pages: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor,
+               cu: torch.Tensor | None = None) -> None:
+    """New keys and values into a paged 4-bit cache (:func:`kv4_pages`): ``k``/``v`` ``[tokens, kv_heads, dim]`` bf16 or fp16,
+    every row 16-byte aligned. Position p of sequence s lies at offset ``p % page_size`` of page ``block_table[s, p //
+    page_size]`` (int32 ``[sequences, pages]``, -1 or any id outside the pool where there is none). ``lengths`` (int32
+    ``[sequences]``) counts the new tokens already, so that one update serves all layers: the tokens ``cu[s] .. cu[s + 1] - 1``
+    become the last ones of ``lengths[s]`` positions (``cu`` int32 ``[sequences + 1]``; without it, one token for each
+    sequence). A page that receives tokens must belong to one sequence alone."""
+    _expect(k.is_cuda and k.dim() == 3 and k.dtype in _ROW_CODE and k.stride(2) == 1 and k.device == pages.device,
+            "k must be CUDA bf16 or fp16 [tokens, kv_heads, dim] on the pages' device, the last dimension contiguous")
+    tokens, kv_heads, dim = k.shape
+    _expect_rows("v", v, k, kv_heads, dim)
+    cache = _kv4_args(pages, block_table, lengths, dim)
+    _expect(kv_heads == cache[2] and v.shape[0] == tokens, "k and v must have the pages' heads and as many rows")
+    if cu is None:
+        _expect(tokens == cache[-1], "without cu there is one token for each sequence")
+    else:
+        _expect_ints("cu", cu, cache[-1] + 1, k.device)
+    if tokens == 0 or cache[-1] == 0:
+        return
+    check(_lib.load().tx_kv4_append(k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
+                                    _ROW_CODE[k.dtype], tokens, None if cu is None else cu.data_ptr(), *cache,
+                                    k.device.index, _stream(k)))
+
+
+def kv4_read(pages: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor, head_dim: int,
+             cu: torch.Tensor | None = None, tokens: int | None = None, dtype: torch.dtype = torch.bfloat16,
+             out: tuple[torch.Tensor, torch.Tensor] | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Rows of a paged 4-bit cache as the values they stand for: ``(k, v)``, each ``[tokens, kv_heads, head_dim]`` packed as
+    :func:`kv4_append` takes them: the last ``cu[s + 1] - cu[s]`` of ``lengths[s]`` positions of every sequence (all of them
+    where ``cu`` is the sums of ``lengths``, as :func:`packed_attention` takes the keys of earlier turns); without ``cu``
+    the last one of each. ``tokens``: the rows in all, ``cu[-1]`` (needed with ``cu`` unless ``out`` is given). Rows that name
+    no position are left as they are."""
+    cache = _kv4_args(pages, block_table, lengths, head_dim)
+    if cu is None:
+        _expect(tokens is None or tokens == cache[-1], "without cu there is one token for each sequence")
+        tokens = cache[-1]
+    else:
+        _expect_ints("cu", cu, cache[-1] + 1, pages.device)
+    if out is None:
+        _expect(tokens is not None and tokens >= 0 and dtype in _ROW_CODE, "tokens is needed with cu; dtype is bf16 or fp16")
+        out = torch.empty((2, tokens, cache[2], head_dim), dtype=dtype, device=pages.device).unbind(0)
+    k, v = out
+    _expect(k.is_cuda and k.dtype in _ROW_CODE and k.device == pages.device, "out must be CUDA bf16 or fp16 on the pages' device")
+    _expect_rows("k", k, k, cache[2], head_dim)
+    _expect_rows("v", v, k, cache[2], head_dim)
+    _expect(v.shape[0] == k.shape[0] and (tokens is None or k.shape[0] == tokens), "k and v must have as many rows as tokens")
+    if k.shape[0] == 0 or cache[-1] == 0:
+        return k, v
+    check(_lib.load().tx_kv4_read(k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
+                                  _ROW_CODE[k.dtype], k.shape[0], None if cu is None else cu.data_ptr(), *cache,
+                                  pages.device.index, _stream(pages)))
+    return k, v
+
+
+def kv4_attention_workspace_bytes(pages: torch.Tensor, block_table: torch.Tensor, heads: int, head_dim: int) -> int:
+    """Device scratch of :func:`kv4_attention`: it depends on shapes alone, not on the lengths."""
+    sequences, max_pages = block_table.shape
+    out = ctypes.c_int64(0)
+    check(_lib.load().tx_kv4_attention_workspace(sequences, heads, pages.shape[1], head_dim, pages.shape[3] * 32 // (17 * head_dim),
+                                                 max_pages, pages.device.index, out))
+    return out.value
+
+
+def kv4_attention(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor, scale: float,
+                  workspace: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of one query token for each sequence over a paged 4-bit cache: ``q`` ``[sequences, heads, dim]`` bf16 or fp16
+    (every query 16-byte aligned) against the ``lengths[s]`` positions that ``block_table[s]`` names (see
+    :func:`kv4_append`); heads a multiple of the pages' KV heads. Returns ``[sequences, heads, dim]``, zeros for an empty
+    sequence. ``workspace``: :func:`kv4_attention_workspace_bytes` bytes that no call running at the same time uses;
+    allocated on the current stream where not given."""
+    _expect(q.is_cuda and q.dim() == 3 and q.dtype in _ROW_CODE and q.stride(2) == 1 and q.device == pages.device,
+            "q must be CUDA bf16 or fp16 [sequences, heads, dim] on the pages' device, the last dimension contiguous")
+    sequences, heads, dim = q.shape
+    cache = _kv4_args(pages, block_table, lengths, dim)
+    _expect(cache[-1] == sequences and heads > 0 and heads % cache[2] == 0,
+            "q must have a row for each sequence and a multiple of the pages' heads")
+    if out is None:
+        out = torch.empty((sequences, heads, dim), dtype=q.dtype, device=q.device)
+    else:
+        _expect_rows("out", out, q, heads, dim)
+        _expect(out.shape[0] == sequences, "out must be shaped like q")
+    if sequences == 0:
+        return out
+    if workspace is None:
+        workspace = torch.empty(kv4_attention_workspace_bytes(pages, block_table, heads, dim), dtype=torch.uint8, device=q.device)
+    _expect(workspace.is_cuda and workspace.is_contiguous() and workspace.device == q.device,
+            "workspace must be a contiguous CUDA tensor on the same device")
+    check(_lib.load().tx_kv4_attention(q.data_ptr(), q.stride(0), q.stride(1), _ROW_CODE[q.dtype], heads, *cache, float(scale),
+                                       workspace.data_ptr(), workspace.nbytes, out.data_ptr(), out.stride(0), out.stride(1),
+                                       q.device.index, _stream(q)))
+    return out
+
+
+def kv4_copy_pages(pages: torch.Tensor, src: list[int], dst: list[int]) -> None:
+    """Page ``src[i]`` to page ``dst[i]`` for every i, in one pool (:func:`kv4_pages`) or in all layers' pools
+    ``[layers, ...]`` at once: a fork copies the last, partly filled page, a compaction moves pages and frees theirs.
+    ``src`` and ``dst`` are host integers (a captured call repeats the copies it was captured with). All copies happen at once:
+    a page that is copied to twice, or both copied from and copied to, is refused."""
+    _expect(pages.is_cuda and pages.dtype == torch.uint8 and pages.dim() in (4, 5) and pages.is_contiguous(),
+            "pages must be contiguous CUDA uint8 [num_pages, kv_heads, 2, page bytes], layers before it or not")
+    count = len(src)
+    _expect(len(dst) == count, "src and dst must have as many pages")
+    if count == 0:
+        return
+    *layers, num_pages, kv_heads, _, half = pages.shape
+    ids = ctypes.c_int64 * count
+    try:
+        sources, targets = ids(*src), ids(*dst)
+    except TypeError as error:
+        raise TexelatorError("src and dst must be integers") from error
+    check(_lib.load().tx_kv4_copy_pages(pages.data_ptr(), layers[0] if layers else 1, num_pages, kv_heads * 2 * half, sources,
+                                        targets, count, pages.device.index, _stream(pages)))
