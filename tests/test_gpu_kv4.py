@@ -164,6 +164,8 @@ ATTEND = [
     ([9, 30000, 700, 1], 4, 4, 64, 64),
     ([(37 * i) % 301 for i in range(150)], 4, 2, 128, 16),  # more sequences than lanes
     ([(53 * i) % 1500 for i in range(70)], 12, 12, 64, 32),
+    ([(29 * i) % 900 for i in range(80)], 16, 4, 128, 64),  # heads that fill the chip: a workgroup each up to 1024 positions
+    ([(29 * i) % 400 for i in range(66)], 33, 1, 64, 16),
 ]
 
 

@@ -51,8 +51,8 @@ REFUSED = [
         *POOL_FAULTS, dict(k=None), dict(v=None), dict(dtype=2), dict(tokens=-1), dict(tokens=1 << 31), dict(cu=None), dict(k=P + 8),
         dict(v=P + 2), dict(k_token=260), dict(v_head=4), dict(cu=P + 2)]),
     *(attend(**c) for c in [
-        *POOL_FAULTS, dict(q=None), dict(out=None), dict(workspace=None), dict(dtype=2), dict(heads=15), dict(heads=0), dict(q=P + 8),
-        dict(q_head=60), dict(q_sequence=4), dict(out=P + 4), dict(out_head=2), dict(workspace=P + 8), dict(workspace_bytes=64),
+        *POOL_FAULTS, dict(q=None), dict(out=None), dict(workspace=None, max_pages=500), dict(dtype=2), dict(heads=15), dict(heads=0), dict(q=P + 8),
+        dict(q_head=60), dict(q_sequence=4), dict(out=P + 4), dict(out_head=2), dict(workspace=P + 8), dict(workspace_bytes=64, max_pages=500),
         dict(max_pages=1 << 24, sequences=4096, kv_heads=16)]),
 ]
 

@@ -5,7 +5,9 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstring>
+#include <limits>
 #include <mutex>
 #include <new>
 #include <string>
@@ -1516,7 +1518,7 @@ int tx_kv4_attention(const void *q, int64_t q_sequence, int64_t q_head, int dtyp
   tx::Kv4Attention a = {};
   const char *bad = kv4_pool(a.pool, pages, num_pages, kv_heads, head_dim, page_size, block_table, table_stride, max_pages,
                              lengths, sequences);
-  if (!bad && (!q || !out || !workspace)) bad = "null pointer";
+  if (!bad && (!q || !out)) bad = "null pointer";
   if (!bad && dtype != TX_DTYPE_F16 && dtype != TX_DTYPE_BF16) bad = "q must be FP16 or BF16";
   if (!bad && (heads <= 0 || heads % kv_heads || heads / kv_heads > 65535)) bad = "heads must be a multiple of kv_heads";
   if (!bad && (reinterpret_cast<uintptr_t>(q) % 16 || (q_sequence | q_head) % 8)) bad = "every query must be 16-byte aligned";
@@ -1532,10 +1534,12 @@ int tx_kv4_attention(const void *q, int64_t q_sequence, int64_t q_head, int dtyp
   a.out_sequence = out_sequence;
   a.out_head = out_head;
   a.group = heads / kv_heads;
-  a.scale = scale;
+  a.sl2 = std::max(std::fabs(scale) * 1.44269504088896340736f, std::numeric_limits<float>::min());
+  a.q_and = scale == 0.f ? 0u : ~0u;
+  a.q_xor = scale < 0.f ? 0x80008000u : 0u;
   a.pieces = static_cast<float *>(workspace);
   tx::kv4_attention_plan(a, head_dim, multiprocessors(device));
-  if (workspace_bytes < a.piece_bytes) return fail(TX_ERR_INVALID, "kv4_attention: workspace too small (tx_kv4_attention_workspace)");
+  if (workspace_bytes < a.piece_bytes || (a.piece_bytes > 0 && !workspace)) return fail(TX_ERR_INVALID, "kv4_attention: workspace too small (tx_kv4_attention_workspace)");
   DeviceGuard guard(device);
   TX_HIP(tx::launch_kv4_attention(a, dtype == TX_DTYPE_F16, head_dim, reinterpret_cast<hipStream_t>(stream)));
   return TX_OK;

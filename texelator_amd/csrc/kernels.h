@@ -251,7 +251,7 @@ hipError_t launch_kv4_copy_pages(uint8_t *pool, int layers, int64_t layer_bytes,
                                  const int64_t *dst, int64_t count, hipStream_t stream);
 struct Kv4Attention;
 bool kv4_attention_fits(const Kv4Pool &pool);
-// Fills in workgroups, least_units and piece_bytes (the workspace's size).
+// Fills in workgroups, whole and piece_bytes (the workspace's size).
 void kv4_attention_plan(Kv4Attention &a, int dim, int cus);
 hipError_t launch_kv4_attention(const Kv4Attention &a, bool f16, int dim, hipStream_t stream);
 

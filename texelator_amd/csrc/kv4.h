@@ -34,10 +34,14 @@ struct Kv4Attention {
   uint16_t *out;
   int64_t out_sequence, out_head;
   int group;  // query heads per KV head
-  float scale;
+  // exp2(sl2 * q . k) is exp(scale * q . k): sl2 is above zero, the scale's sign is put into the queries' bits
+  // ((bits & q_and) ^ q_xor), which are cleared for a scale of zero.
+  float sl2;
+  uint32_t q_and, q_xor;
   float *pieces;        // results of heads that several workgroups share
   int64_t piece_bytes;  // bytes of them
-  int workgroups, least_units;
+  int workgroups;
+  bool whole;  // a workgroup for each head: no pieces
 };
 
 // Bytes of one head's keys (or values) in a page.

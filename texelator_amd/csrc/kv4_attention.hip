@@ -35,10 +35,18 @@ namespace tx {
 
 namespace {
 
-constexpr int kWaves = 4;
-constexpr int kTile = 32;               // positions of a wave's step
-constexpr int kUnit = kWaves * kTile;   // positions of a workgroup's step
-constexpr int kCols = 16;               // queries of an MFMA tile
+constexpr int kCols = 16;  // queries of an MFMA tile
+
+constexpr int kWaves = 4;  // of a workgroup
+
+// Positions of a wave's step (4.25 KiB of cache) and of a workgroup's: a unit.
+template <int DIM>
+constexpr int kTile = 4096 / DIM;
+template <int DIM>
+constexpr int kUnit = kTile<DIM> * kWaves;
+// Workgroups that a CU holds: their registers (and, at dim 64, their LDS) set it. At dim 128 four would spill.
+template <int DIM>
+constexpr int kResident = DIM == 128 ? 3 : 4;
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
@@ -90,18 +98,27 @@ __device__ __forceinline__ float quarters_sum(float v) {
 }
 
 // Units of a sequence's KV head: one even if it is empty, whose output is zeros.
-__device__ __forceinline__ int head_units(int length) { return max(1, (length + kUnit - 1) / kUnit); }
+template <int UNIT>
+__device__ __forceinline__ int head_units(int length) { return max(1, (length + UNIT - 1) / UNIT); }
+
+// What starting and ending a head costs, in units: a head's share of the row of units begins with as many without work.
+constexpr int kStart = 1;
 
 // Units of every workgroup.
 __device__ __forceinline__ int run_units(int total, const Kv4Attention &a) {
-  return max((total + a.workgroups - 1) / a.workgroups, a.least_units);
+  return (total + a.workgroups - 1) / a.workgroups;
 }
+
+// All of the workgroup's LDS accesses so far are done; loads from memory stay in flight.
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 // Floats of a piece: per query its output [dim], then max and sum of all queries.
 __device__ __host__ inline int64_t piece_floats(int group, int dim) { return (int64_t)group * (dim + 2); }
 
 template <bool F16, int DIM>
-__global__ __launch_bounds__(64 * kWaves, 4) void kv4_attention_kernel(Kv4Attention a) {
+__global__ __launch_bounds__(64 * kWaves, kResident<DIM>) void kv4_attention_kernel(Kv4Attention a) {
+  constexpr int kUnit = tx::kUnit<DIM>, kTile = tx::kTile<DIM>;
+  constexpr int kSubs = kTile / 16;       // 16 positions make an MFMA tile of scores
   constexpr int kWords = DIM / 32;        // words of codes a lane holds of a row: 4 or 2
   constexpr int kRow = DIM * 2;           // bytes of a converted row
   constexpr int kMergeRow = DIM + 4;      // floats of a query's output in the merge
@@ -117,110 +134,175 @@ __global__ __launch_bounds__(64 * kWaves, 4) void kv4_attention_kernel(Kv4Attent
   const int col0 = blockIdx.y * kCols;                 // first query (of the group) of this workgroup
   const int cols = min(kCols, a.group - col0);
 
-  auto units_of = [&](int s) { return pool.kv_heads * head_units(kv4_length(pool, s)); };
-  const int total = ragged_total(pool.sequences, units_of);
-  const int run = run_units(total, a);
-  int unit = blockIdx.x * run;
-  if (unit >= total) return;
-  const int end = min(unit + run, total);
-  int sequence, local;
-  ragged_find(pool.sequences, unit, units_of, sequence, local);
-  sequence = __builtin_amdgcn_readfirstlane(sequence);
-  int length = __builtin_amdgcn_readfirstlane(kv4_length(pool, sequence));
-  int units = head_units(length);
-  int head = __builtin_amdgcn_readfirstlane(local / units);
-  int first = __builtin_amdgcn_readfirstlane(local) - head * units;  // first unit of this head to do
-  int slot = 0;                                        // 0: the run's first piece
+  // The run: units [unit, end) of the row of all; the part of one head that lies in it.
+  struct Part {
+    int sequence, head, length, units;
+    int first, until;  // the head's units
+    int slot;          // where its piece goes: 0 for the head in which the run begins
+    bool any;
+  };
+  int unit, end, sequence, head, from, length;
+  if (a.whole) {  // a workgroup for each head
+    sequence = blockIdx.x / pool.kv_heads;
+    head = blockIdx.x % pool.kv_heads;
+    length = __builtin_amdgcn_readfirstlane(kv4_length(pool, sequence));
+    unit = from = 0;
+    end = head_units<kUnit>(length);
+  } else {
+    auto units_of = [&](int s) { return pool.kv_heads * (kStart + head_units<kUnit>(kv4_length(pool, s))); };
+    const RaggedPlace place = ragged_place(pool.sequences, units_of, [&](int total) { return (int)blockIdx.x * run_units(total, a); });
+    const int run = run_units(place.total, a);
+    unit = blockIdx.x * run;
+    end = min(unit + run, place.total);
+    if (unit >= end) return;
+    sequence = place.sequence;
+    length = __builtin_amdgcn_readfirstlane(kv4_length(pool, sequence));
+    head = place.local / (kStart + head_units<kUnit>(length));
+    from = place.local - head * (kStart + head_units<kUnit>(length)) - kStart;  // below 0: units without work
+  }
+  int slot = 0;
+  auto take = [&]() {
+    const int units = head_units<kUnit>(length);
+    const int until = min(units, from + end - unit);
+    const Part part = {sequence, head, length, units, max(from, 0), until, slot, unit < end && until > max(from, 0)};
+    unit += until - from;
+    from = -kStart;
+    slot = 1;
+    if (++head == pool.kv_heads && unit < end) {
+      head = 0;
+      length = __builtin_amdgcn_readfirstlane(kv4_length(pool, ++sequence));
+    }
+    return part;
+  };
 
   const int64_t half_bytes = kv4_half_bytes(pool.page_shift, DIM);
   const int64_t scales_at = (int64_t)(DIM / 2) << pool.page_shift;
-  const float sl2 = a.scale * 1.44269504088896340736f;  // scores in log2 units
+  const float sl2 = a.sl2;  // above zero; the scale's sign is in the queries
   constexpr float kLift = F16 ? 15.f : 0.f;
 
   char *mine = lds[wave];
   // A converted row's 32-byte pieces lie at piece ^ turn(row): rows that one transposing read takes hit distinct banks.
   auto piece_at = [](int row, int piece) { return row * kRow + 32 * (piece ^ (DIM == 128 ? row & 7 : (row >> 1) & 3)); };
 
-  while (unit < end) {
-    const int count = min(units - first, end - unit);
-    const int sequence_pages = (length + (1 << pool.page_shift) - 1) >> pool.page_shift;
-    const int *table = pool.table + sequence * pool.table_stride;
+  // Page ids of a step's positions, fetched a step before its codes are.
+  struct Ids {
+    int page[kSubs];
+  };
+  auto ids_of = [&](const Part &part, int position) __attribute__((always_inline)) {
+    // Constant for the whole launch: scalar loads, whose wait leaves the codes under way alone.
+    const auto *table = (const __attribute__((address_space(4))) int *)(pool.table + part.sequence * pool.table_stride);
+    Ids ids;
+#pragma unroll
+    for (int i = 0; i < kSubs; ++i) ids.page[i] = table[min(position + 16 * i, max(part.length - 1, 0)) >> pool.page_shift];
+    return ids;
+  };
+  struct Tile {
+    Codes k[kSubs], v[kSubs];
+    uint32_t ks[kSubs], vs[kSubs];
+    int valid[kSubs];  // positions of each 16 that count
+  };
+  // A lane's share of row n of each 16 positions.
+  const uint32_t code_lane = n * (DIM / 2) + quarter * (DIM / 8), scale_lane = n * kWords + (DIM == 128 ? quarter : quarter >> 1);
+  auto load = [&](Tile &t, const Part &part, int position, const Ids &ids) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < kSubs; ++i) {
+      const int at = position + 16 * i;
+      const bool known = (uint32_t)ids.page[i] < (uint64_t)pool.num_pages;
+      t.valid[i] = known ? min(max(part.length - at, 0), 16) : 0;
+      const int page = known ? ids.page[i] : 0;
+      const int row = at & ((1 << pool.page_shift) - 1);
+      const uint8_t *codes = pool.pages + ((int64_t)page * pool.kv_heads + part.head) * 2 * half_bytes + row * (DIM / 2);
+      const uint8_t *scales = codes + scales_at - row * (DIM / 2 - kWords);
+      t.k[i] = *reinterpret_cast<const Codes *>(codes + code_lane);
+      t.v[i] = *reinterpret_cast<const Codes *>(codes + half_bytes + code_lane);
+      t.ks[i] = scales[scale_lane];
+      t.vs[i] = (scales + half_bytes)[scale_lane];
+    }
+  };
+  // This wave's steps of a part: every unit's `wave`-th.
+  Tile cur, next;
+  Ids ids;
+  auto start_of = [&](const Part &part) { return part.first * kUnit + wave * kTile; };
+  auto stop_of = [&](const Part &part) { return min(part.until * kUnit, part.length); };
+  auto begin = [&](const Part &part) __attribute__((always_inline)) {
+    const int position = start_of(part);
+    if (!part.any || position >= stop_of(part)) return;
+    ids = ids_of(part, position);
+    load(cur, part, position, ids);
+    ids = ids_of(part, position + kUnit);
+  };
 
+  Part part = take();
+  begin(part);
+  while (part.any) {
+    int position = start_of(part);
+    const int last = stop_of(part);
     // B operands: query n, dimensions DIM/4 * quarter + 8 st ..
     u32x4 qb[kWords];
     {
-      const uint16_t *q = a.q + sequence * a.q_sequence + (head * a.group + col0 + min(n, cols - 1)) * a.q_head + DIM / 4 * quarter;
+      const uint16_t *q = a.q + part.sequence * a.q_sequence + (part.head * a.group + col0 + min(n, cols - 1)) * a.q_head + DIM / 4 * quarter;
 #pragma unroll
-      for (int st = 0; st < kWords; ++st) qb[st] = reinterpret_cast<const u32x4 *>(q)[st];
+      for (int st = 0; st < kWords; ++st) {
+        qb[st] = reinterpret_cast<const u32x4 *>(q)[st];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) qb[st][j] = (qb[st][j] & a.q_and) ^ a.q_xor;
+      }
     }
 
-    struct Tile {
-      Codes k[2], v[2];
-      uint32_t ks[2], vs[2];
-      int valid[2];
-    };
-    // The 16 positions from `position` on: a lane's share of row n.
-    auto load = [&](Tile &t, int position) __attribute__((always_inline)) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int at = position + 16 * i, index = at >> pool.page_shift;
-        int page = index < sequence_pages ? table[index] : -1;
-        int valid = min(max(length - at, 0), 16);
-        if ((uint32_t)page >= (uint64_t)pool.num_pages) page = 0, valid = 0;
-        t.valid[i] = valid;
-        const uint8_t *keys = pool.pages + ((int64_t)page * pool.kv_heads + head) * 2 * half_bytes;
-        const uint8_t *values = keys + half_bytes;
-        const uint32_t row = (uint32_t)(at & ((1 << pool.page_shift) - 1)) + n;
-        const uint32_t codes = row * (DIM / 2) + quarter * (DIM / 8), scale = row * kWords + (DIM == 128 ? quarter : quarter >> 1);
-        t.k[i] = *reinterpret_cast<const Codes *>(keys + codes);
-        t.v[i] = *reinterpret_cast<const Codes *>(values + codes);
-        t.ks[i] = (keys + scales_at)[scale];
-        t.vs[i] = (values + scales_at)[scale];
-      }
-    };
-
-    float m = -INFINITY, l = 0.f;  // running maximum of query n (log2 units), this lane's share of the sum
+    float m = -INFINITY, l = 0.f;  // running maximum of query n (before the scale), this lane's share of the sum
     f32x4 o[DIM / 16];             // o[t][r] = O[query n][dimension 16 t + 4 quarter + r]
 #pragma unroll
     for (int t = 0; t < DIM / 16; ++t) o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-    auto step = [&](const Tile &t) __attribute__((always_inline)) {
-      const bool whole = t.valid[0] + t.valid[1] == kTile;
-      f32x4 sc[2];
+    auto multiply = [&](Tile &t) __attribute__((always_inline)) {
+      int valid = 0;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        sc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-        const bool out = !whole && n >= t.valid[i];
-        const float scale = __uint_as_float((out ? 127u : t.ks[i]) << 23);
+      for (int i = 0; i < kSubs; ++i) valid += t.valid[i];
+      const bool whole = valid == kTile;
+      if (!whole) {
 #pragma unroll
-        for (int st = 0; st < kWords; ++st)
-          sc[i] = mfma16<F16>(kv4_octet<F16>(out ? 0u : t.k[i][st], scale), qb[st], sc[i]);
-      }
-      // sc[i][r]: position 16 i + 4 quarter + r, query n
+        for (int i = 0; i < kSubs; ++i) {
+          const bool out = n >= t.valid[i];
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          sc[i][r] *= sl2;
-          if (!whole) sc[i][r] = 4 * quarter + r < t.valid[i] ? sc[i][r] : -INFINITY;
+          for (int st = 0; st < kWords; ++st) {
+            t.k[i][st] = out ? 0u : t.k[i][st];
+            t.v[i][st] = out ? 0u : t.v[i][st];
+          }
+          t.ks[i] = out ? 127u : t.ks[i];
+          t.vs[i] = out ? 127u : t.vs[i];
         }
+      }
+      f32x4 sc[kSubs];
+#pragma unroll
+      for (int i = 0; i < kSubs; ++i) {
+        sc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        const float scale = __uint_as_float(t.ks[i] << 23);
+#pragma unroll
+        for (int st = 0; st < kWords; ++st) sc[i] = mfma16<F16>(kv4_octet<F16>(t.k[i][st], scale), qb[st], sc[i]);
+      }
       // Values: converted rows into LDS while the scores finish.
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const bool out = !whole && n >= t.valid[i];
-        const float scale = __uint_as_float((out ? 127u : t.vs[i]) << 23);
+      for (int i = 0; i < kSubs; ++i) {
+        const float scale = __uint_as_float(t.vs[i] << 23);
 #pragma unroll
         for (int st = 0; st < kWords; ++st) {
           const int d = DIM / 4 * quarter + 8 * st;  // first dimension of these eight
-          *reinterpret_cast<u32x4 *>(mine + piece_at(16 * i + n, d / 16) + 2 * (d & 8)) =
-              kv4_octet<F16>(out ? 0u : t.v[i][st], scale);
+          *reinterpret_cast<u32x4 *>(mine + piece_at(16 * i + n, d / 16) + 2 * (d & 8)) = kv4_octet<F16>(t.v[i][st], scale);
         }
       }
-      float mx = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])),
-                       fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
+      // sc[i][r]: position 16 i + 4 quarter + r, query n
+      if (!whole) {
+#pragma unroll
+        for (int i = 0; i < kSubs; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) sc[i][r] = 4 * quarter + r < t.valid[i] ? sc[i][r] : -INFINITY;
+      }
+      float mx = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < kSubs; ++i) mx = fmaxf(fmaxf(mx, fmaxf(sc[i][0], sc[i][1])), fmaxf(sc[i][2], sc[i][3]));
       const float mnew = fmaxf(m, quarters_max(mx));
       if (__builtin_amdgcn_ballot_w64(mnew > m) != 0) {
-        const float alpha = mnew > m ? __builtin_amdgcn_exp2f(m - mnew) : 1.f;
+        const float alpha = mnew > m ? __builtin_amdgcn_exp2f((m - mnew) * sl2) : 1.f;
         l *= alpha;
 #pragma unroll
         for (int t = 0; t < DIM / 16; ++t)
@@ -228,61 +310,65 @@ __global__ __launch_bounds__(64 * kWaves, 4) void kv4_attention_kernel(Kv4Attent
           for (int r = 0; r < 4; ++r) o[t][r] *= alpha;
         m = mnew;
       }
-      const float base = m == -INFINITY ? 0.f : m - kLift;  // no position yet: every score is -infinity
-      uint32_t pb[4];
+      const float base = m == -INFINITY ? 0.f : kLift - m * sl2;  // no position yet: every score is -infinity
+      uint32_t pb[2 * kSubs];
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < kSubs; ++i)
 #pragma unroll
         for (int r = 0; r < 4; r += 2)
-          pb[2 * i + r / 2] = pack2<F16>(__builtin_amdgcn_exp2f(sc[i][r] - base), __builtin_amdgcn_exp2f(sc[i][r + 1] - base), l);
-      const u32x4 p = {pb[0], pb[1], pb[2], pb[3]};  // slots 0-3: positions 4 quarter .., slots 4-7: the 16 behind
+          pb[2 * i + r / 2] = pack2<F16>(__builtin_amdgcn_exp2f(__builtin_fmaf(sc[i][r], sl2, base)),
+                                         __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i][r + 1], sl2, base)), l);
       // The wave's own writes, then its reads: LDS runs a wave's operations in order, the fence holds the compiler to it.
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
 #pragma unroll
-      for (int t = 0; t < DIM / 16; ++t) {
-        const int row = 4 * quarter + (n >> 2);
-        const char *lo_at = mine + piece_at(row, t) + 8 * (n & 3), *hi_at = mine + piece_at(row + 16, t) + 8 * (n & 3);
-        const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)lo_at));
-        const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)hi_at));
-        o[t] = mfma16<F16>(u32x4{lo[0], lo[1], hi[0], hi[1]}, p, o[t]);
+      for (int j = 0; j < kSubs / 2; ++j) {
+        const u32x4 p = {pb[4 * j], pb[4 * j + 1], pb[4 * j + 2], pb[4 * j + 3]};  // slots 0-3: positions 4 quarter .., 4-7: the 16 behind
+        const int row = 32 * j + 4 * quarter + (n >> 2);
+#pragma unroll
+        for (int t = 0; t < DIM / 16; ++t) {
+          const char *lo_at = mine + piece_at(row, t) + 8 * (n & 3), *hi_at = mine + piece_at(row + 16, t) + 8 * (n & 3);
+          const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)lo_at));
+          const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)hi_at));
+          o[t] = mfma16<F16>(u32x4{lo[0], lo[1], hi[0], hi[1]}, p, o[t]);
+        }
       }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
     };
-
-    // This wave's tiles: every unit's `wave`-th 32 positions, the next ones loaded before these are used.
-    const int last = min((first + count) * kUnit, length);
-    int position = first * kUnit + wave * kTile;
-    if (position < last) {
-      Tile cur, next;
-      load(cur, position);
-      for (; position + kUnit < last; position += kUnit) {
-        load(next, position + kUnit);
-        step(cur);
-        cur = next;
+    while (position < last) {
+      if (position + kUnit < last) {
+        load(next, part, position + kUnit, ids);
+        ids = ids_of(part, position + 2 * kUnit);
       }
-      step(cur);
+      multiply(cur);
+      cur = next;
+      position += kUnit;
     }
 
-    // The waves' shares meet in LDS. M is -infinity where no position counted: then l = 0 and O = 0 everywhere.
+    // The next part's first codes set out before this part's sums are joined.
+    const Part after = take();
+    begin(after);
+
+    // The waves' shares meet in LDS. M is -infinity where no position counted: then l = 0 and O = 0 everywhere (or NaN,
+    // where all scores were).
     l = quarters_sum(l);
     if (quarter == 0) {
       stats[wave][0][n] = m;
       stats[wave][1][n] = l;
     }
-    __syncthreads();
+    lds_barrier();
     float top = -INFINITY;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) top = fmaxf(top, stats[w][0][n]);
-    const float weight = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
+    const float weight = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - top) * sl2);
     float *merge = reinterpret_cast<float *>(mine);
 #pragma unroll
     for (int t = 0; t < DIM / 16; ++t)
       *reinterpret_cast<f32x4 *>(merge + n * kMergeRow + 16 * t + 4 * quarter) = o[t] * weight;
-    __syncthreads();
-    const bool complete = first == 0 && count == units;
-    float *piece = a.pieces + ((int64_t)(blockIdx.x * 2 + slot)) * piece_floats(a.group, DIM);
+    lds_barrier();
+    const bool complete = part.first == 0 && part.until == part.units;
+    float *piece = a.pieces + ((int64_t)(blockIdx.x * 2 + part.slot)) * piece_floats(a.group, DIM);
     for (int i = threadIdx.x; i < cols * (DIM / 4); i += 64 * kWaves) {
       const int q = i / (DIM / 4), d = 4 * (i % (DIM / 4));
       f32x4 sum = {0.f, 0.f, 0.f, 0.f};
@@ -294,10 +380,10 @@ __global__ __launch_bounds__(64 * kWaves, 4) void kv4_attention_kernel(Kv4Attent
       }
 #pragma unroll
       for (int w = 0; w < kWaves; ++w)
-        ll += stats[w][0][q] == -INFINITY ? stats[w][1][q] : stats[w][1][q] * __builtin_amdgcn_exp2f(stats[w][0][q] - mm);
+        ll += stats[w][0][q] == -INFINITY ? stats[w][1][q] : stats[w][1][q] * __builtin_amdgcn_exp2f((stats[w][0][q] - mm) * sl2);
       if (complete) {
         const float inverse = ll == 0.f ? 0.f : 1.f / ll;
-        uint16_t *out = a.out + sequence * a.out_sequence + (head * a.group + col0 + q) * a.out_head + d;
+        uint16_t *out = a.out + part.sequence * a.out_sequence + (part.head * a.group + col0 + q) * a.out_head + d;
         const uint32_t lo = to_half_bits<F16>(sum[0] * inverse) | (uint32_t)to_half_bits<F16>(sum[1] * inverse) << 16;
         const uint32_t hi = to_half_bits<F16>(sum[2] * inverse) | (uint32_t)to_half_bits<F16>(sum[3] * inverse) << 16;
         *reinterpret_cast<u32x2 *>(out) = u32x2{lo, hi};
@@ -310,97 +396,118 @@ __global__ __launch_bounds__(64 * kWaves, 4) void kv4_attention_kernel(Kv4Attent
         }
       }
     }
-    __syncthreads();  // before the buffers are written again
-    unit += count;
-    first = 0;
-    slot = 1;
-    if (++head == pool.kv_heads) {
-      head = 0;
-      ++sequence;
-      if (unit < end) {
-        length = __builtin_amdgcn_readfirstlane(kv4_length(pool, sequence));
-        units = head_units(length);
-      }
-    }
+    lds_barrier();  // before the buffers are written again
+    part = after;
   }
 }
 
-// Joins the pieces of heads that several workgroups shared. Grid: x = sequence * kv_heads + head, y = query of the group.
-template <bool F16, int DIM>
+// Joins the pieces of heads that several workgroups shared. Grid: x = sequence * kv_heads + head, y = query of the group,
+// z = 4 * LANES dimensions of its output.
+template <bool F16, int DIM, int LANES>
 __global__ __launch_bounds__(256) void kv4_combine_kernel(Kv4Attention a) {
-  constexpr int kLanes = DIM / 4, kGroups = 256 / kLanes;
-  __shared__ float lds[kGroups][DIM + 1];
-  __shared__ float sums[kGroups];
+  constexpr int kUnit = tx::kUnit<DIM>;
+  constexpr int kLanes = LANES, kGroups = 256 / kLanes, kHeld = 4;  // a thread holds kHeld pieces' values at once
+  __shared__ f32x4 lds[kGroups][kLanes];
+  __shared__ float sums[kGroups], tops[4];
   const Kv4Pool &pool = a.pool;
-  auto units_of = [&](int s) { return pool.kv_heads * head_units(kv4_length(pool, s)); };
   const int sequence = blockIdx.x / pool.kv_heads, head = blockIdx.x % pool.kv_heads, q = blockIdx.y;
-  const int run = run_units(ragged_total(pool.sequences, units_of), a);
-  const int units = head_units(kv4_length(pool, sequence));
-  const int begin = ragged_total(sequence, units_of) + head * units;  // this head's units: begin .. begin + units - 1
-  const int w0 = begin / run, w1 = (begin + units - 1) / run;
+  auto units_of = [&](int s) { return pool.kv_heads * (kStart + head_units<kUnit>(kv4_length(pool, s))); };
+  const RaggedPlace place = ragged_before(pool.sequences, units_of, sequence);
+  const int run = run_units(place.total, a);
+  const int units = head_units<kUnit>(kv4_length(pool, sequence));
+  const int begin = place.local + head * (kStart + units), work = begin + kStart;  // units with work: work .. work + units - 1
+  const int w0 = work / run, w1 = (work + units - 1) / run;
   if (w0 == w1) return;  // one workgroup had it all and wrote the output
-  const int group = threadIdx.x / kLanes, d = 4 * (threadIdx.x % kLanes);
-  const int64_t floats = piece_floats(a.group, DIM);
+  const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes, d = 4 * (kLanes * blockIdx.z + lane);
+  const int64_t floats = piece_floats(a.group, DIM), stats_at = (int64_t)a.group * DIM + 2 * q;
   // Only the first workgroup can have had another head before this one.
   auto piece = [&](int w) { return a.pieces + ((int64_t)w * 2 + (w == w0 && begin > w0 * run ? 1 : 0)) * floats; };
-  float top = -INFINITY;
-  for (int w = w0 + (threadIdx.x & 63); w <= w1; w += 64) top = fmaxf(top, piece(w)[(int64_t)a.group * DIM + 2 * q]);
-  top = wave_max(top);
+  // Each thread keeps its own running maximum over its pieces; the threads' sums meet under the largest.
   f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-  float l = 0.f;
-#pragma unroll 4
-  for (int w = w0 + group; w <= w1; w += kGroups) {
-    const float *p = piece(w);
-    const float *s = p + (int64_t)a.group * DIM + 2 * q;
-    const float m = s[0];
-    const float weight = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - top);  // an empty piece holds zeros (or NaN)
-    sum += *reinterpret_cast<const f32x4 *>(p + (int64_t)q * DIM + d) * weight;
-    l += s[1] * weight;
-  }
+  float l = 0.f, m = -INFINITY;
+  for (int w = w0 + group; w <= w1; w += kGroups * kHeld) {
+    f32x4 value[kHeld];
+    float pm[kHeld], pl[kHeld];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) lds[group][d + j] = sum[j];
-  if (d == 0) sums[group] = l;
+    for (int i = 0; i < kHeld; ++i) {
+      const float *p = piece(min(w + i * kGroups, w1));
+      value[i] = *reinterpret_cast<const f32x4 *>(p + (int64_t)q * DIM + d);
+      pm[i] = p[stats_at];
+      pl[i] = p[stats_at + 1];
+    }
+    float mnew = m;
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) mnew = w + i * kGroups <= w1 ? fmaxf(mnew, pm[i]) : mnew;
+    const float alpha = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - mnew) * a.sl2);
+    sum *= alpha;
+    l *= alpha;
+    m = mnew;
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+      if (w + i * kGroups > w1) continue;
+      const float weight = pm[i] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((pm[i] - m) * a.sl2);  // an empty piece holds zeros (or NaN)
+      sum += value[i] * weight;
+      l += pl[i] * weight;
+    }
+  }
+  float top = wave_max(m);
+  if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
   __syncthreads();
-  if (threadIdx.x < DIM) {
+  top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+  const float weight = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - top) * a.sl2);
+  lds[group][lane] = sum * weight;
+  if (lane == 0) sums[group] = l * weight;
+  __syncthreads();
+  if (threadIdx.x < 4 * kLanes) {
+    const float *column = reinterpret_cast<const float *>(&lds[0][0]) + threadIdx.x;
     float total = 0.f, ll = 0.f;
 #pragma unroll
     for (int g = 0; g < kGroups; ++g) {
-      total += lds[g][threadIdx.x];
+      total += column[g * 4 * kLanes];
       ll += sums[g];
     }
-    a.out[sequence * a.out_sequence + (head * a.group + q) * a.out_head + threadIdx.x] =
+    a.out[sequence * a.out_sequence + (head * a.group + q) * a.out_head + 4 * kLanes * blockIdx.z + threadIdx.x] =
         to_half_bits<F16>(ll == 0.f ? 0.f : total / ll);
   }
 }
 
-// Workgroups of a call, from what the host knows: an upper bound on its units.
-int64_t most_units(const Kv4Pool &pool) {
+// An upper bound on a call's units, from what the host knows.
+int64_t most_units(const Kv4Pool &pool, int unit) {
   const int64_t room = (int64_t)pool.max_pages << pool.page_shift;
-  const int64_t units = (room + kUnit - 1) / kUnit;
-  return (int64_t)pool.sequences * pool.kv_heads * (units > 1 ? units : 1);
+  const int64_t units = (room + unit - 1) / unit;
+  return (int64_t)pool.sequences * pool.kv_heads * (kStart + (units > 1 ? units : 1));
 }
 
 }  // namespace
 
-bool kv4_attention_fits(const Kv4Pool &pool) { return most_units(pool) <= (int64_t)1 << 30; }
+bool kv4_attention_fits(const Kv4Pool &pool) { return most_units(pool, kUnit<128>) <= (int64_t)1 << 30; }
 
 void kv4_attention_plan(Kv4Attention &a, int dim, int cus) {
-  const int64_t most = most_units(a.pool);
-  const int64_t fill = 4 * (int64_t)cus;  // four workgroups a CU are resident
-  a.workgroups = (int)(most < fill ? most : fill);
-  a.least_units = 1;
-  a.piece_bytes = (int64_t)a.workgroups * 2 * piece_floats(a.group, dim) * (int64_t)sizeof(float);
+  const int64_t room = (int64_t)a.pool.max_pages << a.pool.page_shift, heads = (int64_t)a.pool.sequences * a.pool.kv_heads;
+  // A workgroup for each head, and no combine kernel, where no head can be long: always up to 512 positions (128
+  // sequences of 500, 4 heads of 64: 7.3 us against 13.3), up to 1024 where the heads fill the chip by themselves (1024 heads
+  // of 64 at 600 positions 14.3 against 16.8; 2 heads of 128 at 700: 9.4 against 8.7).
+  a.whole = room <= 512 || (room <= 1024 && heads >= cus);
+  const int64_t most = most_units(a.pool, dim == 128 ? kUnit<128> : kUnit<64>);
+  const int64_t fill = (dim == 128 ? kResident<128> : kResident<64>) * (int64_t)cus;
+  a.workgroups = (int)(a.whole ? heads : most < fill ? most : fill);
+  a.piece_bytes = a.whole ? 0 : (int64_t)a.workgroups * 2 * piece_floats(a.group, dim) * (int64_t)sizeof(float);
 }
 
 hipError_t launch_kv4_attention(const Kv4Attention &a, bool f16, int dim, hipStream_t stream) {
   const dim3 grid((unsigned)a.workgroups, (unsigned)((a.group + kCols - 1) / kCols));
-  const dim3 combine((unsigned)(a.pool.sequences * a.pool.kv_heads), (unsigned)a.group);
+  const unsigned heads = (unsigned)(a.pool.sequences * a.pool.kv_heads);
   auto launch = [&](auto type, auto d) {
     constexpr bool kF16 = decltype(type)::value;
     constexpr int kDim = decltype(d)::value;
     hipLaunchKernelGGL((kv4_attention_kernel<kF16, kDim>), grid, dim3(64 * kWaves), 0, stream, a);
-    if (a.pool.max_pages > kUnit >> a.pool.page_shift)  // else no head has more than one unit
-      hipLaunchKernelGGL((kv4_combine_kernel<kF16, kDim>), combine, dim3(256), 0, stream, a);
+    if (a.whole) return;
+    // Few outputs are spread over more workgroups, 32 dimensions each (40 heads' queries of 1024 pieces: 5.2 us against
+    // 6.7); many are not (1280 of them 5.2 against 8.0).
+    if ((int64_t)heads * a.group * (kDim / 32) <= 1024)
+      hipLaunchKernelGGL((kv4_combine_kernel<kF16, kDim, 8>), dim3(heads, (unsigned)a.group, kDim / 32), dim3(256), 0, stream, a);
+    else
+      hipLaunchKernelGGL((kv4_combine_kernel<kF16, kDim, kDim / 4>), dim3(heads, (unsigned)a.group), dim3(256), 0, stream, a);
   };
   using std::integral_constant;
   if (f16 && dim == 128) launch(integral_constant<bool, true>{}, integral_constant<int, 128>{});

@@ -116,13 +116,14 @@ __global__ __launch_bounds__(64 * QW * KW, QW * KW * KB == 128 ? 1 : 2) __attrib
   const int hx = blockIdx.x % a.heads;
   const int head = a.heads % kXcds == 0 ? (hx % kXcds) * (a.heads / kXcds) + hx / kXcds : hx;
   auto tiles_of = [&](int s) { return (rows_of(a.cu_q, s, a.total_q).count + 32 * QW - 1) / (32 * QW); };
-  int sequence, tile;
-  if (!ragged_find(a.sequences, blockIdx.x / a.heads, tiles_of, sequence, tile)) return;
-  sequence = __builtin_amdgcn_readfirstlane(sequence);
+  const int wanted = blockIdx.x / a.heads;
+  const RaggedPlace place = ragged_place(a.sequences, tiles_of, [&](int) { return wanted; });
+  if (wanted >= place.total) return;
+  const int sequence = place.sequence;
   const Rows qs = rows_of(a.cu_q, sequence, a.total_q), ks = rows_of(a.cu_k, sequence, a.total_k);
   const int queries = __builtin_amdgcn_readfirstlane(qs.count), keys = __builtin_amdgcn_readfirstlane(ks.count);
   // The heaviest tiles of a sequence (the last) first.
-  tile = (queries + 32 * QW - 1) / (32 * QW) - 1 - __builtin_amdgcn_readfirstlane(tile);
+  const int tile = (queries + 32 * QW - 1) / (32 * QW) - 1 - place.local;
   const int shift = keys - queries;            // query i sees the keys up to i + shift
   const int q0 = (tile * QW + qw) * 32;        // this wave's first query
 

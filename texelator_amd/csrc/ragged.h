@@ -18,37 +18,52 @@ __device__ __forceinline__ int wave_scan(int v) {
   return v;
 }
 
-// Sum of count(s) over all sequences; every wave computes it alone.
-template <typename Count>
-__device__ __forceinline__ int ragged_total(int sequences, Count count) {
+// All sequences' items in one row: how many there are, and where one of them lies.
+struct RaggedPlace {
+  int total;     // items of all sequences
+  int sequence;  // the sequence that holds the item asked for (the last one's number past the end)
+  int local;     // the item's number in it
+};
+
+// The item `target(total)`. Every wave finds it alone; up to 64 sequences count(s) is called once.
+template <typename Count, typename Target>
+__device__ __forceinline__ RaggedPlace ragged_place(int sequences, Count count, Target target) {
   const int lane = threadIdx.x & 63;
-  int total = 0;
+  const int n0 = lane < sequences ? count(lane) : 0;
+  const int sum0 = wave_scan(n0);
+  int total = __builtin_amdgcn_readlane(sum0, 63);
+  for (int first = 64; first < sequences; first += 64)
+    total += __builtin_amdgcn_readlane(wave_scan(first + lane < sequences ? count(first + lane) : 0), 63);
+  const int wanted = target(total);
+  RaggedPlace place = {total, sequences - 1, 0};
+  int before = 0;
   for (int first = 0; first < sequences; first += 64) {
-    const int n = first + lane < sequences ? count(first + lane) : 0;
-    total += __builtin_amdgcn_readlane(wave_scan(n), 63);
+    const int n = first == 0 ? n0 : first + lane < sequences ? count(first + lane) : 0;
+    const int sum = first == 0 ? sum0 : wave_scan(n);
+    const uint64_t past = __builtin_amdgcn_ballot_w64(sum > wanted - before);
+    if (past) {
+      const int at = __builtin_ctzll(past);
+      place.sequence = first + at;
+      place.local = wanted - before - __builtin_amdgcn_readlane(sum - n, at);
+      break;
+    }
+    before += __builtin_amdgcn_readlane(sum, 63);
   }
-  return total;
+  return place;
 }
 
-// The sequence that holds item `target` of all sequences' items in order, and the item's number within it;
-// false past the last one. `before`: items of the earlier sequences.
+// The items in all, and in `local` those before sequence `s`.
 template <typename Count>
-__device__ __forceinline__ bool ragged_find(int sequences, int target, Count count, int &sequence, int &local) {
+__device__ __forceinline__ RaggedPlace ragged_before(int sequences, Count count, int s) {
   const int lane = threadIdx.x & 63;
-  int before = 0;
+  RaggedPlace place = {0, s, 0};
   for (int first = 0; first < sequences; first += 64) {
     const int n = first + lane < sequences ? count(first + lane) : 0;
     const int sum = wave_scan(n);
-    const int total = __builtin_amdgcn_readlane(sum, 63);
-    if (target < before + total) {
-      const int at = __builtin_ctzll(__builtin_amdgcn_ballot_w64(sum > target - before));
-      sequence = first + at;
-      local = target - before - __builtin_amdgcn_readlane(sum - n, at);
-      return true;
-    }
-    before += total;
+    if (s >= first && s < first + 64) place.local = place.total + __builtin_amdgcn_readlane(sum - n, s - first);
+    place.total += __builtin_amdgcn_readlane(sum, 63);
   }
-  return false;
+  return place;
 }
 
 }  // namespace tx
