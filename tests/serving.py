@@ -25,7 +25,8 @@ def attention64(q, k, v, scale, first):
     probabilities changes numerator and denominator by a factor in 1 +- u each: 2 u A. The fp32 scores are off by at most (dim
     + 4) 2^-24 S (sums, the two factors), which changes a probability by that share, again in both: twice; the same for the
     exponential's own 2^-22 and for fp32 sums over m keys and a few joins, (m + 64) 2^-24. The output is rounded once: u |out|, or
-    half of the smallest subnormal. In fp16 a probability below 2^-29 (held times 2^15) is off by up to 2^-40."""
+    half of the smallest subnormal. In fp16 probabilities are held times 2^11 at least, and below 2^-25 (subnormals then, half
+    a step being 2^-25) they are off by up to 2^-36, in numerator and denominator."""
     u = HALF_STEP[q.dtype]
     q, k, v = q.double(), k.double(), v.double()
     n, m, dim = q.shape[0], k.shape[0], q.shape[1]
@@ -42,7 +43,7 @@ def attention64(q, k, v, scale, first):
     loss = 2 * u + 2 * ((dim + 4) * 2.0 ** -24 * spread + 2.0 ** -22 + (m + 64) * 2.0 ** -24)
     bound[seen] = loss * (p @ v.abs()) + u * out[seen].abs() * (1 + loss)
     if u == HALF_STEP[torch.float16]:
-        bound[seen] += 2.0 ** -25 + m * 2.0 ** -39 * v.abs().max()
+        bound[seen] += 2.0 ** -25 + m * 2.0 ** -35 * v.abs().max()
     return out, bound
 
 

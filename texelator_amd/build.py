@@ -30,6 +30,11 @@ HIPCC_FLAGS = [
 ]
 
 
+# Products of the matrix cores go to vector registers, not to accumulation registers that every use would copy from:
+# one wave a SIMD has 512 registers, of which vector instructions reach the first 256.
+EXTRA_FLAGS = {"packed_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+
+
 def hipcc() -> str:
     found = shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
     if not Path(found).exists():
@@ -43,7 +48,7 @@ def sources() -> list[Path]:
 
 def _compile(source: Path, build_dir: Path, defines: tuple[str, ...]) -> Path:
     obj = build_dir / (source.stem + ".o")
-    cmd = [hipcc(), *HIPCC_FLAGS, *(f"-D{d}" for d in defines), "-c", str(source), "-o", str(obj)]
+    cmd = [hipcc(), *HIPCC_FLAGS, *EXTRA_FLAGS.get(source.name, []), *(f"-D{d}" for d in defines), "-c", str(source), "-o", str(obj)]
     result = subprocess.run(cmd, capture_output=True, text=True)
     if result.returncode != 0:
         raise RuntimeError(f"hipcc failed for {source.name}:\n{result.stderr}")

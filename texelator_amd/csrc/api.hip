@@ -1412,6 +1412,13 @@ int tx_rope_rotate_half(const void *q, const void *k, int64_t tokens, int heads,
 
 namespace {
 
+// The scale of an attention call as its kernels take it (sl2, q_and, q_xor).
+void set_scale(float scale, float &sl2, uint32_t &q_and, uint32_t &q_xor) {
+  sl2 = std::max(std::fabs(scale) * 1.44269504088896340736f, std::numeric_limits<float>::min());
+  q_and = scale == 0.f ? 0u : ~0u;
+  q_xor = scale < 0.f ? 0x80008000u : 0u;
+}
+
 // CUs of a device, cheaply enough to ask at every call.
 int multiprocessors(int device) {
   int cus = 0;
@@ -1534,9 +1541,7 @@ int tx_kv4_attention(const void *q, int64_t q_sequence, int64_t q_head, int dtyp
   a.out_sequence = out_sequence;
   a.out_head = out_head;
   a.group = heads / kv_heads;
-  a.sl2 = std::max(std::fabs(scale) * 1.44269504088896340736f, std::numeric_limits<float>::min());
-  a.q_and = scale == 0.f ? 0u : ~0u;
-  a.q_xor = scale < 0.f ? 0x80008000u : 0u;
+  set_scale(scale, a.sl2, a.q_and, a.q_xor);
   a.pieces = static_cast<float *>(workspace);
   tx::kv4_attention_plan(a, head_dim, multiprocessors(device));
   if (workspace_bytes < a.piece_bytes || (a.piece_bytes > 0 && !workspace)) return fail(TX_ERR_INVALID, "kv4_attention: workspace too small (tx_kv4_attention_workspace)");
@@ -1618,10 +1623,11 @@ int tx_packed_attention(const void *q, int64_t q_token, int64_t q_head, const vo
   a.total_k = (int)total_k;
   a.heads = heads;
   a.group = heads / kv_heads;
-  a.scale = scale;
+  a.cus = multiprocessors(device);
+  set_scale(scale, a.sl2, a.q_and, a.q_xor);
+  a.lag = std::min(tx::kPackedLag / a.sl2, std::numeric_limits<float>::max() / 4);
   DeviceGuard guard(device);
-  TX_HIP(tx::launch_packed_attention(a, dtype == TX_DTYPE_F16, head_dim, multiprocessors(device),
-                                     reinterpret_cast<hipStream_t>(stream)));
+  TX_HIP(tx::launch_packed_attention(a, dtype == TX_DTYPE_F16, head_dim, reinterpret_cast<hipStream_t>(stream)));
   return TX_OK;
 }
 

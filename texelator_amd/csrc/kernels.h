@@ -261,9 +261,16 @@ struct PackedAttention {
   uint16_t *out;
   int64_t q_token, q_head, k_token, k_head, v_token, v_head, out_token, out_head;
   const int *cu_q, *cu_k;  // [sequences + 1] first rows
-  int sequences, total_q, total_k, heads, group;
-  float scale;
+  int sequences, total_q, total_k, heads, group, cus;
+  // exp2(sl2 * q . k) is exp(scale * q . k): sl2 is above zero, the scale's sign is put into the queries' bits
+  // ((bits & q_and) ^ q_xor), which are cleared for a scale of zero.
+  float sl2;
+  uint32_t q_and, q_xor;
+  float lag;  // kPackedLag / sl2
 };
-hipError_t launch_packed_attention(const PackedAttention &a, bool f16, int dim, int cus, hipStream_t stream);
+// A query's running maximum follows its scores only where they exceed it by this many powers of two: until then its
+// probabilities are held up to 2^kPackedLag instead of 1, and its outputs need no rescaling.
+constexpr float kPackedLag = 4.f;
+hipError_t launch_packed_attention(const PackedAttention &a, bool f16, int dim, hipStream_t stream);
 
 }  // namespace tx

@@ -6,18 +6,27 @@
 //   out[i][h] = sum_j p_ij v_j / sum_j p_ij,  p_ij = exp(scale * q_i . k_j - max_i),  j <= i + keys - queries
 // within a sequence: its last query sees its last key (keys of earlier turns come first); a query that sees none gets zeros.
 //
-// A workgroup takes 32 * QW queries of one head of one sequence with QW * KW waves; it finds its sequence from cu_q
-// by itself, so the grid needs the totals only. Wave (kw, qw) owns 32 queries and every KW-th block of KB keys (KW > 1
+// A workgroup takes 32 * QW queries of one head of one sequence with QW * KW waves; it finds its place from cu_q by
+// itself, so the grid needs the totals only. Wave (kw, qw) owns 32 queries and every KW-th block of KB keys (KW > 1
 // shortens the chain of dependent key blocks where there are few workgroups; the KW shares meet in LDS at the end).
 //   * scores are computed transposed, S^T = K q^T (v_mfma_f32_32x32x16: A = 32 keys, B = the wave's 32 queries, held in
 //     registers): a lane holds 16 scores of ONE query, so the row maximum is in-lane but for one lane swap, the rescale
 //     factor is a scalar of the lane, and the probabilities, rounded to 16 bits in place, are the B operand of
 //     O^T = V^T P^T: none of them passes through LDS;
+//   * the next 32 keys' scores are computed while these 32 keys' exponentials are, woven by hand: a wave that ran its
+//     products and its exponentials one after the other kept the matrix cores 44% busy, woven 53%;
+//   * a query's running maximum follows its scores only where they pass it by 2^4: rescaling the outputs had been a third of
+//     the vector instructions, since some of a wave's queries almost always finds a new maximum;
 //   * keys and values reach LDS by direct buffer loads one block ahead, as they lie in memory; the descriptors end at
 //     the sequence's last row, rows past it read as zeros. 16-byte chunks of a row are permuted by its number so
 //     that operand reads hit distinct banks; the values' transpose is done by the read (ds_read_b64_tr_b16).
-// Online softmax in fp32 with exp2; the sum runs over the probabilities as rounded. In fp16 they are held times 2^15, so
-// that small ones keep their bits.
+// Online softmax in fp32 with exp2; the sum runs over the probabilities as rounded. In fp16 they are held times 2^11, so
+// that small ones keep their bits and large ones (2^4 more while a maximum lags) stay below fp16's largest.
+//
+// Bound: power. At 8190 tokens and 40/8 heads 1.23 M cycles a SIMD at 1.9 GHz, 655 us (1050 TFLOP/s; a plain 16384^3 product
+// of the library reaches 1370); the same instructions on zeros run at 2.4 GHz. Two waves a SIMD: vector instructions take 2.6
+// cycles each there against 5 of a wave alone. 64 queries a wave (half the LDS reads per product, one wave a SIMD) took
+// 1.73 M cycles, 718 us.
 #include <math.h>
 
 #include <type_traits>
@@ -78,6 +87,15 @@ __device__ __forceinline__ float halves_sum(float v) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+// This wave's loads (to LDS too) and LDS accesses are done, then every wave's. Builtins: the compiler has to know
+// that nothing is under way any more, or it waits again before the reads that follow.
+__device__ __forceinline__ void drain_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
 // First row and rows of a sequence, kept within the array whatever cu holds.
 struct Rows {
   int begin, count;
@@ -89,87 +107,88 @@ __device__ __forceinline__ Rows rows_of(const int *cu, int sequence, int total) 
 
 // Two waves per SIMD, but for <1, 4, 32>, whose four waves have a CU's LDS to themselves.
 template <bool F16, int DIM, int QW, int KW, int KB>
-__global__ __launch_bounds__(64 * QW * KW, QW * KW * KB == 128 ? 1 : 2) __attribute__((amdgpu_num_vgpr(256))) void packed_attention_kernel(
-    PackedAttention a) {
+__global__ __launch_bounds__(64 * QW * KW, QW * KW * KB == 128 ? 1 : 2) void packed_attention_kernel(PackedAttention a) {
   constexpr int kRow = DIM * 2;                 // bytes of a key or value
-  constexpr int kTile = KB * kRow;              // bytes of a key (or value) block
-  constexpr int kLoads = kTile / 1024;          // 1 KiB direct loads per block and array
-  constexpr int kPer = kLoads / QW;             // of them this wave issues
-  constexpr int kChunks = DIM / 8;              // 16-byte chunks of a row = lanes that bring it
-  constexpr int kLoadRows = 64 / kChunks;       // rows of a load
+  constexpr int kTile = KB * kRow;              // bytes of a key group's keys (or values) of a turn
+  constexpr int kSub = 32 * kRow;               // of 32 of them
   constexpr int kSubs = KB / 32;
+  constexpr int kChunks = DIM / 8;              // 16-byte chunks of a row = lanes that bring it
+  constexpr int kLoadRows = 64 / kChunks;       // rows of a 1 KiB load
+  constexpr int kPer = kSub / 1024 / QW;        // loads of this wave for 32 rows
   constexpr int kSteps = DIM / 16, kOut = DIM / 32;
-  constexpr float kLift = F16 ? 15.f : 0.f;
-  static_assert(kPer * QW == kLoads, "loads divide among the waves");
-  // Two buffers, separate LDS objects (the compiler then knows that reads of one do not wait for the
-  // direct loads that fill the other): per key group its key block, then its value block.
-  __shared__ __attribute__((aligned(1024))) char buf0[KW * 2 * kTile];
-  __shared__ __attribute__((aligned(1024))) char buf1[KW * 2 * kTile];
+  constexpr float kLift = F16 ? 15.f - kPackedLag : 0.f;
+  static_assert(kPer * QW * 1024 == kSub, "loads divide among the waves");
+  // Two buffers of each, separate LDS objects: the compiler then knows that reads of one do not wait for the direct
+  // loads that fill the other.
+  __shared__ __attribute__((aligned(1024))) char k_even[KW * kTile];
+  __shared__ __attribute__((aligned(1024))) char k_odd[KW * kTile];
+  __shared__ __attribute__((aligned(1024))) char v_even[KW * kTile];
+  __shared__ __attribute__((aligned(1024))) char v_odd[KW * kTile];
   __shared__ float stats[KW][QW][2][KW > 1 ? 64 : 1];  // (m, l) of every wave, for the merge
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int qw = wave % QW, kw = wave / QW;
   const int n = lane & 31, h = lane >> 5;
-  // Heads fastest; where the head count allows, an XCD (workgroups arrive round-robin) gets neighbouring heads, which
-  // share keys.
-  const int hx = blockIdx.x % a.heads;
+  // The heaviest tiles of all sequences first. Where two workgroups a CU are all there are, the second of a CU come in
+  // reverse order, so that the heaviest meets the lightest (by eights: the order of the XCDs, which workgroups reach
+  // round-robin, stays): 4096 tokens of 16/2 heads 95.1 -> 89.8 us; with more than that 2048 tokens of 40/8 58.4 -> 61.5.
+  // Heads fastest; where the head count allows, an XCD gets neighbouring heads, which share keys.
+  constexpr int kQueries = 32 * QW;
+  int hx = 0;
+  auto tiles_of = [&](int s) { return (rows_of(a.cu_q, s, a.total_q).count + kQueries - 1) / kQueries; };
+  auto before_of = [&](int s) { return (rows_of(a.cu_k, s, a.total_k).count - rows_of(a.cu_q, s, a.total_q).count) / kQueries; };
+  const RaggedPlace place = ragged_heaviest(a.sequences, tiles_of, before_of, [&](int total) {
+    int index = blockIdx.x;
+    const int64_t all = (int64_t)total * a.heads;
+    const int first = a.cus & ~7, end = (int)min((int64_t)2 * first, all) & ~7;
+    if (index >= first && index < end && all <= 2 * first) index = first + (end - 8 - (index & ~7)) + (index & 7);
+    hx = index % a.heads;
+    return index / a.heads;
+  });
+  if (blockIdx.x >= (int64_t)place.total * a.heads) return;
   const int head = a.heads % kXcds == 0 ? (hx % kXcds) * (a.heads / kXcds) + hx / kXcds : hx;
-  auto tiles_of = [&](int s) { return (rows_of(a.cu_q, s, a.total_q).count + 32 * QW - 1) / (32 * QW); };
-  const int wanted = blockIdx.x / a.heads;
-  const RaggedPlace place = ragged_place(a.sequences, tiles_of, [&](int) { return wanted; });
-  if (wanted >= place.total) return;
+  const int tile = place.local;
   const int sequence = place.sequence;
   const Rows qs = rows_of(a.cu_q, sequence, a.total_q), ks = rows_of(a.cu_k, sequence, a.total_k);
   const int queries = __builtin_amdgcn_readfirstlane(qs.count), keys = __builtin_amdgcn_readfirstlane(ks.count);
-  // The heaviest tiles of a sequence (the last) first.
-  const int tile = (queries + 32 * QW - 1) / (32 * QW) - 1 - place.local;
-  const int shift = keys - queries;            // query i sees the keys up to i + shift
-  const int q0 = (tile * QW + qw) * 32;        // this wave's first query
+  const int shift = keys - queries;      // query i sees the keys up to i + shift
+  const int q0 = tile * kQueries + qw * 32;  // this wave's first query
 
   // q as MFMA B operands: column n = query q0 + n (clamped into the sequence), dimensions 16 st + 8 h ...
-  const float sl2 = a.scale * 1.44269504088896340736f;  // scores in log2 units
   u32x4 qb[kSteps];
   {
     const uint16_t *qr = a.q + (qs.begin + min(q0 + n, queries - 1)) * a.q_token + head * a.q_head;
 #pragma unroll
-    for (int st = 0; st < kSteps; ++st) qb[st] = *reinterpret_cast<const u32x4 *>(qr + 16 * st + 8 * h);
+    for (int st = 0; st < kSteps; ++st) {
+      qb[st] = *reinterpret_cast<const u32x4 *>(qr + 16 * st + 8 * h);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) qb[st][j] = (qb[st][j] & a.q_and) ^ a.q_xor;
+    }
   }
 
   const int kv = head / a.group;
   const char *kg = reinterpret_cast<const char *>(a.k + ks.begin * a.k_token + kv * a.k_head);
   const char *vg = reinterpret_cast<const char *>(a.v + ks.begin * a.v_token + kv * a.v_head);
   const uint32_t k_bytes = (uint32_t)a.k_token * 2, v_bytes = (uint32_t)a.v_token * 2;  // between rows
-  // Load i of a block brings rows kLoadRows * i .., lane l landing in chunk l % kChunks of the load's row l / kChunks,
-  // which holds the row's chunk (l % kChunks) ^ turn(row): the row's number mod 16 for keys (mod 16 of its
-  // pair for rows of 128 bytes, two of which make a pass over the banks), 4 times it mod 4 (mod 2 of its pair) for values.
+  // 32 rows from `first` on into LDS. Load i brings rows kLoadRows * i .., lane l landing in chunk l % kChunks of the
+  // load's row l / kChunks, which holds the row's chunk (l % kChunks) ^ turn(row): the row's number mod 16 for keys (mod 16
+  // of its pair for rows of 128 bytes, two of which make a pass over the banks), 4 times it mod 4 (mod 2 of its pair) for values.
   const uint32_t load_row = lane / kChunks;
   const uint32_t k_chunk = 16u * (uint32_t)((lane % kChunks) ^ (lane >> 4));  // but for the load's number
   const uint32_t v_chunk = 16u * (uint32_t)((lane % kChunks) ^ (DIM == 128 ? 4 * (lane >> 4) : 4 * ((lane >> 4) & 1)));
-  auto stage = [&](char *buf, int kb) __attribute__((always_inline)) {
-    const int first = kb * KB, rows = min(KB, keys - first);
-    char *kd = buf + kw * 2 * kTile, *vd = kd + kTile;
-    const __amdgpu_buffer_rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc(
-        const_cast<char *>(kg) + (int64_t)first * k_bytes, (short)0, rows > 0 ? (rows - 1) * k_bytes + kRow : 0, 0x00020000);
-    const __amdgpu_buffer_rsrc_t vr = __builtin_amdgcn_make_buffer_rsrc(
-        const_cast<char *>(vg) + (int64_t)first * v_bytes, (short)0, rows > 0 ? (rows - 1) * v_bytes + kRow : 0, 0x00020000);
+  auto stage = [&](const char *from, uint32_t bytes, uint32_t chunk, bool turned, char *to, int first) __attribute__((always_inline)) {
+    const int rows = min(32, keys - first);
+    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<char *>(from) + (int64_t)first * bytes, (short)0, rows > 0 ? (rows - 1) * bytes + kRow : 0, 0x00020000);
 #pragma unroll
     for (int u = 0; u < kPer; ++u) {
       const int i = qw + QW * u;
-      const uint32_t row = i * kLoadRows + load_row, turn = 64u * (uint32_t)(DIM == 128 ? i & 3 : i & 1);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(kr, (__attribute__((address_space(3))) void *)(kd + i * 1024), 16,
-                                               row * k_bytes + (k_chunk ^ turn), 0, 0, 0);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(vr, (__attribute__((address_space(3))) void *)(vd + i * 1024), 16,
-                                               row * v_bytes + v_chunk, 0, 0, 0);
+      const uint32_t turn = turned ? 64u * (uint32_t)(DIM == 128 ? i & 3 : i & 1) : 0u;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *)(to + i * 1024), 16,
+                                               (i * kLoadRows + load_row) * bytes + (chunk ^ turn), 0, 0, 0);
     }
   };
-
-  float m = -INFINITY, l = 0.f;  // running maximum (log2 units) and this lane's share of the sum, query q0 + n
-  f32x16 o[kOut];                // o[t][r] = O[query q0 + n][dimension 32 t + 8 (r / 4) + 4 h + r % 4]
-#pragma unroll
-  for (int t = 0; t < kOut; ++t)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) o[t][r] = 0.f;
 
   // Byte offsets of this lane's operands in a tile: of key row n, dimensions 16 st + 8 h (chunk 2 st + h) at
   // k_at ^ 32 st; and, for the transposing reads, of key 4 h + (lane % 16) / 4, dimensions
@@ -179,128 +198,167 @@ __global__ __launch_bounds__(64 * QW * KW, QW * KW * KB == 128 ? 1 : 2) __attrib
   const uint32_t v_at = (4u * h + x4) * kRow + 32u * ((lane >> 4) & 1) + 8u * (lane & 3) + 64u * (DIM == 128 ? x4 : x4 >> 1);
   const int limit = min(q0 + n, queries - 1) + shift;  // the last key this lane's query sees
 
-  // NS sub-blocks of 32 keys at once (their score chains are independent); MASK: some keys are past some query's limit.
-  auto block = [&](const char *buf, int k0, auto ns_c, auto mask_c) __attribute__((always_inline)) {
-    constexpr int NS = decltype(ns_c)::value;
-    constexpr bool MASK = decltype(mask_c)::value;
-    const char *kt = buf + kw * 2 * kTile, *vt = kt + kTile;
-    f32x16 sc[NS];
+  float m = -INFINITY, l = 0.f;  // running maximum (before the scale) and this lane's share of the sum, query q0 + n
+  float mx = -INFINITY;          // the largest of the scores at hand
+  f32x16 o[kOut];                // o[t][r] = O[query q0 + n][dimension 32 t + 8 (r / 4) + 4 h + r % 4]
 #pragma unroll
-    for (int s = 0; s < NS; ++s)
+  for (int t = 0; t < kOut; ++t) o[t] = f32x16{};
+
+  auto largest = [&](const f32x16 &sc) __attribute__((always_inline)) {
+    mx = fmaxf(sc[0], sc[1]);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) sc[s][r] = 0.f;
+    for (int r = 2; r < 16; r += 2) mx = fmaxf(fmaxf(mx, sc[r]), sc[r + 1]);
+  };
+  // Before the scores of keys k0 .. k0 + 31 are used (sc[r]: key k0 + 8 (r / 4) + 4 h + r % 4, query q0 + n): hides those
+  // past each query's limit and moves the running maximum. Whether it moves depends on the query's own scores alone,
+  // and one that stays is scaled by exactly 1: a query's output does not depend on which others share the wave.
+  auto settle = [&](f32x16 &sc, int k0) __attribute__((always_inline)) {
+    if (k0 + 31 > q0 + shift) {
+      asm volatile("" ::: "memory");  // stays a branch: few blocks are hidden in part
 #pragma unroll
-    for (int st = 0; st < kSteps; ++st)
-#pragma unroll
-      for (int s = 0; s < NS; ++s) {
-        const u32x4 b = *reinterpret_cast<const u32x4 *>(kt + 32 * s * kRow + (k_at ^ (32u * st)));
-        sc[s] = mfma32<F16>(b, qb[st], sc[s]);
-      }
-    // sc[s][r] = score of key 32 s + 8 (r / 4) + 4 h + r % 4 of the block and query q0 + n
-#pragma unroll
-    for (int s = 0; s < NS; ++s)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        sc[s][r] *= sl2;
-        if (MASK) sc[s][r] = k0 + 32 * s + 8 * (r >> 2) + 4 * h + (r & 3) > limit ? -INFINITY : sc[s][r];
-      }
-    float mx = fmaxf(sc[0][0], sc[0][1]);
-#pragma unroll
-    for (int s = 0; s < NS; ++s)
-#pragma unroll
-      for (int r = s == 0 ? 2 : 0; r < 16; r += 2) mx = fmaxf(fmaxf(mx, sc[s][r]), sc[s][r + 1]);
-    // The running maximum is each query's own: its output does not depend on which others share the wave. It is
-    // finite from the first block on in which the query sees a key (in unmasked blocks all do).
-    const float mnew = fmaxf(m, halves_max(mx));
-    if (__builtin_amdgcn_ballot_w64(mnew > m) != 0) {
-      const float alpha = !MASK || mnew > m ? __builtin_amdgcn_exp2f(m - mnew) : 1.f;
+      for (int r = 0; r < 16; ++r) sc[r] = k0 + 8 * (r >> 2) + 4 * h + (r & 3) > limit ? -INFINITY : sc[r];
+      largest(sc);
+    }
+    const float mnew = halves_max(mx);
+    const bool grow = mnew > m + a.lag;
+    if (__builtin_amdgcn_ballot_w64(grow) != 0) {
+      const float alpha = grow ? __builtin_amdgcn_exp2f((m - mnew) * a.sl2) : 1.f;
       l *= alpha;
 #pragma unroll
       for (int t = 0; t < kOut; ++t)
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[t][r] *= alpha;
-      m = mnew;
+      m = grow ? mnew : m;
     }
-    const float base = MASK && m == -INFINITY ? 0.f : m - kLift;
-    uint32_t pb[NS][8];
-#pragma unroll
-    for (int s = 0; s < NS; ++s)
-#pragma unroll
-      for (int r = 0; r < 16; r += 2)
-        pb[s][r / 2] = pack2<F16>(__builtin_amdgcn_exp2f(sc[s][r] - base), __builtin_amdgcn_exp2f(sc[s][r + 1] - base), l);
-    // O^T += V^T P^T, sixteen keys at a time: slots 0-3 of half h are keys 4 h .. + 3, slots 4-7 the keys 8 on
-#pragma unroll
-    for (int s = 0; s < NS; ++s)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const u32x4 b = {pb[s][4 * j], pb[s][4 * j + 1], pb[s][4 * j + 2], pb[s][4 * j + 3]};
-#pragma unroll
-        for (int t = 0; t < kOut; ++t) {
-          const char *at = vt + (32 * s + 16 * j) * kRow + (v_at ^ (64u * t));
-          const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)at);
-          const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(at + 8 * kRow));
-          const u32x2 lw = __builtin_bit_cast(u32x2, lo), hw = __builtin_bit_cast(u32x2, hi);
-          o[t] = mfma32<F16>(u32x4{lw[0], lw[1], hw[0], hw[1]}, b, o[t]);
-        }
-      }
   };
-  // A key block against this wave's queries: nothing to do for a wave without queries or whose last query ends before it.
-  const int reach = q0 < queries ? min(q0 + 31, queries - 1) + shift : -1;
-  using One = std::integral_constant<int, 1>;
-  using Two = std::integral_constant<int, 2>;
-  auto visit = [&](const char *buf, int kb) __attribute__((always_inline)) {
-    const int k0 = kb * KB;
-    if (k0 > reach) return;
-    if constexpr (kSubs == 2) {
-      if (k0 + 63 <= q0 + shift) block(buf, k0, Two{}, std::false_type{});
-      else if (k0 + 32 <= reach) block(buf, k0, Two{}, std::true_type{});
-      else block(buf, k0, One{}, std::true_type{});
-    } else {
-      if (k0 + 31 <= q0 + shift) block(buf, k0, One{}, std::false_type{});
-      else block(buf, k0, One{}, std::true_type{});
+  // The next 32 keys' scores, and these 32 keys' share of the outputs: O^T += V^T P^T, sixteen keys at a time (slots 0-3 of half h
+  // are keys 4 h .. + 3, slots 4-7 the keys 8 on). The order here is the order of issue (the scheduling barriers hold the
+  // compiler to it): the exponentials in the time of the products, operands read two products ahead, the next scores'
+  // maximum last.
+  auto step = [&](const f32x16 &cur, f32x16 &next, const char *vt, const char *kt_next) __attribute__((always_inline)) {
+    const float base = m == -INFINITY ? 0.f : kLift - m * a.sl2;  // no key yet: every score is -infinity
+    uint32_t pb[8];
+    auto pair = [&](int p) __attribute__((always_inline)) {  // probabilities 2 p and 2 p + 1
+      pb[p] = pack2<F16>(__builtin_amdgcn_exp2f(__builtin_fmaf(cur[2 * p], a.sl2, base)),
+                         __builtin_amdgcn_exp2f(__builtin_fmaf(cur[2 * p + 1], a.sl2, base)), l);
+      asm volatile("" : "+v"(pb[p]));
+    };
+    auto key = [&](int st) __attribute__((always_inline)) { return *reinterpret_cast<const u32x4 *>(kt_next + (k_at ^ (32u * st))); };
+    auto value = [&](int i) __attribute__((always_inline)) {
+      const char *at = vt + 16 * (i / kOut) * kRow + (v_at ^ (64u * (i % kOut)));
+      const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)at));
+      const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(at + 8 * kRow)));
+      return u32x4{lo[0], lo[1], hi[0], hi[1]};
+    };
+    constexpr int kGroups = kSteps + kOut;  // products before the second sixteen keys' probabilities are needed
+    int done = 0;
+    u32x4 x = key(0), y = key(1);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int st = 0; st < kSteps; ++st) {
+      const u32x4 z = st + 2 < kSteps ? key(st + 2) : value(st + 2 - kSteps);
+      next = mfma32<F16>(x, qb[st], st == 0 ? f32x16{} : next);
+#pragma unroll
+      for (; done < max(8 * (st + 1) / kGroups, 4 * (st + 1) / kSteps); ++done) pair(done);
+      x = y;
+      y = z;
+      __builtin_amdgcn_sched_barrier(0);
     }
+#pragma unroll
+    for (int i = 0; i < 2 * kOut; ++i) {
+      const u32x4 z = i + 2 < 2 * kOut ? value(i + 2) : x;
+      const int j = i / kOut, t = i % kOut;
+      o[t] = mfma32<F16>(x, u32x4{pb[4 * j], pb[4 * j + 1], pb[4 * j + 2], pb[4 * j + 3]}, o[t]);
+#pragma unroll
+      for (; i < kOut && done < 8 * (kSteps + i + 1) / kGroups; ++done) pair(done);
+      x = y;
+      y = z;
+      if (i == kOut) largest(next);
+      if (i < kOut) __builtin_amdgcn_sched_barrier(0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
   };
 
-  // Blocks of this key group: kw, kw + KW, ... up to the workgroup's last key; every wave runs every
-  // turn (the barriers are workgroup-wide). A turn's loads were issued a turn before; the barrier
-  // that ends their wait also says that the other buffer is no longer read.
-  const int last_key = min((tile + 1) * QW * 32, queries) - 1 + shift;
-  const int last = last_key < 0 ? -1 : last_key / KB;
-  const int turns = last < 0 ? 0 : last / KW + 1;
-  auto turn = [&](int it, char *cur, char *next) __attribute__((always_inline)) {
-    asm volatile("s_waitcnt vmcnt(0)\n\ts_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    const int kb = it * KW + kw;
-    if (kb + KW <= last) stage(next, kb + KW);
-    if (kb <= last) visit(cur, kb);
+  // Blocks of this key group: kw, kw + KW, ... up to the workgroup's last key; every wave runs every turn (the barriers
+  // are workgroup-wide). In turn `it` the values of block b = it * KW + kw are in LDS, and the keys 32 further on: b's but for
+  // its first 32, then the first 32 of the group's next block. Those of the next turn set out behind the barrier, which also says
+  // that their buffers are no longer read. Scores past the wave's last key are computed from whatever lies there and dropped.
+  const int last_key = min((tile + 1) * kQueries, queries) - 1 + shift;
+  const int blocks = last_key < 0 ? 0 : last_key / KB + 1, turns = (blocks + KW - 1) / KW;
+  const int reach = q0 < queries ? min(q0 + 31, queries - 1) + shift : -1;  // this wave's last key
+  f32x16 s0, s1;
+  auto stage_keys = [&](char *to, int b) __attribute__((always_inline)) {  // those of the turn of block b
+    to += kw * kTile;
+    if (kSubs == 2 && b * KB + 32 <= last_key) stage(kg, k_bytes, k_chunk, true, to, b * KB + 32);
+    if ((b + KW) * KB <= last_key) stage(kg, k_bytes, k_chunk, true, to + (kSubs - 1) * kSub, (b + KW) * KB);
   };
-  if (kw <= last) stage(buf0, kw);
+  auto stage_values = [&](char *to, int b) __attribute__((always_inline)) {
+#pragma unroll
+    for (int s = 0; s < kSubs; ++s)
+      if (b * KB + 32 * s <= last_key) stage(vg, v_bytes, v_chunk, false, to + kw * kTile + s * kSub, b * KB + 32 * s);
+  };
+  auto turn = [&](int it, const char *k_cur, char *k_next, const char *v_cur, char *v_next) __attribute__((always_inline)) {
+    drain_barrier();
+    const int b = it * KW + kw, k0 = b * KB;
+    stage_values(v_next, b + KW);
+    stage_keys(k_next, b + KW);
+    k_cur += kw * kTile;
+    v_cur += kw * kTile;
+    if (k0 > reach) return;
+    if constexpr (kSubs == 2) {
+      step(s0, s1, v_cur, k_cur);
+      if (k0 + 32 > reach) return;
+      settle(s1, k0 + 32);
+      step(s1, s0, v_cur + kSub, k_cur + kSub);
+    } else {
+      step(s0, s1, v_cur, k_cur);
+      s0 = s1;
+    }
+    if (k0 + KW * KB <= reach) settle(s0, k0 + KW * KB);
+  };
+  if (turns > 0) {
+    if (kw * KB <= last_key) stage(kg, k_bytes, k_chunk, true, k_odd + kw * kTile, kw * KB);
+    stage_keys(k_even, kw);
+    stage_values(v_even, kw);
+    drain_barrier();
+    if (kw * KB <= reach) {
+#pragma unroll
+      for (int st = 0; st < kSteps; ++st)
+        s0 = mfma32<F16>(*reinterpret_cast<const u32x4 *>(k_odd + kw * kTile + (k_at ^ (32u * st))), qb[st], st == 0 ? f32x16{} : s0);
+      largest(s0);
+      settle(s0, kw * KB);
+    }
+  }
   int it = 0;
   for (; it + 2 <= turns; it += 2) {
-    turn(it, buf0, buf1);
-    turn(it + 1, buf1, buf0);
+    turn(it, k_even, k_odd, v_even, v_odd);
+    turn(it + 1, k_odd, k_even, v_odd, v_even);
   }
-  if (it < turns) turn(it, buf0, buf1);
+  if (it < turns) turn(it, k_even, k_odd, v_even, v_odd);
 
   l = halves_sum(l);
   if constexpr (KW > 1) {
-    // The groups' (m, l) meet in LDS; with M = max m, every group scales its O by exp2(m - M), and group
+    // The groups' (m, l) meet in LDS; with M = max m, every group scales its O by exp(m - M), and group
     // t % KW sums the output tile t of all. A group whose blocks a query does not see has m = -inf, l = 0, O = 0
     // for it and weighs nothing (or NaN, where its scores were).
-    constexpr int kHalf = kOut / 2;  // output tiles that go through a buffer
-    static_assert(KW * QW * kHalf * 4096 <= KW * 2 * kTile, "half the output tiles of every wave fit a buffer");
+    constexpr int kHalf = kOut / 2;  // output tiles that go through the keys' buffers; the others through the values'
+    static_assert(kHalf * QW * KW * 4096 <= 2 * KW * kTile, "half the output tiles of every wave fit two buffers");
     stats[kw][qw][0][lane] = m;
     stats[kw][qw][1][lane] = l;
     __syncthreads();  // every tile read is done, too
     float mm = m, total = 0.f;
 #pragma unroll
     for (int g = 0; g < KW; ++g) mm = fmaxf(mm, stats[g][qw][0][lane]);
-    auto weight = [&](float mine) { return mine == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mine - mm); };
+    auto weight = [&](float mine) { return mine == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((mine - mm) * a.sl2); };
 #pragma unroll
     for (int g = 0; g < KW; ++g) total += stats[g][qw][1][lane] * weight(stats[g][qw][0][lane]);
     l = total;
     const float alpha = weight(m);
+    // Tile t of wave (g, qw): 4 KiB; those of a half in the even buffer first, then in the odd one.
     auto at = [&](int g, int t) {
-      return reinterpret_cast<float *>(t < kHalf ? buf0 : buf1) + ((g * QW + qw) * kHalf + t % kHalf) * 1024 + lane;
+      const int index = (g * QW + qw) * kHalf + t % kHalf, half = KW * kTile / 4096;
+      char *even = t < kHalf ? k_even : v_even, *odd = t < kHalf ? k_odd : v_odd;
+      return reinterpret_cast<float *>(index < half ? even + index * 4096 : odd + (index - half) * 4096) + lane;
     };
 #pragma unroll
     for (int t = 0; t < kOut; ++t) {
@@ -339,26 +397,31 @@ __global__ __launch_bounds__(64 * QW * KW, QW * KW * KB == 128 ? 1 : 2) __attrib
 }
 
 template <bool F16, int DIM>
-hipError_t launch_typed(const PackedAttention &a, int cus, hipStream_t stream) {
+hipError_t launch_typed(const PackedAttention &a, hipStream_t stream) {
   auto launch = [&](auto kernel, int queries, int waves) {
     const int64_t tiles = a.total_q / queries + a.sequences;  // at least what the sequences' partial tiles make it
     hipLaunchKernelGGL(kernel, dim3((unsigned)(tiles * a.heads)), dim3(64 * waves), 0, stream, a);
   };
-  const int64_t tokens = a.total_q;
-  const int64_t tiles128 = (tokens + 127) / 128 * a.heads, tiles64 = (tokens + 63) / 64 * a.heads,
-                tiles32 = (tokens + 31) / 32 * a.heads;
-  if (4 * tiles128 >= 9 * (int64_t)cus) launch(packed_attention_kernel<F16, DIM, 4, 1, 64>, 128, 4);
-  else if (5 * tiles64 >= 8 * (int64_t)cus) launch(packed_attention_kernel<F16, DIM, 4, 2, 64>, 128, 8);
-  else if (tiles32 <= cus) launch(packed_attention_kernel<F16, DIM, 1, 4, 32>, 32, 4);
-  else launch(packed_attention_kernel<F16, DIM, 2, 4, 32>, 64, 8);
+  // Which split of the waves, by how many tiles of 32 and 64 queries the rows can make and how many keys a sequence has on
+  // average (us, graph replays, at 40/8 heads where no others are named):
+  //   <1, 4, 32> where its workgroups fit the CUs at once and there is a chain of key blocks to shorten: 128 tokens 7.6
+  //              against 8.1 of <4, 1, 64>, 256 tokens of 16/2 heads 8.5 against 10.1; but 12 prompts of up to 60 tokens at
+  //              32/8 heads 12.7 against 6.6, whose chains are short;
+  //   <2, 4, 32> likewise: 1024 tokens of 16/2 heads 17.5 against 23.9; but 512 tokens (320 workgroups) 18.8 against 15.5;
+  //   <4, 1, 64> for all else: 1024 tokens 28.1 against 34.2 of <2, 4, 32>, 8190 tokens 658 against 880.
+  const int64_t tiles32 = (a.total_q + (int64_t)31 * a.sequences) / 32 * a.heads,
+                tiles64 = (a.total_q + (int64_t)63 * a.sequences) / 64 * a.heads;
+  if (tiles32 <= a.cus && a.total_k >= (int64_t)96 * a.sequences) launch(packed_attention_kernel<F16, DIM, 1, 4, 32>, 32, 4);
+  else if (tiles64 <= a.cus && a.total_k >= (int64_t)96 * a.sequences) launch(packed_attention_kernel<F16, DIM, 2, 4, 32>, 64, 8);
+  else launch(packed_attention_kernel<F16, DIM, 4, 1, 64>, 128, 4);
   return hipGetLastError();
 }
 
 }  // namespace
 
-hipError_t launch_packed_attention(const PackedAttention &a, bool f16, int dim, int cus, hipStream_t stream) {
-  if (f16) return dim == 128 ? launch_typed<true, 128>(a, cus, stream) : launch_typed<true, 64>(a, cus, stream);
-  return dim == 128 ? launch_typed<false, 128>(a, cus, stream) : launch_typed<false, 64>(a, cus, stream);
+hipError_t launch_packed_attention(const PackedAttention &a, bool f16, int dim, hipStream_t stream) {
+  if (f16) return dim == 128 ? launch_typed<true, 128>(a, stream) : launch_typed<true, 64>(a, stream);
+  return dim == 128 ? launch_typed<false, 128>(a, stream) : launch_typed<false, 64>(a, stream);
 }
 
 }  // namespace tx

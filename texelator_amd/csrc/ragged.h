@@ -52,6 +52,47 @@ __device__ __forceinline__ RaggedPlace ragged_place(int sequences, Count count, 
   return place;
 }
 
+// Largest value of the lanes of a wave.
+__device__ __forceinline__ int wave_max_int(int v) {
+  v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x111, 0xF, 0xF, false));
+  v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x112, 0xF, 0xF, false));
+  v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x114, 0xF, 0xF, false));
+  v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x118, 0xF, 0xF, false));
+  v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x142, 0xA, 0xF, false));
+  v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x143, 0xC, 0xF, false));
+  return __builtin_amdgcn_readlane(v, 63);
+}
+
+// The item at rank target(total), heaviest first, where item i of sequence s weighs i + offset(s); up to 64 sequences
+// (beyond, the sequences keep their order and each its heaviest items first).
+template <typename Count, typename Offset, typename Target>
+__device__ __forceinline__ RaggedPlace ragged_heaviest(int sequences, Count count, Offset offset, Target target) {
+  if (sequences > 64) {
+    RaggedPlace place = ragged_place(sequences, count, target);
+    place.local = __builtin_amdgcn_readfirstlane(count(place.sequence)) - 1 - place.local;
+    return place;
+  }
+  const int lane = threadIdx.x & 63;
+  const int n = lane < sequences ? count(lane) : 0, o = lane < sequences ? offset(lane) : 0;
+  const int total = __builtin_amdgcn_readlane(wave_scan(n), 63);
+  const int rank = target(total);
+  if (sequences == 1) return {total, 0, total - 1 - rank};
+  // Weights of at least `low` belong to more than `rank` items, of at least `high` to `heavier` <= rank of them.
+  int low = -wave_max_int(n > 0 ? -o : -(1 << 30)), high = wave_max_int(n > 0 ? n + o : -(1 << 30)), heavier = 0;
+  if (rank >= total) return {total, 0, 0};
+  while (high - low > 1) {
+    const int mid = low + ((high - low) >> 1);
+    const int items = __builtin_amdgcn_readlane(wave_scan(min(max(n + o - mid, 0), n)), 63);
+    if (items > rank) low = mid;
+    else high = mid, heavier = items;
+  }
+  const bool has = low >= o && low < n + o;
+  const int among = wave_scan(has ? 1 : 0);  // with every lane: a lane left out would break the sums
+  const uint64_t here = __builtin_amdgcn_ballot_w64(has && among == rank - heavier + 1);
+  const int sequence = here ? __builtin_ctzll(here) : 0;
+  return {total, sequence, low - __builtin_amdgcn_readlane(o, sequence)};
+}
+
 // The items in all, and in `local` those before sequence `s`.
 template <typename Count>
 __device__ __forceinline__ RaggedPlace ragged_before(int sequences, Count count, int s) {
