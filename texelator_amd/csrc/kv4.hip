@@ -105,27 +105,48 @@ __global__ __launch_bounds__(kThreads) void kv4_append_kernel(const uint16_t *k,
   half[((int64_t)(DIM / 2) << pool.page_shift) + row.offset * kGroups + group] = (uint8_t)e;
 }
 
-// The same grid the other way: k_out and v_out [tokens][kv_heads][DIM], row strides as given.
+// The same the other way: k_out and v_out [tokens][kv_heads][DIM], row strides as given. A workgroup finds the places of
+// its kReadRows rows first, one a thread; then a thread turns four bytes of codes into 16 bytes of output, so that a wave stores
+// 1 KiB of consecutive bytes: 20291 tokens of 8 heads of 128 17.7 us (5.9 TB/s), with a group a thread, 64 bytes each, 29.8.
+template <int DIM>
+constexpr int kReadRows = 8192 / DIM;
 template <bool F16, int DIM>
 __global__ __launch_bounds__(kThreads) void kv4_read_kernel(uint16_t *k, int64_t k_token, int64_t k_head, uint16_t *v,
                                                             int64_t v_token, int64_t v_head, int tokens, const int *cu,
                                                             Kv4Pool pool) {
-  constexpr int kGroups = DIM / 32;
+  constexpr int kGroups = DIM / 32, kOctets = DIM / 8, kPasses = kReadRows<DIM> * kOctets / kThreads;
   __shared__ int lds[kCuEntries];
+  __shared__ int pages[kReadRows<DIM>], offsets[kReadRows<DIM>];
   const int *starts = stage_starts(cu, pool.sequences, lds);
-  const int group = threadIdx.x % kGroups;
-  const int64_t index = (int64_t)blockIdx.x * (kThreads / kGroups) + threadIdx.x / kGroups;
-  if (index >= tokens) return;
-  const int token = (int)index, head = blockIdx.y >> 1;
+  const int64_t first = (int64_t)blockIdx.x * kReadRows<DIM>;
+  if (threadIdx.x < kReadRows<DIM>) {
+    Row row = {-1, 0};
+    if (first + threadIdx.x < tokens) row = locate(pool, cu, starts, (int)first + threadIdx.x);
+    pages[threadIdx.x] = (int)row.page;
+    offsets[threadIdx.x] = row.offset;
+  }
+  __syncthreads();
+  const int head = blockIdx.y >> 1;
   const bool values = blockIdx.y & 1;
-  const Row row = locate(pool, cu, starts, token);
-  if (row.page < 0) return;
-  const uint8_t *half = pool.pages + ((row.page * pool.kv_heads + head) * 2 + values) * kv4_half_bytes(pool.page_shift, DIM);
-  const u32x4 codes = *reinterpret_cast<const u32x4 *>(half + row.offset * (DIM / 2) + 16 * group);
-  const float scale = __uint_as_float((uint32_t)half[((int64_t)(DIM / 2) << pool.page_shift) + row.offset * kGroups + group] << 23);
-  uint16_t *dst = (values ? v + token * v_token + head * v_head : k + token * k_token + head * k_head) + 32 * group;
+  const int64_t half_bytes = kv4_half_bytes(pool.page_shift, DIM), scales_at = (int64_t)(DIM / 2) << pool.page_shift;
+  const int octet = threadIdx.x % kOctets;
+  uint16_t *out = (values ? v + head * v_head : k + head * k_head) + 8 * octet;
+  const int64_t stride = values ? v_token : k_token;
+  uint32_t codes[kPasses], scale[kPasses];
+  int page[kPasses];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) reinterpret_cast<u32x4 *>(dst)[i] = kv4_octet<F16>(codes[i], scale);
+  for (int i = 0; i < kPasses; ++i) {
+    const int r = threadIdx.x / kOctets + i * (kThreads / kOctets);
+    page[i] = pages[r];
+    const uint8_t *half = pool.pages + (((int64_t)max(page[i], 0) * pool.kv_heads + head) * 2 + values) * half_bytes;
+    codes[i] = *reinterpret_cast<const uint32_t *>(half + offsets[r] * (DIM / 2) + 4 * octet);
+    scale[i] = half[scales_at + offsets[r] * kGroups + octet / 4];
+  }
+#pragma unroll
+  for (int i = 0; i < kPasses; ++i) {
+    const int64_t token = first + threadIdx.x / kOctets + i * (kThreads / kOctets);
+    if (page[i] >= 0) *reinterpret_cast<u32x4 *>(out + token * stride) = kv4_octet<F16>(codes[i], __uint_as_float(scale[i] << 23));
+  }
 }
 
 // Page pairs travel as kernel arguments: no copy to the device, nothing to keep alive.
@@ -178,7 +199,7 @@ hipError_t launch_kv4_append(const uint16_t *k, int64_t k_token, int64_t k_head,
 
 hipError_t launch_kv4_read(uint16_t *k, int64_t k_token, int64_t k_head, uint16_t *v, int64_t v_token, int64_t v_head,
                            int tokens, bool f16, int dim, const int *cu, const Kv4Pool &pool, hipStream_t stream) {
-  const int rows = kThreads / (dim / 32);
+  const int rows = dim == 128 ? kReadRows<128> : kReadRows<64>;
   by_type(f16, dim, [&](auto type, auto d) {
     hipLaunchKernelGGL((kv4_read_kernel<decltype(type)::value, decltype(d)::value>),
                        dim3((unsigned)((tokens + (int64_t)rows - 1) / rows), (unsigned)pool.kv_heads * 2), dim3(kThreads), 0,

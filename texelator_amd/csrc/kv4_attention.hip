@@ -149,14 +149,15 @@ __global__ __launch_bounds__(64 * kWaves, kResident<DIM>) void kv4_attention_ker
     unit = from = 0;
     end = head_units<kUnit>(length);
   } else {
-    auto units_of = [&](int s) { return pool.kv_heads * (kStart + head_units<kUnit>(kv4_length(pool, s))); };
-    const RaggedPlace place = ragged_place(pool.sequences, units_of, [&](int total) { return (int)blockIdx.x * run_units(total, a); });
+    auto length_of = [&](int s) { return kv4_length(pool, s); };
+    auto units_of = [&](int l) { return pool.kv_heads * (kStart + head_units<kUnit>(l)); };
+    const RaggedPlace place = ragged_place(pool.sequences, length_of, units_of, [&](int total) { return (int)blockIdx.x * run_units(total, a); });
     const int run = run_units(place.total, a);
     unit = blockIdx.x * run;
     end = min(unit + run, place.total);
     if (unit >= end) return;
     sequence = place.sequence;
-    length = __builtin_amdgcn_readfirstlane(kv4_length(pool, sequence));
+    length = place.length;
     head = place.local / (kStart + head_units<kUnit>(length));
     from = place.local - head * (kStart + head_units<kUnit>(length)) - kStart;  // below 0: units without work
   }
@@ -411,10 +412,11 @@ __global__ __launch_bounds__(256) void kv4_combine_kernel(Kv4Attention a) {
   __shared__ float sums[kGroups], tops[4];
   const Kv4Pool &pool = a.pool;
   const int sequence = blockIdx.x / pool.kv_heads, head = blockIdx.x % pool.kv_heads, q = blockIdx.y;
-  auto units_of = [&](int s) { return pool.kv_heads * (kStart + head_units<kUnit>(kv4_length(pool, s))); };
-  const RaggedPlace place = ragged_before(pool.sequences, units_of, sequence);
+  auto length_of = [&](int s) { return kv4_length(pool, s); };
+  auto units_of = [&](int l) { return pool.kv_heads * (kStart + head_units<kUnit>(l)); };
+  const RaggedPlace place = ragged_before(pool.sequences, length_of, units_of, sequence);
   const int run = run_units(place.total, a);
-  const int units = head_units<kUnit>(kv4_length(pool, sequence));
+  const int units = head_units<kUnit>(place.length);
   const int begin = place.local + head * (kStart + units), work = begin + kStart;  // units with work: work .. work + units - 1
   const int w0 = work / run, w1 = (work + units - 1) / run;
   if (w0 == w1) return;  // one workgroup had it all and wrote the output

@@ -136,9 +136,10 @@ __global__ __launch_bounds__(64 * QW * KW, QW * KW * KB == 128 ? 1 : 2) void pac
   // Heads fastest; where the head count allows, an XCD gets neighbouring heads, which share keys.
   constexpr int kQueries = 32 * QW;
   int hx = 0;
-  auto tiles_of = [&](int s) { return (rows_of(a.cu_q, s, a.total_q).count + kQueries - 1) / kQueries; };
+  auto queries_of = [&](int s) { return rows_of(a.cu_q, s, a.total_q).count; };
+  auto tiles_of = [&](int count) { return (count + kQueries - 1) / kQueries; };
   auto before_of = [&](int s) { return (rows_of(a.cu_k, s, a.total_k).count - rows_of(a.cu_q, s, a.total_q).count) / kQueries; };
-  const RaggedPlace place = ragged_heaviest(a.sequences, tiles_of, before_of, [&](int total) {
+  const RaggedPlace place = ragged_heaviest(a.sequences, queries_of, tiles_of, before_of, [&](int total) {
     int index = blockIdx.x;
     const int64_t all = (int64_t)total * a.heads;
     const int first = a.cus & ~7, end = (int)min((int64_t)2 * first, all) & ~7;

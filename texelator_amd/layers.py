@@ -7,6 +7,7 @@ the current stream. Nothing here allocates unless an output is not supplied.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -548,15 +549,18 @@ def swiglu(gate_up: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tens
 _ROW_CODE = {torch.float16: _lib.TX_DTYPE_F16, torch.bfloat16: _lib.TX_DTYPE_BF16}
 
 
+# The messages are put together only for the calls that fail: formatting them took a tenth of a small call's host time.
 def _expect_rows(name: str, t: torch.Tensor, like: torch.Tensor, heads: int, head_dim: int) -> None:
-    _expect(t.dim() == 3 and t.dtype == like.dtype and t.device == like.device and t.shape[1] == heads
-            and t.shape[2] == head_dim and t.stride(2) == 1, f"{name} must be {like.dtype} [rows, {heads}, {head_dim}] on one device, "
-            "the last dimension contiguous")
+    shape = t.shape
+    if (len(shape) != 3 or shape[1] != heads or shape[2] != head_dim or t.dtype != like.dtype or t.device != like.device
+            or t.stride(2) != 1):
+        raise TexelatorError(f"{name} must be {like.dtype} [rows, {heads}, {head_dim}] on one device, the last dimension contiguous")
 
 
 def _expect_ints(name: str, t: torch.Tensor, count: int, device: torch.device) -> None:
-    _expect(t.dtype == torch.int32 and t.dim() == 1 and t.shape[0] == count and t.device == device and t.is_contiguous(),
-            f"{name} must be a contiguous int32 [{count}] on the same device")
+    shape = t.shape
+    if len(shape) != 1 or shape[0] != count or t.dtype != torch.int32 or t.device != device or not t.is_contiguous():
+        raise TexelatorError(f"{name} must be a contiguous int32 [{count}] on the same device")
 
 
 def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor, scale: float,
@@ -567,30 +571,36 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     ``cu_k[s] .. cu_k[s + 1] - 1`` (int32 on the device; ``cu_k`` defaults to ``cu_q``); its last query sees its last key,
     so keys of earlier turns come first. A query that sees no key gets zeros; rows of ``out`` that belong to no
     sequence are left as they are (uninitialised where ``out`` is not given). Returns ``[tokens, heads, dim]``."""
-    _expect(q.is_cuda and q.dim() == 3 and q.dtype in _ROW_CODE and q.stride(2) == 1,
-            "q must be CUDA bf16 or fp16 [tokens, heads, dim], the last dimension contiguous")
-    total, heads, dim = q.shape
-    kv_heads = k.shape[1] if k.dim() == 3 else 0
-    _expect_rows("k", k, q, kv_heads, dim)
-    _expect_rows("v", v, q, kv_heads, dim)
-    _expect(kv_heads > 0 and v.shape[0] == k.shape[0], "k and v must have as many rows and at least one head")
-    _expect(cu_q.dim() == 1 and cu_q.shape[0] > 0, "cu_q must be int32 [sequences + 1]")
+    shape, rows, dtype, device, code = q.shape, k.shape, q.dtype, q.device, _ROW_CODE.get(q.dtype)
+    if code is None or len(shape) != 3 or not q.is_cuda or q.stride(2) != 1:
+        raise TexelatorError("q must be CUDA bf16 or fp16 [tokens, heads, dim], the last dimension contiguous")
+    total, heads, dim = shape
+    if (len(rows) != 3 or rows != v.shape or rows[1] == 0 or rows[2] != dim or k.dtype != dtype or v.dtype != dtype
+            or k.device != device or v.device != device):
+        raise TexelatorError(f"k and v must be {dtype} [keys, kv_heads, {dim}] on q's device")
+    q_strides, k_strides, v_strides = q.stride(), k.stride(), v.stride()
+    if k_strides[2] != 1 or v_strides[2] != 1:
+        raise TexelatorError("the last dimension of k and v must be contiguous")
+    sequences = cu_q.numel() - 1
+    _expect(sequences >= 0, "cu_q must be int32 [sequences + 1]")
+    _expect_ints("cu_q", cu_q, sequences + 1, device)
     if cu_k is None:
-        _expect(k.shape[0] == total, "without cu_k there is a key for each query")
+        _expect(rows[0] == total, "without cu_k there is a key for each query")
         cu_k = cu_q
-    _expect_ints("cu_q", cu_q, cu_q.shape[0], q.device)
-    _expect_ints("cu_k", cu_k, cu_q.shape[0], q.device)
+    else:
+        _expect_ints("cu_k", cu_k, sequences + 1, device)
     if out is None:
-        out = torch.empty((total, heads, dim), dtype=q.dtype, device=q.device)
+        out = torch.empty(shape, dtype=dtype, device=device)
     else:
         _expect_rows("out", out, q, heads, dim)
         _expect(out.shape[0] == total, "out must be shaped like q")
     if total == 0:
         return out
+    out_strides = out.stride()
     check(_lib.load().tx_packed_attention(
-        q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
-        _ROW_CODE[q.dtype], heads, kv_heads, dim, cu_q.data_ptr(), cu_k.data_ptr(), cu_q.shape[0] - 1, total, k.shape[0],
-        float(scale), out.data_ptr(), out.stride(0), out.stride(1), q.device.index, _stream(q)))
+        q.data_ptr(), q_strides[0], q_strides[1], k.data_ptr(), k_strides[0], k_strides[1], v.data_ptr(), v_strides[0],
+        v_strides[1], code, heads, rows[1], dim, cu_q.data_ptr(), cu_k.data_ptr(), sequences, total, rows[0], float(scale),
+        out.data_ptr(), out_strides[0], out_strides[1], device.index, _stream_address(device)))
     return out
 
 
@@ -607,21 +617,34 @@ def kv4_pages(num_pages: int, kv_heads: int, head_dim: int, page_size: int = 64,
     return torch.zeros(shape if layers is None else (layers, *shape), dtype=torch.uint8, device=device)
 
 
-def _kv4_args(pages: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor, head_dim: int) -> tuple:
+def _kv4_args(pages: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor, head_dim: int, device: torch.device) -> tuple:
     """The cache's arguments of a C call, from pages to sequences."""
-    _expect(head_dim in (64, 128), "head_dim must be 64 or 128")
-    _expect(pages.is_cuda and pages.dtype == torch.uint8 and pages.dim() == 4 and pages.shape[2] == 2 and pages.is_contiguous(),
-            "pages must be contiguous CUDA uint8 [num_pages, kv_heads, 2, page bytes]")
-    num_pages, kv_heads, _, half = pages.shape
-    row = head_dim * 17 // 32
-    _expect(half % row == 0, "pages were made for another head_dim")
-    _expect(block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.device == pages.device
-            and (block_table.stride(1) == 1 or block_table.shape[1] == 1),
-            "block_table must be int32 [sequences, pages] on the same device, rows contiguous")
-    sequences, max_pages = block_table.shape
-    _expect_ints("lengths", lengths, sequences, pages.device)
-    return (pages.data_ptr(), num_pages, kv_heads, head_dim, half // row, block_table.data_ptr(), block_table.stride(0),
-            max_pages, lengths.data_ptr(), sequences)
+    shape, table = pages.shape, block_table.shape
+    if (len(shape) != 4 or shape[2] != 2 or pages.dtype != torch.uint8 or not pages.is_cuda or pages.device != device
+            or not pages.is_contiguous()):
+        raise TexelatorError("pages must be contiguous CUDA uint8 [num_pages, kv_heads, 2, page bytes] on the rows' device")
+    if head_dim not in (64, 128):
+        raise TexelatorError("head_dim must be 64 or 128")
+    page_size, rest = divmod(shape[3], head_dim * 17 // 32)
+    if rest:
+        raise TexelatorError("pages were made for another head_dim")
+    if (len(table) != 2 or block_table.dtype != torch.int32 or block_table.device != device
+            or (block_table.stride(1) != 1 and table[1] != 1)):
+        raise TexelatorError("block_table must be int32 [sequences, pages] on the same device, rows contiguous")
+    _expect_ints("lengths", lengths, table[0], device)
+    return (pages.data_ptr(), shape[0], shape[1], head_dim, page_size, block_table.data_ptr(), block_table.stride(0), table[1],
+            lengths.data_ptr(), table[0])
+
+
+def _kv4_rows(k: torch.Tensor, v: torch.Tensor, kv_heads: int, head_dim: int, device: torch.device) -> tuple:
+    """The arguments of a C call that k and v [tokens, kv_heads, head_dim] make, to the token count."""
+    shape, dtype, k_strides, v_strides = k.shape, k.dtype, k.stride(), v.stride()
+    code = _ROW_CODE.get(dtype)
+    if (code is None or len(shape) != 3 or shape != v.shape or shape[1] != kv_heads or shape[2] != head_dim or v.dtype != dtype
+            or k.device != device or v.device != device or k_strides[2] != 1 or v_strides[2] != 1):
+        raise TexelatorError(f"k and v must be CUDA bf16 or fp16 [tokens, {kv_heads}, {head_dim}] on the pages' device, the last "
+                             "dimension contiguous")
+    return k.data_ptr(), k_strides[0], k_strides[1], v.data_ptr(), v_strides[0], v_strides[1], code, shape[0]
 
 
 def kv4_append(k: torch.Tensor, v: torch.Tensor, pages: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor,
@@ -632,21 +655,16 @@ def kv4_append(k: torch.Tensor, v: torch.Tensor, pages: torch.Tensor, block_tabl
     ``[sequences]``) counts the new tokens already, so that one update serves all layers: the tokens ``cu[s] .. cu[s + 1] - 1``
     become the last ones of ``lengths[s]`` positions (``cu`` int32 ``[sequences + 1]``; without it, one token for each
     sequence). A page that receives tokens must belong to one sequence alone."""
-    _expect(k.is_cuda and k.dim() == 3 and k.dtype in _ROW_CODE and k.stride(2) == 1 and k.device == pages.device,
-            "k must be CUDA bf16 or fp16 [tokens, kv_heads, dim] on the pages' device, the last dimension contiguous")
-    tokens, kv_heads, dim = k.shape
-    _expect_rows("v", v, k, kv_heads, dim)
-    cache = _kv4_args(pages, block_table, lengths, dim)
-    _expect(kv_heads == cache[2] and v.shape[0] == tokens, "k and v must have the pages' heads and as many rows")
+    device = pages.device
+    cache = _kv4_args(pages, block_table, lengths, k.shape[-1], device)
+    rows = _kv4_rows(k, v, cache[2], cache[3], device)
+    tokens, sequences = rows[-1], cache[-1]
     if cu is None:
-        _expect(tokens == cache[-1], "without cu there is one token for each sequence")
+        _expect(tokens == sequences, "without cu there is one token for each sequence")
     else:
-        _expect_ints("cu", cu, cache[-1] + 1, k.device)
-    if tokens == 0 or cache[-1] == 0:
-        return
-    check(_lib.load().tx_kv4_append(k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
-                                    _ROW_CODE[k.dtype], tokens, None if cu is None else cu.data_ptr(), *cache,
-                                    k.device.index, _stream(k)))
+        _expect_ints("cu", cu, sequences + 1, device)
+    if tokens and sequences:
+        check(_lib.load().tx_kv4_append(*rows, None if cu is None else cu.data_ptr(), *cache, device.index, _stream_address(device)))
 
 
 def kv4_read(pages: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor, head_dim: int,
@@ -657,35 +675,38 @@ def kv4_read(pages: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tens
     where ``cu`` is the sums of ``lengths``, as :func:`packed_attention` takes the keys of earlier turns); without ``cu``
     the last one of each. ``tokens``: the rows in all, ``cu[-1]`` (needed with ``cu`` unless ``out`` is given). Rows that name
     no position are left as they are."""
-    cache = _kv4_args(pages, block_table, lengths, head_dim)
+    device = pages.device
+    cache = _kv4_args(pages, block_table, lengths, head_dim, device)
+    sequences = cache[-1]
     if cu is None:
-        _expect(tokens is None or tokens == cache[-1], "without cu there is one token for each sequence")
-        tokens = cache[-1]
+        _expect(tokens is None or tokens == sequences, "without cu there is one token for each sequence")
+        tokens = sequences
     else:
-        _expect_ints("cu", cu, cache[-1] + 1, pages.device)
+        _expect_ints("cu", cu, sequences + 1, device)
     if out is None:
         _expect(tokens is not None and tokens >= 0 and dtype in _ROW_CODE, "tokens is needed with cu; dtype is bf16 or fp16")
-        out = torch.empty((2, tokens, cache[2], head_dim), dtype=dtype, device=pages.device).unbind(0)
-    k, v = out
-    _expect(k.is_cuda and k.dtype in _ROW_CODE and k.device == pages.device, "out must be CUDA bf16 or fp16 on the pages' device")
-    _expect_rows("k", k, k, cache[2], head_dim)
-    _expect_rows("v", v, k, cache[2], head_dim)
-    _expect(v.shape[0] == k.shape[0] and (tokens is None or k.shape[0] == tokens), "k and v must have as many rows as tokens")
-    if k.shape[0] == 0 or cache[-1] == 0:
-        return k, v
-    check(_lib.load().tx_kv4_read(k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
-                                  _ROW_CODE[k.dtype], k.shape[0], None if cu is None else cu.data_ptr(), *cache,
-                                  pages.device.index, _stream(pages)))
+        k, v = torch.empty((2, tokens, cache[2], head_dim), dtype=dtype, device=device).unbind(0)
+    else:
+        k, v = out
+    rows = _kv4_rows(k, v, cache[2], head_dim, device)
+    _expect(tokens is None or rows[-1] == tokens, "out must have a row for each token")
+    if rows[-1] and sequences:
+        check(_lib.load().tx_kv4_read(*rows, None if cu is None else cu.data_ptr(), *cache, device.index, _stream_address(device)))
     return k, v
+
+
+@functools.lru_cache(maxsize=256)
+def _kv4_workspace_bytes(*sizes: int) -> int:
+    out = ctypes.c_int64(0)
+    check(_lib.load().tx_kv4_attention_workspace(*sizes, out))
+    return out.value
 
 
 def kv4_attention_workspace_bytes(pages: torch.Tensor, block_table: torch.Tensor, heads: int, head_dim: int) -> int:
     """Device scratch of :func:`kv4_attention`: it depends on shapes alone, not on the lengths."""
     sequences, max_pages = block_table.shape
-    out = ctypes.c_int64(0)
-    check(_lib.load().tx_kv4_attention_workspace(sequences, heads, pages.shape[1], head_dim, pages.shape[3] * 32 // (17 * head_dim),
-                                                 max_pages, pages.device.index, out))
-    return out.value
+    return _kv4_workspace_bytes(sequences, heads, pages.shape[1], head_dim, pages.shape[3] * 32 // (17 * head_dim), max_pages,
+                                pages.device.index)
 
 
 def kv4_attention(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor, scale: float,
@@ -695,26 +716,30 @@ def kv4_attention(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tenso
     :func:`kv4_append`); heads a multiple of the pages' KV heads. Returns ``[sequences, heads, dim]``, zeros for an empty
     sequence. ``workspace``: :func:`kv4_attention_workspace_bytes` bytes that no call running at the same time uses;
     allocated on the current stream where not given."""
-    _expect(q.is_cuda and q.dim() == 3 and q.dtype in _ROW_CODE and q.stride(2) == 1 and q.device == pages.device,
-            "q must be CUDA bf16 or fp16 [sequences, heads, dim] on the pages' device, the last dimension contiguous")
-    sequences, heads, dim = q.shape
-    cache = _kv4_args(pages, block_table, lengths, dim)
+    shape, device, code = q.shape, q.device, _ROW_CODE.get(q.dtype)
+    if code is None or len(shape) != 3 or not q.is_cuda or q.stride(2) != 1:
+        raise TexelatorError("q must be CUDA bf16 or fp16 [sequences, heads, dim], the last dimension contiguous")
+    sequences, heads, dim = shape
+    cache = _kv4_args(pages, block_table, lengths, dim, device)
     _expect(cache[-1] == sequences and heads > 0 and heads % cache[2] == 0,
             "q must have a row for each sequence and a multiple of the pages' heads")
     if out is None:
-        out = torch.empty((sequences, heads, dim), dtype=q.dtype, device=q.device)
+        out = torch.empty(shape, dtype=q.dtype, device=device)
     else:
         _expect_rows("out", out, q, heads, dim)
         _expect(out.shape[0] == sequences, "out must be shaped like q")
     if sequences == 0:
         return out
     if workspace is None:
-        workspace = torch.empty(kv4_attention_workspace_bytes(pages, block_table, heads, dim), dtype=torch.uint8, device=q.device)
-    _expect(workspace.is_cuda and workspace.is_contiguous() and workspace.device == q.device,
-            "workspace must be a contiguous CUDA tensor on the same device")
-    check(_lib.load().tx_kv4_attention(q.data_ptr(), q.stride(0), q.stride(1), _ROW_CODE[q.dtype], heads, *cache, float(scale),
-                                       workspace.data_ptr(), workspace.nbytes, out.data_ptr(), out.stride(0), out.stride(1),
-                                       q.device.index, _stream(q)))
+        size = _kv4_workspace_bytes(sequences, heads, cache[2], dim, cache[4], cache[7], device.index)
+        workspace = torch.empty(size, dtype=torch.uint8, device=device) if size else None  # short sequences need no scratch
+    else:
+        _expect(workspace.is_cuda and workspace.is_contiguous() and workspace.device == device,
+                "workspace must be a contiguous CUDA tensor on the same device")
+        size = workspace.nbytes
+    q_strides, out_strides = q.stride(), out.stride()
+    check(_lib.load().tx_kv4_attention(q.data_ptr(), q_strides[0], q_strides[1], code, heads, *cache, float(scale), _ptr(workspace),
+                                       size, out.data_ptr(), out_strides[0], out_strides[1], device.index, _stream_address(device)))
     return out
 
 
