@@ -136,9 +136,13 @@ __global__ __launch_bounds__(64 * QW * KW, QW * KW * KB == 128 ? 1 : 2) void pac
   // Heads fastest; where the head count allows, an XCD gets neighbouring heads, which share keys.
   constexpr int kQueries = 32 * QW;
   int hx = 0;
-  auto queries_of = [&](int s) { return rows_of(a.cu_q, s, a.total_q).count; };
+  // Up to 64 sequences, lane s keeps the rows of sequence s: they are loaded once.
+  const bool few = a.sequences <= 64;
+  Rows lane_q = {0, 0}, lane_k = {0, 0};
+  if (few && lane < a.sequences) lane_q = rows_of(a.cu_q, lane, a.total_q), lane_k = rows_of(a.cu_k, lane, a.total_k);
+  auto queries_of = [&](int s) { return few ? lane_q.count : rows_of(a.cu_q, s, a.total_q).count; };
   auto tiles_of = [&](int count) { return (count + kQueries - 1) / kQueries; };
-  auto before_of = [&](int s) { return (rows_of(a.cu_k, s, a.total_k).count - rows_of(a.cu_q, s, a.total_q).count) / kQueries; };
+  auto before_of = [&](int) { return (lane_k.count - lane_q.count) / kQueries; };
   const RaggedPlace place = ragged_heaviest(a.sequences, queries_of, tiles_of, before_of, [&](int total) {
     int index = blockIdx.x;
     const int64_t all = (int64_t)total * a.heads;
@@ -151,8 +155,13 @@ __global__ __launch_bounds__(64 * QW * KW, QW * KW * KB == 128 ? 1 : 2) void pac
   const int head = a.heads % kXcds == 0 ? (hx % kXcds) * (a.heads / kXcds) + hx / kXcds : hx;
   const int tile = place.local;
   const int sequence = place.sequence;
-  const Rows qs = rows_of(a.cu_q, sequence, a.total_q), ks = rows_of(a.cu_k, sequence, a.total_k);
-  const int queries = __builtin_amdgcn_readfirstlane(qs.count), keys = __builtin_amdgcn_readfirstlane(ks.count);
+  auto rows_at = [&](Rows of_lane, const int *cu, int total) {
+    const Rows r = few ? Rows{__builtin_amdgcn_readlane(of_lane.begin, sequence), __builtin_amdgcn_readlane(of_lane.count, sequence)}
+                       : rows_of(cu, sequence, total);
+    return Rows{__builtin_amdgcn_readfirstlane(r.begin), __builtin_amdgcn_readfirstlane(r.count)};
+  };
+  const Rows qs = rows_at(lane_q, a.cu_q, a.total_q), ks = rows_at(lane_k, a.cu_k, a.total_k);
+  const int queries = qs.count, keys = ks.count;
   const int shift = keys - queries;      // query i sees the keys up to i + shift
   const int q0 = tile * kQueries + qw * 32;  // this wave's first query
 
