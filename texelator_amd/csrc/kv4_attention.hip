@@ -5,23 +5,30 @@
 //   out[s][h] = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale * q[s][h] . k_j - max),  j < lengths[s]
 //
 // Work: a unit is kUnit positions of one sequence and KV head; the units of all sequences lie in one row, and every
-// workgroup takes an equal run of them, whatever the lengths (it finds its place from the lengths itself). A run
-// that covers a whole (sequence, head) writes its output; the others leave (max, sum, unnormalised output) for the
-// combine kernel, at most two such pieces a workgroup, so the workspace does not grow with the lengths.
+// workgroup takes an equal run of them, whatever the lengths (it finds its place from the lengths itself, so that a captured
+// call serves any). A run that covers a whole (sequence, head) writes its output; the others leave (max, sum,
+// unnormalised output) for the combine kernel, at most two such pieces a workgroup, so the workspace does not grow with the lengths.
 //
-// A wave takes 32 positions at a time and shares nothing with the other waves until its run of a head ends:
+// A wave takes kTile positions (4.25 KiB of cache) at a time and shares nothing with the other waves until its run of a head ends:
 //   * S^T = K q^T (v_mfma_f32_16x16x32: A = 16 keys, B = the head's queries, up to 16): a lane's 16 bytes of codes
 //     (8 at dim 64) lie in one scale group and become MFMA operands by v_cvt_scalef32_pk_*_fp4 alone: the scale rides
 //     along. The queries' dimensions are laid out to match the codes;
-//   * a lane then holds 8 scores of one query: running maximum by two lane swaps, the probabilities, rounded to 16
-//     bits in place, are the B operand of O^T = V^T P^T;
+//   * a lane then holds 4 scores of one query for every 16 keys: running maximum by two lane swaps, the probabilities,
+//     rounded to 16 bits in place, are the B operand of O^T = V^T P^T;
 //   * values are converted the same way and pass through the wave's own LDS, whose transposing reads
 //     (ds_read_b64_tr_b16) give the A operand. 32-byte pieces lie at piece ^ f(row): the reads hit distinct banks;
-//   * the next 32 positions' codes are loaded while these are multiplied.
+//   * the next step's codes set out before these are multiplied, by buffer loads whose page is scalar, and the page ids of the one
+//     after by scalar loads (as vector loads their wait had taken in the codes just set out: 54.8 against 45.4 us below);
+//   * the next head's first codes set out before this head's sums are joined.
 // Positions past the length (the rest of a page is stale) are loaded where they lie and replaced by zeros before they
 // are converted, their scores by -infinity; a page id outside the pool counts as such.
 // Statistics and sums in fp32; sums run over the probabilities as rounded. In fp16 probabilities are held times 2^15,
 // so that small ones keep their bits (p <= 2^15 stays below fp16's largest).
+//
+// Bound: memory for long contexts, 262144 positions of 8 heads of 128 (285 MB) 45 us, 6.3 TB/s with a part of it still cached, and 5
+// for the combine kernel and the gap before it; at dim 64 instruction issue (half the bytes for the same scores), 163 MB at 31 us, 5.3
+// TB/s. A few thousand positions in all: the chain of dependent loads (lengths, page ids, codes), the merge and the second
+// launch, 8 us; a codes' step further ahead, more workgroups a CU and 16-wave workgroups were all slower.
 #include <math.h>
 
 #include <type_traits>
@@ -101,7 +108,8 @@ __device__ __forceinline__ float quarters_sum(float v) {
 template <int UNIT>
 __device__ __forceinline__ int head_units(int length) { return max(1, (length + UNIT - 1) / UNIT); }
 
-// What starting and ending a head costs, in units: a head's share of the row of units begins with as many without work.
+// What starting and ending a head costs, in units: a head's share of the row of units begins with as many without work (96
+// sequences of 1 to 16384 positions, 16 heads of 64: 42.9 us, with none 50.8, with two 44.0).
 constexpr int kStart = 1;
 
 // Units of every workgroup.
@@ -115,7 +123,8 @@ __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(
 // Floats of a piece: per query its output [dim], then max and sum of all queries.
 __device__ __host__ inline int64_t piece_floats(int group, int dim) { return (int64_t)group * (dim + 2); }
 
-template <bool F16, int DIM>
+// SHARE: 16-position groups of a step that lie in one page: a page's, or all of the step's.
+template <bool F16, int DIM, int SHARE>
 __global__ __launch_bounds__(64 * kWaves, kResident<DIM>) void kv4_attention_kernel(Kv4Attention a) {
   constexpr int kUnit = tx::kUnit<DIM>, kTile = tx::kTile<DIM>;
   constexpr int kSubs = kTile / 16;       // 16 positions make an MFMA tile of scores
@@ -186,15 +195,16 @@ __global__ __launch_bounds__(64 * kWaves, kResident<DIM>) void kv4_attention_ker
   auto piece_at = [](int row, int piece) { return row * kRow + 32 * (piece ^ (DIM == 128 ? row & 7 : (row >> 1) & 3)); };
 
   // Page ids of a step's positions, fetched a step before its codes are.
+  constexpr int kPages = kSubs / SHARE;
   struct Ids {
-    int page[kSubs];
+    int page[kPages];
   };
   auto ids_of = [&](const Part &part, int position) __attribute__((always_inline)) {
     // Constant for the whole launch: scalar loads, whose wait leaves the codes under way alone.
     const auto *table = (const __attribute__((address_space(4))) int *)(pool.table + part.sequence * pool.table_stride);
     Ids ids;
 #pragma unroll
-    for (int i = 0; i < kSubs; ++i) ids.page[i] = table[min(position + 16 * i, max(part.length - 1, 0)) >> pool.page_shift];
+    for (int i = 0; i < kPages; ++i) ids.page[i] = table[min(position + 16 * SHARE * i, max(part.length - 1, 0)) >> pool.page_shift];
     return ids;
   };
   struct Tile {
@@ -206,18 +216,30 @@ __global__ __launch_bounds__(64 * kWaves, kResident<DIM>) void kv4_attention_ker
   const uint32_t code_lane = n * (DIM / 2) + quarter * (DIM / 8), scale_lane = n * kWords + (DIM == 128 ? quarter : quarter >> 1);
   auto load = [&](Tile &t, const Part &part, int position, const Ids &ids) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < kSubs; ++i) {
-      const int at = position + 16 * i;
-      const bool known = (uint32_t)ids.page[i] < (uint64_t)pool.num_pages;
-      t.valid[i] = known ? min(max(part.length - at, 0), 16) : 0;
-      const int page = known ? ids.page[i] : 0;
+    for (int p = 0; p < kPages; ++p) {
+      const int at = position + 16 * SHARE * p;
+      const bool known = (uint32_t)ids.page[p] < (uint64_t)pool.num_pages;
+      const int page = known ? ids.page[p] : 0;
       const int row = at & ((1 << pool.page_shift) - 1);
-      const uint8_t *codes = pool.pages + ((int64_t)page * pool.kv_heads + part.head) * 2 * half_bytes + row * (DIM / 2);
-      const uint8_t *scales = codes + scales_at - row * (DIM / 2 - kWords);
-      t.k[i] = *reinterpret_cast<const Codes *>(codes + code_lane);
-      t.v[i] = *reinterpret_cast<const Codes *>(codes + half_bytes + code_lane);
-      t.ks[i] = scales[scale_lane];
-      t.vs[i] = (scales + half_bytes)[scale_lane];
+      // Buffer loads: the page's place is scalar, the lane's share one register for all of them.
+      const __amdgpu_buffer_rsrc_t half2 = __builtin_amdgcn_make_buffer_rsrc(
+          pool.pages + ((int64_t)page * pool.kv_heads + part.head) * 2 * half_bytes, (short)0, (int)(2 * half_bytes), 0x00020000);
+      const int codes = row * (DIM / 2), scales = (int)scales_at + row * kWords;
+#pragma unroll
+      for (int j = 0; j < SHARE; ++j) {
+        const int i = p * SHARE + j;
+        t.valid[i] = known ? min(max(part.length - at - 16 * j, 0), 16) : 0;
+        const uint32_t code = code_lane + 16 * j * (DIM / 2), scale = scale_lane + 16 * j * kWords;
+        if constexpr (DIM == 128) {
+          t.k[i] = __builtin_amdgcn_raw_buffer_load_b128(half2, code, codes, 0);
+          t.v[i] = __builtin_amdgcn_raw_buffer_load_b128(half2, code, codes + (int)half_bytes, 0);
+        } else {
+          t.k[i] = __builtin_amdgcn_raw_buffer_load_b64(half2, code, codes, 0);
+          t.v[i] = __builtin_amdgcn_raw_buffer_load_b64(half2, code, codes + (int)half_bytes, 0);
+        }
+        t.ks[i] = __builtin_amdgcn_raw_buffer_load_b8(half2, scale, scales, 0);
+        t.vs[i] = __builtin_amdgcn_raw_buffer_load_b8(half2, scale, scales + (int)half_bytes, 0);
+      }
     }
   };
   // This wave's steps of a part: every unit's `wave`-th.
@@ -298,9 +320,11 @@ __global__ __launch_bounds__(64 * kWaves, kResident<DIM>) void kv4_attention_ker
 #pragma unroll
           for (int r = 0; r < 4; ++r) sc[i][r] = 4 * quarter + r < t.valid[i] ? sc[i][r] : -INFINITY;
       }
-      float mx = -INFINITY;
+      float mx = fmaxf(sc[0][0], sc[0][1]);
 #pragma unroll
-      for (int i = 0; i < kSubs; ++i) mx = fmaxf(fmaxf(mx, fmaxf(sc[i][0], sc[i][1])), fmaxf(sc[i][2], sc[i][3]));
+      for (int i = 0; i < kSubs; ++i)
+#pragma unroll
+        for (int r = i == 0 ? 2 : 0; r < 4; r += 2) mx = fmaxf(fmaxf(mx, sc[i][r]), sc[i][r + 1]);
       const float mnew = fmaxf(m, quarters_max(mx));
       if (__builtin_amdgcn_ballot_w64(mnew > m) != 0) {
         const float alpha = mnew > m ? __builtin_amdgcn_exp2f((m - mnew) * sl2) : 1.f;
@@ -502,7 +526,10 @@ hipError_t launch_kv4_attention(const Kv4Attention &a, bool f16, int dim, hipStr
   auto launch = [&](auto type, auto d) {
     constexpr bool kF16 = decltype(type)::value;
     constexpr int kDim = decltype(d)::value;
-    hipLaunchKernelGGL((kv4_attention_kernel<kF16, kDim>), grid, dim3(64 * kWaves), 0, stream, a);
+    const int groups = 1 << (a.pool.page_shift - 4);  // of 16 positions, in a page
+    if (groups >= kTile<kDim> / 16) hipLaunchKernelGGL((kv4_attention_kernel<kF16, kDim, kTile<kDim> / 16>), grid, dim3(64 * kWaves), 0, stream, a);
+    else if (groups >= 2) hipLaunchKernelGGL((kv4_attention_kernel<kF16, kDim, 2>), grid, dim3(64 * kWaves), 0, stream, a);
+    else hipLaunchKernelGGL((kv4_attention_kernel<kF16, kDim, 1>), grid, dim3(64 * kWaves), 0, stream, a);
     if (a.whole) return;
     // Few outputs are spread over more workgroups, 32 dimensions each (40 heads' queries of 1024 pieces: 5.2 us against
     // 6.7); many are not (1280 of them 5.2 against 8.0).
