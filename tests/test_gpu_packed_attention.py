@@ -106,6 +106,28 @@ def test_keys_behind_a_query_reach_it_in_no_way(ext):
     assert torch.equal(got[:100], want[:100])  # query 99 sees the keys up to 119
 
 
+@pytest.mark.parametrize("dtype,dim", [(BF16, 128), (FP16, 64), (FP16, 128), (BF16, 64)])
+@pytest.mark.parametrize("new,old,heads,kv_heads", [([150, 9], [20, 3], 8, 2), ([700, 33], [5, 0], 16, 2), ([50] * 40, [i for i in range(40)], 16, 4),
+                                                    ([1000, 70], [30, 90], 40, 8)])
+def test_values_behind_a_query_reach_it_in_no_way(ext, new, old, heads, kv_heads, dtype, dim):
+    """Infinities and NaN among the values: the queries before them, and other columns, are what they were within the bound."""
+    q, k, v = inputs(new, old, heads, kv_heads, dim, dtype, 21)
+    want, bound = reference(q, k, v, new, old, -dim ** -0.5)
+    starts = [sum(new[:s]) + sum(old[:s]) for s in range(len(new))]
+    struck = torch.zeros(sum(new), heads, dim, dtype=torch.bool, device="cuda")
+    q0 = 0
+    for s, (n, o) in enumerate(zip(new, old)):
+        for place, value, head, column in ((o + n // 2, float("inf"), 0, 7), (o + n - 1, float("nan"), kv_heads - 1, dim - 1),
+                                           (o + n // 3, float("-inf"), kv_heads - 1, 33)):
+            v[starts[s] + place, head, column] = value
+            group = heads // kv_heads
+            struck[q0 + place - o:q0 + n, head * group:(head + 1) * group, column] = True
+        q0 += n
+    got = run(q, k, v, new, old, -dim ** -0.5)
+    assert not torch.isfinite(got[struck]).any()
+    assert_within(torch.where(struck, 0, got), want.masked_fill(struck, 0), bound)
+
+
 def test_views_that_agree_with_the_packed_call(ext):
     """The same rows at other strides and offsets, and an output with gaps, give the same bits."""
     new, old = [130, 40], [3, 60]
