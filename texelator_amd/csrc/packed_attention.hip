@@ -168,7 +168,7 @@ __device__ __forceinline__ void seen_keys_alone(const PackedAttention &a, const 
 
 // Two waves per SIMD, but for <1, 4, 32>, whose four waves have a CU's LDS to themselves.
 template <bool F16, int DIM, int QW, int KW, int KB>
-__global__ __launch_bounds__(64 * QW * KW, QW * KW * KB == 128 ? 1 : 2) void packed_attention_kernel(PackedAttention a) {
+__global__ __launch_bounds__(64 * QW * KW, QW == 1 ? 1 : 2) void packed_attention_kernel(PackedAttention a) {
   constexpr int kRow = DIM * 2;                 // bytes of a key or value
   constexpr int kTile = KB * kRow;              // bytes of a key group's keys (or values) of a turn
   constexpr int kSub = 32 * kRow;               // of 32 of them
@@ -306,7 +306,13 @@ __global__ __launch_bounds__(64 * QW * KW, QW * KW * KB == 128 ? 1 : 2) void pac
   // are keys 4 h .. + 3, slots 4-7 the keys 8 on). The order here is the order of issue (the scheduling barriers hold the
   // compiler to it): the exponentials in the time of the products, operands read two products ahead, the next scores'
   // maximum last.
-  auto step = [&](const f32x16 &cur, f32x16 &next, const char *vt, const char *kt_next) __attribute__((always_inline)) {
+  // The first two of a step's key operands set out before its scores' maxima are settled.
+  auto first_keys = [&](const char *kt, u32x4 &x, u32x4 &y) __attribute__((always_inline)) {
+    x = *reinterpret_cast<const u32x4 *>(kt + k_at);
+    y = *reinterpret_cast<const u32x4 *>(kt + (k_at ^ 32u));
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto step = [&](const f32x16 &cur, f32x16 &next, const char *vt, const char *kt_next, u32x4 x, u32x4 y) __attribute__((always_inline)) {
     const float base = m == -INFINITY ? 0.f : kLift - m * a.sl2;  // no key yet: every score is -infinity
     uint32_t pb[8];
     auto pair = [&](int p) __attribute__((always_inline)) {  // probabilities 2 p and 2 p + 1
@@ -323,7 +329,6 @@ __global__ __launch_bounds__(64 * QW * KW, QW * KW * KB == 128 ? 1 : 2) void pac
     };
     constexpr int kGroups = kSteps + kOut;  // products before the second sixteen keys' probabilities are needed
     int done = 0;
-    u32x4 x = key(0), y = key(1);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int st = 0; st < kSteps; ++st) {
@@ -344,7 +349,10 @@ __global__ __launch_bounds__(64 * QW * KW, QW * KW * KB == 128 ? 1 : 2) void pac
       for (; i < kOut && done < 8 * (kSteps + i + 1) / kGroups; ++done) pair(done);
       x = y;
       y = z;
-      if (i == kOut) largest(next);
+      if (i == kOut) {
+        largest(next);
+        asm volatile("" : "+v"(mx));  // here, not where it is used
+      }
       if (i < kOut) __builtin_amdgcn_sched_barrier(0);
     }
     __builtin_amdgcn_sched_barrier(0);
@@ -371,18 +379,21 @@ __global__ __launch_bounds__(64 * QW * KW, QW * KW * KB == 128 ? 1 : 2) void pac
   auto turn = [&](int it, const char *k_cur, char *k_next, const char *v_cur, char *v_next) __attribute__((always_inline)) {
     drain_barrier();
     const int b = it * KW + kw, k0 = b * KB;
+    u32x4 x, y;
+    first_keys(k_cur + kw * kTile, x, y);
     stage_values(v_next, b + KW);
     stage_keys(k_next, b + KW);
     k_cur += kw * kTile;
     v_cur += kw * kTile;
     if (k0 > reach) return;
     if constexpr (kSubs == 2) {
-      step(s0, s1, v_cur, k_cur);
+      step(s0, s1, v_cur, k_cur, x, y);
       if (k0 + 32 > reach) return;
+      first_keys(k_cur + kSub, x, y);
       settle(s1, k0 + 32);
-      step(s1, s0, v_cur + kSub, k_cur + kSub);
+      step(s1, s0, v_cur + kSub, k_cur + kSub, x, y);
     } else {
-      step(s0, s1, v_cur, k_cur);
+      step(s0, s1, v_cur, k_cur, x, y);
       s0 = s1;
     }
     if (k0 + KW * KB <= reach) settle(s0, k0 + KW * KB);
@@ -492,16 +503,25 @@ hipError_t launch_typed(const PackedAttention &a, hipStream_t stream) {
     hipLaunchKernelGGL(kernel, dim3((unsigned)(tiles * a.heads)), dim3(64 * waves), 0, stream, a);
   };
   // Which split of the waves, by how many tiles of 32 and 64 queries the rows can make and how many keys a sequence has on
-  // average (us, graph replays, at 40/8 heads where no others are named):
+  // average (us, graph replays, at 40/8 heads of 128 where no others are named):
   //   <1, 4, 32> where its workgroups fit the CUs at once and there is a chain of key blocks to shorten: 128 tokens 7.6
   //              against 8.1 of <4, 1, 64>, 256 tokens of 16/2 heads 8.5 against 10.1; but 12 prompts of up to 60 tokens at
   //              32/8 heads 12.7 against 6.6, whose chains are short;
   //   <2, 4, 32> likewise: 1024 tokens of 16/2 heads 17.5 against 23.9; but 512 tokens (320 workgroups) 18.8 against 15.5;
-  //   <4, 1, 64> for all else: 1024 tokens 28.1 against 34.2 of <2, 4, 32>, 8190 tokens 658 against 880.
+  //   <2, 2, KB> where the longest chain still outlasts the others' work, keys being many: 3000 tokens of 16/2 heads 54 against
+  //              60 of <4, 1, 64>, 3 turns of up to 400 behind up to 6000 keys 60 against 82 (heads of 64: 39 against 62), 2500
+  //              tokens of 16/2 heads of 64 27 against 37; but 2048 tokens (1280 workgroups) 70 against 60, 6 turns of up to 600
+  //              behind up to 1000 of 32/8 (896) 42 against 34, 12 prompts of up to 600 tokens of 28/4 heads of 64 17 against 14.
+  //              The lengths themselves, on the device, decide as much: of 26 shapes that this rule sends here four got
+  //              slower, by 2 to 16%, and 22 faster, by up to 37%;
+  //   <4, 1, 64> for all else: 1024 tokens 28.1 against 34.2 of <2, 4, 32>, 8190 tokens 650 against 756 of <2, 2, 32>.
   const int64_t tiles32 = (a.total_q + (int64_t)31 * a.sequences) / 32 * a.heads,
                 tiles64 = (a.total_q + (int64_t)63 * a.sequences) / 64 * a.heads;
-  if (tiles32 <= a.cus && a.total_k >= (int64_t)96 * a.sequences) launch(packed_attention_kernel<F16, DIM, 1, 4, 32>, 32, 4);
-  else if (tiles64 <= a.cus && a.total_k >= (int64_t)96 * a.sequences) launch(packed_attention_kernel<F16, DIM, 2, 4, 32>, 64, 8);
+  const bool some_keys = a.total_k >= (int64_t)96 * a.sequences, many_keys = a.total_k >= (int64_t)256 * a.sequences;
+  if (tiles32 <= a.cus && some_keys) launch(packed_attention_kernel<F16, DIM, 1, 4, 32>, 32, 4);
+  else if (tiles64 <= a.cus && some_keys) launch(packed_attention_kernel<F16, DIM, 2, 4, 32>, 64, 8);
+  else if (2 * tiles64 < (DIM == 64 ? 7 : 6) * (int64_t)a.cus && many_keys)
+    launch(packed_attention_kernel<F16, DIM, 2, 2, DIM == 64 ? 64 : 32>, 64, 4);
   else launch(packed_attention_kernel<F16, DIM, 4, 1, 64>, 128, 4);
   return hipGetLastError();
 }
