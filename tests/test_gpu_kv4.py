@@ -376,6 +376,7 @@ def test_copies_of_pages(ext, layer_count, num_pages, kv_heads, dim, page, copie
         layers.kv4_copy_pages(pages, [0, 1], [1])
     with pytest.raises(_lib.TexelatorError, match="integers"):
         layers.kv4_copy_pages(pages, [0.5], [1])
+    layers.kv4_copy_pages(pages, np.array([src[0]]), torch.tensor([dst[0]]))  # integers of other kinds
     assert torch.equal(pages.cpu(), want)
 
 
@@ -386,7 +387,7 @@ def test_wrong_tensors_are_refused(ext):
     q = torch.zeros(3, 6, 64, dtype=BF16, device="cuda")
     wide = torch.zeros(3, 2, 128, dtype=BF16, device="cuda")
     bad_append = [(k[:2], k, None), (k, k.half(), None), (k, k[:, :1], None), (wide, wide, None), (k.float(), k.float(), None),
-                  (k, k, i32([0, 3])), (k, k, i32([0, 1, 2, 3]).long()), (wide[:, :, ::2], k, None), (wide[:, :, 4:68], k, None)]
+                  (k[0, 0, 0], k[0, 0, 0], None), (k, k, i32([0, 3])), (k, k, i32([0, 1, 2, 3]).long()), (wide[:, :, ::2], k, None), (wide[:, :, 4:68], k, None)]
     for a, b, cu in bad_append:
         with pytest.raises(_lib.TexelatorError):
             layers.kv4_append(a, b, pages, table, lengths, cu=cu)

@@ -90,6 +90,13 @@ def test_copies_that_depend_on_their_order_are_refused(src, dst, change, message
     assert message in _lib.load().tx_last_error()
 
 
+@pytest.mark.parametrize("src,dst,message", [([5, 1], [2 ** 30, 2 ** 30], b"copied to twice"), ([7, 2 ** 30], [2 ** 30, 3], b"both"),
+                                             ([0], [2 ** 31 - 2], b"outside")])
+def test_the_same_for_a_pool_far_larger_than_the_lists(src, dst, message):
+    assert copy(src, dst, num_pages=2 ** 31 - 2) == _lib.TX_ERR_INVALID
+    assert message in _lib.load().tx_last_error()
+
+
 def test_no_copies_launch_nothing():
     assert copy([], []) == _lib.TX_OK
 

@@ -1559,16 +1559,28 @@ int tx_kv4_copy_pages(void *pages, int layers, int64_t num_pages, int64_t page_b
     return fail(TX_ERR_INVALID, "kv4_copy_pages: pages must be 16-byte aligned and hold a multiple of 16 bytes");
   if (count < 0 || count > num_pages) return fail(TX_ERR_INVALID, "kv4_copy_pages: more copies than pages");
   try {
-    // Pages are copied all at once: a page is written once, and no page that is read is written.
-    std::vector<int64_t> targets(dst, dst + count);
-    std::sort(targets.begin(), targets.end());
-    if (count && (targets.front() < 0 || targets.back() >= num_pages)) return fail(TX_ERR_INVALID, "kv4_copy_pages: page id outside the pool");
-    if (std::adjacent_find(targets.begin(), targets.end()) != targets.end())
-      return fail(TX_ERR_INVALID, "kv4_copy_pages: a page is copied to twice");
-    for (int64_t i = 0; i < count; ++i) {
-      if (src[i] < 0 || src[i] >= num_pages) return fail(TX_ERR_INVALID, "kv4_copy_pages: page id outside the pool");
-      if (std::binary_search(targets.begin(), targets.end(), src[i]))
-        return fail(TX_ERR_INVALID, "kv4_copy_pages: a page is both copied from and copied to");
+    // Pages are copied all at once: a page is written once, and no page that is read is written. Targets as a bit map
+    // where that is small beside the lists, else sorted.
+    for (int64_t i = 0; i < count; ++i)
+      if (src[i] < 0 || src[i] >= num_pages || dst[i] < 0 || dst[i] >= num_pages)
+        return fail(TX_ERR_INVALID, "kv4_copy_pages: page id outside the pool");
+    const char *twice = "kv4_copy_pages: a page is copied to twice", *both = "kv4_copy_pages: a page is both copied from and copied to";
+    if (num_pages / 64 <= 16 * count + 1024) {
+      std::vector<uint64_t> written((size_t)(num_pages / 64 + 1));
+      for (int64_t i = 0; i < count; ++i) {
+        uint64_t &word = written[(size_t)(dst[i] / 64)];
+        const uint64_t bit = uint64_t(1) << (dst[i] % 64);
+        if (word & bit) return fail(TX_ERR_INVALID, twice);
+        word |= bit;
+      }
+      for (int64_t i = 0; i < count; ++i)
+        if (written[(size_t)(src[i] / 64)] >> (src[i] % 64) & 1) return fail(TX_ERR_INVALID, both);
+    } else {
+      std::vector<int64_t> targets(dst, dst + count);
+      std::sort(targets.begin(), targets.end());
+      if (std::adjacent_find(targets.begin(), targets.end()) != targets.end()) return fail(TX_ERR_INVALID, twice);
+      for (int64_t i = 0; i < count; ++i)
+        if (std::binary_search(targets.begin(), targets.end(), src[i])) return fail(TX_ERR_INVALID, both);
     }
   } catch (const std::bad_alloc &) {
     return fail(TX_ERR_INVALID, "kv4_copy_pages: out of host memory");

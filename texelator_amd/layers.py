@@ -6,6 +6,7 @@ the current stream. Nothing here allocates unless an output is not supplied.
 """
 from __future__ import annotations
 
+import array
 import ctypes
 import functools
 
@@ -570,7 +571,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     ``[q | k | v]`` projection will do). Sequence ``s`` has the queries ``cu_q[s] .. cu_q[s + 1] - 1`` and the keys
     ``cu_k[s] .. cu_k[s + 1] - 1`` (int32 on the device; ``cu_k`` defaults to ``cu_q``); its last query sees its last key,
     so keys of earlier turns come first. A query that sees no key gets zeros; rows of ``out`` that belong to no
-    sequence are left as they are (uninitialised where ``out`` is not given). Returns ``[tokens, heads, dim]``."""
+    sequence are left as they are (uninitialised where ``out`` is not given). Keys that a query does not see,
+    and their values, may hold anything. Returns ``[tokens, heads, dim]``."""
     shape, rows, dtype, device, code = q.shape, k.shape, q.dtype, q.device, _ROW_CODE.get(q.dtype)
     if code is None or len(shape) != 3 or not q.is_cuda or q.stride(2) != 1:
         raise TexelatorError("q must be CUDA bf16 or fp16 [tokens, heads, dim], the last dimension contiguous")
@@ -609,7 +611,8 @@ def kv4_pages(num_pages: int, kv_heads: int, head_dim: int, page_size: int = 64,
     """An empty pool of a paged 4-bit KV cache: uint8 ``[num_pages, kv_heads, 2, page_size * head_dim * 17 / 32]``, behind
     ``layers`` where given (``pages[i]`` is layer i's pool, and one block table serves them all). A key or value takes
     ``head_dim * 17 / 32`` bytes: E2M1 codes and an E8M0 scale for 32 elements. ``page_size``: positions of a page, a
-    power of two from 16 to 1024; ``head_dim`` 64 or 128."""
+    power of two from 16 to 1024; ``head_dim`` 64 or 128. The calls take ``head_dim`` from the rows they are given: a pool made for
+    128 and used with 64 is not told from one of twice the page size."""
     _expect(head_dim in (64, 128), "head_dim must be 64 or 128")
     _expect(16 <= page_size <= 1024 and page_size & (page_size - 1) == 0, "page_size must be a power of two from 16 to 1024")
     _expect(num_pages > 0 and kv_heads > 0 and (layers is None or layers > 0), "bad pool shape")
@@ -656,7 +659,7 @@ def kv4_append(k: torch.Tensor, v: torch.Tensor, pages: torch.Tensor, block_tabl
     become the last ones of ``lengths[s]`` positions (``cu`` int32 ``[sequences + 1]``; without it, one token for each
     sequence). A page that receives tokens must belong to one sequence alone."""
     device = pages.device
-    cache = _kv4_args(pages, block_table, lengths, k.shape[-1], device)
+    cache = _kv4_args(pages, block_table, lengths, k.shape[-1] if k.dim() else 0, device)
     rows = _kv4_rows(k, v, cache[2], cache[3], device)
     tokens, sequences = rows[-1], cache[-1]
     if cu is None:
@@ -755,10 +758,10 @@ def kv4_copy_pages(pages: torch.Tensor, src: list[int], dst: list[int]) -> None:
     if count == 0:
         return
     *layers, num_pages, kv_heads, _, half = pages.shape
-    ids = ctypes.c_int64 * count
     try:
-        sources, targets = ids(*src), ids(*dst)
-    except TypeError as error:
+        sources, targets = array.array("q", src), array.array("q", dst)
+    except (TypeError, OverflowError) as error:
         raise TexelatorError("src and dst must be integers") from error
-    check(_lib.load().tx_kv4_copy_pages(pages.data_ptr(), layers[0] if layers else 1, num_pages, kv_heads * 2 * half, sources,
-                                        targets, count, pages.device.index, _stream(pages)))
+    check(_lib.load().tx_kv4_copy_pages(pages.data_ptr(), layers[0] if layers else 1, num_pages, kv_heads * 2 * half,
+                                        sources.buffer_info()[0], targets.buffer_info()[0], count, pages.device.index,
+                                        _stream(pages)))
