@@ -376,6 +376,8 @@ def test_copies_of_pages(ext, layer_count, num_pages, kv_heads, dim, page, copie
         layers.kv4_copy_pages(pages, [0, 1], [1])
     with pytest.raises(_lib.TexelatorError, match="integers"):
         layers.kv4_copy_pages(pages, [0.5], [1])
+    with pytest.raises(_lib.TexelatorError, match="integers"):
+        layers.kv4_copy_pages(pages, bytes(8), bytes(range(8)))
     layers.kv4_copy_pages(pages, np.array([src[0]]), torch.tensor([dst[0]]))  # integers of other kinds
     assert torch.equal(pages.cpu(), want)
 

@@ -140,6 +140,16 @@ def test_views_that_agree_with_the_packed_call(ext):
     assert torch.equal(wide[:, :, 4:68], want) and (wide[:, :, :4] == 9).all() and (wide[:, :, 68:] == 9).all()
 
 
+def test_heads_farther_apart_than_rows_may_be(ext):
+    """Keys and values with the heads first: 2^24 elements and more between a token's heads."""
+    keys = (1 << 24) // 128 + 100
+    q, k, v = inputs([40], [keys - 40], 4, 2, 128, BF16, 17)
+    k, v = k.contiguous(), v.contiguous()
+    want = run(q, k, v, [40], [keys - 40], 0.1)
+    first = [t.transpose(0, 1).contiguous().transpose(0, 1) for t in (k, v)]
+    assert first[0].stride(1) > 1 << 24 and torch.equal(run(q, *first, [40], [keys - 40], 0.1), want)
+
+
 def test_sequence_starts_outside_the_rows(ext):
     """cu is data: starts past the arrays, below zero or falling are cut to them; nothing outside is written."""
     q, k, v = inputs([100], [0], 4, 2, 128, BF16, 9)

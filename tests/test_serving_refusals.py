@@ -44,7 +44,7 @@ REFUSED = [
     *(packed(**c) for c in [
         dict(q=None), dict(k=None), dict(v=None), dict(out=None), dict(cu_q=None), dict(cu_k=None), dict(dtype=2), dict(head_dim=96),
         dict(heads=15), dict(heads=0), dict(kv_heads=0), dict(sequences=-1), dict(sequences=65536), dict(total_q=-1), dict(total_k=-1),
-        dict(total_q=(1 << 28) + 1), dict(total_q=1 << 28, heads=1024), dict(q=P + 2), dict(k=P + 8), dict(v=P + 4), dict(q_token=2052),
+        dict(total_q=(1 << 28) + 1), dict(total_q=1 << 28, heads=1024), dict(sequences=65535, heads=512), dict(q=P + 2), dict(k=P + 8), dict(v=P + 4), dict(q_token=2052),
         dict(k_token=260), dict(v_head=4), dict(q_head=-128), dict(k_token=1 << 25), dict(k_token=64), dict(v_token=0), dict(out=P + 4),
         dict(out_token=2049), dict(out_head=2), dict(cu_q=P + 2), dict(cu_k=P + 1)]),
     *(rows(name, **c) for name in ("tx_kv4_append", "tx_kv4_read") for c in [
@@ -53,7 +53,7 @@ REFUSED = [
     *(attend(**c) for c in [
         *POOL_FAULTS, dict(q=None), dict(out=None), dict(workspace=None, max_pages=500), dict(dtype=2), dict(heads=15), dict(heads=0), dict(q=P + 8),
         dict(q_head=60), dict(q_sequence=4), dict(out=P + 4), dict(out_head=2), dict(workspace=P + 8), dict(workspace_bytes=64, max_pages=500),
-        dict(max_pages=1 << 24, sequences=4096, kv_heads=16)]),
+        dict(max_pages=1 << 24, sequences=4096, kv_heads=16), dict(max_pages=1, sequences=32768, kv_heads=512, heads=512)]),
 ]
 
 

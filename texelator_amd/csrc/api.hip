@@ -1598,17 +1598,19 @@ int tx_packed_attention(const void *q, int64_t q_token, int64_t q_head, const vo
                         void *out, int64_t out_token, int64_t out_head, int device, void *stream) {
   g_last_error.clear();
   const char *bad = nullptr;
-  auto row = [](int64_t stride) { return stride >= 0 && stride <= (1 << 24) && stride % 8 == 0; };
+  auto row = [](int64_t stride) { return stride >= 0 && stride % 8 == 0; };
   if (!q || !out || !cu_q || !cu_k || (total_k > 0 && (!k || !v))) bad = "null pointer";
   else if (dtype != TX_DTYPE_F16 && dtype != TX_DTYPE_BF16) bad = "q, k and v must be FP16 or BF16";
   else if (head_dim != 64 && head_dim != 128) bad = "head_dim must be 64 or 128";
   else if (kv_heads <= 0 || heads <= 0 || heads > 65535 || heads % kv_heads) bad = "heads must be a multiple of kv_heads";
   else if (sequences < 0 || sequences > 65535 || total_q < 0 || total_k < 0 || total_q > 1 << 28 || total_k > 1 << 28)
     bad = "bad sequence or token count";
-  else if ((total_q / 32 + sequences) * heads > 0x7FFFFFFF) bad = "the grid exceeds the launch limit";
+  else if ((total_q / 128 + sequences) * heads >= 1 << 24) bad = "the grid exceeds the launch limit";  // of 2^32 threads
   else if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) % 16 || !row(q_token) ||
            !row(q_head) || !row(k_token) || !row(k_head) || !row(v_token) || !row(v_head))
     bad = "every row of q, k and v must be 16-byte aligned";
+  // Offsets within a block of keys are 32-bit.
+  else if (k_token > 1 << 24 || v_token > 1 << 24) bad = "rows of k and v must follow within 2^24 elements";
   // A row past the last one must lie past the end of its block's descriptor.
   else if (total_k > 1 && (k_token < head_dim || v_token < head_dim)) bad = "rows of k and v must not overlap";
   else if (reinterpret_cast<uintptr_t>(out) % 8 || (out_token | out_head) % 4) bad = "every output row must be 8-byte aligned";

@@ -506,7 +506,10 @@ int64_t most_units(const Kv4Pool &pool, int unit) {
 
 }  // namespace
 
-bool kv4_attention_fits(const Kv4Pool &pool) { return most_units(pool, kUnit<128>) <= (int64_t)1 << 30; }
+// Unit numbers are 32-bit; a launch has fewer than 2^32 threads, 256 for each head.
+bool kv4_attention_fits(const Kv4Pool &pool) {
+  return most_units(pool, kUnit<128>) <= (int64_t)1 << 30 && (int64_t)pool.sequences * pool.kv_heads < (int64_t)1 << 24;
+}
 
 void kv4_attention_plan(Kv4Attention &a, int dim, int cus) {
   const int64_t room = (int64_t)a.pool.max_pages << a.pool.page_shift, heads = (int64_t)a.pool.sequences * a.pool.kv_heads;

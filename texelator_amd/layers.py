@@ -762,6 +762,7 @@ def kv4_copy_pages(pages: torch.Tensor, src: list[int], dst: list[int]) -> None:
         sources, targets = array.array("q", src), array.array("q", dst)
     except (TypeError, OverflowError) as error:
         raise TexelatorError("src and dst must be integers") from error
+    _expect(len(sources) == len(targets) == count, "src and dst must be integers")  # bytes make one of eight
     check(_lib.load().tx_kv4_copy_pages(pages.data_ptr(), layers[0] if layers else 1, num_pages, kv_heads * 2 * half,
                                         sources.buffer_info()[0], targets.buffer_info()[0], count, pages.device.index,
                                         _stream(pages)))
