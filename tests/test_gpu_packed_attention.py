@@ -53,6 +53,7 @@ CASES = [
     ([200, 333, 5], [500, 0, 64], 28, 4),
     ([700, 3, 129], [0, 10, 70], 40, 8),
     ([1400, 70], [0, 5], 40, 8),
+    ([2200, 70], [0, 5], 40, 8),
     ([70, 190, 0, 2, 33], [2000, 31, 300, 900, 1], 40, 8),
     ([3] * 130, [i % 40 for i in range(130)], 4, 4),  # more sequences than lanes
 ]
@@ -109,7 +110,8 @@ def test_keys_behind_a_query_reach_it_in_no_way(ext):
 
 @pytest.mark.parametrize("dtype,dim", [(BF16, 128), (FP16, 64), (FP16, 128), (BF16, 64)])
 @pytest.mark.parametrize("new,old,heads,kv_heads", [([150, 9], [20, 3], 8, 2), ([700, 33], [5, 0], 16, 2), ([50] * 40, [i for i in range(40)], 16, 4),
-                                                    ([1000, 70], [30, 90], 40, 8), ([1400, 70], [0, 5], 40, 8)])
+                                                    ([1000, 70], [30, 90], 40, 8), ([1400, 70], [0, 5], 40, 8),
+                                                    ([2200, 70], [0, 5], 40, 8)])
 def test_values_behind_a_query_reach_it_in_no_way(ext, new, old, heads, kv_heads, dtype, dim):
     """Infinities and NaN among the values: the queries before them, and other columns, are what they were within the bound."""
     q, k, v = inputs(new, old, heads, kv_heads, dim, dtype, 21)

@@ -166,7 +166,7 @@ __device__ __forceinline__ void seen_keys_alone(const PackedAttention &a, const 
     if (KW == 1 || (2 * e + (lane >> 5)) % KW == kw) out[64 * e + lane] = (uint16_t)half2_bits<F16>(o[e] * inv, 0.f);
 }
 
-// Two waves per SIMD, but for <1, 4, 32>, whose four waves have a CU's LDS to themselves.
+// Two waves per SIMD at least, but for <1, 4, 32>, whose four waves have a CU's LDS to themselves (at 128 dimensions).
 template <bool F16, int DIM, int QW, int KW, int KB>
 __global__ __launch_bounds__(64 * QW * KW, QW == 1 ? 1 : 2) void packed_attention_kernel(PackedAttention a) {
   constexpr int kRow = DIM * 2;                 // bytes of a key or value
@@ -508,21 +508,24 @@ hipError_t launch_typed(const PackedAttention &a, hipStream_t stream) {
   //              against 8.1 of <4, 1, 64>, 256 tokens of 16/2 heads 8.5 against 10.1; but 12 prompts of up to 60 tokens at
   //              32/8 heads 12.7 against 6.6, whose chains are short;
   //   <2, 4, 32> likewise: 1024 tokens of 16/2 heads 17.5 against 23.9; but 512 tokens (320 workgroups) 18.8 against 15.5;
-  //   <2, 2, KB> where the longest chain still outlasts the others' work, keys being many: 3000 tokens of 16/2 heads 54 against
-  //              60 of <4, 1, 64>, 3 turns of up to 400 behind up to 6000 keys 60 against 82 (heads of 64: 39 against 62), 2500
-  //              tokens of 16/2 heads of 64 27 against 37; but 2048 tokens (1280 workgroups) 70 against 60, 6 turns of up to 600
-  //              behind up to 1000 of 32/8 (896) 42 against 34, 12 prompts of up to 600 tokens of 28/4 heads of 64 17 against 14.
-  //              The lengths themselves, on the device, decide as much: of 26 shapes that this rule sends here four got
-  //              slower, by 2 to 16%, and 22 faster, by up to 37%;
+  //   <2, 2, KB> where the longest chain still outlasts the others' work. Heads of 64: KB 64 while all workgroups run at
+  //              once (3 turns of up to 400 behind up to 6000 keys 39 against 62 of <4, 1, 64>, 2500 tokens of 16/2 heads 27
+  //              against 37), beyond KB 32, of which a CU holds three and not two (9 turns of up to 777 behind up to 2500 of
+  //              28/4 heads 34.5 against 40 of KB 64 and of <4, 1, 64>, 2048 tokens of 28/4 30 against 34; but 1477 tokens of
+  //              64/8, 1600 workgroups, 30 against 26). Heads of 128: KB 32 and longer chains (3000 tokens of 16/2 heads 54
+  //              against 60, those 3 turns 60 against 82; but 2048 tokens, 1280 workgroups, 70 against 60, and 3 prompts of up
+  //              to 300 tokens 12.6 against 11.5). The lengths themselves, on the device, decide as much: of 13 shapes of 128
+  //              that the rule sends here three got slower, by 2 to 16%, ten faster, by up to 27%;
   //   <4, 1, 64> for all else: 1024 tokens 28.1 against 34.2 of <2, 4, 32>, 8190 tokens 650 against 756 of <2, 2, 32>.
   const int64_t tiles32 = (a.total_q + (int64_t)31 * a.sequences) / 32 * a.heads,
                 tiles64 = (a.total_q + (int64_t)63 * a.sequences) / 64 * a.heads;
   const bool some_keys = a.total_k >= (int64_t)96 * a.sequences, many_keys = a.total_k >= (int64_t)256 * a.sequences;
   if (tiles32 <= a.cus && some_keys) launch(packed_attention_kernel<F16, DIM, 1, 4, 32>, 32, 4);
   else if (tiles64 <= a.cus && some_keys) launch(packed_attention_kernel<F16, DIM, 2, 4, 32>, 64, 8);
-  else if (2 * tiles64 < (DIM == 64 ? 7 : 6) * (int64_t)a.cus && many_keys)
-    launch(packed_attention_kernel<F16, DIM, 2, 2, DIM == 64 ? 64 : 32>, 64, 4);
-  else launch(packed_attention_kernel<F16, DIM, 4, 1, 64>, 128, 4);
+  else if (DIM == 64 ? tiles64 <= 5 * (int64_t)a.cus && some_keys : tiles64 < 3 * (int64_t)a.cus && many_keys) {
+    if (DIM == 64 && 2 * tiles64 <= 5 * (int64_t)a.cus) launch(packed_attention_kernel<F16, DIM, 2, 2, DIM == 64 ? 64 : 32>, 64, 4);
+    else launch(packed_attention_kernel<F16, DIM, 2, 2, 32>, 64, 4);
+  } else launch(packed_attention_kernel<F16, DIM, 4, 1, 64>, 128, 4);
   return hipGetLastError();
 }
 
