@@ -592,7 +592,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     else:
         _expect_ints("cu_k", cu_k, sequences + 1, device)
     if out is None:
-        out = torch.empty(shape, dtype=dtype, device=device)
+        out = q.new_empty(shape)
     else:
         _expect_rows("out", out, q, heads, dim)
         _expect(out.shape[0] == total, "out must be shaped like q")
@@ -727,7 +727,7 @@ def kv4_attention(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tenso
     _expect(cache[-1] == sequences and heads > 0 and heads % cache[2] == 0,
             "q must have a row for each sequence and a multiple of the pages' heads")
     if out is None:
-        out = torch.empty(shape, dtype=q.dtype, device=device)
+        out = q.new_empty(shape)
     else:
         _expect_rows("out", out, q, heads, dim)
         _expect(out.shape[0] == sequences, "out must be shaped like q")
