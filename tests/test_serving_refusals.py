@@ -5,6 +5,7 @@ import ctypes
 
 import pytest
 import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
 
 from texelator_amd import _lib, layers
 
@@ -115,3 +116,15 @@ def test_tensors_are_checked():
                  lambda: layers.packed_attention(k, k, k, lengths, 1.0)):
         with pytest.raises(_lib.TexelatorError, match="CUDA"):
             call()
+
+
+@pytest.mark.parametrize("shape", [(4, 2, 1, 544), (3, 4, 2, 1, 544), (4, 2, 3, 544), (2, 2, 544), (1, 3, 4, 2, 2, 544)])
+def test_copies_in_pools_of_another_shape_are_refused(shape, monkeypatch):
+    """The bytes of a page follow from the shape, so one without keys and values both never reaches the native call."""
+    calls = []
+    monkeypatch.setattr(_lib, "load", lambda: calls.append(shape))
+    with FakeTensorMode():
+        pages = torch.empty(shape, dtype=torch.uint8, device="cuda:0")
+    with pytest.raises(_lib.TexelatorError, match="kv_heads, 2, page bytes"):
+        layers.kv4_copy_pages(pages, [0], [1])
+    assert not calls

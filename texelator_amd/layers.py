@@ -751,7 +751,8 @@ def kv4_copy_pages(pages: torch.Tensor, src: list[int], dst: list[int]) -> None:
     ``[layers, ...]`` at once: a fork copies the last, partly filled page, a compaction moves pages and frees theirs.
     ``src`` and ``dst`` are host integers (a captured call repeats the copies it was captured with). All copies happen at once:
     a page that is copied to twice, or both copied from and copied to, is refused."""
-    _expect(pages.is_cuda and pages.dtype == torch.uint8 and pages.dim() in (4, 5) and pages.is_contiguous(),
+    # The page's bytes follow from its keys and values both: a pool of one of them would be left past its end.
+    _expect(pages.is_cuda and pages.dtype == torch.uint8 and pages.dim() in (4, 5) and pages.shape[-2] == 2 and pages.is_contiguous(),
             "pages must be contiguous CUDA uint8 [num_pages, kv_heads, 2, page bytes], layers before it or not")
     count = len(src)
     _expect(len(dst) == count, "src and dst must have as many pages")
