@@ -131,6 +131,33 @@ def test_values_behind_a_query_reach_it_in_no_way(ext, new, old, heads, kv_heads
     assert_within(torch.where(struck, 0, got), want.masked_fill(struck, 0), bound)
 
 
+@pytest.mark.parametrize("dtype,dim", [(BF16, 128), (FP16, 64), (FP16, 128), (BF16, 64)])
+@pytest.mark.parametrize("new,old,heads,kv_heads", [([300, 40], [30, 0], 8, 2), ([60, 90], [-20, 10], 8, 2), ([700, 33], [5, 0], 16, 2),
+                                                    ([1000, 70], [30, 90], 28, 4), ([1000, 70], [30, 90], 40, 8),
+                                                    ([50] * 40, [i for i in range(40)], 16, 4), ([2200, 70], [0, 5], 40, 8)])
+def test_scores_of_minus_infinity(ext, new, old, heads, kv_heads, dtype, dim):
+    """Two thirds of each sequence's keys score -infinity: a query that sees no others has no softmax and gets NaN, later ones
+    are what the other keys make them, and one that sees no key at all still gets zeros."""
+    q, k, v = inputs(new, old, heads, kv_heads, dim, dtype, 23)
+    scale, group = dim ** -0.5, heads // kv_heads
+    q[:, :, 3] = q[:, :, 3].abs() + 0.1
+    want, bound = reference(q, k, v, new, old, scale)
+    undefined = torch.zeros(sum(new), heads, dtype=torch.bool, device="cuda")
+    q0 = k0 = 0
+    for n, o in zip(new, old):
+        struck = (n + o) * 2 // 3
+        k[k0:k0 + struck, 0, 3] = float("-inf")
+        first, blind = max(0, struck - o), max(0, -o)  # the first query with a finite score, the queries without a key
+        undefined[q0 + blind:q0 + first, :group] = True
+        for h in range(group):
+            want[q0 + first:q0 + n, h], bound[q0 + first:q0 + n, h] = attention64(
+                q[q0 + first:q0 + n, h], k[k0 + struck:k0 + n + o, 0], v[k0 + struck:k0 + n + o, 0], scale, first + o - struck)
+        q0, k0 = q0 + n, k0 + n + o
+    got = run(q, k, v, new, old, scale)
+    assert torch.isnan(got[undefined]).all() and undefined.any()
+    assert_within(got.masked_fill(undefined[..., None], 0), want.masked_fill(undefined[..., None], 0), bound)
+
+
 def test_views_that_agree_with_the_packed_call(ext):
     """The same rows at other strides and offsets, and an output with gaps, give the same bits."""
     new, old = [130, 40], [3, 60]

@@ -160,7 +160,7 @@ __device__ __forceinline__ void seen_keys_alone(const PackedAttention &a, const 
       for (int e = 0; e < DIM / 64; ++e) o[e] = __builtin_fmaf(p, half_bits_to_float<F16>(v[(k0 + j) * a.v_token + 64 * e + lane]), o[e]);
     }
   }
-  const float inv = l == 0.f ? 0.f : 1.0f / l;
+  const float inv = limit < 0 ? 0.f : 1.0f / l;
 #pragma unroll
   for (int e = 0; e < DIM / 64; ++e)
     if (KW == 1 || (2 * e + (lane >> 5)) % KW == kw) out[64 * e + lane] = (uint16_t)half2_bits<F16>(o[e] * inv, 0.f);
@@ -477,7 +477,8 @@ __global__ __launch_bounds__(64 * QW * KW, QW == 1 ? 1 : 2) void packed_attentio
   const uint64_t odd = __builtin_amdgcn_ballot_w64(query < queries && __builtin_isnan(probe));
   uint32_t again = (uint32_t)(odd | odd >> 32);
   if (again != 0 && !unseen_odd_value<F16, DIM>(a, vg, max(q0 + shift + 1, 0), min(reach | 31, keys - 1), lane)) again = 0;
-  const float inv = l == 0.f ? 0.f : 1.0f / l;
+  // A query that sees no key gets zeros; one whose scores are all -infinity has l = 0 and O = 0 as well, and gets NaN.
+  const float inv = limit < 0 ? 0.f : 1.0f / l;
   uint16_t *dst = a.out + (qs.begin + query) * a.out_token + head * a.out_head + 4 * h;
   if (query < queries && !(again >> n & 1)) {
 #pragma unroll
