@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from oracle import mxfp4
-from tests.serving import Cache, assert_within, cumulative, half_values, i32
+from tests.serving import Cache, assert_within, attention64, cumulative, half_values, i32
 from texelator_amd import _lib, layers
 
 pytestmark = pytest.mark.gpu
@@ -253,6 +253,48 @@ def test_a_nan_reaches_its_own_sequence_and_head_alone(ext, dtype):
     got = layers.kv4_attention(q, cache.pages, cache.table, cache.lengths, 0.1)
     assert torch.equal(got[0], want[0]) and torch.equal(got[2], want[2])
     assert torch.isnan(got[1, :2]).all() and torch.isnan(got[1, 2:, 96:]).all() and torch.equal(got[1, 2:, :96], want[1, 2:, :96])
+
+
+@pytest.mark.parametrize("lengths,heads,kv_heads,dim,page", [([30, 7, 0, 90], 8, 2, 64, 16), ([700, 1, 0, 1024], 16, 2, 128, 64),
+                                                             ([20000, 40, 0, 3000], 5, 1, 128, 128), ([3000, 8, 0, 9000], 8, 2, 64, 32)])
+def test_scores_of_minus_infinity(ext, lengths, heads, kv_heads, dim, page):
+    """Two thirds of sequence 0's positions and all of sequence 1's score -infinity for KV head 0: the first is what its other positions make
+    it, the second has no softmax and gets NaN, the others and a sequence without any position in the pool are what they were."""
+    sequences, scale, group = len(lengths), dim ** -0.5, heads // kv_heads
+    g = torch.Generator().manual_seed(31)
+    x = torch.randn(sum(lengths), 2, kv_heads, dim, generator=g).to(BF16)
+    starts, struck = [sum(lengths[:s]) for s in range(sequences)], lengths[0] * 2 // 3
+    low = torch.zeros(32)
+    low[3] = -2.0 ** 100
+    x[:lengths[0], 0, 0, :32] = 0   # these and the query's 2^100 make 0 or -2^200
+    x[:struck, 0, 0, :32] = low.to(BF16)
+    x[starts[1]:starts[2], 0, 0, :32] = low.to(BF16)
+    q = torch.randn(sequences, heads, dim, generator=g).to(BF16)
+    q[:2, :group, 3] = 2.0 ** 100
+    counts = [-(-n // page) for n in lengths]
+    table = torch.full((sequences + 1, max(counts)), -1, dtype=torch.int32)
+    for s, n in enumerate(counts):
+        table[s, :n] = torch.arange(sum(counts[:s]), sum(counts[:s]) + n)
+    pages, table, positions = layers.kv4_pages(sum(counts), kv_heads, dim, page), table.cuda(), i32([*lengths, 50])
+    gpu = x.cuda()
+    layers.kv4_append(gpu[:, 0], gpu[:, 1], pages, table[:-1], positions[:-1], cu=cumulative(lengths))
+    q = torch.cat([q, q[:1]]).cuda()  # the last sequence has positions, but no page
+    got = layers.kv4_attention(q, pages, table, positions, scale)
+    values = torch.from_numpy(mxfp4.dequantize(*mxfp4.quantize(x.float().numpy()))).cuda()
+    for s, n in enumerate(lengths):
+        for h in range(heads):
+            first = struck if s == 0 and h < group else 0
+            if s == 1 and h < group:
+                assert torch.isnan(got[s, h]).all()
+                continue
+            seen = slice(starts[s] + first, starts[s] + n)
+            k, v = values[seen, 0, h // group], values[seen, 1, h // group]
+            query = q[s, h][None]
+            if s == 0 and h < group:
+                query = query.clone()
+                query[:, :32] = 0  # as these keys are
+            assert_within(got[s, h][None], *attention64(query, k, v, scale, n - first - 1))
+    assert not got[sequences].any()
 
 
 def test_workspace_is_of_the_stated_size_and_needs_no_clearing(ext):

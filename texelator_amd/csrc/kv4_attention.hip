@@ -123,6 +123,19 @@ __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(
 // Floats of a piece: per query its output [dim], then max and sum of all queries.
 __device__ __host__ inline int64_t piece_floats(int group, int dim) { return (int64_t)group * (dim + 2); }
 
+// Whether any position of a sequence lies in the pool, by LANES lanes that ask together. Asked only where no score was above
+// -infinity, to tell zeros (no position) from a softmax that is undefined (NaN): carried along with the maxima it cost 1% at dim 64.
+template <int LANES>
+__device__ __forceinline__ bool any_position(const Kv4Pool &pool, int sequence, int length) {
+  const int lane = threadIdx.x % LANES;
+  for (int64_t first = 0; first << pool.page_shift < length; first += LANES) {
+    const bool inside = (first + lane) << pool.page_shift < length;
+    const bool known = inside && (uint32_t)pool.table[sequence * pool.table_stride + first + lane] < (uint64_t)pool.num_pages;
+    if (LANES == 1 ? known : __builtin_amdgcn_ballot_w64(known) != 0) return true;
+  }
+  return false;
+}
+
 // SHARE: 16-position groups of a step that lie in one page: a page's, or all of the step's.
 template <bool F16, int DIM, int SHARE>
 __global__ __launch_bounds__(64 * kWaves, kResident<DIM>) void kv4_attention_kernel(Kv4Attention a) {
@@ -375,8 +388,8 @@ __global__ __launch_bounds__(64 * kWaves, kResident<DIM>) void kv4_attention_ker
     const Part after = take();
     begin(after);
 
-    // The waves' shares meet in LDS. M is -infinity where no position counted: then l = 0 and O = 0 everywhere (or NaN,
-    // where all scores were).
+    // The waves' shares meet in LDS. M is -infinity where no position counted or no score was above it: then l = 0 and O = 0
+    // everywhere (or NaN, where scores were).
     l = quarters_sum(l);
     if (quarter == 0) {
       stats[wave][0][n] = m;
@@ -407,7 +420,8 @@ __global__ __launch_bounds__(64 * kWaves, kResident<DIM>) void kv4_attention_ker
       for (int w = 0; w < kWaves; ++w)
         ll += stats[w][0][q] == -INFINITY ? stats[w][1][q] : stats[w][1][q] * __builtin_amdgcn_exp2f((stats[w][0][q] - mm) * sl2);
       if (complete) {
-        const float inverse = ll == 0.f ? 0.f : 1.f / ll;
+        // A lane each: a head that one workgroup has to itself has few pages.
+        const float inverse = mm == -INFINITY && !any_position<1>(pool, part.sequence, part.length) ? 0.f : 1.f / ll;
         uint16_t *out = a.out + part.sequence * a.out_sequence + (part.head * a.group + col0 + q) * a.out_head + d;
         const uint32_t lo = to_half_bits<F16>(sum[0] * inverse) | (uint32_t)to_half_bits<F16>(sum[1] * inverse) << 16;
         const uint32_t hi = to_half_bits<F16>(sum[2] * inverse) | (uint32_t)to_half_bits<F16>(sum[3] * inverse) << 16;
@@ -480,6 +494,7 @@ __global__ __launch_bounds__(256) void kv4_combine_kernel(Kv4Attention a) {
   if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
   __syncthreads();
   top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+  const bool none = top == -INFINITY && !any_position<64>(pool, sequence, place.length);
   const float weight = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - top) * a.sl2);
   lds[group][lane] = sum * weight;
   if (lane == 0) sums[group] = l * weight;
@@ -493,7 +508,7 @@ __global__ __launch_bounds__(256) void kv4_combine_kernel(Kv4Attention a) {
       ll += sums[g];
     }
     a.out[sequence * a.out_sequence + (head * a.group + q) * a.out_head + 4 * kLanes * blockIdx.z + threadIdx.x] =
-        to_half_bits<F16>(ll == 0.f ? 0.f : total / ll);
+        to_half_bits<F16>(none ? 0.f : total / ll);
   }
 }
 
