@@ -158,6 +158,27 @@ def test_scores_of_minus_infinity(ext, new, old, heads, kv_heads, dtype, dim):
     assert_within(got.masked_fill(undefined[..., None], 0), want.masked_fill(undefined[..., None], 0), bound)
 
 
+@pytest.mark.parametrize("dtype,dim", [(BF16, 128), (FP16, 64), (FP16, 128), (BF16, 64)])
+@pytest.mark.parametrize("new,old,heads,kv_heads", [([300, 40], [30, 0], 8, 2), ([700, 33], [5, 0], 16, 2), ([1000, 70], [30, 90], 28, 4),
+                                                    ([1000, 70], [30, 90], 40, 8), ([50] * 40, [i for i in range(40)], 16, 4),
+                                                    ([2200, 70], [0, 5], 40, 8), ([100], [9000], 8, 2)])
+def test_the_largest_values(ext, new, old, heads, kv_heads, dtype, dim):
+    """Values of the type's largest magnitude, all of one sign or of both, give finite averages, also to the queries that are
+    computed again because the last key's value is infinite."""
+    q, k, v = inputs(new, old, heads, kv_heads, dim, dtype, 29)
+    v.copy_(torch.where(v > 0, torch.finfo(dtype).max, -torch.finfo(dtype).max))
+    v[..., dim // 2:] = torch.finfo(dtype).max
+    want, bound = reference(q, k, v, new, old, dim ** -0.5)
+    assert_within(run(q, k, v, new, old, dim ** -0.5), want, bound)
+    ends = torch.tensor(new).cumsum(0) - 1
+    v[(torch.tensor(new) + torch.tensor(old)).cumsum(0) - 1, 0, 5] = float("inf")
+    got = run(q, k, v, new, old, dim ** -0.5)
+    group = heads // kv_heads
+    assert not torch.isfinite(got[ends, :group, 5]).any()
+    got[ends, :group, 5] = want[ends, :group, 5].to(dtype)
+    assert_within(got, want, bound)
+
+
 def test_views_that_agree_with_the_packed_call(ext):
     """The same rows at other strides and offsets, and an output with gaps, give the same bits."""
     new, old = [130, 40], [3, 60]

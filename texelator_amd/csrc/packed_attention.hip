@@ -21,7 +21,9 @@
 //     the sequence's last row, rows past it read as zeros. 16-byte chunks of a row are permuted by its number so
 //     that operand reads hit distinct banks; the values' transpose is done by the read (ds_read_b64_tr_b16).
 // Online softmax in fp32 with exp2; the sum runs over the probabilities as rounded. In fp16 they are held times 2^11, so
-// that small ones keep their bits and large ones (2^4 more while a maximum lags) stay below fp16's largest.
+// that small ones keep their bits and large ones (2^4 more while a maximum lags) stay below fp16's largest; in bf16 times a power
+// of two below 1 / (2^4 keys), so that sums of the type's largest values stay finite (in turn values below 2^-110, at 8190 keys, lose
+// bits to fp32's smallest; held unscaled, sums of values above 2^111 overflowed).
 //
 // Bound: power. At 8190 tokens and 40/8 heads 1.23 M cycles a SIMD at 1.9 GHz, 655 us (1050 TFLOP/s; a plain 16384^3 product
 // of the library reaches 1370); the same instructions on zeros run at 2.4 GHz. Two waves a SIMD: vector instructions take 2.6
@@ -105,6 +107,9 @@ __device__ __forceinline__ Rows rows_of(const int *cu, int sequence, int total) 
   return {begin, min(max(cu[sequence + 1], begin), total) - begin};
 }
 
+// Bits of a count: it is below 2^bits.
+__device__ __forceinline__ float bits_of(int count) { return (float)(32 - __builtin_clz(count | 1)); }
+
 // Whether values of the rows first .. last hold an infinity or a NaN: asked by a whole wave.
 template <bool F16, int DIM>
 __device__ __forceinline__ bool unseen_odd_value(const PackedAttention &a, const char *vg, int first, int last, int lane) {
@@ -146,7 +151,7 @@ __device__ __forceinline__ void seen_keys_alone(const PackedAttention &a, const 
   for (int k0 = 0; k0 <= limit; k0 += 64) m = fmaxf(m, score(k0 + lane));
 #pragma unroll
   for (int w = 1; w < 64; w *= 2) m = fmaxf(m, __shfl_xor(m, w));
-  const float base = m == -INFINITY ? 0.f : -m * a.sl2;
+  const float base = m == -INFINITY ? 0.f : -bits_of(limit + 1) - m * a.sl2;  // the sum of the largest values stays finite
   float l = 0.f, o[DIM / 64] = {};
 #pragma unroll 1
   for (int k0 = 0; k0 <= limit; k0 += 64) {
@@ -177,7 +182,6 @@ __global__ __launch_bounds__(64 * QW * KW, QW == 1 ? 1 : 2) void packed_attentio
   constexpr int kLoadRows = 64 / kChunks;       // rows of a 1 KiB load
   constexpr int kPer = kSub / 1024 / QW;        // loads of this wave for 32 rows
   constexpr int kSteps = DIM / 16, kOut = DIM / 32;
-  constexpr float kLift = F16 ? 15.f - kPackedLag : 0.f;
   static_assert(kPer * QW * 1024 == kSub, "loads divide among the waves");
   // Two buffers of each, separate LDS objects: the compiler then knows that reads of one do not wait for the direct
   // loads that fill the other.
@@ -224,6 +228,7 @@ __global__ __launch_bounds__(64 * QW * KW, QW == 1 ? 1 : 2) void packed_attentio
   const Rows qs = rows_at(lane_q, a.cu_q, a.total_q), ks = rows_at(lane_k, a.cu_k, a.total_k);
   const int queries = qs.count, keys = ks.count;
   const int shift = keys - queries;      // query i sees the keys up to i + shift
+  const float lift = F16 ? 15.f - kPackedLag : -kPackedLag - 1.f - bits_of(keys);  // probabilities are held times 2^lift
   const int q0 = tile * kQueries + qw * 32;  // this wave's first query
 
   // q as MFMA B operands: column n = query q0 + n (clamped into the sequence), dimensions 16 st + 8 h ...
@@ -313,7 +318,7 @@ __global__ __launch_bounds__(64 * QW * KW, QW == 1 ? 1 : 2) void packed_attentio
     __builtin_amdgcn_sched_barrier(0);
   };
   auto step = [&](const f32x16 &cur, f32x16 &next, const char *vt, const char *kt_next, u32x4 x, u32x4 y) __attribute__((always_inline)) {
-    const float base = m == -INFINITY ? 0.f : kLift - m * a.sl2;  // no key yet: every score is -infinity
+    const float base = m == -INFINITY ? 0.f : lift - m * a.sl2;  // no key yet: every score is -infinity
     uint32_t pb[8];
     auto pair = [&](int p) __attribute__((always_inline)) {  // probabilities 2 p and 2 p + 1
       pb[p] = pack2<F16>(__builtin_amdgcn_exp2f(__builtin_fmaf(cur[2 * p], a.sl2, base)),
