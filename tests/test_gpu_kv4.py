@@ -297,6 +297,32 @@ def test_scores_of_minus_infinity(ext, lengths, heads, kv_heads, dim, page):
     assert not got[sequences].any()
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("lengths,heads,kv_heads,dim,page", [([30, 7, 0, 90], 8, 2, 64, 16), ([700, 1, 0, 1024], 16, 2, 128, 64),
+                                                             ([20000, 40, 0, 3000], 5, 1, 128, 128), ([3000, 8, 0, 9000], 8, 2, 64, 32)])
+def test_the_largest_values(ext, lengths, heads, kv_heads, dim, page, dtype):
+    """Values of the largest magnitude that a cache of the type holds, all of one sign or of both, give finite averages."""
+    g = torch.Generator().manual_seed(37)
+    x = torch.randn(sum(lengths), 2, kv_heads, dim, generator=g).to(dtype)
+    largest = 6 * 2.0 ** (125 if dtype == BF16 else 13)
+    x[:, 1] = torch.where(x[:, 1] > 0, largest, -largest)
+    x[:, 1, :, dim // 2:] = largest
+    counts = [-(-n // page) for n in lengths]
+    table = torch.full((len(lengths), max(counts)), -1, dtype=torch.int32)
+    for s, n in enumerate(counts):
+        table[s, :n] = torch.arange(sum(counts[:s]), sum(counts[:s]) + n)
+    pages, table, gpu = layers.kv4_pages(sum(counts), kv_heads, dim, page), table.cuda(), x.cuda()
+    layers.kv4_append(gpu[:, 0], gpu[:, 1], pages, table, i32(lengths), cu=cumulative(lengths))
+    q = torch.randn(len(lengths), heads, dim, generator=g).to(dtype).cuda()
+    got = layers.kv4_attention(q, pages, table, i32(lengths), dim ** -0.5)
+    values = torch.from_numpy(mxfp4.dequantize(*mxfp4.quantize(x.float().numpy()))).cuda()
+    assert torch.equal(values[:, 1].cpu(), x[:, 1].double())
+    for s, n in enumerate(lengths):
+        for h in range(heads):
+            k, v = (values[sum(lengths[:s]):sum(lengths[:s + 1]), i, h // (heads // kv_heads)] for i in (0, 1))
+            assert_within(got[s, h][None], *attention64(q[s, h][None], k, v, dim ** -0.5, n - 1))
+
+
 def test_workspace_is_of_the_stated_size_and_needs_no_clearing(ext):
     cache = Cache([5000, 17, 900], 2, 128, 64, 9)
     q = torch.randn(3, 10, 128).to(BF16).cuda()
