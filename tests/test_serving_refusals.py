@@ -128,3 +128,19 @@ def test_copies_in_pools_of_another_shape_are_refused(shape, monkeypatch):
     with pytest.raises(_lib.TexelatorError, match="kv_heads, 2, page bytes"):
         layers.kv4_copy_pages(pages, [0], [1])
     assert not calls
+
+
+@pytest.mark.parametrize("head_dim", [64, 128])
+@pytest.mark.parametrize("group", range(1, 18))
+def test_pieces_of_the_workspace_are_whole_vectors(head_dim, group):
+    """Partial results, two for each workgroup, are accessed 16 bytes at a time: each begins on 16 bytes, with room for a query's output,
+    maximum and sum."""
+    lib, sizes = _lib.load(), []
+    for heads in (4, group):  # of groups of four the size is exact: 4 (head_dim + 2) floats a piece
+        size = ctypes.c_int64()
+        assert lib.tx_kv4_attention_workspace(3, heads, 1, head_dim, 64, 500, 0, size) == _lib.TX_OK
+        sizes.append(size.value)
+    pieces, rest = divmod(sizes[0], 4 * (head_dim + 2) * 4)
+    assert rest == 0 and pieces % 2 == 0 and pieces > 0
+    piece, rest = divmod(sizes[1], pieces)
+    assert rest == 0 and piece % 16 == 0 and 0 <= piece - group * (head_dim + 2) * 4 < 16

@@ -40,6 +40,7 @@ struct Kv4Attention {
   uint32_t q_and, q_xor;
   float *pieces;        // results of heads that several workgroups share
   int64_t piece_bytes;  // bytes of them
+  int piece_floats;     // of each: per query its output [dim], then max and sum of all queries; whole vectors of four
   int workgroups;
   bool whole;  // a workgroup for each head: no pieces
 };

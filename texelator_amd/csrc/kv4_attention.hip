@@ -121,9 +121,6 @@ __device__ __forceinline__ int run_units(int total, const Kv4Attention &a) {
 // All of the workgroup's LDS accesses so far are done; loads from memory stay in flight.
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-// Floats of a piece: per query its output [dim], then max and sum of all queries.
-__device__ __host__ inline int64_t piece_floats(int group, int dim) { return (int64_t)group * (dim + 2); }
-
 // Whether any position of a sequence lies in the pool, by LANES lanes that ask together. Asked only where no score was above
 // -infinity, to tell zeros (no position) from a softmax that is undefined (NaN): carried along with the maxima it cost 1% at dim 64.
 template <int LANES>
@@ -414,7 +411,7 @@ __global__ __launch_bounds__(64 * kWaves, kResident<DIM>) void kv4_attention_ker
       *reinterpret_cast<f32x4 *>(merge + n * kMergeRow + 16 * t + 4 * quarter) = o[t] * weight;
     lds_barrier();
     const bool complete = part.first == 0 && part.until == part.units;
-    float *piece = a.pieces + ((int64_t)(blockIdx.x * 2 + part.slot)) * piece_floats(a.group, DIM);
+    float *piece = a.pieces + ((int64_t)(blockIdx.x * 2 + part.slot)) * a.piece_floats;
     for (int i = threadIdx.x; i < cols * (DIM / 4); i += 64 * kWaves) {
       const int q = i / (DIM / 4), d = 4 * (i % (DIM / 4));
       f32x4 sum = {0.f, 0.f, 0.f, 0.f};
@@ -467,7 +464,7 @@ __global__ __launch_bounds__(256) void kv4_combine_kernel(Kv4Attention a) {
   const int w0 = work / run, w1 = (work + units - 1) / run;
   if (w0 == w1) return;  // one workgroup had it all and wrote the output
   const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes, d = 4 * (kLanes * blockIdx.z + lane);
-  const int64_t floats = piece_floats(a.group, DIM), stats_at = (int64_t)a.group * DIM + 2 * q;
+  const int64_t floats = a.piece_floats, stats_at = (int64_t)a.group * DIM + 2 * q;
   // Only the first workgroup can have had another head before this one.
   auto piece = [&](int w) { return a.pieces + ((int64_t)w * 2 + (w == w0 && begin > w0 * run ? 1 : 0)) * floats; };
   // Each thread keeps its own running maximum over its pieces; the threads' sums meet under the largest.
@@ -543,7 +540,8 @@ void kv4_attention_plan(Kv4Attention &a, int dim, int cus) {
   const int64_t most = most_units(a.pool, dim == 128 ? kUnit<128> : kUnit<64>);
   const int64_t fill = (dim == 128 ? kResident<128> : kResident<64>) * (int64_t)cus;
   a.workgroups = (int)(a.whole ? heads : most < fill ? most : fill);
-  a.piece_bytes = a.whole ? 0 : (int64_t)a.workgroups * 2 * piece_floats(a.group, dim) * (int64_t)sizeof(float);
+  a.piece_floats = (a.group * (dim + 2) + 3) & ~3;
+  a.piece_bytes = a.whole ? 0 : (int64_t)a.workgroups * 2 * a.piece_floats * (int64_t)sizeof(float);
 }
 
 hipError_t launch_kv4_attention(const Kv4Attention &a, bool f16, int dim, hipStream_t stream) {
