@@ -223,6 +223,27 @@ def test_strided_queries_outputs_and_tables(ext):
     assert torch.equal(same[2], want[2])
 
 
+@pytest.mark.parametrize("heads", [1, 3])
+def test_strides_of_dimensions_of_one(ext, heads):
+    """One sequence, one head: whatever stride the tensor names there, in every call."""
+    cache = Cache([77], 1, 64, 16, 5, extra_columns=0)
+    g = torch.Generator().manual_seed(3)
+    q, k, v = (torch.randn(1, h, 64, generator=g).to(BF16).cuda() for h in (heads, 1, 1))
+
+    def odd(t):
+        return t.as_strided(t.shape, [s if n > 1 else o for n, s, o in zip(t.shape, t.stride(), (3, 5, 1))])
+
+    pages = cache.pages.clone()
+    layers.kv4_append(k, v, cache.pages, cache.table, cache.lengths)
+    layers.kv4_append(odd(k), odd(v), pages, cache.table.as_strided(cache.table.shape, (7, 1)), cache.lengths)
+    assert torch.equal(pages, cache.pages)
+    want, rows = layers.kv4_attention(q, pages, cache.table, cache.lengths, 0.1), layers.kv4_read(pages, cache.table, cache.lengths, 64)
+    out, back = torch.zeros_like(q), [torch.zeros_like(k) for _ in range(2)]
+    layers.kv4_attention(odd(q), pages, cache.table, cache.lengths, 0.1, out=odd(out))
+    layers.kv4_read(pages, cache.table, cache.lengths, 64, out=tuple(odd(t) for t in back))
+    assert torch.equal(out, want) and want.any() and torch.equal(torch.stack(back), torch.stack(rows)) and back[0].any()
+
+
 def test_pages_outside_the_pool_take_no_part(ext):
     """Unknown page ids are skipped wherever they occur, and lengths past the table or below zero are cut to it."""
     page, dim = 32, 64

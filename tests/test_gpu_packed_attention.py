@@ -190,6 +190,20 @@ def test_views_that_agree_with_the_packed_call(ext):
     assert torch.equal(wide[:, :, 4:68], want) and (wide[:, :, :4] == 9).all() and (wide[:, :, 68:] == 9).all()
 
 
+@pytest.mark.parametrize("old", [0, 40])
+@pytest.mark.parametrize("heads", [1, 4])
+def test_strides_of_dimensions_of_one(ext, heads, old):
+    """One query, one head, one key: whatever stride the tensor names there."""
+    q, k, v = (t.contiguous() for t in inputs([1], [old], heads, 1, 64, BF16, 19))
+    want = run(q, k, v, [1], [old], 0.1)
+    odd = [t.as_strided(t.shape, [s if n > 1 else o for n, s, o in zip(t.shape, t.stride(), (3, 5, 1))]) for t in (q, k, v)]
+    far = [t.as_strided(t.shape, [s if n > 1 else 1 << 40 for n, s in zip(t.shape, t.stride())]) for t in (q, k, v)]
+    for views in (odd, far):
+        out = torch.zeros_like(want)
+        run(*views, [1], [old], 0.1, out=out.as_strided(out.shape, [views[0].stride(0), views[0].stride(1), 1]))
+        assert torch.equal(out, want) and torch.isfinite(want).all() and want.any()
+
+
 def test_heads_farther_apart_than_rows_may_be(ext):
     """Keys and values with the heads first: 2^24 elements and more between a token's heads."""
     keys = (1 << 24) // 128 + 100

@@ -1451,6 +1451,11 @@ const char *kv4_pool(tx::Kv4Pool &pool, const void *pages, int64_t num_pages, in
   return nullptr;
 }
 
+// A dimension of one has no stride: what a tensor names there is neither checked nor used.
+void drop_strides(int64_t size, int64_t &a, int64_t &b) {
+  if (size <= 1) a = b = 0;
+}
+
 const char *kv4_rows(const void *k, int64_t k_token, int64_t k_head, const void *v, int64_t v_token, int64_t v_head,
                      int dtype, int64_t tokens, const int *cu, int sequences) {
   if (!k || !v) return "null pointer";
@@ -1473,6 +1478,8 @@ int tx_kv4_append(const void *k, int64_t k_token, int64_t k_head, const void *v,
   tx::Kv4Pool pool;
   const char *bad = kv4_pool(pool, pages, num_pages, kv_heads, head_dim, page_size, block_table, table_stride, max_pages,
                              lengths, sequences);
+  drop_strides(tokens, k_token, v_token);
+  drop_strides(kv_heads, k_head, v_head);
   if (!bad) bad = kv4_rows(k, k_token, k_head, v, v_token, v_head, dtype, tokens, cu, sequences);
   if (bad) return fail(TX_ERR_INVALID, std::string("kv4_append: ") + bad);
   if (tokens == 0 || sequences == 0) return TX_OK;
@@ -1491,6 +1498,8 @@ int tx_kv4_read(void *k, int64_t k_token, int64_t k_head, void *v, int64_t v_tok
   tx::Kv4Pool pool;
   const char *bad = kv4_pool(pool, pages, num_pages, kv_heads, head_dim, page_size, block_table, table_stride, max_pages,
                              lengths, sequences);
+  drop_strides(tokens, k_token, v_token);
+  drop_strides(kv_heads, k_head, v_head);
   if (!bad) bad = kv4_rows(k, k_token, k_head, v, v_token, v_head, dtype, tokens, cu, sequences);
   if (bad) return fail(TX_ERR_INVALID, std::string("kv4_read: ") + bad);
   if (tokens == 0 || sequences == 0) return TX_OK;
@@ -1525,6 +1534,8 @@ int tx_kv4_attention(const void *q, int64_t q_sequence, int64_t q_head, int dtyp
   tx::Kv4Attention a = {};
   const char *bad = kv4_pool(a.pool, pages, num_pages, kv_heads, head_dim, page_size, block_table, table_stride, max_pages,
                              lengths, sequences);
+  drop_strides(sequences, q_sequence, out_sequence);
+  drop_strides(heads, q_head, out_head);
   if (!bad && (!q || !out)) bad = "null pointer";
   if (!bad && dtype != TX_DTYPE_F16 && dtype != TX_DTYPE_BF16) bad = "q must be FP16 or BF16";
   if (!bad && (heads <= 0 || heads % kv_heads || heads / kv_heads > 65535)) bad = "heads must be a multiple of kv_heads";
@@ -1599,6 +1610,10 @@ int tx_packed_attention(const void *q, int64_t q_token, int64_t q_head, const vo
   g_last_error.clear();
   const char *bad = nullptr;
   auto row = [](int64_t stride) { return stride >= 0 && stride % 8 == 0; };
+  drop_strides(total_q, q_token, out_token);
+  drop_strides(heads, q_head, out_head);
+  drop_strides(kv_heads, k_head, v_head);
+  if (total_k <= 1) k_token = v_token = head_dim;  // a row past the only one has to lie past its end
   if (!q || !out || !cu_q || !cu_k || (total_k > 0 && (!k || !v))) bad = "null pointer";
   else if (dtype != TX_DTYPE_F16 && dtype != TX_DTYPE_BF16) bad = "q, k and v must be FP16 or BF16";
   else if (head_dim != 64 && head_dim != 128) bad = "head_dim must be 64 or 128";
