@@ -144,3 +144,25 @@ def test_pieces_of_the_workspace_are_whole_vectors(head_dim, group):
     assert rest == 0 and pieces % 2 == 0 and pieces > 0
     piece, rest = divmod(sizes[1], pieces)
     assert rest == 0 and piece % 16 == 0 and 0 <= piece - group * (head_dim + 2) * 4 < 16
+
+
+def test_shapes_without_heads_or_of_other_pools_are_refused(monkeypatch):
+    """Pools without KV heads, layered ones, and sizes of rows that no pool has: the error of every other bad argument."""
+    monkeypatch.setattr(_lib, "load", lambda: pytest.fail("reached the native call"))
+    def pool(*shape):
+        with FakeTensorMode():
+            return torch.empty(shape, dtype=torch.uint8, device="cuda:0")
+
+    with FakeTensorMode():
+        table, lengths = (torch.empty(s, dtype=torch.int32, device="cuda:0") for s in ((3, 2), (3,)))
+        q = torch.empty(3, 4, 64, dtype=torch.bfloat16, device="cuda:0")
+    for pages in (pool(4, 0, 2, 544), pool(2, 4, 2, 2, 544), pool(4, 2, 1, 544), pool(4, 2, 2, 545)):
+        with pytest.raises(_lib.TexelatorError, match="pages"):
+            layers.kv4_attention(q, pages, table, lengths, 1.0)
+        with pytest.raises(_lib.TexelatorError, match="pages"):
+            layers.kv4_attention_workspace_bytes(pages, table, 4, 64)
+    for head_dim in (0, 32, 96):
+        with pytest.raises(_lib.TexelatorError, match="head_dim"):
+            layers.kv4_attention_workspace_bytes(pool(4, 2, 2, 544), table, 4, head_dim)
+    with pytest.raises(_lib.TexelatorError, match="block_table"):
+        layers.kv4_attention_workspace_bytes(pool(4, 2, 2, 544), lengths, 4, 64)

@@ -620,17 +620,24 @@ def kv4_pages(num_pages: int, kv_heads: int, head_dim: int, page_size: int = 64,
     return torch.zeros(shape if layers is None else (layers, *shape), dtype=torch.uint8, device=device)
 
 
-def _kv4_args(pages: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor, head_dim: int, device: torch.device) -> tuple:
-    """The cache's arguments of a C call, from pages to sequences."""
-    shape, table = pages.shape, block_table.shape
-    if (len(shape) != 4 or shape[2] != 2 or pages.dtype != torch.uint8 or not pages.is_cuda or pages.device != device
-            or not pages.is_contiguous()):
-        raise TexelatorError("pages must be contiguous CUDA uint8 [num_pages, kv_heads, 2, page bytes] on the rows' device")
+def _kv4_page_size(shape: torch.Size, head_dim: int) -> int:
+    """Positions of a page of a pool [num_pages, kv_heads, 2, page bytes]."""
+    if len(shape) != 4 or shape[1] == 0 or shape[2] != 2:
+        raise TexelatorError("pages must be [num_pages, kv_heads, 2, page bytes]")
     if head_dim not in (64, 128):
         raise TexelatorError("head_dim must be 64 or 128")
     page_size, rest = divmod(shape[3], head_dim * 17 // 32)
     if rest:
         raise TexelatorError("pages were made for another head_dim")
+    return page_size
+
+
+def _kv4_args(pages: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor, head_dim: int, device: torch.device) -> tuple:
+    """The cache's arguments of a C call, from pages to sequences."""
+    shape, table = pages.shape, block_table.shape
+    if pages.dtype != torch.uint8 or not pages.is_cuda or pages.device != device or not pages.is_contiguous():
+        raise TexelatorError("pages must be contiguous CUDA uint8 [num_pages, kv_heads, 2, page bytes] on the rows' device")
+    page_size = _kv4_page_size(shape, head_dim)
     if (len(table) != 2 or block_table.dtype != torch.int32 or block_table.device != device
             or (block_table.stride(1) != 1 and table[1] != 1)):
         raise TexelatorError("block_table must be int32 [sequences, pages] on the same device, rows contiguous")
@@ -707,9 +714,10 @@ def _kv4_workspace_bytes(*sizes: int) -> int:
 
 def kv4_attention_workspace_bytes(pages: torch.Tensor, block_table: torch.Tensor, heads: int, head_dim: int) -> int:
     """Device scratch of :func:`kv4_attention`: it depends on shapes alone, not on the lengths."""
+    _expect(pages.is_cuda and block_table.dim() == 2, "pages must be a CUDA tensor, block_table [sequences, pages]")
     sequences, max_pages = block_table.shape
-    return _kv4_workspace_bytes(sequences, heads, pages.shape[1], head_dim, pages.shape[3] * 32 // (17 * head_dim), max_pages,
-                                pages.device.index)
+    page_size = _kv4_page_size(pages.shape, head_dim)
+    return _kv4_workspace_bytes(sequences, heads, pages.shape[1], head_dim, page_size, max_pages, pages.device.index)
 
 
 def kv4_attention(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor, scale: float,
