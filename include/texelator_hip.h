@@ -446,7 +446,7 @@ int tx_rope_kv_cache_prefill_split(uint64_t qkv_handle, const void *partials, in
  * that sees no key gets zeros. Keys that a query does not see, and their values, may hold anything. Rows of out
  * [total_q][heads][head_dim] that belong to no sequence are left as they are. head_dim 64 or 128; heads a multiple of
  * kv_heads; rows of q, k and v 16-byte aligned, of out 8-byte. Rows of k and v do not overlap and follow each other within 2^24
- * elements. out must not overlap the inputs. fp32 scores, softmax statistics and sums; the probabilities are rounded to the
+ * elements. out must not overlap the inputs (columns of one buffer are told apart). fp32 scores, softmax statistics and sums; the probabilities are rounded to the
  * rows' type before they meet the values. Finite values give finite outputs where the scores are finite. */
 int tx_packed_attention(const void *q, int64_t q_token, int64_t q_head, const void *k, int64_t k_token, int64_t k_head,
                         const void *v, int64_t v_token, int64_t v_head, int dtype, int heads, int kv_heads, int head_dim,

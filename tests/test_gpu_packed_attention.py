@@ -214,6 +214,22 @@ def test_heads_farther_apart_than_rows_may_be(ext):
     assert first[0].stride(1) > 1 << 24 and torch.equal(run(q, *first, [40], [keys - 40], 0.1), want)
 
 
+@pytest.mark.parametrize("tokens", [1, 150])
+def test_an_output_among_the_columns_of_its_inputs(ext, tokens):
+    """q, k, v and the output side by side in one buffer run as apart; an output that shares a column with them is refused."""
+    heads, kv_heads, dim = 6, 2, 64
+    wide = torch.randn(tokens, 2 * heads + 2 * kv_heads, dim, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1)).to(BF16)
+    q, k, v, out = wide.split([heads, kv_heads, kv_heads, heads], dim=1)
+    want = run(q.clone(), k.clone(), v.clone(), [tokens], [0], 0.1)
+    before = wide.clone()
+    run(q, k, v, [tokens], [0], 0.1, out=out)
+    assert torch.equal(out, want) and torch.equal(wide[:, :-heads], before[:, :-heads])
+    for column in (0, 1, heads - 1, heads, heads + 2 * kv_heads - 1):
+        with pytest.raises(_lib.TexelatorError, match="overlap"):
+            run(q, k, v, [tokens], [0], 0.1, out=wide[:, column:column + heads])
+    assert torch.equal(wide[:, :-heads], before[:, :-heads])
+
+
 def test_sequence_starts_outside_the_rows(ext):
     """cu is data: starts past the arrays, below zero or falling are cut to them; nothing outside is written."""
     q, k, v = inputs([100], [0], 4, 2, 128, BF16, 9)

@@ -166,3 +166,22 @@ def test_shapes_without_heads_or_of_other_pools_are_refused(monkeypatch):
             layers.kv4_attention_workspace_bytes(pool(4, 2, 2, 544), table, 4, head_dim)
     with pytest.raises(_lib.TexelatorError, match="block_table"):
         layers.kv4_attention_workspace_bytes(pool(4, 2, 2, 544), lengths, 4, 64)
+
+
+FAR = 1 << 40  # away from everything else
+# Rows of 40 heads of 128 of one buffer: q in the first 16, k in the next 2, v in the next 2, 20 heads between the rows' ends.
+FUSED = dict(q=P, q_token=5120, k=P + 2 * 2048, k_token=5120, v=P + 2 * 2304, v_token=5120, out_token=5120)
+
+
+@pytest.mark.parametrize("change", [
+    dict(k=FAR, v=FAR, out=P), dict(q=FAR, v=2 * FAR, out=P), dict(q=FAR, k=2 * FAR, out=P),    # the same rows
+    dict(k=FAR, v=FAR, out=P + 9 * 4096), dict(k=FAR, v=FAR, out=P + 8, out_head=64),           # the last row of q, the middle of one
+    dict(k=FAR, v=FAR, out=P + 2048, out_token=4096),                                           # other strides within q's ends
+    dict(FUSED, out=P + 2 * 2044), dict(FUSED, out=P + 2 * 2304), dict(FUSED, out=P + 2 * 5120 * 7),
+    dict(FUSED, out=P + 2 * (5120 - 2048 + 128)), dict(FUSED, total_q=1, out=P + 2 * 5120 * 3 + 2 * 2048),
+], ids=str)
+def test_outputs_that_overlap_inputs_are_refused(change):
+    name, arguments = packed(**change)
+    lib = _lib.load()
+    assert getattr(lib, name)(*arguments.values()) == _lib.TX_ERR_INVALID
+    assert b"overlap q, k or v" in lib.tx_last_error()

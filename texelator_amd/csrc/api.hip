@@ -1470,6 +1470,38 @@ const char *kv4_rows(const void *k, int64_t k_token, int64_t k_head, const void 
 
 }  // namespace
 
+namespace {
+
+// [rows][heads][dim] elements of 16 bits.
+struct RowBlock {
+  const void *at;
+  int64_t rows, token, heads, head, dim;
+  uintptr_t begin() const { return reinterpret_cast<uintptr_t>(at); }
+  uintptr_t end() const { return rows > 0 ? begin() + 2 * ((rows - 1) * token + (heads - 1) * head + dim) : begin(); }
+};
+
+// Whether two blocks share an element: exact where their rows follow each other alike (columns of one buffer do); blocks that lie
+// within each other's ends with other strides count as sharing.
+bool overlap(const RowBlock &a, const RowBlock &b) {
+  if (a.begin() == a.end() || b.begin() == b.end() || a.end() <= b.begin() || b.end() <= a.begin()) return false;
+  if ((a.rows > 1 && b.rows > 1 && a.token != b.token) || a.heads * b.heads > 1 << 16) return true;
+  const int64_t stride = a.rows > 1 ? a.token : b.token, dim = std::max(a.dim, b.dim);
+  const int64_t apart = (int64_t)(b.begin() - a.begin()) / 2;
+  for (int64_t i = 0; i < a.heads; ++i)
+    for (int64_t j = 0; j < b.heads; ++j) {
+      // Row r of a and row s of b are x + (s - r) * stride apart.
+      const int64_t x = apart + j * b.head - i * a.head;
+      int64_t most = b.rows - 1, least = 1 - a.rows;  // of s - r
+      if (stride == 0) most = least = 0;
+      const int64_t near = stride == 0 ? 0 : -x / stride;
+      for (int64_t d = near - 1; d <= near + 1; ++d)
+        if (d >= least && d <= most && std::abs(x + d * stride) < dim) return true;
+    }
+  return false;
+}
+
+}  // namespace
+
 int tx_kv4_append(const void *k, int64_t k_token, int64_t k_head, const void *v, int64_t v_token, int64_t v_head, int dtype,
                   int64_t tokens, const int *cu, void *pages, int64_t num_pages, int kv_heads, int head_dim, int page_size,
                   const int *block_table, int64_t table_stride, int max_pages, const int *lengths, int sequences,
@@ -1632,6 +1664,10 @@ int tx_packed_attention(const void *q, int64_t q_token, int64_t q_head, const vo
   else if ((reinterpret_cast<uintptr_t>(cu_q) | reinterpret_cast<uintptr_t>(cu_k)) % 4) bad = "cu must be 4-byte aligned";
   if (bad) return fail(TX_ERR_INVALID, std::string("packed_attention: ") + bad);
   if (sequences == 0 || total_q == 0) return TX_OK;
+  const RowBlock to = {out, total_q, out_token, heads, out_head, head_dim};
+  if (overlap(to, {q, total_q, q_token, heads, q_head, head_dim}) || overlap(to, {k, total_k, k_token, kv_heads, k_head, head_dim}) ||
+      overlap(to, {v, total_k, v_token, kv_heads, v_head, head_dim}))
+    return fail(TX_ERR_INVALID, "packed_attention: out must not overlap q, k or v");
   tx::PackedAttention a = {};
   a.q = static_cast<const uint16_t *>(q);
   a.k = static_cast<const uint16_t *>(k);
