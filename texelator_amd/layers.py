@@ -571,8 +571,10 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     ``[q | k | v]`` projection will do). Sequence ``s`` has the queries ``cu_q[s] .. cu_q[s + 1] - 1`` and the keys
     ``cu_k[s] .. cu_k[s + 1] - 1`` (int32 on the device; ``cu_k`` defaults to ``cu_q``); its last query sees its last key,
     so keys of earlier turns come first. A query that sees no key gets zeros; rows of ``out`` that belong to no
-    sequence are left as they are (uninitialised where ``out`` is not given). Keys that a query does not see,
-    and their values, may hold anything. Returns ``[tokens, heads, dim]``."""
+    sequence are left as they are (uninitialised where ``out`` is not given); ``out`` shares no element with q, k and v, but
+    may be columns of their buffer. Keys that a query does not see, and their values, may hold anything. Scores, softmax statistics
+    and sums are fp32; the probabilities are rounded to the rows' type before they meet the values, and the sum that divides is of
+    the rounded ones. Returns ``[tokens, heads, dim]``."""
     shape, rows, dtype, device, code = q.shape, k.shape, q.dtype, q.device, _ROW_CODE.get(q.dtype)
     if code is None or len(shape) != 3 or not q.is_cuda or q.stride(2) != 1:
         raise TexelatorError("q must be CUDA bf16 or fp16 [tokens, heads, dim], the last dimension contiguous")
@@ -725,7 +727,9 @@ def kv4_attention(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tenso
     """Attention of one query token for each sequence over a paged 4-bit cache: ``q`` ``[sequences, heads, dim]`` bf16 or fp16
     (every query 16-byte aligned) against the ``lengths[s]`` positions that ``block_table[s]`` names (see
     :func:`kv4_append`); heads a multiple of the pages' KV heads. Returns ``[sequences, heads, dim]``, zeros for an empty
-    sequence. ``workspace``: :func:`kv4_attention_workspace_bytes` bytes that no call running at the same time uses;
+    sequence (one without a position in the pool). Scores, statistics and sums are fp32; the probabilities are rounded to q's type, and
+    the sum that divides is of the rounded ones. Cached values become q's type: exact in bf16; in fp16 they are rounded where they are
+    subnormal and infinite beyond 65504. ``workspace``: :func:`kv4_attention_workspace_bytes` bytes that no call running at the same time uses;
     allocated on the current stream where not given."""
     shape, device, code = q.shape, q.device, _ROW_CODE.get(q.dtype)
     if code is None or len(shape) != 3 or not q.is_cuda or q.stride(2) != 1:
