@@ -446,8 +446,9 @@ int tx_rope_kv_cache_prefill_split(uint64_t qkv_handle, const void *partials, in
  * that sees no key gets zeros. Keys that a query does not see, and their values, may hold anything. Rows of out
  * [total_q][heads][head_dim] that belong to no sequence are left as they are. head_dim 64 or 128; heads a multiple of
  * kv_heads; rows of q, k and v 16-byte aligned, of out 8-byte. Rows of k and v do not overlap and follow each other within 2^24
- * elements. out must not overlap the inputs (columns of one buffer are told apart). fp32 scores, softmax statistics and sums; the probabilities are rounded to the
- * rows' type before they meet the values. Finite values give finite outputs where the scores are finite. */
+ * elements. out must not overlap the inputs (columns of one buffer are told apart). At most 65535 sequences, 65535 heads and 2^28
+ * rows. fp32 scores, softmax statistics and sums; the probabilities are rounded to the rows' type before they meet the values. Finite
+ * values give finite outputs where the scores are finite; a query whose scores are all -infinity gets NaN. */
 int tx_packed_attention(const void *q, int64_t q_token, int64_t q_head, const void *k, int64_t k_token, int64_t k_head,
                         const void *v, int64_t v_token, int64_t v_head, int dtype, int heads, int kv_heads, int head_dim,
                         const int *cu_q, const int *cu_k, int sequences, int64_t total_q, int64_t total_k, float scale,
@@ -459,7 +460,7 @@ int tx_packed_attention(const void *q, int64_t q_token, int64_t q_head, const vo
  * [page_size][head_dim / 32], one for 32 elements. head_dim 64 or 128. Position p of sequence s lies at offset
  * p % page_size of page block_table[s][p / page_size] (rows of max_pages entries, table_stride apart). lengths[s]: the positions
  * in use, those that a call appends included; above max_pages * page_size they count as that, below 0 as 0. A page id outside the
- * pool is allowed: its positions are skipped.
+ * pool is allowed: its positions are skipped. At most 65535 sequences of 2^30 positions, 1024 KV heads.
  *
  * tx_kv4_append: token rows k and v [tokens][kv_heads][head_dim] into the cache. cu [sequences + 1]: the tokens
  * cu[s] .. cu[s + 1] - 1 become the last ones of sequence s's lengths[s] positions; NULL: one token for each sequence.
@@ -480,7 +481,7 @@ int tx_kv4_read(void *k, int64_t k_token, int64_t k_head, void *v, int64_t v_tok
                 void *stream);
 
 /* One query token per sequence over the cache: q [sequences][heads][head_dim] against the lengths[s] positions of its
- * sequence; out the same shape, zeros for an empty sequence. heads a multiple of kv_heads; every query 16-byte
+ * sequence; out the same shape, zeros for a sequence without a position in the pool, NaN where all scores are -infinity. heads a multiple of kv_heads; every query 16-byte
  * aligned, every output row 8-byte. workspace: at least tx_kv4_attention_workspace bytes, 16-byte aligned, not shared
  * with a call that may run at the same time; it need not be cleared. fp32 scores, statistics and sums; probabilities rounded
  * to q's type. Finite values give finite outputs where the scores are finite. In fp16, cached values beyond 65504 (a cache

@@ -26,7 +26,7 @@
 // so that small ones keep their bits (p <= 2^15 stays below fp16's largest); in bf16 times a power of two below 1 / (2 length), so
 // that sums of the largest values stay finite (in turn values below 2^-110, at 8191 positions, lose bits to fp32's smallest).
 //
-// Bound: memory for long contexts, 262144 positions of 8 heads of 128 (285 MB) 45 us, 6.3 TB/s with a part of it still cached, and 5
+// Bound: memory for long contexts, 262144 positions of 8 heads of 128 (285 MB) 44 to 47 us, 6.0 to 6.5 TB/s with a part of it still cached, and 5
 // for the combine kernel and the gap before it; at dim 64 instruction issue (half the bytes for the same scores), 163 MB at 31 us, 5.3
 // TB/s. A few thousand positions in all: the chain of dependent loads (lengths, page ids, codes), the merge and the second
 // launch, 8 us; a codes' step further ahead, more workgroups a CU and 16-wave workgroups were all slower.

@@ -14,7 +14,7 @@
 //     factor is a scalar of the lane, and the probabilities, rounded to 16 bits in place, are the B operand of
 //     O^T = V^T P^T: none of them passes through LDS;
 //   * the next 32 keys' scores are computed while these 32 keys' exponentials are, woven by hand: a wave that ran its
-//     products and its exponentials one after the other kept the matrix cores 44% busy, woven 53%;
+//     products and its exponentials one after the other kept the matrix cores 44% busy, woven 54%;
 //   * a query's running maximum follows its scores only where they pass it by 2^4: rescaling the outputs had been a third of
 //     the vector instructions, since some of a wave's queries almost always finds a new maximum;
 //   * keys and values reach LDS by direct buffer loads one block ahead, as they lie in memory; the descriptors end at
@@ -25,10 +25,11 @@
 // of two below 1 / (2^4 keys), so that sums of the type's largest values stay finite (in turn values below 2^-110, at 8190 keys, lose
 // bits to fp32's smallest; held unscaled, sums of values above 2^111 overflowed).
 //
-// Bound: power. At 8190 tokens and 40/8 heads 1.23 M cycles a SIMD at 1.9 GHz, 655 us (1050 TFLOP/s; a plain 16384^3 product
-// of the library reaches 1370); the same instructions on zeros run at 2.4 GHz. Two waves a SIMD: vector instructions take 2.6
-// cycles each there against 5 of a wave alone. 64 queries a wave (half the LDS reads per product, one wave a SIMD) took
-// 1.73 M cycles, 718 us.
+// Bound: power. At 8190 tokens and 40/8 heads 1.22 M cycles a SIMD, 54% of them with products, at 1.83 GHz, 650 to 669 us by card (1030
+// to 1060 TFLOP/s; a plain 16384^3 product of the library reaches 1370); on zeros as many cycles at 2.4 GHz, 494 us. At 64 dimensions
+// 0.73 M cycles, 45% of them with products, 68% with vector instructions, 372 us, on zeros 296. Two waves a SIMD: vector
+// instructions take 2.6 cycles each there against 5 of a wave alone. 64 queries a wave (half the LDS reads per product, one wave a
+// SIMD) took 1.73 M cycles, 718 us.
 #include <math.h>
 
 #include <type_traits>
@@ -514,9 +515,9 @@ hipError_t launch_typed(const PackedAttention &a, hipStream_t stream) {
   //              against 8.1 of <4, 1, 64>, 256 tokens of 16/2 heads 8.5 against 10.1; but 12 prompts of up to 60 tokens at
   //              32/8 heads 12.7 against 6.6, whose chains are short;
   //   <2, 4, 32> likewise: 1024 tokens of 16/2 heads 17.5 against 23.9; but 512 tokens (320 workgroups) 18.8 against 15.5;
-  //   <2, 2, KB> where the longest chain still outlasts the others' work. Heads of 64: KB 64 while all workgroups run at
-  //              once (3 turns of up to 400 behind up to 6000 keys 39 against 62 of <4, 1, 64>, 2500 tokens of 16/2 heads 27
-  //              against 37), beyond KB 32, of which a CU holds three and not two (9 turns of up to 777 behind up to 2500 of
+  //   <2, 2, KB> where the longest chain still outlasts the others' work. Heads of 64: KB 64 up to two and a half
+  //              workgroups a CU, which holds two (3 turns of up to 400 behind up to 6000 keys 39 against 62 of <4, 1, 64>, 2500
+  //              tokens of 16/2 heads 27 against 37), beyond KB 32, of which a CU holds four (9 turns of up to 777 behind up to 2500 of
   //              28/4 heads 34.5 against 40 of KB 64 and of <4, 1, 64>, 2048 tokens of 28/4 30 against 34; but 1477 tokens of
   //              64/8, 1600 workgroups, 30 against 26). Heads of 128: KB 32 and longer chains (3000 tokens of 16/2 heads 54
   //              against 60, those 3 turns 60 against 82; but 2048 tokens, 1280 workgroups, 70 against 60, and 3 prompts of up
