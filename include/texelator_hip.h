@@ -481,11 +481,11 @@ int tx_kv4_read(void *k, int64_t k_token, int64_t k_head, void *v, int64_t v_tok
                 void *stream);
 
 /* One query token per sequence over the cache: q [sequences][heads][head_dim] against the lengths[s] positions of its
- * sequence; out the same shape, zeros for a sequence without a position in the pool, NaN where all scores are -infinity. heads a multiple of kv_heads; every query 16-byte
- * aligned, every output row 8-byte. workspace: at least tx_kv4_attention_workspace bytes, 16-byte aligned, not shared
- * with a call that may run at the same time; it need not be cleared. fp32 scores, statistics and sums; probabilities rounded
- * to q's type. Finite values give finite outputs where the scores are finite. In fp16, cached values beyond 65504 (a cache
- * written from bf16) read as infinities. */
+ * sequence; out the same shape, zeros for a sequence without a position in the pool, NaN where all scores are -infinity. heads a
+ * multiple of kv_heads; every query 16-byte aligned, every output row 8-byte. workspace: at least tx_kv4_attention_workspace
+ * bytes, 16-byte aligned, not shared with a call that may run at the same time; it need not be cleared. fp32 scores, statistics
+ * and sums; probabilities rounded to q's type. Finite values give finite outputs where the scores are finite. In fp16, cached
+ * values beyond 65504 (a cache written from bf16) read as infinities. */
 int tx_kv4_attention_workspace(int sequences, int heads, int kv_heads, int head_dim, int page_size, int max_pages, int device,
                                int64_t *bytes);
 int tx_kv4_attention(const void *q, int64_t q_sequence, int64_t q_head, int dtype, int heads, const void *pages,

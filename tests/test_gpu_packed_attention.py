@@ -179,6 +179,15 @@ def test_the_largest_values(ext, new, old, heads, kv_heads, dtype, dim):
     assert_within(got, want, bound)
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("new,old,heads,kv_heads", [([300, 40], [30, 0], 8, 2), ([50] * 40, [i for i in range(40)], 16, 4), ([100], [9000], 8, 2)])
+def test_small_values_keep_their_bits(ext, new, old, heads, kv_heads, dim):
+    """Values of 2^-100: the power of two that keeps sums of the largest values finite does not cost them any."""
+    q, k, v = inputs(new, old, heads, kv_heads, dim, BF16, 31)
+    v.mul_(2.0 ** -100)
+    assert_within(run(q, k, v, new, old, dim ** -0.5), *reference(q, k, v, new, old, dim ** -0.5))
+
+
 def test_views_that_agree_with_the_packed_call(ext):
     """The same rows at other strides and offsets, and an output with gaps, give the same bits."""
     new, old = [130, 40], [3, 60]

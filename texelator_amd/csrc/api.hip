@@ -1487,6 +1487,11 @@ bool overlap(const RowBlock &a, const RowBlock &b) {
   if ((a.rows > 1 && b.rows > 1 && a.token != b.token) || a.heads * b.heads > 1 << 16) return true;
   const int64_t stride = a.rows > 1 ? a.token : b.token, dim = std::max(a.dim, b.dim);
   const int64_t apart = (int64_t)(b.begin() - a.begin()) / 2;
+  // Columns of one buffer: b's begin behind all of a's and end before a's next row. Else every pair of heads is looked at.
+  if (stride > 0) {
+    const int64_t behind = (apart % stride + stride) % stride;
+    if (behind >= (a.heads - 1) * a.head + dim && behind + (b.heads - 1) * b.head + dim <= stride) return false;
+  }
   for (int64_t i = 0; i < a.heads; ++i)
     for (int64_t j = 0; j < b.heads; ++j) {
       // Row r of a and row s of b are x + (s - r) * stride apart.
