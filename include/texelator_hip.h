@@ -500,6 +500,75 @@ int tx_kv4_attention(const void *q, int64_t q_sequence, int64_t q_head, int dtyp
 int tx_kv4_copy_pages(void *pages, int layers, int64_t num_pages, int64_t page_bytes, const int64_t *src, const int64_t *dst,
                       int64_t count, int device, void *stream);
 
+/* ---- A drafted step over the paged 4-bit cache (speculative decoding; no reference counterpart) ----
+ * For every sequence the target model runs its last token and some drafted tokens together. cu [sequences + 1]: sequence s has the
+ * rows cu[s] .. cu[s + 1] - 1, at most 64 (those behind the 64th are neither read nor written, but count for the places of
+ * all); row 0 is its last token, the others are drafts. parents [tokens]: row i follows row parents[i] of its sequence; a
+ * value outside the sequence's rows: nothing but the context; NULL: each row follows the one before it. lengths count the rows, as
+ * tx_kv4_append takes them: they are the last positions of their sequence.
+ *
+ * tx_kv4_append_rope: tx_kv4_append of keys turned by their positions, and the queries q [tokens][heads][head_dim] turned into
+ * q_out, in one launch. Dimensions below `rotary` (a multiple of 16, at most head_dim) of every query and key head are turned in
+ * pairs (i, i + rotary / 2), with `interleaved` (2 i, 2 i + 1): a cos - b sin, b cos + a sin, pair i's cosine and sine at
+ * cos[position * cos_row + i] and sin[position * sin_row + i] (fp32 [table_rows][rotary / 2]; a scaling for long contexts lies
+ * in the tables). positions [tokens], or NULL: every token's place in its sequence; a position outside the tables turns into NaN.
+ * q_out is rounded once, from 32 bits; what is stored is the nearest code to the exact value, a value beyond fp32's largest
+ * counts as infinite. k_out [tokens][kv_heads][head_dim], or NULL: the turned keys, rounded once. q_out and k_out must not
+ * overlap q, k, v or each other. Rows of tokens outside cu are left as they are. Rows 16-byte aligned. */
+int tx_kv4_append_rope(const void *q, int64_t q_token, int64_t q_head, const void *k, int64_t k_token, int64_t k_head, const void *v,
+                       int64_t v_token, int64_t v_head, int dtype, int64_t tokens, int heads, const float *cos, int64_t cos_row,
+                       const float *sin, int64_t sin_row, int64_t table_rows, int rotary, int interleaved, const int *positions,
+                       const int *cu, void *pages, int64_t num_pages, int kv_heads, int head_dim, int page_size,
+                       const int *block_table, int64_t table_stride, int max_pages, const int *lengths, int sequences, void *q_out,
+                       int64_t q_out_token, int64_t q_out_head, void *k_out, int64_t k_out_token, int64_t k_out_head, int device,
+                       void *stream);
+
+/* tx_kv4_tree_attention: the rows' queries q [tokens][heads][head_dim] over the cache. Row i of a sequence sees the positions before
+ * all of its rows, itself and the rows that its parents lead to. out the same shape: zeros for a row that sees no position in the
+ * pool, NaN where all scores are -infinity. Positions that a row does not see, and their values, may hold anything. out must not
+ * overlap q; queries 16-byte aligned, output rows 8-byte. Arithmetic, workspace rules and limits as tx_kv4_attention, and at
+ * most 2^22 rows. */
+int tx_kv4_tree_attention_workspace(int sequences, int64_t tokens, int heads, int kv_heads, int head_dim, int page_size, int max_pages,
+                                    int device, int64_t *bytes);
+int tx_kv4_tree_attention(const void *q, int64_t q_token, int64_t q_head, int dtype, int64_t tokens, int heads, const int *cu,
+                          const int *parents, const void *pages, int64_t num_pages, int kv_heads, int head_dim, int page_size,
+                          const int *block_table, int64_t table_stride, int max_pages, const int *lengths, int sequences, float scale,
+                          void *workspace, int64_t workspace_bytes, void *out, int64_t out_token, int64_t out_head, int device,
+                          void *stream);
+
+/* tx_verify_drafts: which drafts the target accepts, and the token behind them. logits [tokens][vocab] (F16, BF16 or F32, rows
+ * logits_row elements apart): the target's at every row; p_v = softmax(logits[v] / temperature). ids [tokens]: the rows'
+ * tokens (row 0's is not used). uniforms [tokens]: numbers in [0, 1), one for each draft's test, row 0's for the closing token.
+ * From row 0 on, the drafts behind the row v reached so far are tried in the order of their rows:
+ *   without draft_logits a draft x is accepted where u (1 - sum of the earlier drafts' p_v) < p_v(x), one that repeats an earlier
+ *     one's token never; where none is, the closing token is drawn from p_v without their tokens;
+ *   with draft_logits [tokens][vocab] (chains alone: parents must be NULL; x was drawn from q_v = softmax(draft_logits[v] /
+ *     temperature)) where u q_v(x) < p_v(x); else the closing token is drawn from max(p_v - q_v, 0).
+ * Where that leaves nothing, it is drawn from p_v. A token is drawn as the first whose running sum in the vocabulary's order
+ * exceeds u times the whole sum, in 64 bits; the tests use sums of 32-bit terms (off by some 1e-7). temperatures [sequences], or
+ * NULL: `temperature` for all. A temperature that is not above 0: the largest logit's token is accepted and closes, of equal ones
+ * the first. Logits of -infinity have no weight; where a row that is reached holds a NaN, at temperatures above 0 an infinity, or
+ * nothing above -infinity, no draft behind it is accepted and the closing token is -1.
+ * accepted [sequences]: accepted drafts, -1 for a sequence without rows. path [tokens]: path[cu[s] + j] is the row at step j, 0 to
+ * accepted[s] (0 first). next [tokens]: next[cu[s] + j] the new tokens, accepted[s] drafts and the closing one. Both -1 behind.
+ * At most 65535 rows and 2^24 tokens of vocabulary. The outputs must not overlap the inputs, each other or the workspace, which is
+ * at least tx_verify_drafts_workspace bytes, 16-byte aligned, not shared with a call that may run at the same time, and need
+ * not be cleared. */
+int tx_verify_drafts_workspace(int dtype, int64_t tokens, int64_t vocab, int sequences, int sampled, int device, int64_t *bytes);
+int tx_verify_drafts(const void *logits, int64_t logits_row, const void *draft_logits, int64_t draft_row, int dtype, int64_t tokens,
+                     int64_t vocab, const int64_t *ids, const float *uniforms, const int *cu, const int *parents, int sequences,
+                     const float *temperatures, float temperature, void *workspace, int64_t workspace_bytes, int *accepted, int *path,
+                     int64_t *next, int device, void *stream);
+
+/* tx_kv4_keep_path: the rows of an accepted path moved together in each of `layers` pools [layers][num_pages][..]: row path[cu[s] + j]
+ * of sequence s moves to row j's place, j = 1 .. accepted[s] (as tx_verify_drafts leaves them; an entry outside the sequence's rows
+ * moves nothing, nor does one whose place or row j's lies in no page), all at once. lengths_out [sequences], another array than
+ * lengths: the positions that are left, lengths[s] - rows + accepted[s] + 1. A page that rows move within or into must be
+ * one sequence's alone. */
+int tx_kv4_keep_path(void *pages, int layers, int64_t num_pages, int kv_heads, int head_dim, int page_size, const int *block_table,
+                     int64_t table_stride, int max_pages, const int *lengths, int sequences, const int *cu, int64_t tokens,
+                     const int *path, const int *accepted, int *lengths_out, int device, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -95,6 +95,16 @@ SIGNATURES = {
     "tx_kv4_attention": (_I32, [_P, _I64, _I64, _I32, _I32, _P, _I64, _I32, _I32, _I32, _P, _I64, _I32, _P, _I32,
                                 ctypes.c_float, _P, _I64, _P, _I64, _I64, _I32, _P]),
     "tx_kv4_copy_pages": (_I32, [_P, _I32, _I64, _I64, _P, _P, _I64, _I32, _P]),
+    "tx_kv4_append_rope": (_I32, [_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I32, _I64, _I32, _P, _I64, _P, _I64, _I64, _I32,
+                                  _I32, _P, _P, _P, _I64, _I32, _I32, _I32, _P, _I64, _I32, _P, _I32, _P, _I64, _I64, _P, _I64,
+                                  _I64, _I32, _P]),
+    "tx_kv4_tree_attention_workspace": (_I32, [_I32, _I64, _I32, _I32, _I32, _I32, _I32, _I32, ctypes.POINTER(_I64)]),
+    "tx_kv4_tree_attention": (_I32, [_P, _I64, _I64, _I32, _I64, _I32, _P, _P, _P, _I64, _I32, _I32, _I32, _P, _I64, _I32, _P,
+                                     _I32, ctypes.c_float, _P, _I64, _P, _I64, _I64, _I32, _P]),
+    "tx_verify_drafts_workspace": (_I32, [_I32, _I64, _I64, _I32, _I32, _I32, ctypes.POINTER(_I64)]),
+    "tx_verify_drafts": (_I32, [_P, _I64, _P, _I64, _I32, _I64, _I64, _P, _P, _P, _P, _I32, _P, ctypes.c_float, _P, _I64, _P, _P,
+                                _P, _I32, _P]),
+    "tx_kv4_keep_path": (_I32, [_P, _I32, _I64, _I32, _I32, _I32, _P, _I64, _I32, _P, _I32, _P, _I64, _P, _P, _P, _I32, _P]),
 }
 
 _LIB = None

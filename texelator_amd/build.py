@@ -32,7 +32,7 @@ HIPCC_FLAGS = [
 
 # Products of the matrix cores go to vector registers, not to accumulation registers that every use would copy from:
 # one wave a SIMD has 512 registers, of which vector instructions reach the first 256.
-EXTRA_FLAGS = {"packed_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+EXTRA_FLAGS = {name: ["-mllvm", "-amdgpu-mfma-vgpr-form=1"] for name in ("packed_attention.hip", "tree_attention.hip")}
 
 
 def hipcc() -> str:

@@ -1640,6 +1640,264 @@ int tx_kv4_copy_pages(void *pages, int layers, int64_t num_pages, int64_t page_b
   return TX_OK;
 }
 
+namespace {
+
+// What the calls for drafted rows share: cu and the row count.
+const char *draft_rows(const int *cu, int64_t tokens, const int *parents) {
+  if (!cu) return "null pointer";
+  if (reinterpret_cast<uintptr_t>(cu) % 4 || reinterpret_cast<uintptr_t>(parents) % 4) return "cu and parents must be 4-byte aligned";
+  if (tokens < 0 || tokens > 1 << 22) return "bad row count";
+  return nullptr;
+}
+
+// [begin, end) in bytes against [begin, end).
+bool bytes_overlap(const void *a, int64_t a_bytes, const void *b, int64_t b_bytes) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return a_bytes > 0 && b_bytes > 0 && x < y + (uintptr_t)b_bytes && y < x + (uintptr_t)a_bytes;
+}
+
+}  // namespace
+
+int tx_kv4_append_rope(const void *q, int64_t q_token, int64_t q_head, const void *k, int64_t k_token, int64_t k_head, const void *v,
+                       int64_t v_token, int64_t v_head, int dtype, int64_t tokens, int heads, const float *cos, int64_t cos_row,
+                       const float *sin, int64_t sin_row, int64_t table_rows, int rotary, int interleaved, const int *positions,
+                       const int *cu, void *pages, int64_t num_pages, int kv_heads, int head_dim, int page_size,
+                       const int *block_table, int64_t table_stride, int max_pages, const int *lengths, int sequences, void *q_out,
+                       int64_t q_out_token, int64_t q_out_head, void *k_out, int64_t k_out_token, int64_t k_out_head, int device,
+                       void *stream) {
+  g_last_error.clear();
+  tx::Kv4Pool pool;
+  const char *bad = kv4_pool(pool, pages, num_pages, kv_heads, head_dim, page_size, block_table, table_stride, max_pages, lengths,
+                             sequences);
+  drop_strides(tokens, q_token, q_out_token);
+  drop_strides(tokens, k_token, v_token);
+  drop_strides(heads, q_head, q_out_head);
+  drop_strides(kv_heads, k_head, v_head);
+  int64_t unused = 0;
+  drop_strides(tokens, k_out_token, unused);
+  drop_strides(kv_heads, k_out_head, unused);
+  if (!bad) bad = kv4_rows(k, k_token, k_head, v, v_token, v_head, dtype, tokens, cu, sequences);
+  if (!bad && (!q || !q_out || !cos || !sin)) bad = "null pointer";
+  if (!bad && (heads <= 0 || heads > 32768)) bad = "bad head count";
+  if (!bad && ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(q_out) | reinterpret_cast<uintptr_t>(k_out)) % 16 ||
+               (q_token | q_head | q_out_token | q_out_head) % 8 || (k_out && (k_out_token | k_out_head) % 8)))
+    bad = "every row must be 16-byte aligned";
+  if (!bad && (q_token | q_head | k_token | k_head | v_token | v_head | q_out_token | q_out_head) < 0) bad = "negative strides";
+  if (!bad && k_out && (k_out_token | k_out_head) < 0) bad = "negative strides";
+  if (!bad && (rotary <= 0 || rotary > head_dim || rotary % 16)) bad = "the rotated dimensions must be a multiple of 16 within the head";
+  if (!bad && ((reinterpret_cast<uintptr_t>(cos) | reinterpret_cast<uintptr_t>(sin) | reinterpret_cast<uintptr_t>(positions)) % 4 ||
+               cos_row < 0 || sin_row < 0 || table_rows < 0 || table_rows > 0x7FFFFFFF))
+    bad = "bad tables or positions";
+  if (!bad && tokens > 0) {
+    const RowBlock in[3] = {{q, tokens, q_token, heads, q_head, head_dim},
+                            {k, tokens, k_token, kv_heads, k_head, head_dim},
+                            {v, tokens, v_token, kv_heads, v_head, head_dim}};
+    const RowBlock out_q = {q_out, tokens, q_out_token, heads, q_out_head, head_dim};
+    const RowBlock out_k = {k_out, tokens, k_out_token, kv_heads, k_out_head, head_dim};
+    for (const RowBlock &block : in)
+      if (overlap(out_q, block) || (k_out && overlap(out_k, block))) bad = "the rotated rows must not overlap q, k or v";
+    if (!bad && k_out && overlap(out_q, out_k)) bad = "the rotated rows must not overlap each other";
+  }
+  if (bad) return fail(TX_ERR_INVALID, std::string("kv4_append_rope: ") + bad);
+  if (tokens == 0 || sequences == 0) return TX_OK;
+  tx::Kv4Rope a = {};
+  a.q = static_cast<const uint16_t *>(q);
+  a.k = static_cast<const uint16_t *>(k);
+  a.v = static_cast<const uint16_t *>(v);
+  a.q_token = q_token, a.q_head = q_head, a.k_token = k_token, a.k_head = k_head, a.v_token = v_token, a.v_head = v_head;
+  a.q_out = static_cast<uint16_t *>(q_out);
+  a.k_out = static_cast<uint16_t *>(k_out);
+  a.q_out_token = q_out_token, a.q_out_head = q_out_head, a.k_out_token = k_out_token, a.k_out_head = k_out_head;
+  a.cos = cos, a.sin = sin, a.cos_row = cos_row, a.sin_row = sin_row, a.table_rows = table_rows;
+  a.positions = positions;
+  a.cu = cu;
+  a.heads = heads, a.rotary = rotary, a.tokens = (int)tokens;
+  DeviceGuard guard(device);
+  TX_HIP(tx::launch_kv4_append_rope(a, interleaved != 0, dtype == TX_DTYPE_F16, head_dim, pool, reinterpret_cast<hipStream_t>(stream)));
+  return TX_OK;
+}
+
+int tx_kv4_keep_path(void *pages, int layers, int64_t num_pages, int kv_heads, int head_dim, int page_size, const int *block_table,
+                     int64_t table_stride, int max_pages, const int *lengths, int sequences, const int *cu, int64_t tokens,
+                     const int *path, const int *accepted, int *lengths_out, int device, void *stream) {
+  g_last_error.clear();
+  tx::Kv4Pool pool;
+  const char *bad = kv4_pool(pool, pages, num_pages, kv_heads, head_dim, page_size, block_table, table_stride, max_pages, lengths,
+                             sequences);
+  if (!bad) bad = draft_rows(cu, tokens, path);
+  if (!bad && (layers <= 0 || layers > 65535)) bad = "bad pool shape";
+  if (!bad && ((tokens > 0 && !path) || !accepted || !lengths_out)) bad = "null pointer";
+  if (!bad && (reinterpret_cast<uintptr_t>(accepted) | reinterpret_cast<uintptr_t>(lengths_out)) % 4) bad = "integers must be 4-byte aligned";
+  const int64_t bytes = (int64_t)sequences * 4;
+  if (!bad && (bytes_overlap(lengths_out, bytes, lengths, bytes) || bytes_overlap(lengths_out, bytes, cu, bytes + 4) ||
+               bytes_overlap(lengths_out, bytes, accepted, bytes) || bytes_overlap(lengths_out, bytes, path, tokens * 4)))
+    bad = "the new lengths must not overlap the other arrays";
+  if (bad) return fail(TX_ERR_INVALID, std::string("kv4_keep_path: ") + bad);
+  if (sequences == 0) return TX_OK;
+  DeviceGuard guard(device);
+  const int64_t layer_bytes = num_pages * kv_heads * 2 * tx::kv4_half_bytes(pool.page_shift, head_dim);
+  TX_HIP(tx::launch_kv4_keep_path(pool, head_dim, layers, layer_bytes, cu, (int)tokens, path, accepted, lengths_out,
+                                  reinterpret_cast<hipStream_t>(stream)));
+  return TX_OK;
+}
+
+int tx_kv4_tree_attention_workspace(int sequences, int64_t tokens, int heads, int kv_heads, int head_dim, int page_size, int max_pages,
+                                    int device, int64_t *bytes) {
+  g_last_error.clear();
+  if (!bytes) return fail(TX_ERR_INVALID, "kv4_tree_attention_workspace: null pointer");
+  static int dummy;
+  tx::Kv4Tree a = {};
+  const char *bad = kv4_pool(a.pool, reinterpret_cast<void *>(16), 1, kv_heads, head_dim, page_size, &dummy, max_pages, max_pages,
+                             &dummy, sequences);
+  if (!bad) bad = draft_rows(&dummy, tokens, nullptr);
+  if (!bad && (heads <= 0 || heads % kv_heads || heads > 65535)) bad = "heads must be a multiple of kv_heads";
+  if (!bad) {
+    a.tokens = (int)tokens;
+    a.group = heads / kv_heads;
+    if (!tx::kv4_tree_fits(a)) bad = "sequences x heads x positions too large";
+  }
+  if (bad) return fail(TX_ERR_INVALID, std::string("kv4_tree_attention_workspace: ") + bad);
+  tx::kv4_tree_plan(a, head_dim, multiprocessors(device));
+  *bytes = a.piece_bytes;
+  return TX_OK;
+}
+
+int tx_kv4_tree_attention(const void *q, int64_t q_token, int64_t q_head, int dtype, int64_t tokens, int heads, const int *cu,
+                          const int *parents, const void *pages, int64_t num_pages, int kv_heads, int head_dim, int page_size,
+                          const int *block_table, int64_t table_stride, int max_pages, const int *lengths, int sequences, float scale,
+                          void *workspace, int64_t workspace_bytes, void *out, int64_t out_token, int64_t out_head, int device,
+                          void *stream) {
+  g_last_error.clear();
+  tx::Kv4Tree a = {};
+  const char *bad = kv4_pool(a.pool, pages, num_pages, kv_heads, head_dim, page_size, block_table, table_stride, max_pages, lengths,
+                             sequences);
+  drop_strides(tokens, q_token, out_token);
+  drop_strides(heads, q_head, out_head);
+  if (!bad) bad = draft_rows(cu, tokens, parents);
+  if (!bad && (!q || !out)) bad = "null pointer";
+  if (!bad && dtype != TX_DTYPE_F16 && dtype != TX_DTYPE_BF16) bad = "q must be FP16 or BF16";
+  if (!bad && (heads <= 0 || heads % kv_heads || heads > 65535)) bad = "heads must be a multiple of kv_heads";
+  if (!bad && (reinterpret_cast<uintptr_t>(q) % 16 || (q_token | q_head) % 8)) bad = "every query must be 16-byte aligned";
+  if (!bad && (reinterpret_cast<uintptr_t>(out) % 8 || (out_token | out_head) % 4)) bad = "every output row must be 8-byte aligned";
+  if (!bad && (q_token | q_head | out_token | out_head) < 0) bad = "negative strides";
+  if (!bad && reinterpret_cast<uintptr_t>(workspace) % 16) bad = "the workspace must be 16-byte aligned";
+  if (!bad) {
+    a.tokens = (int)tokens;
+    a.group = heads / kv_heads;
+    if (!tx::kv4_tree_fits(a)) bad = "sequences x heads x positions too large";
+  }
+  if (!bad && overlap({out, tokens, out_token, heads, out_head, head_dim}, {q, tokens, q_token, heads, q_head, head_dim}))
+    bad = "the output must not overlap q";
+  if (bad) return fail(TX_ERR_INVALID, std::string("kv4_tree_attention: ") + bad);
+  if (sequences == 0 || tokens == 0) return TX_OK;
+  a.q = static_cast<const uint16_t *>(q);
+  a.q_token = q_token;
+  a.q_head = q_head;
+  a.out = static_cast<uint16_t *>(out);
+  a.out_token = out_token;
+  a.out_head = out_head;
+  a.cu = cu;
+  a.parents = parents;
+  set_scale(scale, a.sl2, a.q_and, a.q_xor);
+  a.lag = tx::kPackedLag / a.sl2;
+  a.pieces = static_cast<float *>(workspace);
+  tx::kv4_tree_plan(a, head_dim, multiprocessors(device));
+  if (workspace_bytes < a.piece_bytes || (a.piece_bytes > 0 && !workspace))
+    return fail(TX_ERR_INVALID, "kv4_tree_attention: workspace too small (tx_kv4_tree_attention_workspace)");
+  DeviceGuard guard(device);
+  TX_HIP(tx::launch_kv4_tree(a, dtype == TX_DTYPE_F16, head_dim, reinterpret_cast<hipStream_t>(stream)));
+  return TX_OK;
+}
+
+namespace {
+
+// A verification's sizes as its kernels take them; a message where they cannot.
+const char *verify_sizes(tx::Verify &a, int dtype, int64_t tokens, int64_t vocab, int sequences, bool sampled, int device) {
+  if (dtype != TX_DTYPE_F16 && dtype != TX_DTYPE_BF16 && dtype != TX_DTYPE_F32) return "logits must be FP16, BF16 or FP32";
+  if (tokens < 0 || tokens > 65535 || sequences < 0 || sequences > 65535) return "at most 65535 rows and sequences";
+  if (vocab <= 0 || vocab > 1 << 24) return "the vocabulary must have 1 to 2^24 tokens";
+  a.tokens = (int)tokens;
+  a.sequences = sequences;
+  a.vocab = (int)vocab;
+  a.draft = sampled ? &a : nullptr;  // whether there is one
+  tx::verify_plan(a, dtype == TX_DTYPE_F32 ? 4 : 2, multiprocessors(device));
+  return nullptr;
+}
+
+}  // namespace
+
+int tx_verify_drafts_workspace(int dtype, int64_t tokens, int64_t vocab, int sequences, int sampled, int device, int64_t *bytes) {
+  g_last_error.clear();
+  if (!bytes) return fail(TX_ERR_INVALID, "verify_drafts_workspace: null pointer");
+  tx::Verify a = {};
+  const char *bad = verify_sizes(a, dtype, tokens, vocab, sequences, sampled != 0, device);
+  if (bad) return fail(TX_ERR_INVALID, std::string("verify_drafts_workspace: ") + bad);
+  *bytes = a.workspace_bytes;
+  return TX_OK;
+}
+
+int tx_verify_drafts(const void *logits, int64_t logits_row, const void *draft_logits, int64_t draft_row, int dtype, int64_t tokens,
+                     int64_t vocab, const int64_t *ids, const float *uniforms, const int *cu, const int *parents, int sequences,
+                     const float *temperatures, float temperature, void *workspace, int64_t workspace_bytes, int *accepted, int *path,
+                     int64_t *next, int device, void *stream) {
+  g_last_error.clear();
+  tx::Verify a = {};
+  const char *bad = verify_sizes(a, dtype, tokens, vocab, sequences, draft_logits != nullptr, device);
+  if (!bad) bad = draft_rows(cu, tokens, parents);
+  if (!bad && ((sequences > 0 && !accepted) || (tokens > 0 && (!logits || !ids || !uniforms || !path || !next)))) bad = "null pointer";
+  if (!bad && draft_logits && parents) bad = "sampled drafts are chains: draft logits go without parents";
+  const int size = dtype == TX_DTYPE_F32 ? 4 : 2;
+  if (!bad && ((reinterpret_cast<uintptr_t>(logits) | reinterpret_cast<uintptr_t>(draft_logits)) % size || logits_row < 0 || draft_row < 0))
+    bad = "logits must be aligned to their type, rows forward";
+  if (!bad && ((reinterpret_cast<uintptr_t>(ids) | reinterpret_cast<uintptr_t>(next)) % 8 ||
+               (reinterpret_cast<uintptr_t>(uniforms) | reinterpret_cast<uintptr_t>(temperatures) | reinterpret_cast<uintptr_t>(accepted) |
+                reinterpret_cast<uintptr_t>(path)) % 4))
+    bad = "tokens must be 8-byte aligned, the other arrays 4-byte";
+  if (!bad && reinterpret_cast<uintptr_t>(workspace) % 16) bad = "the workspace must be 16-byte aligned";
+  if (!bad && (workspace_bytes < a.workspace_bytes || (a.workspace_bytes > 0 && !workspace)))
+    bad = "workspace too small (tx_verify_drafts_workspace)";
+  if (!bad) {
+    struct Bytes {
+      const void *at;
+      int64_t count;
+    };
+    auto logit_bytes = [&](const void *at, int64_t row) { return Bytes{at, at && tokens > 0 ? ((tokens - 1) * row + vocab) * size : 0}; };
+    const Bytes in[] = {{ids, tokens * 8},
+                        {uniforms, tokens * 4},
+                        {cu, (int64_t)sequences * 4 + 4},
+                        {parents, parents ? tokens * 4 : 0},
+                        {temperatures, temperatures ? (int64_t)sequences * 4 : 0},
+                        {workspace, a.workspace_bytes},
+                        logit_bytes(logits, logits_row),
+                        logit_bytes(draft_logits, draft_row)};
+    const Bytes out[] = {{accepted, (int64_t)sequences * 4}, {path, tokens * 4}, {next, tokens * 8}};
+    for (int i = 0; i < 3; ++i) {
+      for (const Bytes &other : in)
+        if (bytes_overlap(out[i].at, out[i].count, other.at, other.count)) bad = "the outputs must not overlap the inputs or the workspace";
+      for (int j = 0; j < i; ++j)
+        if (bytes_overlap(out[i].at, out[i].count, out[j].at, out[j].count)) bad = "the outputs must not overlap each other";
+    }
+  }
+  if (bad) return fail(TX_ERR_INVALID, std::string("verify_drafts: ") + bad);
+  if (sequences == 0) return TX_OK;
+  a.target = logits;
+  a.target_row = logits_row;
+  a.draft = draft_logits;
+  a.draft_row = draft_row;
+  a.ids = ids;
+  a.uniforms = uniforms;
+  a.cu = cu;
+  a.parents = parents;
+  a.temperatures = temperatures;
+  a.temperature = temperature;
+  a.accepted = accepted;
+  a.path = path;
+  a.next = next;
+  DeviceGuard guard(device);
+  TX_HIP(tx::launch_verify(a, dtype, static_cast<char *>(workspace), reinterpret_cast<hipStream_t>(stream)));
+  return TX_OK;
+}
+
 int tx_packed_attention(const void *q, int64_t q_token, int64_t q_head, const void *k, int64_t k_token, int64_t k_head,
                         const void *v, int64_t v_token, int64_t v_head, int dtype, int heads, int kv_heads, int head_dim,
                         const int *cu_q, const int *cu_k, int sequences, int64_t total_q, int64_t total_k, float scale,

@@ -22,6 +22,13 @@ __device__ __forceinline__ float half_bits_to_float(uint16_t v) {
 // Round to bf16, nearest-even.
 __device__ __forceinline__ uint16_t to_bf(float f) { return __builtin_bit_cast(uint16_t, (__bf16)f); }
 
+// Round to a 16-bit type, nearest-even.
+template <bool F16>
+__device__ __forceinline__ uint16_t to_half_bits(float f) {
+  if constexpr (F16) return __builtin_bit_cast(uint16_t, (_Float16)f);
+  else return to_bf(f);
+}
+
 // Reductions over the 16 lanes of a DPP row (xor 1, xor 2, half-row mirror, row mirror): every
 // lane of the row ends with the same value.
 template <int CTRL>

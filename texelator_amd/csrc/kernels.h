@@ -246,6 +246,11 @@ hipError_t launch_kv4_append(const uint16_t *k, int64_t k_token, int64_t k_head,
                              hipStream_t stream);
 hipError_t launch_kv4_read(uint16_t *k, int64_t k_token, int64_t k_head, uint16_t *v, int64_t v_token, int64_t v_head,
                            int tokens, bool f16, int dim, const int *cu, const Kv4Pool &pool, hipStream_t stream);
+// The same with keys (and queries) rotated on the way, and the accepted rows of drafts moved together, in `layers` pools.
+struct Kv4Rope;
+hipError_t launch_kv4_append_rope(Kv4Rope a, bool interleaved, bool f16, int dim, const Kv4Pool &pool, hipStream_t stream);
+hipError_t launch_kv4_keep_path(const Kv4Pool &pool, int dim, int layers, int64_t layer_bytes, const int *cu, int tokens,
+                                const int *path, const int *accepted, int *lengths_out, hipStream_t stream);
 constexpr int kKv4Pairs = 448;  // page pairs of one copy launch: 3.5 KiB of kernel arguments
 hipError_t launch_kv4_copy_pages(uint8_t *pool, int layers, int64_t layer_bytes, int64_t page_bytes, const int64_t *src,
                                  const int64_t *dst, int64_t count, hipStream_t stream);
@@ -254,6 +259,35 @@ bool kv4_attention_fits(const Kv4Pool &pool);
 // Fills in workgroups, whole and piece_bytes (the workspace's size).
 void kv4_attention_plan(Kv4Attention &a, int dim, int cus);
 hipError_t launch_kv4_attention(const Kv4Attention &a, bool f16, int dim, hipStream_t stream);
+
+// Attention of drafted rows over the cache (tree_attention.hip).
+struct Kv4Tree;
+bool kv4_tree_fits(const Kv4Tree &a);
+// Fills in workgroups, passes, whole and piece_bytes (the workspace's size).
+void kv4_tree_plan(Kv4Tree &a, int dim, int cus);
+hipError_t launch_kv4_tree(const Kv4Tree &a, bool f16, int dim, hipStream_t stream);
+
+// Verification of drafted tokens (verify.hip). Rows of target and draft logits are target_row and draft_row elements apart.
+struct Verify {
+  const void *target, *draft;  // draft: null where the drafts are given ones
+  int64_t target_row, draft_row;
+  const int64_t *ids;     // [tokens]
+  const float *uniforms;  // [tokens]
+  const int *cu, *parents;    // [sequences + 1]; [tokens] or null: chains
+  const float *temperatures;  // [sequences], or null: `temperature` for all
+  float temperature;
+  int tokens, sequences, vocab;
+  int *accepted, *path;  // [sequences], [tokens]
+  int64_t *next;         // [tokens]
+  // Filled in by verify_plan: spans of a row's statistics, workgroups, parts and tokens a part of a last row; the workspace.
+  int spans, groups, parts, part;
+  int64_t closings_at, sums_at, workspace_bytes;
+  float2 *partials;
+  void *closings, *sums;
+};
+constexpr int kVerifyF16 = 0, kVerifyBf16 = 1, kVerifyF32 = 2;
+void verify_plan(Verify &a, int dtype_bytes, int cus);
+hipError_t launch_verify(Verify a, int dtype, char *workspace, hipStream_t stream);
 
 // Causal attention of packed sequences (packed_attention.hip). Strides in elements.
 struct PackedAttention {

@@ -45,6 +45,41 @@ struct Kv4Attention {
   bool whole;  // a workgroup for each head: no pieces
 };
 
+// Rows of one sequence that a drafted step takes: a lane of a wave for each.
+constexpr int kMostDrafts = 64;
+
+// Token rows of a call that stores rotated keys (strides in elements).
+struct Kv4Rope {
+  const uint16_t *q, *k, *v;
+  int64_t q_token, q_head, k_token, k_head, v_token, v_head;
+  uint16_t *q_out, *k_out;  // k_out may be null
+  int64_t q_out_token, q_out_head, k_out_token, k_out_head;
+  const float *cos, *sin;  // [table_rows][rotary / 2], rows cos_row and sin_row apart
+  int64_t cos_row, sin_row, table_rows;
+  const int *positions;  // [tokens], or null: every token's place in the cache
+  const int *cu;
+  int heads, rotary, tokens;
+  int per;  // heads of a workgroup, filled in by the launch
+};
+
+// Attention of drafted rows; sl2, q_and and q_xor as above.
+struct Kv4Tree {
+  Kv4Pool pool;
+  const uint16_t *q;  // query h of row i at q + i * q_token + h * q_head (elements)
+  int64_t q_token, q_head;
+  uint16_t *out;
+  int64_t out_token, out_head;
+  const int *cu;       // [sequences + 1] first rows
+  const int *parents;  // [tokens] within the sequence, or null: each row follows the one before it
+  int tokens, group;
+  float sl2, lag;  // lag: kPackedLag / sl2
+  uint32_t q_and, q_xor;
+  float *pieces;  // results of heads that several workgroups share
+  int64_t piece_bytes;
+  int piece_floats, workgroups, most_passes;
+  bool whole;  // a workgroup for each sequence, head and pass: no pieces
+};
+
 // Bytes of one head's keys (or values) in a page.
 __host__ __device__ inline int64_t kv4_half_bytes(int page_shift, int dim) { return ((int64_t)dim * 17 / 32) << page_shift; }
 

@@ -6,7 +6,7 @@
 // e = max(floor(log2(amax)) - 2 + 127, 0), each code the E2M1 value nearest to v * 2^(127 - e), ties to the even code,
 // saturated at 6. A group that holds an infinity or a NaN gets e = 255 and reads back as NaN.
 //
-// All three are copies with arithmetic on the way, bound by memory; the scale and the codes of a group never leave its thread.
+// All are copies with arithmetic on the way, bound by memory.
 #include "elementwise.h"
 #include "kernels.h"
 #include "kv4.h"
@@ -27,7 +27,12 @@ struct Row {
   int offset;
 };
 
-__device__ __forceinline__ Row locate(const Kv4Pool &pool, const int *cu, const int *starts, int token) {
+// The sequence that has a token and the token's position in it, which may be below zero; sequence -1: no sequence has it.
+struct Place {
+  int sequence, position;
+};
+
+__device__ __forceinline__ Place place_of(const Kv4Pool &pool, const int *cu, const int *starts, int token) {
   int sequence = token, back = 1;  // `back`: how far before the sequence's end the token lies
   if (cu) {
     if (token < cu[0] || token >= cu[pool.sequences]) return {-1, 0};
@@ -40,11 +45,19 @@ __device__ __forceinline__ Row locate(const Kv4Pool &pool, const int *cu, const 
     sequence = low;
     back = cu[low + 1] - token;
   }
-  const int position = kv4_length(pool, sequence) - back;
-  if (position < 0 || back <= 0 || (cu == nullptr && token >= pool.sequences)) return {-1, 0};
-  const int page = pool.table[sequence * pool.table_stride + (position >> pool.page_shift)];
+  if (back <= 0 || (cu == nullptr && token >= pool.sequences)) return {-1, 0};
+  return {sequence, kv4_length(pool, sequence) - back};
+}
+
+__device__ __forceinline__ Row row_at(const Kv4Pool &pool, const Place &place) {
+  if (place.sequence < 0 || place.position < 0) return {-1, 0};
+  const int page = pool.table[place.sequence * pool.table_stride + (place.position >> pool.page_shift)];
   if ((uint32_t)page >= (uint64_t)pool.num_pages) return {-1, 0};
-  return {page, position & ((1 << pool.page_shift) - 1)};
+  return {page, place.position & ((1 << pool.page_shift) - 1)};
+}
+
+__device__ __forceinline__ Row locate(const Kv4Pool &pool, const int *cu, const int *starts, int token) {
+  return row_at(pool, place_of(pool, cu, starts, token));
 }
 
 // Sequence starts into LDS where they fit, for the binary search.
@@ -149,6 +162,168 @@ __global__ __launch_bounds__(kThreads) void kv4_read_kernel(uint16_t *k, int64_t
   }
 }
 
+// A value of two 16-bit numbers turned: a cos - b sin, rounded to 32 bits so that no comparison of the quantizer comes out
+// otherwise than for the exact value: towards an odd last bit where it is not exact (borders of codes and scales are even by
+// many bits). The products are exact in 64 bits.
+__device__ __forceinline__ float turned_to_odd(float a, float cos, float b, float sin) {
+  const double exact = __builtin_fma((double)a, (double)cos, -((double)b * (double)sin));
+  const float near = (float)exact;
+  const double back = (double)near;
+  uint32_t bits = __float_as_uint(near);
+  if (back != exact && !(bits & 1) && (bits & 0x7F800000u) != 0x7F800000u) bits += fabs(exact) > fabs(back) ? 1u : ~0u;
+  return __uint_as_float(bits);
+}
+
+// kv4_append with the rotary embedding on the way, and the queries' rotation in the same launch. Dimensions below `rotary` of
+// every query and key head are turned in pairs (i, i + rotary / 2), or (2i, 2i + 1) where INTERLEAVED, by the angle that the tables'
+// row of the token's position has for pair i; the others pass. Grid: x token blocks, y blocks of `per` heads of [q | k | v]. A
+// thread has eight elements of one token and loads their cosines and sines once for all its heads; four neighbours share a
+// group's scale. Queries and rotated key rows (k_out, where given) are rounded once, from 32 bits (a value next to a rounding
+// border of 16 bits is off by 2^-24 of itself more); what is stored is quantized from the exact value (turned_to_odd): a
+// slowly turning key stays so near the 16-bit value that it was that 32 bits put it midway between two codes.
+template <bool F16, int DIM, bool INTERLEAVED>
+__global__ __launch_bounds__(kThreads) void kv4_append_rope_kernel(Kv4Rope a, Kv4Pool pool) {
+  constexpr int kChunks = DIM / 8, kGroups = DIM / 32;
+  __shared__ int lds[kCuEntries];
+  const int *starts = stage_starts(a.cu, pool.sequences, lds);
+  const int chunk = threadIdx.x % kChunks;
+  const int64_t index = (int64_t)blockIdx.x * (kThreads / kChunks) + threadIdx.x / kChunks;
+  if (index >= a.tokens) return;
+  const int token = (int)index;
+  const Place place = place_of(pool, a.cu, starts, token);
+  if (place.sequence < 0) return;
+  const Row row = row_at(pool, place);
+  const int position = a.positions ? a.positions[token] : place.position;
+  const bool turns = 8 * chunk < a.rotary;
+  // Pairs of this thread: eight where the halves pair up (its elements' partners are another chunk), else four.
+  const int half = a.rotary / 2;
+  const bool second = !INTERLEAVED && 8 * chunk >= half;  // of the half layout: b cos + a sin
+  const int pair = INTERLEAVED ? 4 * chunk : 8 * chunk - (second ? half : 0);
+  const int partner = second ? -half : half;
+  constexpr int kPairs = INTERLEAVED ? 4 : 8;
+  float cs[kPairs], sn[kPairs];
+  if (turns) {
+    const bool known = (uint32_t)position < (uint64_t)a.table_rows;
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) {
+      cs[i] = known ? a.cos[position * a.cos_row + pair + i] : NAN;
+      sn[i] = known ? a.sin[position * a.sin_row + pair + i] : NAN;
+    }
+  }
+  const int heads = a.heads + 2 * pool.kv_heads, first = blockIdx.y * a.per, last = min(first + a.per, heads);
+  for (int h = first; h < last; ++h) {
+    const int which = h < a.heads ? 0 : h < a.heads + pool.kv_heads ? 1 : 2;
+    const int head = h - (which == 0 ? 0 : which == 1 ? a.heads : a.heads + pool.kv_heads);
+    const uint16_t *src = 8 * chunk + (which == 0   ? a.q + token * a.q_token + head * a.q_head
+                                       : which == 1 ? a.k + token * a.k_token + head * a.k_head
+                                                    : a.v + token * a.v_token + head * a.v_head);
+    const u32x4 mine = *reinterpret_cast<const u32x4 *>(src);
+    u32x4 theirs = mine;
+    const bool turned = turns && which != 2;
+    if (!INTERLEAVED && turned) theirs = *reinterpret_cast<const u32x4 *>(src + partner);
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = half_bits_to_float<F16>((uint16_t)(mine[i / 2] >> (16 * (i % 2))));
+    if (turned) {
+      float y[8], old[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        old[i] = x[i];
+        y[i] = half_bits_to_float<F16>((uint16_t)(theirs[i / 2] >> (16 * (i % 2))));
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int p = INTERLEAVED ? i / 2 : i;
+        const float other = INTERLEAVED ? old[i ^ 1] : y[i];
+        const float s = (INTERLEAVED ? i % 2 == 1 : second) ? -sn[p] : sn[p];
+        x[i] = which == 0 ? old[i] * cs[p] - other * s : turned_to_odd(old[i], cs[p], other, s);
+      }
+    }
+    if (which != 2) {
+      uint16_t *out = which == 0 ? a.q_out + token * a.q_out_token + head * a.q_out_head
+                      : a.k_out  ? a.k_out + token * a.k_out_token + head * a.k_out_head
+                                 : nullptr;
+      if (out) {
+        u32x4 packed = mine;
+        if (turned) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            packed[i] = to_half_bits<F16>(x[2 * i]) | (uint32_t)to_half_bits<F16>(x[2 * i + 1]) << 16;
+        }
+        *reinterpret_cast<u32x4 *>(out + 8 * chunk) = packed;
+      }
+    }
+    if (which == 0 || row.page < 0) continue;  // all four threads of a group alike
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);
+    top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0xB1, 0xF, 0xF, false));  // quad_perm [1,0,3,2]
+    top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0x4E, 0xF, 0xF, false));  // quad_perm [2,3,0,1]
+    const uint32_t field = top >> 23;
+    const uint32_t e = field == 255 ? 255 : (uint32_t)max((int)field - 2, 0);
+    const float inverse = __uint_as_float((254u - min(e, 254u)) << 23);  // 2^(127 - e), exact
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] *= inverse;
+    uint8_t *cache = pool.pages + ((row.page * pool.kv_heads + head) * 2 + (which - 1)) * kv4_half_bytes(pool.page_shift, DIM);
+    *reinterpret_cast<uint32_t *>(cache + row.offset * (DIM / 2) + 4 * chunk) = e == 255 ? 0u : e2m1_octet(x);
+    if (chunk % 4 == 0) cache[((int64_t)(DIM / 2) << pool.page_shift) + row.offset * kGroups + chunk / 4] = (uint8_t)e;
+  }
+}
+
+// The rows of an accepted path moved together: of sequence s, whose last cu[s + 1] - cu[s] positions are drafted rows, row path[cu[s] + j]
+// moves to the place of row j, j = 1 .. accepted[s]. A wave has one head's keys or values of one sequence and layer: it holds
+// every piece that moves before it stores the first, so paths may run in any order. Grid: x sequences, y heads and halves by
+// kKeepWaves, z layers.
+constexpr int kKeepWaves = 4;
+template <int DIM>
+__global__ __launch_bounds__(64 * kKeepWaves) void kv4_keep_path_kernel(Kv4Pool pool, int64_t layer_bytes, const int *cu,
+                                                                        int tokens, const int *path, const int *accepted,
+                                                                        int *lengths_out) {
+  constexpr int kGroups = DIM / 32, kHeld = kMostDrafts * kGroups / 64;
+  const int sequence = blockIdx.x, lane = threadIdx.x & 63, half = blockIdx.y * kKeepWaves + (threadIdx.x >> 6);
+  const int begin = min(max(cu[sequence], 0), tokens), count = min(max(cu[sequence + 1], begin), tokens) - begin;
+  const int rows = min(count, kMostDrafts);
+  const int length = kv4_length(pool, sequence), context = length - count;
+  const int kept = min(max(accepted[sequence], -1), rows - 1);
+  if (half == 0 && lane == 0 && blockIdx.z == 0) lengths_out[sequence] = context + kept + 1;
+  if (half >= 2 * pool.kv_heads || kept < 1) return;
+  const int64_t half_bytes = kv4_half_bytes(pool.page_shift, DIM), scales_at = (int64_t)(DIM / 2) << pool.page_shift;
+  uint8_t *layer = pool.pages + blockIdx.z * layer_bytes;
+  const int group = lane % kGroups;
+  auto at = [&](int position) -> uint8_t * {  // this group's codes; null where there is none
+    const Row row = row_at(pool, {sequence, position});
+    if (row.page < 0) return nullptr;
+    return layer + (row.page * pool.kv_heads * 2 + half) * half_bytes + row.offset * (DIM / 2) + 16 * group;
+  };
+  auto scale_of = [&](uint8_t *codes, int position) {  // beside the codes at `at(position)`
+    const int offset = position & ((1 << pool.page_shift) - 1);
+    return codes - offset * (DIM / 2) - 16 * group + scales_at + offset * kGroups + group;
+  };
+  u32x4 codes[kHeld];
+  uint8_t scale[kHeld];
+  uint8_t *to[kHeld];
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) {
+    const int j = 1 + (64 * i + lane) / kGroups;
+    to[i] = nullptr;
+    if (j > kept) continue;
+    const int from = path[begin + j];
+    if (from < 0 || from >= rows || from == j) continue;
+    uint8_t *source = at(context + from);
+    to[i] = source ? at(context + j) : nullptr;
+    if (!to[i]) continue;
+    codes[i] = *reinterpret_cast<const u32x4 *>(source);
+    scale[i] = *scale_of(source, context + from);
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // everything is held
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) {
+    if (!to[i]) continue;
+    *reinterpret_cast<u32x4 *>(to[i]) = codes[i];
+    *scale_of(to[i], context + 1 + (64 * i + lane) / kGroups) = scale[i];
+  }
+}
+
 // Page pairs travel as kernel arguments: no copy to the device, nothing to keep alive.
 struct Kv4Pairs {
   uint32_t src[kKv4Pairs], dst[kKv4Pairs];
@@ -205,6 +380,32 @@ hipError_t launch_kv4_read(uint16_t *k, int64_t k_token, int64_t k_head, uint16_
                        dim3((unsigned)((tokens + (int64_t)rows - 1) / rows), (unsigned)pool.kv_heads * 2), dim3(kThreads), 0,
                        stream, k, k_token, k_head, v, v_token, v_head, tokens, cu, pool);
   });
+  return hipGetLastError();
+}
+
+hipError_t launch_kv4_append_rope(Kv4Rope a, bool interleaved, bool f16, int dim, const Kv4Pool &pool, hipStream_t stream) {
+  const int heads = a.heads + 2 * pool.kv_heads, rows = kThreads / (dim / 8);
+  const int64_t blocks = (a.tokens + (int64_t)rows - 1) / rows;
+  a.per = 1;
+  by_type(f16, dim, [&](auto type, auto d) {
+    auto launch = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, dim3((unsigned)blocks, (unsigned)((heads + a.per - 1) / a.per)), dim3(kThreads), 0, stream, a, pool);
+    };
+    constexpr bool kF16 = decltype(type)::value;
+    constexpr int kDim = decltype(d)::value;
+    if (interleaved) launch(kv4_append_rope_kernel<kF16, kDim, true>);
+    else launch(kv4_append_rope_kernel<kF16, kDim, false>);
+  });
+  return hipGetLastError();
+}
+
+hipError_t launch_kv4_keep_path(const Kv4Pool &pool, int dim, int layers, int64_t layer_bytes, const int *cu, int tokens,
+                                const int *path, const int *accepted, int *lengths_out, hipStream_t stream) {
+  const dim3 grid((unsigned)pool.sequences, (unsigned)((2 * pool.kv_heads + kKeepWaves - 1) / kKeepWaves), (unsigned)layers);
+  if (dim == 128) hipLaunchKernelGGL(kv4_keep_path_kernel<128>, grid, dim3(64 * kKeepWaves), 0, stream, pool, layer_bytes, cu, tokens, path,
+                                   accepted, lengths_out);
+  else hipLaunchKernelGGL(kv4_keep_path_kernel<64>, grid, dim3(64 * kKeepWaves), 0, stream, pool, layer_bytes, cu, tokens, path,
+                                   accepted, lengths_out);
   return hipGetLastError();
 }
 

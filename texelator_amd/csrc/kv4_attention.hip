@@ -85,12 +85,6 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, float &sum) {
   }
 }
 
-template <bool F16>
-__device__ __forceinline__ uint16_t to_half_bits(float v) {
-  if constexpr (F16) return __builtin_bit_cast(uint16_t, (_Float16)v);
-  else return to_bf(v);
-}
-
 // Over the four lanes that hold one query (lane, + 16, + 32, + 48).
 __device__ __forceinline__ float quarters_max(float v) {
   auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);

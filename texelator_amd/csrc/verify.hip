@@ -1,0 +1,510 @@
+// Verification of drafted tokens against the target model's probabilities (gfx950), from given random numbers.
+//
+// No reference counterpart: the reference decodes one token at a time.
+//
+// A sequence's rows are a tree: row 0 its last token, row i a draft behind row parents[i]. p_v = softmax(logits[v] / T). From
+// row 0 on, the drafts behind the row v that is reached are tried in the order of their rows:
+//   * given drafts: draft i is accepted where u_i (1 - sum of the earlier drafts' p_v) < p_v(token i), a token that an earlier one
+//     of them has never; where none is, the closing token is drawn from p_v without their tokens;
+//   * chains sampled from a draft model, q_v = softmax(draft_logits[v] / T): accepted where u_i q_v(token i) < p_v(token i); else the
+//     closing token is drawn from max(p_v - q_v, 0);
+//   * T = 0: accepted where the token is the largest logit's (of equal ones the first), which is the closing token too.
+// A token is drawn as the first whose running sum in the vocabulary's order exceeds u_0 times the whole sum.
+//
+// Three launches. The first reads all logits once, a wave 64 * kLoads * 16 bytes of a row, and leaves the maximum and the sum
+// of exponentials of each such span, in 32 bits: enough for the tests (off by some 1e-7). The second finds every sequence's path: a
+// lane has a row, all drafts are tested at once and a row is reached where all rows that lead to it are taken. Its
+// workgroups then share the last row reached and sum its weights in 64 bits, a wave a span: a draw is as exact as those
+// sums are, and 150 thousand borders lie close. The third finds the span, then the token in it. For the residual max(p - q, 0) the
+// sums of p and q are only known after the second launch: it sums p's and q's weights over the tokens where p > q by the
+// first launch's sums; a token that those put on the wrong side adds at most 1e-7 of its own probability.
+#include <math.h>
+
+#include "elementwise.h"
+#include "kernels.h"
+#include "kv4.h"
+#include "ragged.h"
+
+namespace tx {
+
+namespace {
+
+constexpr int kThreads = 256, kWaves = kThreads / 64;
+constexpr int kLoads = 4;  // 16-byte loads of a lane
+
+// Elements of a lane's load, and of a wave's span.
+template <typename T>
+constexpr int kVector = 16 / (int)sizeof(T);
+template <typename T>
+constexpr int kSpan = 64 * kLoads * kVector<T>;
+
+struct Bf16 {
+  uint16_t bits;
+};
+struct Fp16 {
+  uint16_t bits;
+};
+__device__ __forceinline__ float widen(Bf16 v) { return bf(v.bits); }
+__device__ __forceinline__ float widen(Fp16 v) { return hf(v.bits); }
+__device__ __forceinline__ float widen(float v) { return v; }
+
+// 16 bytes at any element's address: rows of odd widths begin anywhere.
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
+
+template <typename T>
+__device__ __forceinline__ void widen_all(u32x4 raw, float *x) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(raw[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = widen(T{(uint16_t)(raw[i / 2] >> (16 * (i % 2)))});
+  }
+}
+
+// ln(2)^k / k!: 2^f is the sum of these times f^k.
+constexpr double power_of_ln2(int k) { return k == 0 ? 1.0 : power_of_ln2(k - 1) * 0.693147180559945309417232121458 / k; }
+
+// 2^y of y <= 0 in 64 bits: the Taylor sum of 2^f, |f| <= 1/2, to the twelfth power (off by 2e-16). NaN stays.
+__device__ __forceinline__ double exp2_64(double y) {
+  if (!(y >= -1100.0)) return y != y ? y : 0.0;
+  constexpr double kTerm[13] = {power_of_ln2(0), power_of_ln2(1), power_of_ln2(2),  power_of_ln2(3),  power_of_ln2(4),
+                                power_of_ln2(5), power_of_ln2(6), power_of_ln2(7),  power_of_ln2(8),  power_of_ln2(9),
+                                power_of_ln2(10), power_of_ln2(11), power_of_ln2(12)};
+  const double whole = rint(y), f = y - whole;
+  double sum = kTerm[12];
+#pragma unroll
+  for (int i = 11; i >= 0; --i) sum = __builtin_fma(sum, f, kTerm[i]);
+  return ldexp(sum, (int)whole);
+}
+
+// log2(e) / T; above zero and finite for every T above zero.
+__device__ __forceinline__ double rate_of(float temperature) { return fmin(1.44269504088896340736 / (double)temperature, 1e300); }
+
+struct Rows {
+  int begin, count;  // a sequence's rows: at most kMostDrafts
+};
+__device__ __forceinline__ Rows rows_of(const Verify &a, int sequence) {
+  const int begin = min(max(a.cu[sequence], 0), a.tokens);
+  return {begin, min(min(max(a.cu[sequence + 1], begin), a.tokens) - begin, kMostDrafts)};
+}
+__device__ __forceinline__ float temperature_of(const Verify &a, int sequence) {
+  return a.temperatures ? a.temperatures[sequence] : a.temperature;
+}
+__device__ __forceinline__ int wave_min_int(int v) { return -wave_max_int(-v); }
+
+// Grid: x spans by kWaves, y rows, z target and draft logits. Partial of a span: (maximum, sum of exp((x - maximum) / T)), or at
+// T = 0 (maximum, its first index); a NaN among the logits makes the sum (at T = 0 the maximum) NaN.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void verify_stats_kernel(Verify a) {
+  const int lane = threadIdx.x & 63, span = blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int row = blockIdx.y;
+  if (span >= a.spans) return;
+  const bool draft = blockIdx.z != 0;
+  const T *logits = reinterpret_cast<const T *>(draft ? a.draft : a.target) + row * (draft ? a.draft_row : a.target_row);
+  // The row's sequence: as many starts behind the first lie at or before it.
+  int sequence = 0;
+  for (int first = 0; first < a.sequences; first += 64) {
+    const bool before = first + lane < a.sequences && a.cu[first + lane + 1] <= row;
+    sequence += __builtin_popcountll(__builtin_amdgcn_ballot_w64(before));
+  }
+  if (sequence >= a.sequences || row < a.cu[0]) return;
+  const Rows rows = rows_of(a, sequence);
+  const int local = row - rows.begin;
+  if (local < 0 || local >= rows.count || (draft && local + 1 >= rows.count)) return;  // a chain's last row has no draft behind it
+  const float temperature = temperature_of(a, sequence);
+  if (draft && !(temperature > 0.f)) return;
+
+  constexpr int kVector = tx::kVector<T>;
+  const int first = span * kSpan<T> + lane * kVector;
+  float x[kLoads][kVector];
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) {
+    const int at = first + i * 64 * kVector;
+    if (at + kVector <= a.vocab) {
+      widen_all<T>(*reinterpret_cast<const u32x4_any *>(logits + at), x[i]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < kVector; ++j) x[i][j] = at + j < a.vocab ? widen(logits[at + j]) : -INFINITY;
+    }
+  }
+  float top = -INFINITY;
+  bool odd = false;
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i)
+#pragma unroll
+    for (int j = 0; j < kVector; ++j) top = fmaxf(top, x[i][j]);
+  top = wave_max(top);
+  float2 *partial = a.partials + ((int64_t)(draft ? a.tokens : 0) + row) * a.spans + span;
+  if (!(temperature > 0.f)) {
+    int index = 0x7FFFFFFF;
+#pragma unroll
+    for (int i = kLoads - 1; i >= 0; --i)
+#pragma unroll
+      for (int j = kVector - 1; j >= 0; --j) {
+        if (x[i][j] == top) index = first + i * 64 * kVector + j;
+        odd |= x[i][j] != x[i][j];
+      }
+    index = wave_min_int(index);
+    if (__builtin_amdgcn_ballot_w64(odd) != 0) top = NAN;
+    if (lane == 0) *partial = make_float2(top, __int_as_float(index));
+    return;
+  }
+  const float rate = (float)fmin(rate_of(temperature), 1e30), base = top == -INFINITY ? 0.f : top;
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i)
+#pragma unroll
+    for (int j = 0; j < kVector; ++j) sum += x[i][j] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((x[i][j] - base) * rate);
+  sum = wave_sum(sum);
+  if (lane == 0) *partial = make_float2(top, sum);
+}
+
+// What the second launch leaves of a sequence for the third.
+struct Closing {
+  int row;        // the last row reached, in the packed rows; -1: nothing to draw
+  int first;      // the sequence's first row
+  int slot;       // where the token goes
+  int residual;   // drawn from max(p - q, 0)
+  float temperature;
+  float top, draft_top;
+  int removed;  // tokens that are left out
+  int64_t tokens[kMostDrafts];
+};
+
+// Sums of a span of the last row: all weights of p and of q; of the tokens that may be drawn, those of p and of q.
+struct Sums {
+  double p, q, rest_p, rest_q;
+};
+
+template <typename T>
+__device__ __forceinline__ float logit(const void *logits, int64_t row_stride, int64_t row, int64_t token) {
+  return widen(reinterpret_cast<const T *>(logits)[row * row_stride + token]);
+}
+
+__device__ __forceinline__ double wave_sum64(double v) {
+#pragma unroll
+  for (int w = 1; w < 64; w *= 2) v += __shfl_xor(v, w);
+  return v;
+}
+
+// The weights of one token of the last row: of p, of q, and whether it may be drawn.
+template <typename T>
+struct Weights {
+  const Verify &a;
+  const Closing &c;
+  double rate;
+  double scale_p, scale_q;  // 1 / sums of p and of q, as well as they are known
+  __device__ __forceinline__ void at(int token, double &p, double &q, bool &rest) const {
+    const float x = logit<T>(a.target, a.target_row, c.row, token);
+    p = x == -INFINITY ? 0.0 : exp2_64(((double)x - (double)c.top) * rate);
+    q = 0.0;
+    rest = true;
+    if (c.residual) {
+      const float y = logit<T>(a.draft, a.draft_row, c.row, token);
+      q = y == -INFINITY ? 0.0 : exp2_64(((double)y - (double)c.draft_top) * rate);
+      rest = p * scale_p > q * scale_q;
+    }
+    for (int i = 0; i < c.removed; ++i) rest &= c.tokens[i] != token;
+  }
+};
+
+// Grid: x workgroups of a sequence, y sequences.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void verify_walk_kernel(Verify a) {
+  __shared__ float tops[2][kMostDrafts];    // maxima of the rows; of the draft's
+  __shared__ double sums[2][kMostDrafts];   // sums of their weights; at T = 0 the target's first largest token
+  __shared__ Closing closing;
+  __shared__ int order[kMostDrafts];  // the path's rows
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), sequence = blockIdx.y;
+  const Rows rows = rows_of(a, sequence);
+  Closing *kept = reinterpret_cast<Closing *>(a.closings) + sequence;
+  const bool writes = blockIdx.x == 0;
+  if (rows.count <= 0) {
+    if (writes && threadIdx.x == 0) {
+      a.accepted[sequence] = -1;
+      kept->row = -1;
+    }
+    return;
+  }
+  const float temperature = temperature_of(a, sequence);
+  const bool greedy = !(temperature > 0.f);
+  const double rate = greedy ? 0.0 : rate_of(temperature);
+  // The rows' statistics from their spans'.
+  const int kinds = a.draft && !greedy ? 2 : 1;
+  for (int i = wave; i < rows.count * kinds; i += kWaves) {
+    const int kind = i / rows.count, local = i % rows.count;
+    if (kind == 1 && local + 1 >= rows.count) continue;
+    const float2 *partial = a.partials + ((int64_t)(kind ? a.tokens : 0) + rows.begin + local) * a.spans;
+    float top = -INFINITY;
+    bool odd = false;
+    for (int s = lane; s < a.spans; s += 64) {
+      const float2 v = partial[s];
+      odd |= v.x != v.x;
+      top = fmaxf(top, v.x);
+    }
+    top = wave_max(top);
+    odd = __builtin_amdgcn_ballot_w64(odd) != 0;
+    if (greedy) {
+      int index = 0x7FFFFFFF;
+      for (int s = lane; s < a.spans; s += 64) {
+        const float2 v = partial[s];
+        if (v.x == top) index = min(index, __float_as_int(v.y));
+      }
+      index = wave_min_int(index);
+      if (lane == 0) sums[0][local] = odd || top == -INFINITY ? -1.0 : (double)index;
+    } else {
+      double sum = 0.0;
+      for (int s = lane; s < a.spans; s += 64) {
+        const float2 v = partial[s];
+        sum += v.x == -INFINITY ? (double)v.y : (double)v.y * exp2_64(((double)v.x - (double)top) * rate);
+      }
+      sum = wave_sum64(sum);
+      if (lane == 0) {
+        tops[kind][local] = top;
+        sums[kind][local] = sum;
+      }
+    }
+  }
+  __syncthreads();
+  if (wave == 0) {
+    // Lane i is row i.
+    const bool row = lane < rows.count;
+    int parent = -1;
+    int64_t token = -1;
+    float u = 0.f;
+    if (row) {
+      parent = a.parents ? a.parents[rows.begin + lane] : lane - 1;
+      token = a.ids[rows.begin + lane];
+      u = a.uniforms[rows.begin + lane];
+    }
+    if (lane == 0 || (uint32_t)parent >= (uint32_t)rows.count) parent = -1;
+    const bool child = row && parent >= 0, known = child && token >= 0 && token < a.vocab;
+    double p = 0.0, q = 0.0;
+    if (known) {
+      if (greedy) {
+        p = sums[0][parent] == (double)token ? 1.0 : 0.0;
+      } else {
+        const float x = logit<T>(a.target, a.target_row, rows.begin + parent, token);
+        p = x == -INFINITY ? 0.0 : exp2_64(((double)x - (double)tops[0][parent]) * rate) / sums[0][parent];
+        if (a.draft) {
+          const float y = logit<T>(a.draft, a.draft_row, rows.begin + parent, token);
+          q = y == -INFINITY ? 0.0 : exp2_64(((double)y - (double)tops[1][parent]) * rate) / sums[1][parent];
+        }
+      }
+    }
+    // Earlier drafts behind the same row: their tokens and probabilities.
+    double before = 0.0;
+    bool again = false;
+    for (int j = 1; j < rows.count; ++j) {
+      const int theirs = __shfl(parent, j);
+      const int64_t their_token = __shfl(token, j);
+      const double their_p = __shfl(again ? 0.0 : p, j);
+      const bool earlier = child && j < lane && theirs == parent;
+      again |= earlier && their_token == token;
+      before += earlier ? their_p : 0.0;
+    }
+    bool accept = p > 0.0 && !again;
+    if (!greedy) accept = accept && (a.draft ? (double)u * q < p : (double)u * (1.0 - before) < p);
+    const uint64_t accepts = __builtin_amdgcn_ballot_w64(accept);
+    // The first accepted draft behind a row is taken.
+    bool taken = accept;
+    for (int j = 1; j < rows.count; ++j) {
+      const int theirs = __shfl(parent, j);
+      taken &= !(j < lane && theirs == parent && (accepts >> j & 1));
+    }
+    const uint64_t fine = __builtin_amdgcn_ballot_w64(taken) | 1;
+    // The rows that lead to each, by doubled pointers; reached: row 0 is among them and all are taken.
+    uint64_t leads = (uint64_t)1 << lane;
+    int up = parent;
+#pragma unroll
+    for (int i = 0; i < 6; ++i) {
+      const int from = max(up, 0);
+      const uint64_t theirs = __shfl(leads, from);
+      const int further = __shfl(up, from);
+      leads |= up >= 0 ? theirs : 0;
+      up = up >= 0 ? further : -1;
+    }
+    const bool reached = row && (leads & 1) && (leads & ~fine) == 0;
+    const int depth = __builtin_popcountll(leads) - 1;
+    const int count = __builtin_popcountll(__builtin_amdgcn_ballot_w64(reached)) - 1;  // accepted drafts
+    const int last = __builtin_ctzll(__builtin_amdgcn_ballot_w64(reached && depth == count));
+    const uint64_t followers = __builtin_amdgcn_ballot_w64(child && parent == last);
+    if (writes) {
+      order[lane] = -1;
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      if (reached) order[depth] = lane;
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      const int at = order[lane], behind = order[min(lane + 1, kMostDrafts - 1)];
+      const int64_t theirs = __shfl(token, max(behind, 0));
+      if (row) a.path[rows.begin + lane] = at;
+      if (row && lane != count) a.next[rows.begin + lane] = lane < count ? theirs : -1;
+      if (lane == 0) a.accepted[sequence] = count;
+    }
+    if (lane == 0) {
+      closing.row = greedy ? -1 : rows.begin + last;
+      closing.first = rows.begin;
+      closing.slot = rows.begin + count;
+      closing.residual = a.draft && followers != 0;
+      closing.temperature = temperature;
+      closing.removed = a.draft ? 0 : __builtin_popcountll(followers);
+      if (!greedy) {
+        closing.top = tops[0][last];
+        closing.draft_top = closing.residual ? tops[1][last] : 0.f;
+      } else if (writes) {
+        a.next[rows.begin + count] = (int64_t)sums[0][last];
+      }
+    }
+    if (!a.draft && (followers >> lane & 1)) closing.tokens[__builtin_popcountll(followers & (((uint64_t)1 << lane) - 1))] = token;
+    if (lane == 0 && !greedy) {  // as well as they are known
+      sums[0][0] = 1.0 / sums[0][last];
+      sums[1][0] = closing.residual ? 1.0 / sums[1][last] : 0.0;
+    }
+  }
+  __syncthreads();
+  if (writes)
+    for (int i = threadIdx.x; i * sizeof(int) < sizeof(Closing); i += kThreads)
+      reinterpret_cast<int *>(kept)[i] = reinterpret_cast<const int *>(&closing)[i];
+  if (closing.row < 0) return;
+  const Weights<T> weights = {a, closing, rate, sums[0][0], sums[1][0]};
+  const int part = blockIdx.x * kWaves + wave, begin = part * a.part, end = min(begin + a.part, a.vocab);
+  Sums mine = {0.0, 0.0, 0.0, 0.0};
+  for (int token = begin + lane; token < end; token += 64) {
+    double p, q;
+    bool rest;
+    weights.at(token, p, q, rest);
+    mine.p += p;
+    mine.q += q;
+    mine.rest_p += rest ? p : 0.0;
+    mine.rest_q += rest ? q : 0.0;
+  }
+  mine.p = wave_sum64(mine.p);
+  mine.q = wave_sum64(mine.q);
+  mine.rest_p = wave_sum64(mine.rest_p);
+  mine.rest_q = wave_sum64(mine.rest_q);
+  if (lane == 0) reinterpret_cast<Sums *>(a.sums)[(int64_t)sequence * a.parts + part] = mine;
+}
+
+// Inclusive sum over the lanes of a wave.
+__device__ __forceinline__ double wave_scan64(double v, int lane) {
+#pragma unroll
+  for (int w = 1; w < 64; w *= 2) {
+    const double other = __shfl_up(v, w);
+    v += lane >= w ? other : 0.0;
+  }
+  return v;
+}
+
+// The first lane whose running sum exceeds `target`, the sums before it added to `before`; else the last lane with a weight, else -1.
+__device__ __forceinline__ int crossing(double v, double target, double &before, int lane) {
+  const double sum = before + wave_scan64(v, lane);
+  const uint64_t past = __builtin_amdgcn_ballot_w64(sum > target && v > 0.0), some = __builtin_amdgcn_ballot_w64(v > 0.0);
+  if (some == 0) return -1;
+  const int at = past ? __builtin_ctzll(past) : 63 - __builtin_clzll(some);
+  before = __shfl(sum - v, at);
+  return at;
+}
+
+// The closing token: the part of the last row in which the running sum passes, then the token in it. One wave a sequence.
+template <typename T>
+__global__ __launch_bounds__(64) void verify_pick_kernel(Verify a) {
+  const int lane = threadIdx.x, sequence = blockIdx.x;
+  const Closing &closing = reinterpret_cast<const Closing *>(a.closings)[sequence];
+  if (closing.row < 0) return;
+  const Sums *sums = reinterpret_cast<const Sums *>(a.sums) + (int64_t)sequence * a.parts;
+  // Lane l has the parts l * each .. of the row.
+  const int each = (a.parts + 63) / 64, first = lane * each, last = min(first + each, a.parts);
+  Sums mine = {0.0, 0.0, 0.0, 0.0};
+  for (int i = first; i < last; ++i) {
+    mine.p += sums[i].p;
+    mine.q += sums[i].q;
+    mine.rest_p += sums[i].rest_p;
+    mine.rest_q += sums[i].rest_q;
+  }
+  const double all_p = wave_sum64(mine.p), all_q = wave_sum64(mine.q);
+  const double scale_p = 1.0 / all_p, scale_q = closing.residual ? 1.0 / all_q : 0.0;
+  const bool residual = closing.residual;
+  // What counts of a sum, and whether anything does: else it is drawn from all of p.
+  auto rest_of = [&](const Sums &s) { return residual ? fmax(s.rest_p * scale_p - s.rest_q * scale_q, 0.0) : s.rest_p; };
+  const bool all = !(wave_sum64(rest_of(mine)) > 0.0);
+  auto value_of = [&](const Sums &s) { return all ? s.p : rest_of(s); };
+  double value = 0.0;
+  for (int i = first; i < last; ++i) value += value_of(sums[i]);
+  const double total = wave_sum64(value);
+  int64_t token = -1;
+  if (total > 0.0 && !(residual && !(all_q > 0.0))) {
+    const double target = (double)a.uniforms[closing.first] * total;
+    double before = 0.0;
+    // The lane, its part, the part's tokens: 64 runs of them a lane each, and the token.
+    const int l = crossing(value, target, before, lane);
+    const int base = l * each, count = min(base + each, a.parts) - base;
+    double held = lane < count ? value_of(sums[base + lane]) : 0.0;
+    const int part = base + crossing(held, target, before, lane);
+    const Weights<T> weights = {a, closing, rate_of(closing.temperature), scale_p, scale_q};
+    const int begin = part * a.part, end = min(begin + a.part, a.vocab), run = (end - begin + 63) / 64;
+    const int from = min(begin + lane * run, end), to = min(from + run, end);
+    // Once more with all of p where a part's rest was nothing but rounding.
+    for (int turn = 0; turn < 2 && token < 0; ++turn) {
+      auto weight_of = [&](int t) {
+        double p, q;
+        bool rest;
+        weights.at(t, p, q, rest);
+        return all || turn ? p : !rest ? 0.0 : residual ? p * scale_p - q * scale_q : p;
+      };
+      held = 0.0;
+      for (int t = from; t < to; ++t) held += weight_of(t);
+      double sum = before;
+      const int at = crossing(held, target, sum, lane);
+      if (at == lane) {
+        for (int t = from; t < to; ++t) {
+          const double w = weight_of(t);
+          sum += w;
+          if (w > 0.0) {
+            token = t;
+            if (sum > target) break;
+          }
+        }
+      }
+      token = __shfl(token, max(at, 0));
+    }
+  }
+  if (lane == 0) a.next[closing.slot] = token;
+}
+
+}  // namespace
+
+void verify_plan(Verify &a, int dtype_bytes, int cus) {
+  const int span = 64 * kLoads * 16 / dtype_bytes;
+  a.spans = (a.vocab + span - 1) / span;
+  // Workgroups that share a sequence's last row: two a CU in all, of at least 512 tokens each.
+  int64_t groups = 2 * (int64_t)cus / (a.sequences > 0 ? a.sequences : 1);
+  if (groups > a.vocab / 512) groups = a.vocab / 512;
+  if (groups > 64) groups = 64;
+  if (groups < 1) groups = 1;
+  a.groups = (int)groups;
+  a.parts = a.groups * kWaves;
+  a.part = (a.vocab + a.parts - 1) / a.parts;
+  auto whole = [](int64_t bytes) { return (bytes + 15) & ~(int64_t)15; };
+  a.closings_at = whole((int64_t)a.tokens * (a.draft ? 2 : 1) * a.spans * sizeof(float2));
+  a.sums_at = a.closings_at + whole((int64_t)a.sequences * sizeof(Closing));
+  a.workspace_bytes = a.sums_at + (int64_t)a.sequences * a.parts * sizeof(Sums);
+}
+
+hipError_t launch_verify(Verify a, int dtype, char *workspace, hipStream_t stream) {
+  a.partials = reinterpret_cast<float2 *>(workspace);
+  a.closings = workspace + a.closings_at;
+  a.sums = workspace + a.sums_at;
+  const dim3 stats((unsigned)((a.spans + kWaves - 1) / kWaves), (unsigned)a.tokens, a.draft ? 2 : 1);
+  auto launch = [&](auto type) {
+    using T = decltype(type);
+    if (a.tokens > 0) hipLaunchKernelGGL(verify_stats_kernel<T>, stats, dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL(verify_walk_kernel<T>, dim3((unsigned)a.groups, (unsigned)a.sequences), dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL(verify_pick_kernel<T>, dim3((unsigned)a.sequences), dim3(64), 0, stream, a);
+  };
+  if (dtype == kVerifyF32) launch(0.f);
+  else if (dtype == kVerifyF16) launch(Fp16{});
+  else launch(Bf16{});
+  return hipGetLastError();
+}
+
+}  // namespace tx

@@ -779,3 +779,227 @@ def kv4_copy_pages(pages: torch.Tensor, src: list[int], dst: list[int]) -> None:
     check(_lib.load().tx_kv4_copy_pages(pages.data_ptr(), layers[0] if layers else 1, num_pages, kv_heads * 2 * half,
                                         sources.buffer_info()[0], targets.buffer_info()[0], count, pages.device.index,
                                         _stream(pages)))
+
+
+# ---------------------------------------------------------------------------------------------
+# A drafted step: for every sequence the target model runs its last token and some drafted ones together
+
+MOST_DRAFT_ROWS = 64  # rows of one sequence
+
+
+def kv4_append_rope(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, pages: torch.Tensor,
+                    block_table: torch.Tensor, lengths: torch.Tensor, cu: torch.Tensor | None = None,
+                    positions: torch.Tensor | None = None, interleaved: bool = False, out: torch.Tensor | None = None,
+                    k_out: torch.Tensor | None = None) -> torch.Tensor:
+    """:func:`kv4_append` of keys turned by their positions (rotary embedding), and the queries turned, in one launch: returns
+    ``q`` ``[tokens, heads, dim]`` turned (into ``out`` where given), stores turned ``k`` and ``v`` as they are. ``cos`` and ``sin``: float32
+    ``[rows, rotary / 2]``, one angle for each pair of the first ``rotary`` dimensions (a multiple of 16, at most dim; the others pass), so
+    that a scaling for long contexts lies in the tables. Pairs are (i, i + rotary / 2), or (2 i, 2 i + 1) with ``interleaved``.
+    ``positions`` (int32 ``[tokens]``): each token's row of the tables, its place in the sequence where not given (the rows of a tree
+    of drafts are placed one behind the other, but their positions follow their depth); one outside the tables turns to NaN.
+    Queries are rounded once, from 32 bits; a key is stored as the nearest code to its exact value. ``k_out`` ``[tokens, kv_heads,
+    dim]`` receives the turned keys, where a prompt's attention needs them. ``out`` and ``k_out`` share no element with q, k and v."""
+    shape, device, code = q.shape, pages.device, _ROW_CODE.get(q.dtype)
+    if code is None or len(shape) != 3 or not q.is_cuda or q.device != device or q.stride(2) != 1 or q.dtype != k.dtype:
+        raise TexelatorError("q must be CUDA bf16 or fp16 [tokens, heads, dim] like k and v, the last dimension contiguous")
+    tokens, heads, dim = shape
+    cache = _kv4_args(pages, block_table, lengths, dim, device)
+    rows = _kv4_rows(k, v, cache[2], dim, device)
+    sequences = cache[-1]
+    _expect(rows[-1] == tokens and heads > 0, "q, k and v must have as many tokens")
+    if cu is None:
+        _expect(tokens == sequences, "without cu there is one token for each sequence")
+    else:
+        _expect_ints("cu", cu, sequences + 1, device)
+    if (cos.dtype != torch.float32 or sin.dtype != torch.float32 or len(cos.shape) != 2 or cos.shape != sin.shape or cos.device != device
+            or sin.device != device or (cos.stride(1) != 1 and cos.shape[1] != 1) or (sin.stride(1) != 1 and sin.shape[1] != 1)):
+        raise TexelatorError("cos and sin must be float32 [rows, rotary / 2] on the pages' device, rows contiguous")
+    if positions is not None:
+        _expect_ints("positions", positions, tokens, device)
+    if out is None:
+        out = torch.empty(shape, dtype=q.dtype, device=device)
+    else:
+        _expect_rows("out", out, q, heads, dim)
+        _expect(out.shape[0] == tokens, "out must be shaped like q")
+    if k_out is not None:
+        _expect_rows("k_out", k_out, q, cache[2], dim)
+        _expect(k_out.shape[0] == tokens, "k_out must be shaped like k")
+    if tokens == 0 or sequences == 0:
+        return out
+    q_strides, out_strides, k_out_strides = q.stride(), out.stride(), (0, 0) if k_out is None else k_out.stride()
+    check(_lib.load().tx_kv4_append_rope(
+        q.data_ptr(), q_strides[0], q_strides[1], *rows, heads, cos.data_ptr(), cos.stride(0), sin.data_ptr(), sin.stride(0),
+        cos.shape[0], 2 * cos.shape[1], bool(interleaved), _ptr(positions), _ptr(cu), *cache, out.data_ptr(), out_strides[0],
+        out_strides[1], _ptr(k_out), k_out_strides[0], k_out_strides[1], device.index, _stream_address(device)))
+    return out
+
+
+@functools.lru_cache(maxsize=256)
+def _kv4_tree_workspace_bytes(*sizes: int) -> int:
+    out = ctypes.c_int64(0)
+    check(_lib.load().tx_kv4_tree_attention_workspace(*sizes, out))
+    return out.value
+
+
+def kv4_tree_attention_workspace_bytes(pages: torch.Tensor, block_table: torch.Tensor, tokens: int, heads: int, head_dim: int) -> int:
+    """Device scratch of :func:`kv4_tree_attention`: it depends on shapes alone, not on the lengths or the rows' sequences."""
+    _expect(pages.is_cuda and block_table.dim() == 2, "pages must be a CUDA tensor, block_table [sequences, pages]")
+    sequences, max_pages = block_table.shape
+    page_size = _kv4_page_size(pages.shape, head_dim)
+    return _kv4_tree_workspace_bytes(sequences, tokens, heads, pages.shape[1], head_dim, page_size, max_pages, pages.device.index)
+
+
+def kv4_tree_attention(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor, cu: torch.Tensor,
+                       scale: float, parents: torch.Tensor | None = None, workspace: torch.Tensor | None = None,
+                       out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of drafted rows over a paged 4-bit cache: ``q`` ``[tokens, heads, dim]`` bf16 or fp16 (every query 16-byte aligned).
+    Sequence s has the rows ``cu[s] .. cu[s + 1] - 1`` (int32 ``[sequences + 1]``, at most :data:`MOST_DRAFT_ROWS` of each; those behind
+    are left as they are), which are the last of its ``lengths[s]`` positions, stored already (:func:`kv4_append_rope`). A row sees
+    the positions before all of its sequence's rows, itself, and the rows that lead to it: row i follows row ``parents[i]`` of
+    its sequence (int32 ``[tokens]``, -1 or any number outside for none), without ``parents`` the row before it. Returns ``[tokens,
+    heads, dim]``: zeros for a row that sees no position in the pool; rows that belong to no sequence are left as they are.
+    What a row does not see may hold anything. ``out`` shares no element with q. Arithmetic as in :func:`kv4_attention`.
+    ``workspace``: :func:`kv4_tree_attention_workspace_bytes` bytes that no call running at the same time uses; allocated on the
+    current stream where not given."""
+    shape, device, code = q.shape, q.device, _ROW_CODE.get(q.dtype)
+    if code is None or len(shape) != 3 or not q.is_cuda or q.stride(2) != 1:
+        raise TexelatorError("q must be CUDA bf16 or fp16 [tokens, heads, dim], the last dimension contiguous")
+    tokens, heads, dim = shape
+    cache = _kv4_args(pages, block_table, lengths, dim, device)
+    sequences = cache[-1]
+    _expect(heads > 0 and heads % cache[2] == 0, "q must have a multiple of the pages' heads")
+    _expect_ints("cu", cu, sequences + 1, device)
+    if parents is not None:
+        _expect_ints("parents", parents, tokens, device)
+    if out is None:
+        out = q.new_empty(shape)
+    else:
+        _expect_rows("out", out, q, heads, dim)
+        _expect(out.shape[0] == tokens, "out must be shaped like q")
+    if sequences == 0 or tokens == 0:
+        return out
+    if workspace is None:
+        size = _kv4_tree_workspace_bytes(sequences, tokens, heads, cache[2], dim, cache[4], cache[7], device.index)
+        workspace = torch.empty(size, dtype=torch.uint8, device=device) if size else None  # short sequences need no scratch
+    else:
+        _expect(workspace.is_cuda and workspace.is_contiguous() and workspace.device == device,
+                "workspace must be a contiguous CUDA tensor on the same device")
+        size = workspace.nbytes
+    q_strides, out_strides = q.stride(), out.stride()
+    check(_lib.load().tx_kv4_tree_attention(
+        q.data_ptr(), q_strides[0], q_strides[1], code, tokens, heads, cu.data_ptr(), _ptr(parents), *cache, float(scale),
+        _ptr(workspace), size, out.data_ptr(), out_strides[0], out_strides[1], device.index, _stream_address(device)))
+    return out
+
+
+_LOGIT_CODE = {**_ROW_CODE, torch.float32: _lib.TX_DTYPE_F32}
+
+
+@functools.lru_cache(maxsize=256)
+def _verify_workspace_bytes(*sizes: int) -> int:
+    out = ctypes.c_int64(0)
+    check(_lib.load().tx_verify_drafts_workspace(*sizes, out))
+    return out.value
+
+
+def verify_drafts_workspace_bytes(logits: torch.Tensor, sequences: int, sampled: bool = False) -> int:
+    """Device scratch of :func:`verify_drafts`; ``sampled``: with ``draft_logits``."""
+    _expect(logits.is_cuda and logits.dim() == 2 and logits.dtype in _LOGIT_CODE, "logits must be CUDA bf16, fp16 or fp32 [tokens, vocab]")
+    return _verify_workspace_bytes(_LOGIT_CODE[logits.dtype], *logits.shape, sequences, bool(sampled), logits.device.index)
+
+
+def verify_drafts(logits: torch.Tensor, ids: torch.Tensor, uniforms: torch.Tensor, cu: torch.Tensor,
+                  parents: torch.Tensor | None = None, draft_logits: torch.Tensor | None = None,
+                  temperature: torch.Tensor | float = 1.0, workspace: torch.Tensor | None = None,
+                  out: tuple[torch.Tensor, torch.Tensor, torch.Tensor] | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Which drafted tokens the target model accepts, and the token behind them, from given random numbers. ``logits`` ``[tokens,
+    vocab]`` (bf16, fp16 or fp32): the target's at every row; the rows ``cu[s] .. cu[s + 1] - 1`` of a sequence (at most
+    :data:`MOST_DRAFT_ROWS`) are its last token and, behind it, drafts ``ids`` (int64 ``[tokens]``; row 0's is not used), row i
+    behind row ``parents[i]`` (int32 ``[tokens]``; without, each behind the one before it). ``uniforms``: float32 ``[tokens]`` in
+    [0, 1), a draft's for its test, row 0's for the closing token. With p the softmax of a row's logits over ``temperature`` (a number, or
+    float32 ``[sequences]``), the drafts behind the row that is reached are tried in order:
+
+    * given drafts: x is accepted where ``u * (1 - sum of earlier ones' p) < p(x)``; where none is, the closing token is drawn from p
+      without them (the distribution of the new tokens is p's own, whatever the drafts);
+    * ``draft_logits`` ``[tokens, vocab]``, chains alone: x, drawn from their softmax q at the same temperature, is accepted where
+      ``u * q(x) < p(x)``; else the closing token is drawn from max(p - q, 0);
+    * temperature 0 (or below): the largest logit's token, of equal ones the first, is accepted and closes.
+
+    Draws are exact to 64-bit sums. Returns ``(accepted, path, next)``: int32 ``[sequences]``, accepted drafts (-1 for a sequence without
+    rows); int32 ``[tokens]``, the rows of the path from row 0 on; int64 ``[tokens]``, the new tokens, the closing one last; both
+    from ``cu[s]`` on, -1 behind. The closing token is -1 where the last row's probabilities are undefined (a NaN or, above
+    temperature 0, an infinity among the logits, or nothing above -infinity). Rows that belong to no sequence are left as they are.
+    ``workspace``: :func:`verify_drafts_workspace_bytes` bytes that no call running at the same time uses."""
+    shape, device, code = logits.shape, logits.device, _LOGIT_CODE.get(logits.dtype)
+    if code is None or len(shape) != 2 or not logits.is_cuda or (logits.stride(1) != 1 and shape[1] != 1):
+        raise TexelatorError("logits must be CUDA bf16, fp16 or fp32 [tokens, vocab], rows contiguous")
+    tokens, vocab = shape
+    sequences = cu.numel() - 1
+    _expect(sequences >= 0, "cu must be int32 [sequences + 1]")
+    _expect_ints("cu", cu, sequences + 1, device)
+    if ids.dtype != torch.int64 or ids.shape != (tokens,) or ids.device != device or not ids.is_contiguous():
+        raise TexelatorError(f"ids must be a contiguous int64 [{tokens}] on the same device")
+    if uniforms.dtype != torch.float32 or uniforms.shape != (tokens,) or uniforms.device != device or not uniforms.is_contiguous():
+        raise TexelatorError(f"uniforms must be a contiguous float32 [{tokens}] on the same device")
+    if parents is not None:
+        _expect_ints("parents", parents, tokens, device)
+    if draft_logits is not None:
+        _expect(parents is None, "sampled drafts are chains: draft_logits go without parents")
+        if (draft_logits.dtype != logits.dtype or draft_logits.shape != shape or draft_logits.device != device
+                or (draft_logits.stride(1) != 1 and vocab != 1)):
+            raise TexelatorError("draft_logits must be like logits, rows contiguous")
+    heat = None
+    if isinstance(temperature, torch.Tensor):
+        heat, temperature = temperature, 0.0
+        if heat.dtype != torch.float32 or heat.shape != (sequences,) or heat.device != device or not heat.is_contiguous():
+            raise TexelatorError(f"temperature must be a number or a contiguous float32 [{sequences}] on the same device")
+    if out is None:
+        accepted, path = (torch.empty(n, dtype=torch.int32, device=device) for n in (sequences, tokens))
+        following = torch.empty(tokens, dtype=torch.int64, device=device)
+    else:
+        accepted, path, following = out
+        _expect_ints("accepted", accepted, sequences, device)
+        _expect_ints("path", path, tokens, device)
+        if following.dtype != torch.int64 or following.shape != (tokens,) or following.device != device or not following.is_contiguous():
+            raise TexelatorError(f"next must be a contiguous int64 [{tokens}] on the same device")
+    if sequences == 0:
+        return accepted, path, following
+    if workspace is None:
+        size = _verify_workspace_bytes(code, tokens, vocab, sequences, draft_logits is not None, device.index)
+        workspace = torch.empty(size, dtype=torch.uint8, device=device)
+    else:
+        _expect(workspace.is_cuda and workspace.is_contiguous() and workspace.device == device,
+                "workspace must be a contiguous CUDA tensor on the same device")
+        size = workspace.nbytes
+    check(_lib.load().tx_verify_drafts(
+        logits.data_ptr(), logits.stride(0), _ptr(draft_logits), 0 if draft_logits is None else draft_logits.stride(0), code, tokens,
+        vocab, ids.data_ptr(), uniforms.data_ptr(), cu.data_ptr(), _ptr(parents), sequences, _ptr(heat), float(temperature),
+        workspace.data_ptr(), size, accepted.data_ptr(), path.data_ptr(), following.data_ptr(), device.index, _stream_address(device)))
+    return accepted, path, following
+
+
+def kv4_keep_path(pages: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor, cu: torch.Tensor, path: torch.Tensor,
+                  accepted: torch.Tensor, head_dim: int, out: torch.Tensor | None = None) -> torch.Tensor:
+    """The rows of every sequence's accepted path (:func:`verify_drafts`) moved together in one pool (:func:`kv4_pages`) or in all
+    layers' pools ``[layers, ...]`` at once: the row of step j to the place of row j. Returns the lengths that are left, int32
+    ``[sequences]``, ``lengths - rows + accepted + 1`` (into ``out`` where given, which is not ``lengths`` itself). What rows lie
+    behind is stale, as any position past a length."""
+    _expect(pages.is_cuda and pages.dtype == torch.uint8 and pages.dim() in (4, 5) and pages.is_contiguous(),
+            "pages must be contiguous CUDA uint8 [num_pages, kv_heads, 2, page bytes], layers before it or not")
+    layered = pages.dim() == 5
+    _expect(not layered or pages.shape[0] > 0, "pages must have layers")
+    device = pages.device
+    cache = _kv4_args(pages[0] if layered else pages, block_table, lengths, head_dim, device)
+    sequences = cache[-1]
+    tokens = path.numel()
+    _expect_ints("cu", cu, sequences + 1, device)
+    _expect_ints("path", path, tokens, device)
+    _expect_ints("accepted", accepted, sequences, device)
+    if out is None:
+        out = torch.empty(sequences, dtype=torch.int32, device=device)
+    else:
+        _expect_ints("out", out, sequences, device)
+    if sequences:
+        check(_lib.load().tx_kv4_keep_path(cache[0], pages.shape[0] if layered else 1, *cache[1:], cu.data_ptr(), tokens,
+                                           path.data_ptr(), accepted.data_ptr(), out.data_ptr(), device.index, _stream_address(device)))
+    return out
