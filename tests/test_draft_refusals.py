@@ -104,7 +104,7 @@ def test_sizes_of_workspaces():
         assert lib.tx_kv4_tree_attention_workspace(3, tokens, 16, 2, 128, 64, 500, 0, out) == _lib.TX_OK
         sizes.append(out.value)
     assert sizes == sorted(sizes) and sizes[0] > 0 and all(n % 16 == 0 for n in sizes)
-    for bad in ((3, 20, 15, 2, 128, 64, 5), (3, -1, 16, 2, 128, 64, 5), (3, 20, 16, 2, 96, 64, 5), (-1, 20, 16, 2, 128, 64, 5),
+    for bad in ((3, 20, 15, 2, 128, 64, 5), (3, 20, 1 << 14, 2, 128, 64, 5), (3, -1, 16, 2, 128, 64, 5), (3, 20, 16, 2, 96, 64, 5), (-1, 20, 16, 2, 128, 64, 5),
                 (4096, 20, 16, 2, 128, 1024, 1 << 20)):
         assert lib.tx_kv4_tree_attention_workspace(*bad, 0, out) == _lib.TX_ERR_INVALID
     assert lib.tx_kv4_tree_attention_workspace(3, 20, 16, 2, 128, 64, 5, 0, None) == _lib.TX_ERR_INVALID

@@ -1750,7 +1750,7 @@ int tx_kv4_tree_attention_workspace(int sequences, int64_t tokens, int heads, in
   const char *bad = kv4_pool(a.pool, reinterpret_cast<void *>(16), 1, kv_heads, head_dim, page_size, &dummy, max_pages, max_pages,
                              &dummy, sequences);
   if (!bad) bad = draft_rows(&dummy, tokens, nullptr);
-  if (!bad && (heads <= 0 || heads % kv_heads || heads > 65535)) bad = "heads must be a multiple of kv_heads";
+  if (!bad && (heads <= 0 || heads % kv_heads || heads / kv_heads > 4096)) bad = "heads must be a multiple of kv_heads, at most 4096 of it";
   if (!bad) {
     a.tokens = (int)tokens;
     a.group = heads / kv_heads;
@@ -1776,7 +1776,7 @@ int tx_kv4_tree_attention(const void *q, int64_t q_token, int64_t q_head, int dt
   if (!bad) bad = draft_rows(cu, tokens, parents);
   if (!bad && (!q || !out)) bad = "null pointer";
   if (!bad && dtype != TX_DTYPE_F16 && dtype != TX_DTYPE_BF16) bad = "q must be FP16 or BF16";
-  if (!bad && (heads <= 0 || heads % kv_heads || heads > 65535)) bad = "heads must be a multiple of kv_heads";
+  if (!bad && (heads <= 0 || heads % kv_heads || heads / kv_heads > 4096)) bad = "heads must be a multiple of kv_heads, at most 4096 of it";
   if (!bad && (reinterpret_cast<uintptr_t>(q) % 16 || (q_token | q_head) % 8)) bad = "every query must be 16-byte aligned";
   if (!bad && (reinterpret_cast<uintptr_t>(out) % 8 || (out_token | out_head) % 4)) bad = "every output row must be 8-byte aligned";
   if (!bad && (q_token | q_head | out_token | out_head) < 0) bad = "negative strides";
@@ -1798,8 +1798,9 @@ int tx_kv4_tree_attention(const void *q, int64_t q_token, int64_t q_head, int dt
   a.out_head = out_head;
   a.cu = cu;
   a.parents = parents;
+  a.group_inverse = (uint32_t)((((uint64_t)1 << 32) + a.group - 1) / a.group);  // not used where it is 2^32
   set_scale(scale, a.sl2, a.q_and, a.q_xor);
-  a.lag = tx::kPackedLag / a.sl2;
+  a.lag = std::min(tx::kPackedLag / a.sl2, 1e38f);  // finite: beyond a maximum of -infinity too
   a.pieces = static_cast<float *>(workspace);
   tx::kv4_tree_plan(a, head_dim, multiprocessors(device));
   if (workspace_bytes < a.piece_bytes || (a.piece_bytes > 0 && !workspace))

@@ -72,6 +72,7 @@ struct Kv4Tree {
   const int *cu;       // [sequences + 1] first rows
   const int *parents;  // [tokens] within the sequence, or null: each row follows the one before it
   int tokens, group;
+  uint32_t group_inverse;  // ceil(2^32 / group)
   float sl2, lag;  // lag: kPackedLag / sl2
   uint32_t q_and, q_xor;
   float *pieces;  // results of heads that several workgroups share

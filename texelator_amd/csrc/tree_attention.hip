@@ -6,22 +6,23 @@
 // of a sequence's `length` positions the last `rows` are its drafted rows; row i sees every position before them (the context)
 // and the rows that its parents lead to, itself included.
 //
-// A KV head's queries are columns, row by row and query head by query head: rows * group of them, in blocks of 32. Work: a unit
-// is kTile positions of one sequence, KV head and pass (of up to four column blocks); the units of all lie in one row, and every
-// workgroup takes an equal run of them, whatever the lengths (it finds its place from the lengths itself, so that a captured call serves
-// any). A run that covers a whole (sequence, head, pass) writes its output; the others leave (max, sum, unnormalised
-// output) for the combine kernel, at most two such pieces a workgroup.
+// A KV head's queries are columns, row by row and query head by query head: rows * group of them, in blocks of 32, up to four blocks
+// a pass. Work: a tile is kTile positions of one sequence, KV head and pass, and weighs as many ticks as its blocks take time;
+// the ticks of all lie in one row, and every workgroup takes an equal run of them, whatever the lengths (it finds its place from
+// the lengths itself, so that a captured call serves any). A run that covers a whole (sequence, head, pass) writes its output; the
+// others leave (max, sum, unnormalised output) for the combine kernel, at most two such pieces a workgroup.
 //
-// A workgroup converts a unit's codes once, into LDS (each thread one scale group of keys and one of values); a wave then has one
-// column block and, where there are fewer blocks than waves, a share of the positions:
+// A workgroup converts a tile's codes once, into LDS, each thread a scale group of keys and one of values: the conversion is what
+// single tokens' attention spends most on, and what the columns share. A wave then has one column block and, where there are
+// fewer blocks than waves, a share of the positions:
 //   * S^T = K q^T (v_mfma_f32_32x32x16: A = 32 keys, B = the block's queries, held in registers): a lane holds 16 scores of one
 //     query, the maximum is in-lane but for one lane swap, and the probabilities, rounded to 16 bits in place, are the B operand of
 //     O^T = V^T P^T, whose A operand the transposing LDS reads give;
-//   * a query's running maximum follows its scores only where they pass it by 2^4;
-//   * the next unit's codes are under way while this one is multiplied.
-// Positions past the length, and those of pages outside the pool, are stored as zeros and their scores hidden. A draft's values that are
-// not finite are stored as zeros too and reach the rows that see them by themselves: zero probabilities of the others would
-// make them NaN.
+//   * a query's running maximum follows its scores only where they pass it by 2^4: rescaling is 64 multiplications;
+//   * the next tile's codes are under way while this one is multiplied, from pages whose ids are scalar loads a tile earlier.
+// Positions past the length, and those of pages outside the pool, become zeros before they are converted and their scores
+// -infinity. A draft's values that are not finite become zeros too and are added, for the rows that see them, at the end: zero
+// probabilities of the others would make them NaN.
 // Statistics and sums in fp32; sums run over the probabilities as rounded. In fp16 they are held times 2^11, in bf16 times a power
 // of two below 1 / (2^4 length), so that sums of the largest values stay finite.
 #include <math.h>
@@ -41,10 +42,13 @@ constexpr int kWaves = 4, kThreads = 64 * kWaves;
 constexpr int kCols = 32;      // columns of a block
 constexpr int kPass = kWaves;  // blocks of a pass
 
-// Positions of a unit: a thread converts one group of 32 elements of its keys and one of its values.
+// Positions of a tile: a thread converts one group of 32 elements of its keys and one of its values.
 template <int DIM>
 constexpr int kTile = kThreads / (DIM / 32);
-constexpr int kResident = 3;  // workgroups that a CU holds
+// Workgroups that a CU holds. Three of head dimension 128 have 168 registers a thread and spill 37: 173 us instead of 175 for 80
+// columns and 262,144 positions, but 35 instead of 28 for 24 trees, whose runs are short.
+template <int DIM>
+constexpr int kResident = DIM == 128 ? 2 : 3;
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
@@ -89,43 +93,62 @@ __device__ __forceinline__ float halves_sum(float v) {
 // All of the workgroup's LDS accesses so far are done; loads from memory stay in flight.
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-// What starting and ending a (head, pass) costs, in units.
-constexpr int kStart = 1;
+// What starting and ending a (head, pass) costs, in ticks.
+constexpr int kStart = 6;
+// What a tile costs: up to two blocks a wave has 32 of its positions (at dim 64 two blocks or one 64 or 32), else all of them.
+constexpr int kMostWeight = 3;
+__device__ __forceinline__ int weight_of(int blocks) { return blocks <= 2 ? 2 : kMostWeight; }
+
+// A value that all lanes have, in a scalar register.
+__device__ __forceinline__ int scalar(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
 // A sequence as the grid sees it.
 struct Drafts {
   int begin, rows;  // its first row, and how many: at most kMostDrafts
   int length, context;
-  int columns, passes;
+  int columns, passes, blocks;  // column blocks of every pass but the last, which may have fewer
 };
-__device__ __forceinline__ Drafts drafts_of(const Kv4Tree &a, int sequence) {
+__host__ __device__ __forceinline__ int pieces_of(int count, int most) { return (count + most - 1) / most; }
+__device__ __forceinline__ Drafts drafts_of(const Kv4Tree &a, int first, int end, int length) {
   Drafts d;
-  const int first = min(max(a.cu[sequence], 0), a.tokens), end = min(max(a.cu[sequence + 1], first), a.tokens);
+  first = min(max(first, 0), a.tokens);
+  end = min(max(end, first), a.tokens);
   d.begin = first;
-  d.length = kv4_length(a.pool, sequence);
-  d.context = d.length - (end - first);
+  d.length = length;
+  d.context = length - (end - first);
   d.rows = min(end - first, kMostDrafts);
   d.columns = d.rows * a.group;
-  d.passes = (d.columns + kCols * kPass - 1) / (kCols * kPass);
+  const int blocks = pieces_of(d.columns, kCols);
+  d.passes = pieces_of(blocks, kPass);
+  d.blocks = d.passes <= 1 ? blocks : pieces_of(blocks, d.passes);
   return d;
 }
+__device__ __forceinline__ Drafts drafts_of(const Kv4Tree &a, int sequence) {
+  return drafts_of(a, a.cu[sequence], a.cu[sequence + 1], kv4_length(a.pool, sequence));
+}
+// The same of a sequence that all lanes ask for, in scalar registers: page ids then stay scalar.
+__device__ __forceinline__ Drafts scalar_drafts(const Kv4Tree &a, int sequence) {
+  return drafts_of(a, scalar(a.cu[sequence]), scalar(a.cu[sequence + 1]), scalar(kv4_length(a.pool, sequence)));
+}
+
 template <int TILE>
 __device__ __forceinline__ int tiles_of(int length) { return max(1, (length + TILE - 1) / TILE); }
+// Ticks of a (head, pass), the start among them: passes count alike, whatever their blocks.
 template <int TILE>
-__device__ __forceinline__ int units_of(const Kv4Tree &a, const Drafts &d) {
-  return a.pool.kv_heads * d.passes * (kStart + tiles_of<TILE>(d.length));
-}
-__device__ __forceinline__ int run_units(int total, const Kv4Tree &a) { return (total + a.workgroups - 1) / a.workgroups; }
+__device__ __forceinline__ int part_ticks(const Drafts &d) { return kStart + weight_of(d.blocks) * tiles_of<TILE>(d.length); }
+template <int TILE>
+__device__ __forceinline__ int ticks_of(const Kv4Tree &a, const Drafts &d) { return a.pool.kv_heads * d.passes * part_ticks<TILE>(d); }
+// Ticks of every workgroup: at least one tile's.
+__device__ __forceinline__ int run_ticks(int total, const Kv4Tree &a) { return max((total + a.workgroups - 1) / a.workgroups, kMostWeight); }
 
-// Column blocks are shared out evenly over the passes.
-__device__ __forceinline__ int blocks_a_pass(const Drafts &d) {
-  const int blocks = (d.columns + kCols - 1) / kCols;
-  return (blocks + d.passes - 1) / d.passes;
-}
-
-__device__ __forceinline__ bool known_position(const Kv4Pool &pool, int sequence, int position) {
-  if (position < 0) return false;
-  return (uint32_t)pool.table[sequence * pool.table_stride + (position >> pool.page_shift)] < (uint64_t)pool.num_pages;
+// The row of a column, and its query head in the KV head's group: column / a.group by the host's ceil(2^32 / group), exact for
+// columns times group below 2^32.
+struct Query {
+  int row, head;
+};
+__device__ __forceinline__ Query query_of(const Kv4Tree &a, int column) {
+  const int row = a.group == 1 ? column : (int)__umulhi((uint32_t)column, a.group_inverse);
+  return {row, column - row * a.group};
 }
 
 __device__ __forceinline__ int parent_of(const Kv4Tree &a, const Drafts &d, int row) {
@@ -133,118 +156,158 @@ __device__ __forceinline__ int parent_of(const Kv4Tree &a, const Drafts &d, int 
   return (uint32_t)parent < (uint32_t)d.rows ? parent : -1;
 }
 
-// Whether row `row` of a sequence sees any position in the pool. Asked only where no score was above -infinity, to tell zeros (none)
-// from a softmax that is undefined (NaN).
-__device__ __forceinline__ bool sees_any(const Kv4Tree &a, const Drafts &d, int sequence, int row) {
-  for (int64_t position = 0; position < d.context; position += (int64_t)1 << a.pool.page_shift)
-    if (known_position(a.pool, sequence, (int)position)) return true;
-  for (int step = 0; step < kMostDrafts && row >= 0; ++step, row = parent_of(a, d, row))
-    if (known_position(a.pool, sequence, d.context + row)) return true;
-  return false;
+// A query's sum where all its scores are -infinity: above zero, so that it is told from a query without a position, whose outputs are
+// zeros; next to any other share's sum it is nothing.
+constexpr float kNoScore = 1e-30f;
+__device__ __forceinline__ float inverse_of(float top, float sum) {
+  return top == -INFINITY ? (sum == 0.f ? 0.f : NAN) : 1.f / sum;
 }
 
+// Whether a word of two 16-bit values holds an infinity or a NaN.
+template <bool F16>
+__device__ __forceinline__ bool not_finite(uint32_t word) {
+  constexpr uint32_t kExponent = F16 ? 0x7C00u : 0x7F80u;
+  return (word & kExponent) == kExponent || (word >> 16 & kExponent) == kExponent;
+}
+
+// Elements e and e + 1 of a cached row in the rows' type: `half` its head's keys or values in its page, `at` its place there.
 template <bool F16, int DIM>
-__global__ __launch_bounds__(kThreads, kResident) void kv4_tree_kernel(Kv4Tree a) {
+__device__ __forceinline__ uint32_t cached_pair(const uint8_t *half, int64_t scales_at, int at, int e) {
+  return kv4_pair<F16, 0>(half[at * (DIM / 2) + e / 2], __uint_as_float((uint32_t)half[scales_at + at * (DIM / 32) + e / 32] << 23));
+}
+// A query's score of a cached key, before the scale.
+template <bool F16, int DIM>
+__device__ __forceinline__ float cached_score(const Kv4Tree &a, const uint16_t *q, const uint8_t *half, int64_t scales_at, int at) {
+  float score = 0.f;
+#pragma unroll 1
+  for (int e = 0; e < DIM; e += 2) {
+    const uint32_t k = cached_pair<F16, DIM>(half, scales_at, at, e), x = (*reinterpret_cast<const uint32_t *>(q + e) & a.q_and) ^ a.q_xor;
+    score = __builtin_fmaf(half_bits_to_float<F16>((uint16_t)x), half_bits_to_float<F16>((uint16_t)k), score);
+    score = __builtin_fmaf(half_bits_to_float<F16>((uint16_t)(x >> 16)), half_bits_to_float<F16>((uint16_t)(k >> 16)), score);
+  }
+  return score;
+}
+
+// Of a block's piece: its outputs in the order of the registers, [DIM / 8][64 lanes][4], then the columns' maxima and sums.
+template <int DIM>
+constexpr int kPieceFloats = kCols * DIM + 2 * kCols;
+
+template <bool F16, int DIM>
+__global__ __launch_bounds__(kThreads, kResident<DIM>) void kv4_tree_kernel(Kv4Tree a) {
   constexpr int kTile = tx::kTile<DIM>, kSubs = kTile / 32, kGroups = DIM / 32;
   constexpr int kRow = DIM * 2;  // bytes of a converted row
   constexpr int kSteps = DIM / 16, kOut = DIM / 32;
-  __shared__ __attribute__((aligned(1024))) char lds[2 * kTile * kRow];  // keys, then values; later the shares' outputs
+  __shared__ __attribute__((aligned(1024))) char keys[kTile * kRow];
+  __shared__ __attribute__((aligned(1024))) char values[kTile * kRow];
   __shared__ float stats[kWaves][2][64];
-  __shared__ uint8_t known[kTile / 16], odd[kTile];
-  char *const keys = lds, *const values = lds + kTile * kRow;
+  __shared__ uint64_t sees[kMostDrafts];  // the rows that each row sees, a bit each
+  __shared__ uint64_t mads;               // drafted rows of whose values a group was left out
+  __shared__ __attribute__((aligned(8))) uint8_t known[8];  // whether each 16 positions of the tile lie in the pool
 
   const Kv4Pool &pool = a.pool;
   const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave = scalar(threadIdx.x >> 6);
   const int n = lane & 31, h = lane >> 5;
 
-  // The run: units [unit, end) of the row of all; a part is what of one (head, pass) lies in it.
+  // The run: ticks [tick, end) of the row of all; `from` of the part's ticks with work, below 0 before them.
   Drafts d;
-  int unit, end, sequence, head, pass, from, slot = 0;
+  int tick, end, sequence, head, pass, from, slot = 0;
   if (a.whole) {  // a workgroup for each (sequence, head, pass)
     pass = blockIdx.x % a.most_passes;
     head = blockIdx.x / a.most_passes % pool.kv_heads;
     sequence = blockIdx.x / a.most_passes / pool.kv_heads;
-    d = drafts_of(a, sequence);
+    d = scalar_drafts(a, sequence);
     if (pass >= d.passes) return;
-    unit = from = 0;
-    end = tiles_of<kTile>(d.length);
+    tick = from = 0;
+    end = part_ticks<kTile>(d) - kStart;
   } else {
     const RaggedPlace place = ragged_place(
-        pool.sequences, [](int s) { return s; }, [&](int s) { return units_of<kTile>(a, drafts_of(a, s)); },
-        [&](int total) { return (int)blockIdx.x * run_units(total, a); });
-    const int run = run_units(place.total, a);
-    unit = blockIdx.x * run;
-    end = min(unit + run, place.total);
-    if (unit >= end) return;
-    sequence = place.sequence;
-    d = drafts_of(a, sequence);
-    const int share = kStart + tiles_of<kTile>(d.length), index = place.local / share;
-    head = index / d.passes;
-    pass = index % d.passes;
-    from = place.local - index * share - kStart;  // below 0: units without work
+        pool.sequences, [](int s) { return s; }, [&](int s) { return ticks_of<kTile>(a, drafts_of(a, s)); },
+        [&](int total) { return (int)blockIdx.x * run_ticks(total, a); });
+    const int run = run_ticks(place.total, a);
+    tick = scalar(blockIdx.x * run);
+    end = scalar(min(tick + run, place.total));
+    if (tick >= end) return;
+    sequence = scalar(place.sequence);
+    d = scalar_drafts(a, sequence);
+    const int ticks = part_ticks<kTile>(d), index = scalar(place.local / ticks);
+    head = scalar(index / d.passes);
+    pass = index - head * d.passes;
+    from = scalar(place.local) - index * ticks - kStart;
   }
 
-  // This thread's part of a conversion: position p of the unit, elements 32 g .. 32 g + 31.
+  // This thread's part of a conversion: position p of the tile, elements 32 g .. 32 g + 31.
   const int p = threadIdx.x / kGroups, g = threadIdx.x % kGroups;
   const int64_t half_bytes = kv4_half_bytes(pool.page_shift, DIM), scales_at = (int64_t)(DIM / 2) << pool.page_shift;
+  const int64_t head_bytes = 2 * half_bytes, page_bytes = head_bytes * pool.kv_heads;
   const int page_mask = (1 << pool.page_shift) - 1;
   // 16-byte chunk c of row r lies at chunk c ^ turn: operand reads and these stores hit distinct banks.
   const int k_turn = DIM == 128 ? p & 15 : (p >> 1) & 7;
   const int v_turn = DIM == 128 ? 5 * (p & 3) : 4 * ((p >> 1) & 1) ^ ((p >> 1) & 3);
   // Operands: key row n, dimensions 16 st + 8 h at k_at ^ 32 st; by the transposing reads key 4 h + (lane % 16) / 4,
   // dimensions 32 t + 16 ((lane / 16) % 2) + 4 (lane % 4) at v_at ^ 64 t.
-  const uint32_t x4 = (lane >> 2) & 3;
   const uint32_t k_at = (uint32_t)n * kRow + 16u * (uint32_t)(h ^ (DIM == 128 ? n & 15 : (n >> 1) & 7));
-  const uint32_t v_row = 4u * h + x4, v_chunk = 2u * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+  const uint32_t v_row = 4u * h + ((lane >> 2) & 3), v_chunk = 2u * ((lane >> 4) & 1) + ((lane & 3) >> 1);
   const uint32_t v_at = v_row * kRow + 8u * (lane & 1) +
                         16u * (v_chunk ^ (DIM == 128 ? 5 * (v_row & 3) : 4 * ((v_row >> 1) & 1) ^ ((v_row >> 1) & 3)));
 
-  struct Codes {
-    u32x4 k, v;
-    uint32_t ks, vs;
-    bool valid;
-  };
-  Codes codes;
-
-  while (unit < end) {
-    const int share_tiles = tiles_of<kTile>(d.length);
-    const int first = max(from, 0), until = min(share_tiles, from + end - unit);
-    const bool any = until > first;
-    if (any) {
-      const int per_pass = blocks_a_pass(d), col0 = pass * per_pass * kCols;
-      const int columns = min(per_pass * kCols, d.columns - col0);  // above zero
-      const int blocks = (columns + kCols - 1) / kCols;
-      const int shares = blocks >= 3 ? 1 : min(kWaves / blocks, kSubs);  // waves that share a block's positions
-      const int block = wave % blocks, share = wave / blocks;
-      const bool works = share < shares;
-      const int column = col0 + block * kCols + n;  // this lane's query
-      const int row = min(column, d.columns - 1) / a.group;
-      const bool mine = column < d.columns && column < col0 + columns;
-
+  while (tick < end) {
+    const int weight = weight_of(d.blocks), tiles = tiles_of<kTile>(d.length);
+    const int to = min(tiles * weight, from + end - tick);
+    // Tiles whose first tick lies in the run.
+    const int first = scalar((max(from, 0) + weight - 1) / weight), until = scalar((max(to, 0) + weight - 1) / weight);
+    if (until > first) {
+      const int col0 = pass * d.blocks * kCols;
+      const int blocks = min(d.blocks, pieces_of(d.columns - col0, kCols));
+      // Waves that share a block's positions: all of them for one block (at dim 128 two), pairs for two.
+      const int shares = blocks >= 3 ? 1 : blocks == 2 ? 2 : min(kWaves, kSubs);
+      const int block = blocks >= 3 ? wave : blocks == 2 ? wave & 1 : 0, share = blocks >= 3 ? 0 : blocks == 2 ? wave >> 1 : wave;
+      const bool works = block < blocks && share < shares;
       const int stop = min(until * kTile, d.length);
-      auto load = [&](int tile) {
-        const int position = tile * kTile + p;
-        int page = -1;
-        if (position < d.length) page = pool.table[sequence * pool.table_stride + (position >> pool.page_shift)];
-        codes.valid = (uint32_t)page < (uint64_t)pool.num_pages;
-        codes.k = codes.v = u32x4{0, 0, 0, 0};
-        codes.ks = codes.vs = 127;
-        if (codes.valid) {
-          const uint8_t *half = pool.pages + ((int64_t)page * pool.kv_heads + head) * 2 * half_bytes;
-          const int at = position & page_mask;
-          codes.k = *reinterpret_cast<const u32x4 *>(half + at * (DIM / 2) + 16 * g);
-          codes.v = *reinterpret_cast<const u32x4 *>(half + half_bytes + at * (DIM / 2) + 16 * g);
-          codes.ks = half[scales_at + at * kGroups + g];
-          codes.vs = half[half_bytes + scales_at + at * kGroups + g];
-        }
-      };
-      load(first);
 
+      // Page ids of this wave's positions of a tile (at dim 64 twice 16 of them), a tile before its codes.
+      constexpr int kIds = kTile / kWaves / 16;
+      struct Ids {
+        int page[kIds];
+      };
+      auto ids_of = [&](int tile) __attribute__((always_inline)) {
+        // Constant for the whole launch: scalar loads.
+        const auto *table = (const __attribute__((address_space(4))) int *)(pool.table + sequence * pool.table_stride);
+        Ids ids;
+#pragma unroll
+        for (int i = 0; i < kIds; ++i)
+          ids.page[i] = table[min(tile * kTile + wave * (kTile / kWaves) + 16 * i, max(d.length - 1, 0)) >> pool.page_shift];
+        return ids;
+      };
+      u32x4 k_codes, v_codes;
+      uint32_t k_scale, v_scale;
+      int there;  // of this thread's position: whether its page is known
+      auto load = [&](int tile, const Ids &ids) __attribute__((always_inline)) {
+        const int position = tile * kTile + p, at = position & page_mask;
+        const uint8_t *half[kIds];
+        int known_page[kIds];
+#pragma unroll
+        for (int i = 0; i < kIds; ++i) {
+          known_page[i] = (uint32_t)ids.page[i] < (uint64_t)pool.num_pages;
+          half[i] = pool.pages + (known_page[i] ? ids.page[i] : 0) * page_bytes + head * head_bytes;
+        }
+        const bool second = kIds == 2 && lane >= 32;
+        const uint8_t *mine = second ? half[kIds - 1] : half[0];
+        there = second ? known_page[kIds - 1] : known_page[0];
+        k_codes = *reinterpret_cast<const u32x4 *>(mine + at * (DIM / 2) + 16 * g);
+        v_codes = *reinterpret_cast<const u32x4 *>(mine + half_bytes + at * (DIM / 2) + 16 * g);
+        k_scale = mine[scales_at + at * kGroups + g];
+        v_scale = mine[half_bytes + scales_at + at * kGroups + g];
+      };
+      Ids ids = ids_of(first);
+      load(first, ids);
+      ids = ids_of(first + 1);
+
+      const int column = col0 + block * kCols + n;  // this lane's query
+      const Query query = query_of(a, min(column, d.columns - 1));
       u32x4 qb[kSteps];
       {
-        const int c = min(column, d.columns - 1);
-        const uint16_t *q = a.q + (int64_t)(d.begin + row) * a.q_token + (head * a.group + c % a.group) * a.q_head + 8 * h;
+        const uint16_t *q = a.q + (int64_t)(d.begin + query.row) * a.q_token + (head * a.group + query.head) * a.q_head + 8 * h;
 #pragma unroll
         for (int st = 0; st < kSteps; ++st) {
           qb[st] = *reinterpret_cast<const u32x4 *>(q + 16 * st);
@@ -252,13 +315,12 @@ __global__ __launch_bounds__(kThreads, kResident) void kv4_tree_kernel(Kv4Tree a
           for (int j = 0; j < 4; ++j) qb[st][j] = (qb[st][j] & a.q_and) ^ a.q_xor;
         }
       }
-      // The rows that this lane's row sees, a bit each: pointers doubled, so that any parents end.
-      uint64_t seen = 0;
-      if (until * kTile > d.context) {
-        if (a.parents) {
+      if (wave == 0 && until * kTile > d.context) {
+        uint64_t seen = ((uint64_t)2 << lane) - 1;
+        if (a.parents) {  // pointers doubled, so that any parents end
           int up = lane < d.rows ? parent_of(a, d, lane) : -1;
           seen = (uint64_t)1 << lane;
-#pragma unroll
+#pragma unroll 1
           for (int i = 0; i < 6; ++i) {
             const int from_lane = max(up, 0);
             const uint64_t theirs = __shfl(seen, from_lane);
@@ -266,73 +328,93 @@ __global__ __launch_bounds__(kThreads, kResident) void kv4_tree_kernel(Kv4Tree a
             seen |= up >= 0 ? theirs : 0;
             up = up >= 0 ? further : -1;
           }
-          seen = __shfl(seen, row);
-        } else {
-          seen = ((uint64_t)2 << row) - 1;
         }
+        sees[lane] = seen;  // the others read it behind a barrier
       }
+      if (threadIdx.x == 0) mads = 0;
 
       const float lift = F16 ? 15.f - kPackedLag : -kPackedLag - 1.f - (float)(32 - __builtin_clz(d.length | 1));
       float m = -INFINITY, l = 0.f;  // running maximum of the query (before the scale), this lane's share of the sum
+      bool any = false;              // whether the query sees a position of this wave's
       f32x16 o[kOut];                // o[t][r] = O[query][dimension 32 t + 8 (r / 4) + 4 h + r % 4]
 #pragma unroll
       for (int t = 0; t < kOut; ++t) o[t] = f32x16{};
 
+#pragma unroll 1
       for (int tile = first; tile < until; ++tile) {
-        const bool drafts = (tile + 1) * kTile > d.context;  // some positions are drafted rows
-        lds_barrier();  // the last unit is read
+        const int base0 = tile * kTile;
+        lds_barrier();  // the last tile is read
         {
-          const float ks = __uint_as_float(codes.ks << 23), vs = __uint_as_float(codes.vs << 23);
-          u32x4 x[4];
+          const int position = base0 + p;
+          const bool counts = there && position < d.length;
+          uint32_t ks = k_scale, vs = v_scale;
+          if (base0 + kTile > min(d.context, d.length)) {
+            asm volatile("" ::: "memory");  // stays a branch: the last tiles of a sequence
+            bool odd = false;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) x[i] = kv4_octet<F16>(codes.v[i], vs);
-          if (drafts) {
-            constexpr uint32_t kExponent = F16 ? 0x7C00u : 0x7F80u;
-            bool mad = false;
+            for (int i = 0; i < 4; ++i) {
+              const u32x4 x = kv4_octet<F16>(v_codes[i], __uint_as_float(vs << 23));
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+              for (int j = 0; j < 4; ++j) odd |= not_finite<F16>(x[j]);
+            }
+            odd = odd && counts && position >= d.context;
+            const int row = position - d.context;
+            if (odd && row < kMostDrafts) atomicOr((unsigned long long *)&mads, 1ull << row);
+            vs = odd ? 127u : vs;
 #pragma unroll
-              for (int j = 0; j < 4; ++j)
-                mad |= (x[i][j] & kExponent) == kExponent || (x[i][j] >> 16 & kExponent) == kExponent;
-            const uint64_t all = __builtin_amdgcn_ballot_w64(mad);
-            const bool out = tile * kTile + p >= d.context && (all >> (lane - g) & ((1 << kGroups) - 1)) != 0;
-            if (g == 0) odd[p] = out;
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-              for (int j = 0; j < 4; ++j) x[i][j] = out ? 0u : x[i][j];
+            for (int i = 0; i < 4; ++i) v_codes[i] = odd ? 0u : v_codes[i];
           }
+          ks = counts ? ks : 127u;
+          vs = counts ? vs : 127u;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            *reinterpret_cast<u32x4 *>(keys + p * kRow + 16 * ((4 * g + i) ^ k_turn)) = kv4_octet<F16>(codes.k[i], ks);
-            *reinterpret_cast<u32x4 *>(values + p * kRow + 16 * ((4 * g + i) ^ v_turn)) = x[i];
+            const uint32_t kc = counts ? k_codes[i] : 0u, vc = counts ? v_codes[i] : 0u;
+            *reinterpret_cast<u32x4 *>(keys + p * kRow + 16 * ((4 * g + i) ^ k_turn)) = kv4_octet<F16>(kc, __uint_as_float(ks << 23));
+            *reinterpret_cast<u32x4 *>(values + p * kRow + 16 * ((4 * g + i) ^ v_turn)) = kv4_octet<F16>(vc, __uint_as_float(vs << 23));
           }
-          if (g == 0 && p % 16 == 0) known[p / 16] = codes.valid;
+          if (g == 0 && p % 16 == 0) known[p / 16] = (uint8_t)there;
         }
-        if (tile + 1 < until) load(tile + 1);
+        if (tile + 1 < until) {
+          load(tile + 1, ids);
+          ids = ids_of(tile + 2);
+        }
         lds_barrier();
         if (!works) continue;
 #pragma unroll 1
         for (int sub = share; sub < kSubs; sub += shares) {
-          const int base = tile * kTile + 32 * sub;
+          const int base = base0 + 32 * sub;
           if (base >= stop) break;
           const char *kt = keys + 32 * sub * kRow, *vt = values + 32 * sub * kRow;
-          f32x16 sc = {};
+          const uint32_t pages = *reinterpret_cast<const uint16_t *>(known + 2 * sub);
+          f32x16 sc;
+          {
+            constexpr int kAhead = kSteps < 4 ? kSteps : 4;
+            auto key = [&](int st) __attribute__((always_inline)) { return *reinterpret_cast<const u32x4 *>(kt + (k_at ^ (32u * st))); };
+            u32x4 x[kAhead];
 #pragma unroll
-          for (int st = 0; st < kSteps; ++st) sc = mfma32<F16>(*reinterpret_cast<const u32x4 *>(kt + (k_at ^ (32u * st))), qb[st], sc);
-          // sc[r]: position base + 8 (r / 4) + 4 h + r % 4
-          uint32_t there = (known[2 * sub] ? 0xFFFFu : 0u) | (known[2 * sub + 1] ? 0xFFFF0000u : 0u);
-          if (stop - base < 32) there &= (1u << (stop - base)) - 1u;
-          there = __builtin_amdgcn_readfirstlane(there);
-          uint32_t sees = there;  // a bit for each of the 32 positions
-          if (base + 32 > d.context) {
-            const int ahead = d.context - base;  // of the rows: the first of them, above or below the base
-            sees &= ahead >= 0 ? (uint32_t)(seen << ahead) | ((1u << ahead) - 1u) : ahead > -64 ? (uint32_t)(seen >> -ahead) : 0u;
+            for (int i = 0; i < kAhead; ++i) x[i] = key(i);
+#pragma unroll
+            for (int st = 0; st < kSteps; ++st) {
+              sc = mfma32<F16>(x[st % kAhead], qb[st], st == 0 ? f32x16{} : sc);
+              if (st + kAhead < kSteps) x[st % kAhead] = key(st + kAhead);
+            }
           }
-          if (there != ~0u || base + 32 > d.context) {
-            const uint32_t bits = sees >> (4 * h);
+          // sc[r]: position base + 8 (r / 4) + 4 h + r % 4
+          if (scalar(pages) != 0x0101 || base + 32 > min(stop, d.context)) {
+            asm volatile("" ::: "memory");
+            uint32_t bits = (pages & 1 ? 0xFFFFu : 0u) | (pages >> 8 ? 0xFFFF0000u : 0u);
+            if (stop - base < 32) bits &= (1u << (stop - base)) - 1u;
+            const int ahead = d.context - base;  // where the first drafted row lies, counted from the base
+            if (ahead < 32) {
+              const uint64_t rows = sees[query.row];
+              bits &= ahead >= 0 ? (uint32_t)(rows << ahead) | ((1u << ahead) - 1u) : ahead > -64 ? (uint32_t)(rows >> -ahead) : 0u;
+            }
+            any |= bits != 0;
+            bits >>= 4 * h;
 #pragma unroll
             for (int r = 0; r < 16; ++r) sc[r] = bits >> (8 * (r >> 2) + (r & 3)) & 1 ? sc[r] : -INFINITY;
+          } else {
+            any = true;
           }
           float mx = fmaxf(sc[0], sc[1]);
 #pragma unroll
@@ -354,85 +436,99 @@ __global__ __launch_bounds__(kThreads, kResident) void kv4_tree_kernel(Kv4Tree a
           for (int i = 0; i < 8; ++i)
             pb[i] = pack2<F16>(__builtin_amdgcn_exp2f(__builtin_fmaf(sc[2 * i], a.sl2, zero)),
                                __builtin_amdgcn_exp2f(__builtin_fmaf(sc[2 * i + 1], a.sl2, zero)), l);
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const u32x4 pr = {pb[4 * j], pb[4 * j + 1], pb[4 * j + 2], pb[4 * j + 3]};  // slots 0-3: positions 16 j + 4 h .., 4-7: the 8 behind
-#pragma unroll
-            for (int t = 0; t < kOut; ++t) {
-              const char *at = vt + 16 * j * kRow + (v_at ^ (64u * t));
+          {
+            constexpr int kAhead = 3;
+            auto value = [&](int i) __attribute__((always_inline)) {
+              const char *at = vt + 16 * (i / kOut) * kRow + (v_at ^ (64u * (i % kOut)));
               const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)at));
               const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(at + 8 * kRow)));
-              o[t] = mfma32<F16>(u32x4{lo[0], lo[1], hi[0], hi[1]}, pr, o[t]);
-            }
-          }
-          if (drafts) {
-            // Drafts whose values are not finite: their share, for the queries that see them alone.
-            uint32_t mad = (uint32_t)__builtin_amdgcn_ballot_w64(h == 0 && odd[32 * sub + n]);
-            for (; mad != 0; mad &= mad - 1) {
-              const int j = __builtin_ctz(mad), position = base + j;
-              uint32_t word = 0;
+              return u32x4{lo[0], lo[1], hi[0], hi[1]};  // slots 0-3: positions 4 h .., 4-7: the 8 behind
+            };
+            u32x4 x[kAhead];
 #pragma unroll
-              for (int i = 0; i < 8; ++i) word = i == 2 * (j >> 3) + ((j & 3) >> 1) ? pb[i] : word;
-              word = __shfl(word, n + 32 * (j >> 2 & 1));
-              const float pj = half_bits_to_float<F16>((uint16_t)(j & 1 ? word >> 16 : word));
-              const bool does = sees >> j & 1;
-              const int page = pool.table[sequence * pool.table_stride + (position >> pool.page_shift)];
-              const uint8_t *half = pool.pages + (((int64_t)page * pool.kv_heads + head) * 2 + 1) * half_bytes;
-              const int at = position & page_mask;
+            for (int i = 0; i < kAhead; ++i) x[i] = value(i);
 #pragma unroll
-              for (int t = 0; t < kOut; ++t) {
-                const float scale = __uint_as_float((uint32_t)half[scales_at + at * kGroups + t] << 23);
-#pragma unroll
-                for (int rq = 0; rq < 4; ++rq) {
-                  const uint32_t word4 = *reinterpret_cast<const uint16_t *>(half + at * (DIM / 2) + 16 * t + 4 * rq + 2 * h);
-                  const uint32_t pair[2] = {kv4_pair<F16, 0>(word4, scale), kv4_pair<F16, 1>(word4, scale)};
-#pragma unroll
-                  for (int e = 0; e < 4; ++e) {
-                    const float v = half_bits_to_float<F16>((uint16_t)(pair[e / 2] >> (16 * (e % 2))));
-                    o[t][4 * rq + e] = does ? __builtin_fmaf(pj, v, o[t][4 * rq + e]) : o[t][4 * rq + e];
-                  }
-                }
-              }
+            for (int i = 0; i < 2 * kOut; ++i) {
+              const int j = i / kOut, t = i % kOut;
+              o[t] = mfma32<F16>(x[i % kAhead], u32x4{pb[4 * j], pb[4 * j + 1], pb[4 * j + 2], pb[4 * j + 3]}, o[t]);
+              if (i + kAhead < 2 * kOut) x[i % kAhead] = value(i + kAhead);
             }
           }
         }
       }
 
-      // The shares of a block meet in LDS. A share without a score above -infinity has l = 0 and O = 0 (or NaN, where scores were).
+      // The shares of a block meet in LDS, in the tiles' place. A share without a score above -infinity has l = 0 and O = 0 (or NaN,
+      // where scores were).
       l = halves_sum(l);
+      if (m == -INFINITY && any) l += kNoScore;
+      lds_barrier();  // the last tile is read
+      const uint64_t lost = mads;
       if (shares > 1) {
-        lds_barrier();  // the last unit is read
+        // Share s of a block: 4 KiB for each 32 dimensions, share 1 and 2 in the keys' place, 3 in the values'.
+        auto region = [&](int s) {
+          const int index = (s - 1) * blocks + block, in_keys = kTile * kRow / (kOut * 4096);
+          return reinterpret_cast<f32x4 *>(index < in_keys ? keys + index * kOut * 4096 : values + (index - in_keys) * kOut * 4096) + lane;
+        };
         if (works && share > 0) {
           stats[wave][0][lane] = m;
           stats[wave][1][lane] = l;
-          float *to = reinterpret_cast<float *>(lds) + ((share - 1) * blocks + block) * kOut * 1024 + lane;
+          f32x4 *put = region(share);
 #pragma unroll
           for (int t = 0; t < kOut; ++t)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) to[(16 * t + r) * 64] = o[t][r];
+            for (int rq = 0; rq < 4; ++rq) put[64 * (4 * t + rq)] = f32x4{o[t][4 * rq], o[t][4 * rq + 1], o[t][4 * rq + 2], o[t][4 * rq + 3]};
         }
         lds_barrier();
-        if (share == 0) {
+        if (works && share == 0) {
+#pragma unroll 1
           for (int s = 1; s < shares; ++s) {
-            const float m2 = stats[s * blocks + block][0][lane], l2 = stats[s * blocks + block][1][lane];
-            const float top = fmaxf(m, m2);
+            const int theirs = blocks == 2 ? 2 * s + block : s;
+            const float m2 = stats[theirs][0][lane], l2 = stats[theirs][1][lane], top = fmaxf(m, m2);
             const float w1 = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - top) * a.sl2);
             const float w2 = m2 == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m2 - top) * a.sl2);
-            const float *theirs = reinterpret_cast<const float *>(lds) + ((s - 1) * blocks + block) * kOut * 1024 + lane;
+            const f32x4 *from_share = region(s);
 #pragma unroll
             for (int t = 0; t < kOut; ++t)
 #pragma unroll
-              for (int r = 0; r < 16; ++r) o[t][r] = o[t][r] * w1 + theirs[(16 * t + r) * 64] * w2;
+              for (int rq = 0; rq < 4; ++rq) {
+                const f32x4 x = from_share[64 * (4 * t + rq)];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) o[t][4 * rq + r] = o[t][4 * rq + r] * w1 + x[r] * w2;
+              }
             l = l * w1 + l2 * w2;
             m = top;
           }
         }
       }
-      if (share == 0) {
-        if (first == 0 && until == share_tiles) {
-          if (mine) {
-            const float inverse = m == -INFINITY && !sees_any(a, d, sequence, row) ? 0.f : 1.f / l;
-            uint16_t *out = a.out + (int64_t)(d.begin + row) * a.out_token + (head * a.group + column % a.group) * a.out_head + 4 * h;
+      if (works && share == 0) {
+        // Groups of value rows that the products left out, for the queries that see them: slow, and seldom.
+        uint64_t rows = lost;
+#pragma unroll 1
+        for (; __builtin_expect(rows != 0, 0); rows &= rows - 1) {
+          const int row = __builtin_ctzll(rows), at = (d.context + row) & page_mask;
+          const int page = pool.table[sequence * pool.table_stride + ((d.context + row) >> pool.page_shift)];
+          const uint8_t *k_half = pool.pages + page * page_bytes + head * head_bytes, *v_half = k_half + half_bytes;
+          uint32_t out = 0;  // a bit for each group
+#pragma unroll 1
+          for (int e = 0; e < DIM; e += 2) out |= (uint32_t)not_finite<F16>(cached_pair<F16, DIM>(v_half, scales_at, at, e)) << (e / 32);
+          const uint16_t *q = a.q + (int64_t)(d.begin + query.row) * a.q_token + (head * a.group + query.head) * a.q_head;
+          const float prob = __builtin_amdgcn_exp2f((cached_score<F16, DIM>(a, q, k_half, scales_at, at) - m) * a.sl2 + lift);
+          const bool does = sees[query.row] >> row & 1;
+#pragma unroll
+          for (int t = 0; t < kOut; ++t) {
+            if (!does || !(out >> t & 1)) continue;
+#pragma unroll
+            for (int r = 0; r < 16; r += 2) {
+              const uint32_t v = cached_pair<F16, DIM>(v_half, scales_at, at, 32 * t + 8 * (r >> 2) + 4 * h + (r & 3));
+              o[t][r] = __builtin_fmaf(prob, half_bits_to_float<F16>((uint16_t)v), o[t][r]);
+              o[t][r + 1] = __builtin_fmaf(prob, half_bits_to_float<F16>((uint16_t)(v >> 16)), o[t][r + 1]);
+            }
+          }
+        }
+        if (first == 0 && until == tiles) {
+          const float inverse = inverse_of(m, l);
+          uint16_t *out = a.out + (int64_t)(d.begin + query.row) * a.out_token + (head * a.group + query.head) * a.out_head + 4 * h;
+          if (column < d.columns) {
 #pragma unroll
             for (int t = 0; t < kOut; ++t)
 #pragma unroll
@@ -444,128 +540,153 @@ __global__ __launch_bounds__(kThreads, kResident) void kv4_tree_kernel(Kv4Tree a
               }
           }
         } else {
-          // A block's piece: its outputs four registers at a time [4 kOut][64 lanes][4], then max and sum of its queries.
-          float *piece = a.pieces + ((int64_t)blockIdx.x * 2 + slot) * a.piece_floats + block * (kOut * 1024 + 64);
+          float *piece = a.pieces + ((int64_t)blockIdx.x * 2 + slot) * a.piece_floats + block * kPieceFloats<DIM>;
 #pragma unroll
           for (int t = 0; t < kOut; ++t)
 #pragma unroll
             for (int rq = 0; rq < 4; ++rq)
-              *reinterpret_cast<f32x4 *>(piece + (4 * t + rq) * 256 + 4 * lane) =
-                  f32x4{o[t][4 * rq], o[t][4 * rq + 1], o[t][4 * rq + 2], o[t][4 * rq + 3]};
+              reinterpret_cast<f32x4 *>(piece)[64 * (4 * t + rq) + lane] = f32x4{o[t][4 * rq], o[t][4 * rq + 1], o[t][4 * rq + 2], o[t][4 * rq + 3]};
           if (h == 0) {
-            piece[kOut * 1024 + n] = m;
-            piece[kOut * 1024 + 32 + n] = l;
+            piece[kCols * DIM + n] = m;
+            piece[kCols * DIM + kCols + n] = l;
           }
         }
       }
+      lds_barrier();  // before LDS is written again
     }
-    unit += until - from;
+    tick += to - from;
     from = -kStart;
     slot = 1;
-    if (unit < end && ++pass == d.passes) {
+    if (tick < end && ++pass == d.passes) {
       pass = 0;
       if (++head == pool.kv_heads) {
         head = 0;
-        do d = drafts_of(a, ++sequence);
-        while (d.rows == 0);  // one with work follows: unit < end
+        do d = scalar_drafts(a, ++sequence);
+        while (d.rows == 0);  // one with work follows: tick < end
       }
     }
   }
 }
 
-// Joins the pieces of (head, pass)es that several workgroups shared. Grid: x = (sequence * kv_heads + head) * most_passes + pass, y =
-// column block, z = four output registers of a lane; a wave takes every fourth piece.
-template <bool F16, int DIM>
+// Joins the pieces of (head, pass)es that several workgroups shared. Grid: y = block of the pass. BORDERS: x = the borders of runs, of
+// which the first in a part joins it, a wave every fourth slice of 1 KiB of its outputs. Else x = the (sequence, head, pass)es, z = the
+// slices, a wave every fourth piece: few parts of many pieces.
+template <bool F16, int DIM, bool BORDERS>
 __global__ __launch_bounds__(kThreads) void kv4_tree_combine_kernel(Kv4Tree a) {
-  constexpr int kTile = tx::kTile<DIM>, kOut = DIM / 32, kHeld = 4;
-  __shared__ f32x4 sums[kWaves][64];
-  __shared__ float stats[kWaves][2][32];
+  constexpr int kTile = tx::kTile<DIM>, kSlices = DIM / 8, kHeld = 4, kStride = BORDERS ? 1 : kWaves;
+  __shared__ f32x4 sums[BORDERS ? 1 : kWaves][64];
+  __shared__ float stats[BORDERS ? 1 : kWaves][2][64];
   const Kv4Pool &pool = a.pool;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, h = lane >> 5;
-  const int pass = blockIdx.x % a.most_passes, head = blockIdx.x / a.most_passes % pool.kv_heads;
-  const int sequence = blockIdx.x / a.most_passes / pool.kv_heads, block = blockIdx.y, quad = blockIdx.z;
-  const Drafts d = drafts_of(a, sequence);
-  if (pass >= d.passes) return;
-  const int per_pass = blocks_a_pass(d);
-  const int column = (pass * per_pass + block) * kCols + n;
-  if (block >= per_pass || (pass * per_pass + block) * kCols >= d.columns) return;
-  const RaggedPlace place = ragged_before(
-      pool.sequences, [](int s) { return s; }, [&](int s) { return units_of<kTile>(a, drafts_of(a, s)); }, sequence);
-  const int run = run_units(place.total, a);
-  const int tiles = tiles_of<kTile>(d.length);
-  const int begin = place.local + (head * d.passes + pass) * (kStart + tiles), work = begin + kStart;  // units with work from here on
-  const int w0 = work / run, w1 = (work + tiles - 1) / run;
+  const int lane = threadIdx.x & 63, wave = scalar(threadIdx.x >> 6);
+  int sequence, head, pass, begin, run;  // begin: the part's first tick in the row of all
+  Drafts d;
+  auto ticks = [&](int s) { return ticks_of<kTile>(a, drafts_of(a, s)); };
+  if constexpr (BORDERS) {
+    int at = 0;
+    const RaggedPlace place = ragged_place(pool.sequences, [](int s) { return s; }, ticks, [&](int total) { return at = ((int)blockIdx.x + 1) * run_ticks(total, a); });
+    if (at >= place.total) return;
+    run = run_ticks(place.total, a);
+    sequence = scalar(place.sequence);
+    d = scalar_drafts(a, sequence);
+    const int a_part = part_ticks<kTile>(d), index = scalar(place.local / a_part);
+    head = scalar(index / d.passes);
+    pass = index - head * d.passes;
+    begin = at - place.local + index * a_part;
+  } else {
+    sequence = blockIdx.x / a.most_passes / pool.kv_heads;
+    pass = blockIdx.x % a.most_passes;
+    head = blockIdx.x / a.most_passes % pool.kv_heads;
+    d = scalar_drafts(a, sequence);
+    if (pass >= d.passes) return;
+    const RaggedPlace place = ragged_before(pool.sequences, [](int s) { return s; }, ticks, sequence);
+    run = run_ticks(place.total, a);
+    begin = place.local + (head * d.passes + pass) * part_ticks<kTile>(d);
+  }
+  const int block = blockIdx.y, col0 = (pass * d.blocks + block) * kCols;
+  if (block >= d.blocks || col0 >= d.columns) return;
+  const int work = begin + kStart;
+  const int w0 = work / run, w1 = (work + (tiles_of<kTile>(d.length) - 1) * weight_of(d.blocks)) / run;  // of the first and last tile
   if (w0 == w1) return;  // one workgroup had it all and wrote the output
+  if (BORDERS && (int)blockIdx.x != w0) return;
   // Only the first workgroup can have had another part before this one.
   auto piece = [&](int w) {
-    return a.pieces + ((int64_t)w * 2 + (w == w0 && begin > w0 * run ? 1 : 0)) * a.piece_floats + block * (kOut * 1024 + 64);
+    return a.pieces + ((int64_t)w * 2 + (w == w0 && begin > w0 * run ? 1 : 0)) * a.piece_floats + block * kPieceFloats<DIM>;
   };
-  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-  float l = 0.f, m = -INFINITY;
-  for (int w = w0 + wave; w <= w1; w += kWaves * kHeld) {
-    f32x4 value[kHeld];
-    float pm[kHeld], pl[kHeld];
+  const int n = lane & 31, column = col0 + n;
+  const Query query = query_of(a, min(column, d.columns - 1));
+  auto put = [&](int slice, f32x4 sum, float top, float ll) __attribute__((always_inline)) {
+    sum *= inverse_of(top, ll);
+    if (column < d.columns)
+      *reinterpret_cast<u32x2 *>(a.out + (int64_t)(d.begin + query.row) * a.out_token + (head * a.group + query.head) * a.out_head +
+                                 8 * slice + 4 * (lane >> 5)) =
+          u32x2{to_half_bits<F16>(sum[0]) | (uint32_t)to_half_bits<F16>(sum[1]) << 16,
+                to_half_bits<F16>(sum[2]) | (uint32_t)to_half_bits<F16>(sum[3]) << 16};
+  };
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i) {
-      const float *at = piece(min(w + i * kWaves, w1));
-      value[i] = *reinterpret_cast<const f32x4 *>(at + quad * 256 + 4 * lane);
-      pm[i] = at[kOut * 1024 + n];
-      pl[i] = at[kOut * 1024 + 32 + n];
+  for (int slice = BORDERS ? wave : blockIdx.z; slice < kSlices; slice += BORDERS ? kWaves : kSlices) {
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+    float l = 0.f, m = -INFINITY;
+    for (int w = w0 + (BORDERS ? 0 : wave); w <= w1; w += kStride * kHeld) {
+      f32x4 value[kHeld];
+      float pm[kHeld], pl[kHeld];
+#pragma unroll
+      for (int i = 0; i < kHeld; ++i) {
+        const float *at = piece(min(w + i * kStride, w1));
+        value[i] = *reinterpret_cast<const f32x4 *>(at + 256 * slice + 4 * lane);
+        pm[i] = at[kCols * DIM + n];
+        pl[i] = at[kCols * DIM + kCols + n];
+      }
+      float mnew = m;
+#pragma unroll
+      for (int i = 0; i < kHeld; ++i) mnew = w + i * kStride <= w1 ? fmaxf(mnew, pm[i]) : mnew;
+      const float alpha = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - mnew) * a.sl2);
+      sum *= alpha;
+      l *= alpha;
+      m = mnew;
+#pragma unroll
+      for (int i = 0; i < kHeld; ++i) {
+        if (w + i * kStride > w1) continue;
+        const float weight = pm[i] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((pm[i] - m) * a.sl2);  // an empty piece holds zeros (or NaN)
+        sum += value[i] * weight;
+        l += pl[i] * weight;
+      }
     }
-    float mnew = m;
+    if constexpr (BORDERS) {
+      put(slice, sum, m, l);
+    } else {
+      sums[wave][lane] = sum;
+      stats[wave][0][lane] = m;
+      stats[wave][1][lane] = l;
+      __syncthreads();
+      if (wave != 0) return;
+      float top = -INFINITY, ll = 0.f;
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i) mnew = w + i * kWaves <= w1 ? fmaxf(mnew, pm[i]) : mnew;
-    const float alpha = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - mnew) * a.sl2);
-    sum *= alpha;
-    l *= alpha;
-    m = mnew;
+      for (int w = 0; w < kWaves; ++w) top = fmaxf(top, stats[w][0][lane]);
+      f32x4 total = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i) {
-      if (w + i * kWaves > w1) continue;
-      const float weight = pm[i] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((pm[i] - m) * a.sl2);  // an empty piece holds zeros (or NaN)
-      sum += value[i] * weight;
-      l += pl[i] * weight;
+      for (int w = 0; w < kWaves; ++w) {
+        const float weight = stats[w][0][lane] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((stats[w][0][lane] - top) * a.sl2);
+        total += sums[w][lane] * weight;
+        ll += stats[w][1][lane] * weight;
+      }
+      put(slice, total, top, ll);
     }
   }
-  sums[wave][lane] = sum;
-  if (h == 0) {
-    stats[wave][0][n] = m;
-    stats[wave][1][n] = l;
-  }
-  __syncthreads();
-  if (wave != 0 || column >= d.columns) return;
-  float top = -INFINITY;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) top = fmaxf(top, stats[w][0][n]);
-  f32x4 total = {0.f, 0.f, 0.f, 0.f};
-  float ll = 0.f;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
-    const float weight = stats[w][0][n] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((stats[w][0][n] - top) * a.sl2);
-    total += sums[w][lane] * weight;
-    ll += stats[w][1][n] * weight;
-  }
-  const int row = column / a.group;
-  total *= top == -INFINITY && !sees_any(a, d, sequence, row) ? 0.f : 1.f / ll;
-  uint16_t *out = a.out + (int64_t)(d.begin + row) * a.out_token + (head * a.group + column % a.group) * a.out_head + 4 * h;
-  *reinterpret_cast<u32x2 *>(out + 32 * (quad / 4) + 8 * (quad % 4)) =
-      u32x2{to_half_bits<F16>(total[0]) | (uint32_t)to_half_bits<F16>(total[1]) << 16,
-            to_half_bits<F16>(total[2]) | (uint32_t)to_half_bits<F16>(total[3]) << 16};
 }
 
 // Upper bounds of a call from what the host knows.
-int64_t most_columns(const Kv4Tree &a) { return (int64_t)(a.tokens < kMostDrafts ? a.tokens : kMostDrafts) * a.group; }
-int64_t most_passes(const Kv4Tree &a) { return (most_columns(a) + kCols * kPass - 1) / (kCols * kPass); }
-int64_t most_units(const Kv4Tree &a, int tile) {
+int64_t most_blocks(const Kv4Tree &a) { return ((int64_t)(a.tokens < kMostDrafts ? a.tokens : kMostDrafts) * a.group + kCols - 1) / kCols; }
+int64_t most_passes(const Kv4Tree &a) { return (most_blocks(a) + kPass - 1) / kPass; }
+int64_t most_ticks(const Kv4Tree &a, int tile) {
   const int64_t room = (int64_t)a.pool.max_pages << a.pool.page_shift, tiles = (room + tile - 1) / tile;
-  return (int64_t)a.pool.sequences * a.pool.kv_heads * most_passes(a) * (kStart + tiles);
+  return (int64_t)a.pool.sequences * a.pool.kv_heads * most_passes(a) * (kStart + kMostWeight * tiles);
 }
 
 }  // namespace
 
-// Unit numbers are 32-bit; a launch has fewer than 2^32 threads, 256 for each (head, pass).
+// Ticks are 32-bit; a launch has fewer than 2^32 threads, 256 for each (head, pass).
 bool kv4_tree_fits(const Kv4Tree &a) {
-  return most_units(a, kTile<128>) <= (int64_t)1 << 30 && (int64_t)a.pool.sequences * a.pool.kv_heads * most_passes(a) < (int64_t)1 << 24;
+  return most_ticks(a, kTile<128>) <= (int64_t)1 << 30 && (int64_t)a.pool.sequences * a.pool.kv_heads * most_passes(a) < (int64_t)1 << 24;
 }
 
 void kv4_tree_plan(Kv4Tree &a, int dim, int cus) {
@@ -573,10 +694,10 @@ void kv4_tree_plan(Kv4Tree &a, int dim, int cus) {
   const int64_t parts = (int64_t)a.pool.sequences * a.pool.kv_heads * most_passes(a);
   a.most_passes = (int)most_passes(a);
   a.whole = room <= 512;
-  const int64_t most = most_units(a, dim == 128 ? kTile<128> : kTile<64>), fill = kResident * (int64_t)cus;
+  const int64_t most = most_ticks(a, dim == 128 ? kTile<128> : kTile<64>), fill = (dim == 128 ? kResident<128> : kResident<64>) * (int64_t)cus;
   a.workgroups = (int)(a.whole ? parts : most < fill ? most : fill);
-  const int64_t blocks = (most_columns(a) + kCols - 1) / kCols;
-  a.piece_floats = (int)(blocks < kPass ? blocks : kPass) * (kCols * dim + 64);
+  const int64_t blocks = most_blocks(a) < kPass ? most_blocks(a) : kPass;
+  a.piece_floats = (int)blocks * (dim == 128 ? kPieceFloats<128> : kPieceFloats<64>);
   a.piece_bytes = a.whole ? 0 : (int64_t)a.workgroups * 2 * a.piece_floats * (int64_t)sizeof(float);
 }
 
@@ -586,10 +707,12 @@ hipError_t launch_kv4_tree(const Kv4Tree &a, bool f16, int dim, hipStream_t stre
     constexpr int kDim = decltype(dims)::value;
     hipLaunchKernelGGL((kv4_tree_kernel<kF16, kDim>), dim3((unsigned)a.workgroups), dim3(kThreads), 0, stream, a);
     if (a.whole) return;
-    const int64_t blocks = (most_columns(a) + kCols - 1) / kCols;
-    hipLaunchKernelGGL((kv4_tree_combine_kernel<kF16, kDim>),
-                       dim3((unsigned)(a.pool.sequences * a.pool.kv_heads * a.most_passes), (unsigned)(blocks < kPass ? blocks : kPass), kDim / 8),
-                       dim3(kThreads), 0, stream, a);
+    const int64_t parts = (int64_t)a.pool.sequences * a.pool.kv_heads * a.most_passes;
+    const unsigned in_pass = (unsigned)(most_blocks(a) < kPass ? most_blocks(a) : kPass);
+    if (parts <= 128)
+      hipLaunchKernelGGL((kv4_tree_combine_kernel<kF16, kDim, false>), dim3((unsigned)parts, in_pass, kDim / 8), dim3(kThreads), 0, stream, a);
+    else if (a.workgroups > 1)
+      hipLaunchKernelGGL((kv4_tree_combine_kernel<kF16, kDim, true>), dim3((unsigned)a.workgroups - 1, in_pass), dim3(kThreads), 0, stream, a);
   };
   using std::integral_constant;
   if (f16 && dim == 128) launch(integral_constant<bool, true>{}, integral_constant<int, 128>{});
