@@ -7,10 +7,11 @@
 // and the rows that its parents lead to, itself included.
 //
 // A KV head's queries are columns, row by row and query head by query head: rows * group of them, in blocks of 32, up to four blocks
-// a pass. Work: a tile is kTile positions of one sequence, KV head and pass, and weighs as many ticks as its blocks take time;
-// the ticks of all lie in one row, and every workgroup takes an equal run of them, whatever the lengths (it finds its place from
-// the lengths itself, so that a captured call serves any). A run that covers a whole (sequence, head, pass) writes its output; the
-// others leave (max, sum, unnormalised output) for the combine kernel, at most two such pieces a workgroup.
+// a pass. Work: a part is one (sequence, KV head, pass); a tile is kTile positions of it, and weighs as many ticks as its blocks take
+// time. A part of about as many ticks as an even share of the grid, or fewer, is one workgroup's, which writes its output; a longer
+// one is cut into even pieces, a workgroup each, that leave (max, sum, unnormalised output) for the combine kernel. Every workgroup
+// finds its piece from the lengths itself, so that a captured call serves any; pieces of cut parts come first in the grid, and parts
+// of a sequence are cut alike.
 //
 // A workgroup converts a tile's codes once, into LDS, each thread a scale group of keys and one of values: the conversion is what
 // single tokens' attention spends most on, and what the columns share. A wave then has one column block and, where there are
@@ -48,7 +49,7 @@ constexpr int kTile = kThreads / (DIM / 32);
 // Workgroups that a CU holds. Three of head dimension 128 have 168 registers a thread and spill 37: 173 us instead of 175 for 80
 // columns and 262,144 positions, but 35 instead of 28 for 24 trees, whose runs are short.
 template <int DIM>
-constexpr int kResident = DIM == 128 ? 2 : 3;
+constexpr int kResident = 2;
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
@@ -93,10 +94,9 @@ __device__ __forceinline__ float halves_sum(float v) {
 // All of the workgroup's LDS accesses so far are done; loads from memory stay in flight.
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-// What starting and ending a (head, pass) costs, in ticks.
-constexpr int kStart = 6;
-// What a tile costs: up to two blocks a wave has 32 of its positions (at dim 64 two blocks or one 64 or 32), else all of them.
-constexpr int kMostWeight = 3;
+// Ticks: what starting and ending a piece costs, and a tile of up to two blocks, whose waves share its positions, or more.
+constexpr int kStart = 6, kMostWeight = 3;
+constexpr int kLeast = 3;  // of a share: a tile a piece, 9.4 us for one tree behind 700 positions, where a share of 6 takes 11.0 and of 9 12.0
 __device__ __forceinline__ int weight_of(int blocks) { return blocks <= 2 ? 2 : kMostWeight; }
 
 // A value that all lanes have, in a scalar register.
@@ -133,13 +133,59 @@ __device__ __forceinline__ Drafts scalar_drafts(const Kv4Tree &a, int sequence) 
 
 template <int TILE>
 __device__ __forceinline__ int tiles_of(int length) { return max(1, (length + TILE - 1) / TILE); }
-// Ticks of a (head, pass), the start among them: passes count alike, whatever their blocks.
+// Ticks of a part, the start among them: passes count alike, whatever their blocks.
 template <int TILE>
 __device__ __forceinline__ int part_ticks(const Drafts &d) { return kStart + weight_of(d.blocks) * tiles_of<TILE>(d.length); }
+
+// How the parts are cut: into as many pieces as they have even shares of the grid, rounded; the pieces of cut parts are fewer than
+// twice the grid's even shares.
+struct Cut {
+  int sequence, part, piece, pieces;  // part: head * passes + pass
+  int before;                         // pieces of cut parts before this part
+};
+// Piece `wanted` of all (`wanted` >= 0), or with wanted = ~sequence the first piece of that sequence. sequence < 0: there is none.
 template <int TILE>
-__device__ __forceinline__ int ticks_of(const Kv4Tree &a, const Drafts &d) { return a.pool.kv_heads * d.passes * part_ticks<TILE>(d); }
-// Ticks of every workgroup: at least one tile's.
-__device__ __forceinline__ int run_ticks(int total, const Kv4Tree &a) { return max((total + a.workgroups - 1) / a.workgroups, kMostWeight); }
+__device__ __forceinline__ Cut cut_at(const Kv4Tree &a, int wanted) {
+  const int lane = threadIdx.x & 63, sequences = a.pool.sequences;
+  int parts = 0, ticks = 0, tiles = 0;  // of the lane's sequence
+  auto load = [&](int first) {
+    parts = ticks = tiles = 0;
+    if (first + lane < sequences) {
+      const Drafts d = drafts_of(a, first + lane);
+      parts = a.pool.kv_heads * d.passes;
+      tiles = tiles_of<TILE>(d.length);
+      ticks = part_ticks<TILE>(d);
+    }
+  };
+  int total = 0;
+  for (int first = 0; first < sequences; first += 64) {
+    load(first);
+    total += __builtin_amdgcn_readlane(wave_scan(parts * ticks), 63);
+  }
+  const int share = max((total + a.workgroups - 1) / a.workgroups, kLeast);
+  auto pieces_now = [&] { return max(min((int)((2u * ticks + share) / (2u * share)), tiles), 1); };
+  int before = 0;
+#pragma unroll 1
+  for (int cut = 1; cut >= 0; --cut) {  // the cut parts, then the others
+    for (int first = 0; first < sequences; first += 64) {
+      if (sequences > 64) load(first);
+      const int pieces = pieces_now(), n = (pieces > 1) == (cut != 0) ? pieces * parts : 0, sum = wave_scan(n);
+      uint64_t past;
+      if (wanted >= 0)
+        past = __builtin_amdgcn_ballot_w64(before + sum > wanted);
+      else
+        past = __builtin_amdgcn_ballot_w64(first + lane == ~wanted);
+      if (past) {
+        const int at = __builtin_ctzll(past), each = __builtin_amdgcn_readlane(pieces, at);
+        const int start = before + __builtin_amdgcn_readlane(sum - n, at), local = scalar(max(wanted, start)) - start;
+        const int part = scalar(local / each);
+        return {first + at, part, local - part * each, each, start + part * each};
+      }
+      before += __builtin_amdgcn_readlane(sum, 63);
+    }
+  }
+  return {-1, 0, 0, 1, 0};
+}
 
 // The row of a column, and its query head in the KV head's group: column / a.group by the host's ceil(2^32 / group), exact for
 // columns times group below 2^32.
@@ -197,44 +243,39 @@ __global__ __launch_bounds__(kThreads, kResident<DIM>) void kv4_tree_kernel(Kv4T
   constexpr int kTile = tx::kTile<DIM>, kSubs = kTile / 32, kGroups = DIM / 32;
   constexpr int kRow = DIM * 2;  // bytes of a converted row
   constexpr int kSteps = DIM / 16, kOut = DIM / 32;
-  __shared__ __attribute__((aligned(1024))) char keys[kTile * kRow];
-  __shared__ __attribute__((aligned(1024))) char values[kTile * kRow];
+  __shared__ __attribute__((aligned(1024))) char keys[2][kTile * kRow];
+  __shared__ __attribute__((aligned(1024))) char values[2][kTile * kRow];
   __shared__ float stats[kWaves][2][64];
   __shared__ uint64_t sees[kMostDrafts];  // the rows that each row sees, a bit each
   __shared__ uint64_t mads;               // drafted rows of whose values a group was left out
-  __shared__ __attribute__((aligned(8))) uint8_t known[8];  // whether each 16 positions of the tile lie in the pool
+  __shared__ __attribute__((aligned(8))) uint8_t known[2][8];  // whether each 16 positions of the tile lie in the pool
 
   const Kv4Pool &pool = a.pool;
   const int lane = threadIdx.x & 63;
   const int wave = scalar(threadIdx.x >> 6);
   const int n = lane & 31, h = lane >> 5;
 
-  // The run: ticks [tick, end) of the row of all; `from` of the part's ticks with work, below 0 before them.
   Drafts d;
-  int tick, end, sequence, head, pass, from, slot = 0;
-  if (a.whole) {  // a workgroup for each (sequence, head, pass)
+  int sequence, head, pass, piece = 0, pieces = 1;
+  if (a.whole) {  // a workgroup for each part
     pass = blockIdx.x % a.most_passes;
     head = blockIdx.x / a.most_passes % pool.kv_heads;
     sequence = blockIdx.x / a.most_passes / pool.kv_heads;
     d = scalar_drafts(a, sequence);
     if (pass >= d.passes) return;
-    tick = from = 0;
-    end = part_ticks<kTile>(d) - kStart;
   } else {
-    const RaggedPlace place = ragged_place(
-        pool.sequences, [](int s) { return s; }, [&](int s) { return ticks_of<kTile>(a, drafts_of(a, s)); },
-        [&](int total) { return (int)blockIdx.x * run_ticks(total, a); });
-    const int run = run_ticks(place.total, a);
-    tick = scalar(blockIdx.x * run);
-    end = scalar(min(tick + run, place.total));
-    if (tick >= end) return;
-    sequence = scalar(place.sequence);
+    const Cut cut = cut_at<kTile>(a, blockIdx.x);
+    if (cut.sequence < 0) return;
+    sequence = cut.sequence;
     d = scalar_drafts(a, sequence);
-    const int ticks = part_ticks<kTile>(d), index = scalar(place.local / ticks);
-    head = scalar(index / d.passes);
-    pass = index - head * d.passes;
-    from = scalar(place.local) - index * ticks - kStart;
+    head = scalar(cut.part / d.passes);
+    pass = cut.part - head * d.passes;
+    piece = cut.piece;
+    pieces = cut.pieces;
   }
+  const int tiles = tiles_of<kTile>(d.length);
+  // Products pass 32 bits.
+  const int first = (int)((uint64_t)tiles * piece / pieces), until = (int)((uint64_t)tiles * (piece + 1) / pieces);
 
   // This thread's part of a conversion: position p of the tile, elements 32 g .. 32 g + 31.
   const int p = threadIdx.x / kGroups, g = threadIdx.x % kGroups;
@@ -251,367 +292,328 @@ __global__ __launch_bounds__(kThreads, kResident<DIM>) void kv4_tree_kernel(Kv4T
   const uint32_t v_at = v_row * kRow + 8u * (lane & 1) +
                         16u * (v_chunk ^ (DIM == 128 ? 5 * (v_row & 3) : 4 * ((v_row >> 1) & 1) ^ ((v_row >> 1) & 3)));
 
-  while (tick < end) {
-    const int weight = weight_of(d.blocks), tiles = tiles_of<kTile>(d.length);
-    const int to = min(tiles * weight, from + end - tick);
-    // Tiles whose first tick lies in the run.
-    const int first = scalar((max(from, 0) + weight - 1) / weight), until = scalar((max(to, 0) + weight - 1) / weight);
-    if (until > first) {
-      const int col0 = pass * d.blocks * kCols;
-      const int blocks = min(d.blocks, pieces_of(d.columns - col0, kCols));
-      // Waves that share a block's positions: all of them for one block (at dim 128 two), pairs for two.
-      const int shares = blocks >= 3 ? 1 : blocks == 2 ? 2 : min(kWaves, kSubs);
-      const int block = blocks >= 3 ? wave : blocks == 2 ? wave & 1 : 0, share = blocks >= 3 ? 0 : blocks == 2 ? wave >> 1 : wave;
-      const bool works = block < blocks && share < shares;
-      const int stop = min(until * kTile, d.length);
+  const int col0 = pass * d.blocks * kCols;
+  const int blocks = min(d.blocks, pieces_of(d.columns - col0, kCols));
+  // Waves that share a block's positions: all of them for one block (at dim 128 two), pairs for two.
+  const int shares = blocks >= 3 ? 1 : blocks == 2 ? 2 : min(kWaves, kSubs);
+  const int block = blocks >= 3 ? wave : blocks == 2 ? wave & 1 : 0, share = blocks >= 3 ? 0 : blocks == 2 ? wave >> 1 : wave;
+  const bool works = block < blocks && share < shares;
+  const int stop = min(until * kTile, d.length);
 
-      // Page ids of this wave's positions of a tile (at dim 64 twice 16 of them), a tile before its codes.
-      constexpr int kIds = kTile / kWaves / 16;
-      struct Ids {
-        int page[kIds];
-      };
-      auto ids_of = [&](int tile) __attribute__((always_inline)) {
-        // Constant for the whole launch: scalar loads.
-        const auto *table = (const __attribute__((address_space(4))) int *)(pool.table + sequence * pool.table_stride);
-        Ids ids;
+  // Page ids of this wave's positions of a tile (at dim 64 twice 16 of them), a tile before its codes.
+  constexpr int kIds = kTile / kWaves / 16;
+  struct Ids {
+    int page[kIds];
+  };
+  auto ids_of = [&](int tile) __attribute__((always_inline)) {
+    // Constant for the whole launch: scalar loads.
+    const auto *table = (const __attribute__((address_space(4))) int *)(pool.table + sequence * pool.table_stride);
+    Ids ids;
 #pragma unroll
-        for (int i = 0; i < kIds; ++i)
-          ids.page[i] = table[min(tile * kTile + wave * (kTile / kWaves) + 16 * i, max(d.length - 1, 0)) >> pool.page_shift];
-        return ids;
-      };
-      u32x4 k_codes, v_codes;
-      uint32_t k_scale, v_scale;
-      int there;  // of this thread's position: whether its page is known
-      auto load = [&](int tile, const Ids &ids) __attribute__((always_inline)) {
-        const int position = tile * kTile + p, at = position & page_mask;
-        const uint8_t *half[kIds];
-        int known_page[kIds];
+    for (int i = 0; i < kIds; ++i)
+      ids.page[i] = table[min(tile * kTile + wave * (kTile / kWaves) + 16 * i, max(d.length - 1, 0)) >> pool.page_shift];
+    return ids;
+  };
+  u32x4 k_codes, v_codes;
+  uint32_t k_scale, v_scale;
+  int there;  // of this thread's position: whether its page is known
+  auto load = [&](int tile, const Ids &ids) __attribute__((always_inline)) {
+    const int position = tile * kTile + p, at = position & page_mask;
+    const uint8_t *half[kIds];
+    int known_page[kIds];
 #pragma unroll
-        for (int i = 0; i < kIds; ++i) {
-          known_page[i] = (uint32_t)ids.page[i] < (uint64_t)pool.num_pages;
-          half[i] = pool.pages + (known_page[i] ? ids.page[i] : 0) * page_bytes + head * head_bytes;
-        }
-        const bool second = kIds == 2 && lane >= 32;
-        const uint8_t *mine = second ? half[kIds - 1] : half[0];
-        there = second ? known_page[kIds - 1] : known_page[0];
-        k_codes = *reinterpret_cast<const u32x4 *>(mine + at * (DIM / 2) + 16 * g);
-        v_codes = *reinterpret_cast<const u32x4 *>(mine + half_bytes + at * (DIM / 2) + 16 * g);
-        k_scale = mine[scales_at + at * kGroups + g];
-        v_scale = mine[half_bytes + scales_at + at * kGroups + g];
-      };
-      Ids ids = ids_of(first);
-      load(first, ids);
-      ids = ids_of(first + 1);
+    for (int i = 0; i < kIds; ++i) {
+      known_page[i] = (uint32_t)ids.page[i] < (uint64_t)pool.num_pages;
+      half[i] = pool.pages + (known_page[i] ? ids.page[i] : 0) * page_bytes + head * head_bytes;
+    }
+    const bool second = kIds == 2 && lane >= 32;
+    const uint8_t *mine = second ? half[kIds - 1] : half[0];
+    there = second ? known_page[kIds - 1] : known_page[0];
+    k_codes = *reinterpret_cast<const u32x4 *>(mine + at * (DIM / 2) + 16 * g);
+    v_codes = *reinterpret_cast<const u32x4 *>(mine + half_bytes + at * (DIM / 2) + 16 * g);
+    k_scale = mine[scales_at + at * kGroups + g];
+    v_scale = mine[half_bytes + scales_at + at * kGroups + g];
+  };
+  Ids ids = ids_of(first);
+  load(first, ids);
+  ids = ids_of(first + 1);
 
-      const int column = col0 + block * kCols + n;  // this lane's query
-      const Query query = query_of(a, min(column, d.columns - 1));
-      u32x4 qb[kSteps];
+  const int column = col0 + block * kCols + n;  // this lane's query
+  const Query query = query_of(a, min(column, d.columns - 1));
+  u32x4 qb[kSteps];
+  {
+    const uint16_t *q = a.q + (int64_t)(d.begin + query.row) * a.q_token + (head * a.group + query.head) * a.q_head + 8 * h;
+#pragma unroll
+    for (int st = 0; st < kSteps; ++st) {
+      qb[st] = *reinterpret_cast<const u32x4 *>(q + 16 * st);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) qb[st][j] = (qb[st][j] & a.q_and) ^ a.q_xor;
+    }
+  }
+  if (wave == 0 && until * kTile > d.context) {
+    uint64_t seen = ((uint64_t)2 << lane) - 1;
+    if (a.parents) {  // pointers doubled, so that any parents end
+      int up = lane < d.rows ? parent_of(a, d, lane) : -1;
+      seen = (uint64_t)1 << lane;
+#pragma unroll 1
+      for (int i = 0; i < 6; ++i) {
+        const int from_lane = max(up, 0);
+        const uint64_t theirs = __shfl(seen, from_lane);
+        const int further = __shfl(up, from_lane);
+        seen |= up >= 0 ? theirs : 0;
+        up = up >= 0 ? further : -1;
+      }
+    }
+    sees[lane] = seen;  // the others read it behind a barrier
+  }
+  if (threadIdx.x == 0) mads = 0;
+  const float lift = F16 ? 15.f - kPackedLag : -kPackedLag - 1.f - (float)(32 - __builtin_clz(d.length | 1));
+  float m = -INFINITY, l = 0.f;  // running maximum of the query (before the scale), this lane's share of the sum
+  bool any = false;              // whether the query sees a position of this wave's
+  f32x16 o[kOut];                // o[t][r] = O[query][dimension 32 t + 8 (r / 4) + 4 h + r % 4]
+#pragma unroll
+  for (int t = 0; t < kOut; ++t) o[t] = f32x16{};
+
+  // The codes in registers, converted into the buffers of their tile.
+  auto convert = [&](int tile) __attribute__((always_inline)) {
+    char *const kb = keys[tile & 1] + p * kRow, *const vb = values[tile & 1] + p * kRow;
+    const int position = tile * kTile + p;
+    const bool counts = there && position < d.length;
+    uint32_t ks = k_scale, vs = v_scale;
+    if (tile * kTile + kTile > min(d.context, d.length)) {
+      asm volatile("" ::: "memory");  // stays a branch: the last tiles of a sequence
+      bool odd = false;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const u32x4 x = kv4_octet<F16>(v_codes[i], __uint_as_float(vs << 23));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) odd |= not_finite<F16>(x[j]);
+      }
+      odd = odd && counts && position >= d.context;
+      const int row = position - d.context;
+      if (odd && row < kMostDrafts) atomicOr((unsigned long long *)&mads, 1ull << row);
+      vs = odd ? 127u : vs;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v_codes[i] = odd ? 0u : v_codes[i];
+    }
+    ks = counts ? ks : 127u;
+    vs = counts ? vs : 127u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t kc = counts ? k_codes[i] : 0u, vc = counts ? v_codes[i] : 0u;
+      *reinterpret_cast<u32x4 *>(kb + 16 * ((4 * g + i) ^ k_turn)) = kv4_octet<F16>(kc, __uint_as_float(ks << 23));
+      *reinterpret_cast<u32x4 *>(vb + 16 * ((4 * g + i) ^ v_turn)) = kv4_octet<F16>(vc, __uint_as_float(vs << 23));
+    }
+    if (g == 0 && p % 16 == 0) known[tile & 1][p / 16] = (uint8_t)there;
+  };
+  lds_barrier();  // `mads` is clear
+  convert(first);
+  if (first + 1 < until) {
+    load(first + 1, ids);
+    ids = ids_of(first + 2);
+  }
+
+#pragma unroll 1
+  for (int tile = first; tile < until; ++tile) {
+    const int base0 = tile * kTile;
+    lds_barrier();  // this tile is converted, the last one read
+    if (tile + 1 < until) {
+      convert(tile + 1);
+      if (tile + 2 < until) {
+        load(tile + 2, ids);
+        ids = ids_of(tile + 3);
+      }
+    }
+    if (!works) continue;
+#pragma unroll 1
+    for (int sub = share; sub < kSubs; sub += shares) {
+      const int base = base0 + 32 * sub;
+      if (base >= stop) break;
+      const char *kt = keys[tile & 1] + 32 * sub * kRow, *vt = values[tile & 1] + 32 * sub * kRow;
+      const uint32_t pages = *reinterpret_cast<const uint16_t *>(known[tile & 1] + 2 * sub);
+      f32x16 sc;
       {
-        const uint16_t *q = a.q + (int64_t)(d.begin + query.row) * a.q_token + (head * a.group + query.head) * a.q_head + 8 * h;
+        constexpr int kAhead = kSteps < 4 ? kSteps : 4;
+        auto key = [&](int st) __attribute__((always_inline)) { return *reinterpret_cast<const u32x4 *>(kt + (k_at ^ (32u * st))); };
+        u32x4 x[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) x[i] = key(i);
 #pragma unroll
         for (int st = 0; st < kSteps; ++st) {
-          qb[st] = *reinterpret_cast<const u32x4 *>(q + 16 * st);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) qb[st][j] = (qb[st][j] & a.q_and) ^ a.q_xor;
+          sc = mfma32<F16>(x[st % kAhead], qb[st], st == 0 ? f32x16{} : sc);
+          if (st + kAhead < kSteps) x[st % kAhead] = key(st + kAhead);
         }
       }
-      if (wave == 0 && until * kTile > d.context) {
-        uint64_t seen = ((uint64_t)2 << lane) - 1;
-        if (a.parents) {  // pointers doubled, so that any parents end
-          int up = lane < d.rows ? parent_of(a, d, lane) : -1;
-          seen = (uint64_t)1 << lane;
-#pragma unroll 1
-          for (int i = 0; i < 6; ++i) {
-            const int from_lane = max(up, 0);
-            const uint64_t theirs = __shfl(seen, from_lane);
-            const int further = __shfl(up, from_lane);
-            seen |= up >= 0 ? theirs : 0;
-            up = up >= 0 ? further : -1;
-          }
+      // sc[r]: position base + 8 (r / 4) + 4 h + r % 4
+      if (scalar(pages) != 0x0101 || base + 32 > min(stop, d.context)) {
+        asm volatile("" ::: "memory");
+        uint32_t bits = (pages & 1 ? 0xFFFFu : 0u) | (pages >> 8 ? 0xFFFF0000u : 0u);
+        if (stop - base < 32) bits &= (1u << (stop - base)) - 1u;
+        const int ahead = d.context - base;  // where the first drafted row lies, counted from the base
+        if (ahead < 32) {
+          const uint64_t rows = sees[query.row];
+          bits &= ahead >= 0 ? (uint32_t)(rows << ahead) | ((1u << ahead) - 1u) : ahead > -64 ? (uint32_t)(rows >> -ahead) : 0u;
         }
-        sees[lane] = seen;  // the others read it behind a barrier
+        any |= bits != 0;
+        bits >>= 4 * h;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sc[r] = bits >> (8 * (r >> 2) + (r & 3)) & 1 ? sc[r] : -INFINITY;
+      } else {
+        any = true;
       }
-      if (threadIdx.x == 0) mads = 0;
-
-      const float lift = F16 ? 15.f - kPackedLag : -kPackedLag - 1.f - (float)(32 - __builtin_clz(d.length | 1));
-      float m = -INFINITY, l = 0.f;  // running maximum of the query (before the scale), this lane's share of the sum
-      bool any = false;              // whether the query sees a position of this wave's
-      f32x16 o[kOut];                // o[t][r] = O[query][dimension 32 t + 8 (r / 4) + 4 h + r % 4]
+      float mx = fmaxf(sc[0], sc[1]);
 #pragma unroll
-      for (int t = 0; t < kOut; ++t) o[t] = f32x16{};
-
-#pragma unroll 1
-      for (int tile = first; tile < until; ++tile) {
-        const int base0 = tile * kTile;
-        lds_barrier();  // the last tile is read
-        {
-          const int position = base0 + p;
-          const bool counts = there && position < d.length;
-          uint32_t ks = k_scale, vs = v_scale;
-          if (base0 + kTile > min(d.context, d.length)) {
-            asm volatile("" ::: "memory");  // stays a branch: the last tiles of a sequence
-            bool odd = false;
+      for (int r = 2; r < 16; r += 2) mx = fmaxf(fmaxf(mx, sc[r]), sc[r + 1]);
+      const float mnew = halves_max(mx);
+      const bool grow = mnew > m + a.lag;
+      if (__builtin_amdgcn_ballot_w64(grow) != 0) {
+        const float alpha = grow ? __builtin_amdgcn_exp2f((m - mnew) * a.sl2) : 1.f;
+        l *= alpha;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const u32x4 x = kv4_octet<F16>(v_codes[i], __uint_as_float(vs << 23));
+        for (int t = 0; t < kOut; ++t)
 #pragma unroll
-              for (int j = 0; j < 4; ++j) odd |= not_finite<F16>(x[j]);
-            }
-            odd = odd && counts && position >= d.context;
-            const int row = position - d.context;
-            if (odd && row < kMostDrafts) atomicOr((unsigned long long *)&mads, 1ull << row);
-            vs = odd ? 127u : vs;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v_codes[i] = odd ? 0u : v_codes[i];
-          }
-          ks = counts ? ks : 127u;
-          vs = counts ? vs : 127u;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t kc = counts ? k_codes[i] : 0u, vc = counts ? v_codes[i] : 0u;
-            *reinterpret_cast<u32x4 *>(keys + p * kRow + 16 * ((4 * g + i) ^ k_turn)) = kv4_octet<F16>(kc, __uint_as_float(ks << 23));
-            *reinterpret_cast<u32x4 *>(values + p * kRow + 16 * ((4 * g + i) ^ v_turn)) = kv4_octet<F16>(vc, __uint_as_float(vs << 23));
-          }
-          if (g == 0 && p % 16 == 0) known[p / 16] = (uint8_t)there;
-        }
-        if (tile + 1 < until) {
-          load(tile + 1, ids);
-          ids = ids_of(tile + 2);
-        }
-        lds_barrier();
-        if (!works) continue;
-#pragma unroll 1
-        for (int sub = share; sub < kSubs; sub += shares) {
-          const int base = base0 + 32 * sub;
-          if (base >= stop) break;
-          const char *kt = keys + 32 * sub * kRow, *vt = values + 32 * sub * kRow;
-          const uint32_t pages = *reinterpret_cast<const uint16_t *>(known + 2 * sub);
-          f32x16 sc;
-          {
-            constexpr int kAhead = kSteps < 4 ? kSteps : 4;
-            auto key = [&](int st) __attribute__((always_inline)) { return *reinterpret_cast<const u32x4 *>(kt + (k_at ^ (32u * st))); };
-            u32x4 x[kAhead];
-#pragma unroll
-            for (int i = 0; i < kAhead; ++i) x[i] = key(i);
-#pragma unroll
-            for (int st = 0; st < kSteps; ++st) {
-              sc = mfma32<F16>(x[st % kAhead], qb[st], st == 0 ? f32x16{} : sc);
-              if (st + kAhead < kSteps) x[st % kAhead] = key(st + kAhead);
-            }
-          }
-          // sc[r]: position base + 8 (r / 4) + 4 h + r % 4
-          if (scalar(pages) != 0x0101 || base + 32 > min(stop, d.context)) {
-            asm volatile("" ::: "memory");
-            uint32_t bits = (pages & 1 ? 0xFFFFu : 0u) | (pages >> 8 ? 0xFFFF0000u : 0u);
-            if (stop - base < 32) bits &= (1u << (stop - base)) - 1u;
-            const int ahead = d.context - base;  // where the first drafted row lies, counted from the base
-            if (ahead < 32) {
-              const uint64_t rows = sees[query.row];
-              bits &= ahead >= 0 ? (uint32_t)(rows << ahead) | ((1u << ahead) - 1u) : ahead > -64 ? (uint32_t)(rows >> -ahead) : 0u;
-            }
-            any |= bits != 0;
-            bits >>= 4 * h;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) sc[r] = bits >> (8 * (r >> 2) + (r & 3)) & 1 ? sc[r] : -INFINITY;
-          } else {
-            any = true;
-          }
-          float mx = fmaxf(sc[0], sc[1]);
-#pragma unroll
-          for (int r = 2; r < 16; r += 2) mx = fmaxf(fmaxf(mx, sc[r]), sc[r + 1]);
-          const float mnew = halves_max(mx);
-          const bool grow = mnew > m + a.lag;
-          if (__builtin_amdgcn_ballot_w64(grow) != 0) {
-            const float alpha = grow ? __builtin_amdgcn_exp2f((m - mnew) * a.sl2) : 1.f;
-            l *= alpha;
-#pragma unroll
-            for (int t = 0; t < kOut; ++t)
-#pragma unroll
-              for (int r = 0; r < 16; ++r) o[t][r] *= alpha;
-            m = grow ? mnew : m;
-          }
-          const float zero = m == -INFINITY ? 0.f : lift - m * a.sl2;  // no position yet: every score is -infinity
-          uint32_t pb[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            pb[i] = pack2<F16>(__builtin_amdgcn_exp2f(__builtin_fmaf(sc[2 * i], a.sl2, zero)),
-                               __builtin_amdgcn_exp2f(__builtin_fmaf(sc[2 * i + 1], a.sl2, zero)), l);
-          {
-            constexpr int kAhead = 3;
-            auto value = [&](int i) __attribute__((always_inline)) {
-              const char *at = vt + 16 * (i / kOut) * kRow + (v_at ^ (64u * (i % kOut)));
-              const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)at));
-              const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(at + 8 * kRow)));
-              return u32x4{lo[0], lo[1], hi[0], hi[1]};  // slots 0-3: positions 4 h .., 4-7: the 8 behind
-            };
-            u32x4 x[kAhead];
-#pragma unroll
-            for (int i = 0; i < kAhead; ++i) x[i] = value(i);
-#pragma unroll
-            for (int i = 0; i < 2 * kOut; ++i) {
-              const int j = i / kOut, t = i % kOut;
-              o[t] = mfma32<F16>(x[i % kAhead], u32x4{pb[4 * j], pb[4 * j + 1], pb[4 * j + 2], pb[4 * j + 3]}, o[t]);
-              if (i + kAhead < 2 * kOut) x[i % kAhead] = value(i + kAhead);
-            }
-          }
-        }
+          for (int r = 0; r < 16; ++r) o[t][r] *= alpha;
+        m = grow ? mnew : m;
       }
-
-      // The shares of a block meet in LDS, in the tiles' place. A share without a score above -infinity has l = 0 and O = 0 (or NaN,
-      // where scores were).
-      l = halves_sum(l);
-      if (m == -INFINITY && any) l += kNoScore;
-      lds_barrier();  // the last tile is read
-      const uint64_t lost = mads;
-      if (shares > 1) {
-        // Share s of a block: 4 KiB for each 32 dimensions, share 1 and 2 in the keys' place, 3 in the values'.
-        auto region = [&](int s) {
-          const int index = (s - 1) * blocks + block, in_keys = kTile * kRow / (kOut * 4096);
-          return reinterpret_cast<f32x4 *>(index < in_keys ? keys + index * kOut * 4096 : values + (index - in_keys) * kOut * 4096) + lane;
+      const float zero = m == -INFINITY ? 0.f : lift - m * a.sl2;  // no position yet: every score is -infinity
+      uint32_t pb[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        pb[i] = pack2<F16>(__builtin_amdgcn_exp2f(__builtin_fmaf(sc[2 * i], a.sl2, zero)),
+                           __builtin_amdgcn_exp2f(__builtin_fmaf(sc[2 * i + 1], a.sl2, zero)), l);
+      {
+        constexpr int kAhead = 3;
+        auto value = [&](int i) __attribute__((always_inline)) {
+          const char *at = vt + 16 * (i / kOut) * kRow + (v_at ^ (64u * (i % kOut)));
+          const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)at));
+          const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(at + 8 * kRow)));
+          return u32x4{lo[0], lo[1], hi[0], hi[1]};  // slots 0-3: positions 4 h .., 4-7: the 8 behind
         };
-        if (works && share > 0) {
-          stats[wave][0][lane] = m;
-          stats[wave][1][lane] = l;
-          f32x4 *put = region(share);
+        u32x4 x[kAhead];
 #pragma unroll
-          for (int t = 0; t < kOut; ++t)
+        for (int i = 0; i < kAhead; ++i) x[i] = value(i);
 #pragma unroll
-            for (int rq = 0; rq < 4; ++rq) put[64 * (4 * t + rq)] = f32x4{o[t][4 * rq], o[t][4 * rq + 1], o[t][4 * rq + 2], o[t][4 * rq + 3]};
-        }
-        lds_barrier();
-        if (works && share == 0) {
-#pragma unroll 1
-          for (int s = 1; s < shares; ++s) {
-            const int theirs = blocks == 2 ? 2 * s + block : s;
-            const float m2 = stats[theirs][0][lane], l2 = stats[theirs][1][lane], top = fmaxf(m, m2);
-            const float w1 = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - top) * a.sl2);
-            const float w2 = m2 == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m2 - top) * a.sl2);
-            const f32x4 *from_share = region(s);
-#pragma unroll
-            for (int t = 0; t < kOut; ++t)
-#pragma unroll
-              for (int rq = 0; rq < 4; ++rq) {
-                const f32x4 x = from_share[64 * (4 * t + rq)];
-#pragma unroll
-                for (int r = 0; r < 4; ++r) o[t][4 * rq + r] = o[t][4 * rq + r] * w1 + x[r] * w2;
-              }
-            l = l * w1 + l2 * w2;
-            m = top;
-          }
+        for (int i = 0; i < 2 * kOut; ++i) {
+          const int j = i / kOut, t = i % kOut;
+          o[t] = mfma32<F16>(x[i % kAhead], u32x4{pb[4 * j], pb[4 * j + 1], pb[4 * j + 2], pb[4 * j + 3]}, o[t]);
+          if (i + kAhead < 2 * kOut) x[i % kAhead] = value(i + kAhead);
         }
       }
-      if (works && share == 0) {
-        // Groups of value rows that the products left out, for the queries that see them: slow, and seldom.
-        uint64_t rows = lost;
-#pragma unroll 1
-        for (; __builtin_expect(rows != 0, 0); rows &= rows - 1) {
-          const int row = __builtin_ctzll(rows), at = (d.context + row) & page_mask;
-          const int page = pool.table[sequence * pool.table_stride + ((d.context + row) >> pool.page_shift)];
-          const uint8_t *k_half = pool.pages + page * page_bytes + head * head_bytes, *v_half = k_half + half_bytes;
-          uint32_t out = 0;  // a bit for each group
-#pragma unroll 1
-          for (int e = 0; e < DIM; e += 2) out |= (uint32_t)not_finite<F16>(cached_pair<F16, DIM>(v_half, scales_at, at, e)) << (e / 32);
-          const uint16_t *q = a.q + (int64_t)(d.begin + query.row) * a.q_token + (head * a.group + query.head) * a.q_head;
-          const float prob = __builtin_amdgcn_exp2f((cached_score<F16, DIM>(a, q, k_half, scales_at, at) - m) * a.sl2 + lift);
-          const bool does = sees[query.row] >> row & 1;
-#pragma unroll
-          for (int t = 0; t < kOut; ++t) {
-            if (!does || !(out >> t & 1)) continue;
-#pragma unroll
-            for (int r = 0; r < 16; r += 2) {
-              const uint32_t v = cached_pair<F16, DIM>(v_half, scales_at, at, 32 * t + 8 * (r >> 2) + 4 * h + (r & 3));
-              o[t][r] = __builtin_fmaf(prob, half_bits_to_float<F16>((uint16_t)v), o[t][r]);
-              o[t][r + 1] = __builtin_fmaf(prob, half_bits_to_float<F16>((uint16_t)(v >> 16)), o[t][r + 1]);
-            }
-          }
-        }
-        if (first == 0 && until == tiles) {
-          const float inverse = inverse_of(m, l);
-          uint16_t *out = a.out + (int64_t)(d.begin + query.row) * a.out_token + (head * a.group + query.head) * a.out_head + 4 * h;
-          if (column < d.columns) {
-#pragma unroll
-            for (int t = 0; t < kOut; ++t)
-#pragma unroll
-              for (int rq = 0; rq < 4; ++rq) {
-                const f32x4 v = f32x4{o[t][4 * rq], o[t][4 * rq + 1], o[t][4 * rq + 2], o[t][4 * rq + 3]} * inverse;
-                *reinterpret_cast<u32x2 *>(out + 32 * t + 8 * rq) =
-                    u32x2{to_half_bits<F16>(v[0]) | (uint32_t)to_half_bits<F16>(v[1]) << 16,
-                          to_half_bits<F16>(v[2]) | (uint32_t)to_half_bits<F16>(v[3]) << 16};
-              }
-          }
-        } else {
-          float *piece = a.pieces + ((int64_t)blockIdx.x * 2 + slot) * a.piece_floats + block * kPieceFloats<DIM>;
-#pragma unroll
-          for (int t = 0; t < kOut; ++t)
-#pragma unroll
-            for (int rq = 0; rq < 4; ++rq)
-              reinterpret_cast<f32x4 *>(piece)[64 * (4 * t + rq) + lane] = f32x4{o[t][4 * rq], o[t][4 * rq + 1], o[t][4 * rq + 2], o[t][4 * rq + 3]};
-          if (h == 0) {
-            piece[kCols * DIM + n] = m;
-            piece[kCols * DIM + kCols + n] = l;
-          }
-        }
-      }
-      lds_barrier();  // before LDS is written again
     }
-    tick += to - from;
-    from = -kStart;
-    slot = 1;
-    if (tick < end && ++pass == d.passes) {
-      pass = 0;
-      if (++head == pool.kv_heads) {
-        head = 0;
-        do d = scalar_drafts(a, ++sequence);
-        while (d.rows == 0);  // one with work follows: tick < end
+  }
+
+  // The shares of a block meet in LDS, in the tiles' place. A share without a score above -infinity has l = 0 and O = 0 (or NaN,
+  // where scores were).
+  l = halves_sum(l);
+  if (m == -INFINITY && any) l += kNoScore;
+  lds_barrier();  // the last tile is read
+  const uint64_t lost = mads;
+  if (shares > 1) {
+    // Share s of a block: 4 KiB for each 32 dimensions, of which the keys' place has 8.
+    auto region = [&](int s) { return reinterpret_cast<f32x4 *>(keys[0] + ((s - 1) * blocks + block) * kOut * 4096) + lane; };
+    if (works && share > 0) {
+      stats[wave][0][lane] = m;
+      stats[wave][1][lane] = l;
+      f32x4 *put = region(share);
+#pragma unroll
+      for (int t = 0; t < kOut; ++t)
+#pragma unroll
+        for (int rq = 0; rq < 4; ++rq) put[64 * (4 * t + rq)] = f32x4{o[t][4 * rq], o[t][4 * rq + 1], o[t][4 * rq + 2], o[t][4 * rq + 3]};
+    }
+    lds_barrier();
+    if (works && share == 0) {
+#pragma unroll 1
+      for (int s = 1; s < shares; ++s) {
+        const int theirs = blocks == 2 ? 2 * s + block : s;
+        const float m2 = stats[theirs][0][lane], l2 = stats[theirs][1][lane], top = fmaxf(m, m2);
+        const float w1 = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - top) * a.sl2);
+        const float w2 = m2 == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m2 - top) * a.sl2);
+        const f32x4 *from_share = region(s);
+#pragma unroll
+        for (int t = 0; t < kOut; ++t)
+#pragma unroll
+          for (int rq = 0; rq < 4; ++rq) {
+            const f32x4 x = from_share[64 * (4 * t + rq)];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[t][4 * rq + r] = o[t][4 * rq + r] * w1 + x[r] * w2;
+          }
+        l = l * w1 + l2 * w2;
+        m = top;
+      }
+    }
+  }
+  if (works && share == 0) {
+    // Groups of value rows that the products left out, for the queries that see them: slow, and seldom.
+    uint64_t rows = lost;
+#pragma unroll 1
+    for (; __builtin_expect(rows != 0, 0); rows &= rows - 1) {
+      const int row = __builtin_ctzll(rows), at = (d.context + row) & page_mask;
+      const int page = pool.table[sequence * pool.table_stride + ((d.context + row) >> pool.page_shift)];
+      const uint8_t *k_half = pool.pages + page * page_bytes + head * head_bytes, *v_half = k_half + half_bytes;
+      uint32_t out = 0;  // a bit for each group
+#pragma unroll 1
+      for (int e = 0; e < DIM; e += 2) out |= (uint32_t)not_finite<F16>(cached_pair<F16, DIM>(v_half, scales_at, at, e)) << (e / 32);
+      const uint16_t *q = a.q + (int64_t)(d.begin + query.row) * a.q_token + (head * a.group + query.head) * a.q_head;
+      const float prob = __builtin_amdgcn_exp2f((cached_score<F16, DIM>(a, q, k_half, scales_at, at) - m) * a.sl2 + lift);
+      const bool does = sees[query.row] >> row & 1;
+#pragma unroll
+      for (int t = 0; t < kOut; ++t) {
+        if (!does || !(out >> t & 1)) continue;
+#pragma unroll
+        for (int r = 0; r < 16; r += 2) {
+          const uint32_t v = cached_pair<F16, DIM>(v_half, scales_at, at, 32 * t + 8 * (r >> 2) + 4 * h + (r & 3));
+          o[t][r] = __builtin_fmaf(prob, half_bits_to_float<F16>((uint16_t)v), o[t][r]);
+          o[t][r + 1] = __builtin_fmaf(prob, half_bits_to_float<F16>((uint16_t)(v >> 16)), o[t][r + 1]);
+        }
+      }
+    }
+    if (pieces == 1) {
+      const float inverse = inverse_of(m, l);
+      uint16_t *out = a.out + (int64_t)(d.begin + query.row) * a.out_token + (head * a.group + query.head) * a.out_head + 4 * h;
+      if (column < d.columns) {
+#pragma unroll
+        for (int t = 0; t < kOut; ++t)
+#pragma unroll
+          for (int rq = 0; rq < 4; ++rq) {
+            const f32x4 v = f32x4{o[t][4 * rq], o[t][4 * rq + 1], o[t][4 * rq + 2], o[t][4 * rq + 3]} * inverse;
+            *reinterpret_cast<u32x2 *>(out + 32 * t + 8 * rq) =
+                u32x2{to_half_bits<F16>(v[0]) | (uint32_t)to_half_bits<F16>(v[1]) << 16,
+                      to_half_bits<F16>(v[2]) | (uint32_t)to_half_bits<F16>(v[3]) << 16};
+          }
+      }
+    } else {
+      float *piece = a.pieces + (int64_t)blockIdx.x * a.piece_floats + block * kPieceFloats<DIM>;
+#pragma unroll
+      for (int t = 0; t < kOut; ++t)
+#pragma unroll
+        for (int rq = 0; rq < 4; ++rq)
+          reinterpret_cast<f32x4 *>(piece)[64 * (4 * t + rq) + lane] = f32x4{o[t][4 * rq], o[t][4 * rq + 1], o[t][4 * rq + 2], o[t][4 * rq + 3]};
+      if (h == 0) {
+        piece[kCols * DIM + n] = m;
+        piece[kCols * DIM + kCols + n] = l;
       }
     }
   }
 }
 
-// Joins the pieces of (head, pass)es that several workgroups shared. Grid: y = block of the pass. BORDERS: x = the borders of runs, of
-// which the first in a part joins it, a wave every fourth slice of 1 KiB of its outputs. Else x = the (sequence, head, pass)es, z = the
-// slices, a wave every fourth piece: few parts of many pieces.
-template <bool F16, int DIM, bool BORDERS>
+// Joins the pieces of the parts that were cut. Grid: x = parts, y = block of the pass. SHARED: z = slices of 1 KiB of a block's
+// outputs, of which the waves each take every fourth piece; else each wave has a quarter of the slices.
+template <bool F16, int DIM, bool SHARED>
 __global__ __launch_bounds__(kThreads) void kv4_tree_combine_kernel(Kv4Tree a) {
-  constexpr int kTile = tx::kTile<DIM>, kSlices = DIM / 8, kHeld = 4, kStride = BORDERS ? 1 : kWaves;
-  __shared__ f32x4 sums[BORDERS ? 1 : kWaves][64];
-  __shared__ float stats[BORDERS ? 1 : kWaves][2][64];
+  constexpr int kTile = tx::kTile<DIM>, kHeld = 4, kStride = SHARED ? kWaves : 1, kSlices = SHARED ? 1 : DIM / 8 / kWaves;
+  __shared__ f32x4 sums[SHARED ? kWaves : 1][64];
+  __shared__ float stats[SHARED ? kWaves : 1][2][64];
   const Kv4Pool &pool = a.pool;
   const int lane = threadIdx.x & 63, wave = scalar(threadIdx.x >> 6);
-  int sequence, head, pass, begin, run;  // begin: the part's first tick in the row of all
-  Drafts d;
-  auto ticks = [&](int s) { return ticks_of<kTile>(a, drafts_of(a, s)); };
-  if constexpr (BORDERS) {
-    int at = 0;
-    const RaggedPlace place = ragged_place(pool.sequences, [](int s) { return s; }, ticks, [&](int total) { return at = ((int)blockIdx.x + 1) * run_ticks(total, a); });
-    if (at >= place.total) return;
-    run = run_ticks(place.total, a);
-    sequence = scalar(place.sequence);
-    d = scalar_drafts(a, sequence);
-    const int a_part = part_ticks<kTile>(d), index = scalar(place.local / a_part);
-    head = scalar(index / d.passes);
-    pass = index - head * d.passes;
-    begin = at - place.local + index * a_part;
-  } else {
-    sequence = blockIdx.x / a.most_passes / pool.kv_heads;
-    pass = blockIdx.x % a.most_passes;
-    head = blockIdx.x / a.most_passes % pool.kv_heads;
-    d = scalar_drafts(a, sequence);
-    if (pass >= d.passes) return;
-    const RaggedPlace place = ragged_before(pool.sequences, [](int s) { return s; }, ticks, sequence);
-    run = run_ticks(place.total, a);
-    begin = place.local + (head * d.passes + pass) * part_ticks<kTile>(d);
-  }
-  const int block = blockIdx.y, col0 = (pass * d.blocks + block) * kCols;
-  if (block >= d.blocks || col0 >= d.columns) return;
-  const int work = begin + kStart;
-  const int w0 = work / run, w1 = (work + (tiles_of<kTile>(d.length) - 1) * weight_of(d.blocks)) / run;  // of the first and last tile
-  if (w0 == w1) return;  // one workgroup had it all and wrote the output
-  if (BORDERS && (int)blockIdx.x != w0) return;
-  // Only the first workgroup can have had another part before this one.
-  auto piece = [&](int w) {
-    return a.pieces + ((int64_t)w * 2 + (w == w0 && begin > w0 * run ? 1 : 0)) * a.piece_floats + block * kPieceFloats<DIM>;
-  };
+  const int pass = blockIdx.x % a.most_passes, head = blockIdx.x / a.most_passes % pool.kv_heads;
+  const int sequence = blockIdx.x / a.most_passes / pool.kv_heads, block = blockIdx.y;
+  const Drafts d = scalar_drafts(a, sequence);
+  const int col0 = (pass * d.blocks + block) * kCols;
+  if (pass >= d.passes || block >= d.blocks || col0 >= d.columns) return;
+  const Cut cut = cut_at<kTile>(a, ~sequence);
+  const int w1 = cut.pieces - 1, slice0 = SHARED ? blockIdx.z : wave * kSlices;
+  if (w1 == 0) return;  // one workgroup had it all and wrote the output
+  const float *pieces = a.pieces + (int64_t)(cut.before + (head * d.passes + pass) * cut.pieces) * a.piece_floats + block * kPieceFloats<DIM>;
   const int n = lane & 31, column = col0 + n;
   const Query query = query_of(a, min(column, d.columns - 1));
   auto put = [&](int slice, f32x4 sum, float top, float ll) __attribute__((always_inline)) {
@@ -622,97 +624,100 @@ __global__ __launch_bounds__(kThreads) void kv4_tree_combine_kernel(Kv4Tree a) {
           u32x2{to_half_bits<F16>(sum[0]) | (uint32_t)to_half_bits<F16>(sum[1]) << 16,
                 to_half_bits<F16>(sum[2]) | (uint32_t)to_half_bits<F16>(sum[3]) << 16};
   };
+  f32x4 sum[kSlices] = {};
+  float l = 0.f, m = -INFINITY;
+  for (int w = SHARED ? wave : 0; w <= w1; w += kStride * kHeld) {
+    f32x4 value[kHeld][kSlices];
+    float pm[kHeld], pl[kHeld];
 #pragma unroll
-  for (int slice = BORDERS ? wave : blockIdx.z; slice < kSlices; slice += BORDERS ? kWaves : kSlices) {
-    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-    float l = 0.f, m = -INFINITY;
-    for (int w = w0 + (BORDERS ? 0 : wave); w <= w1; w += kStride * kHeld) {
-      f32x4 value[kHeld];
-      float pm[kHeld], pl[kHeld];
+    for (int i = 0; i < kHeld; ++i) {
+      const float *at = pieces + (int64_t)min(w + i * kStride, w1) * a.piece_floats;
+      pm[i] = at[kCols * DIM + n];
+      pl[i] = at[kCols * DIM + kCols + n];
 #pragma unroll
-      for (int i = 0; i < kHeld; ++i) {
-        const float *at = piece(min(w + i * kStride, w1));
-        value[i] = *reinterpret_cast<const f32x4 *>(at + 256 * slice + 4 * lane);
-        pm[i] = at[kCols * DIM + n];
-        pl[i] = at[kCols * DIM + kCols + n];
-      }
-      float mnew = m;
-#pragma unroll
-      for (int i = 0; i < kHeld; ++i) mnew = w + i * kStride <= w1 ? fmaxf(mnew, pm[i]) : mnew;
-      const float alpha = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - mnew) * a.sl2);
-      sum *= alpha;
-      l *= alpha;
-      m = mnew;
-#pragma unroll
-      for (int i = 0; i < kHeld; ++i) {
-        if (w + i * kStride > w1) continue;
-        const float weight = pm[i] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((pm[i] - m) * a.sl2);  // an empty piece holds zeros (or NaN)
-        sum += value[i] * weight;
-        l += pl[i] * weight;
-      }
+      for (int j = 0; j < kSlices; ++j) value[i][j] = *reinterpret_cast<const f32x4 *>(at + 256 * (slice0 + j) + 4 * lane);
     }
-    if constexpr (BORDERS) {
-      put(slice, sum, m, l);
-    } else {
-      sums[wave][lane] = sum;
-      stats[wave][0][lane] = m;
-      stats[wave][1][lane] = l;
-      __syncthreads();
-      if (wave != 0) return;
-      float top = -INFINITY, ll = 0.f;
+    float mnew = m;
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) top = fmaxf(top, stats[w][0][lane]);
-      f32x4 total = {0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < kHeld; ++i) mnew = w + i * kStride <= w1 ? fmaxf(mnew, pm[i]) : mnew;
+    const float alpha = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - mnew) * a.sl2);
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) {
-        const float weight = stats[w][0][lane] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((stats[w][0][lane] - top) * a.sl2);
-        total += sums[w][lane] * weight;
-        ll += stats[w][1][lane] * weight;
-      }
-      put(slice, total, top, ll);
+    for (int j = 0; j < kSlices; ++j) sum[j] *= alpha;
+    l *= alpha;
+    m = mnew;
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+      if (w + i * kStride > w1) continue;
+      const float weight = pm[i] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((pm[i] - m) * a.sl2);  // an empty piece holds zeros (or NaN)
+#pragma unroll
+      for (int j = 0; j < kSlices; ++j) sum[j] += value[i][j] * weight;
+      l += pl[i] * weight;
     }
+  }
+  if constexpr (!SHARED) {
+#pragma unroll
+    for (int j = 0; j < kSlices; ++j) put(slice0 + j, sum[j], m, l);
+  } else {
+    sums[wave][lane] = sum[0];
+    stats[wave][0][lane] = m;
+    stats[wave][1][lane] = l;
+    __syncthreads();
+    if (wave != 0) return;
+    float top = -INFINITY, ll = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) top = fmaxf(top, stats[w][0][lane]);
+    f32x4 total = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const float weight = stats[w][0][lane] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((stats[w][0][lane] - top) * a.sl2);
+      total += sums[w][lane] * weight;
+      ll += stats[w][1][lane] * weight;
+    }
+    put(slice0, total, top, ll);
   }
 }
 
 // Upper bounds of a call from what the host knows.
 int64_t most_blocks(const Kv4Tree &a) { return ((int64_t)(a.tokens < kMostDrafts ? a.tokens : kMostDrafts) * a.group + kCols - 1) / kCols; }
 int64_t most_passes(const Kv4Tree &a) { return (most_blocks(a) + kPass - 1) / kPass; }
+int64_t most_parts(const Kv4Tree &a) { return (int64_t)a.pool.sequences * a.pool.kv_heads * most_passes(a); }
 int64_t most_ticks(const Kv4Tree &a, int tile) {
   const int64_t room = (int64_t)a.pool.max_pages << a.pool.page_shift, tiles = (room + tile - 1) / tile;
-  return (int64_t)a.pool.sequences * a.pool.kv_heads * most_passes(a) * (kStart + kMostWeight * tiles);
+  return most_parts(a) * (kStart + kMostWeight * tiles);
 }
 
 }  // namespace
 
 // Ticks are 32-bit; a launch has fewer than 2^32 threads, 256 for each (head, pass).
 bool kv4_tree_fits(const Kv4Tree &a) {
-  return most_ticks(a, kTile<128>) <= (int64_t)1 << 30 && (int64_t)a.pool.sequences * a.pool.kv_heads * most_passes(a) < (int64_t)1 << 24;
+  return most_ticks(a, kTile<128>) <= (int64_t)1 << 30 && most_parts(a) < (int64_t)1 << 24;
 }
 
 void kv4_tree_plan(Kv4Tree &a, int dim, int cus) {
   const int64_t room = (int64_t)a.pool.max_pages << a.pool.page_shift;
-  const int64_t parts = (int64_t)a.pool.sequences * a.pool.kv_heads * most_passes(a);
   a.most_passes = (int)most_passes(a);
   a.whole = room <= 512;
-  const int64_t most = most_ticks(a, dim == 128 ? kTile<128> : kTile<64>), fill = (dim == 128 ? kResident<128> : kResident<64>) * (int64_t)cus;
-  a.workgroups = (int)(a.whole ? parts : most < fill ? most : fill);
+  const int64_t shares = most_ticks(a, dim == 128 ? kTile<128> : kTile<64>) / kLeast + 1;
+  const int64_t fill = (dim == 128 ? kResident<128> : kResident<64>) * (int64_t)cus;
+  a.workgroups = (int)(shares < fill ? shares : fill);
   const int64_t blocks = most_blocks(a) < kPass ? most_blocks(a) : kPass;
   a.piece_floats = (int)blocks * (dim == 128 ? kPieceFloats<128> : kPieceFloats<64>);
-  a.piece_bytes = a.whole ? 0 : (int64_t)a.workgroups * 2 * a.piece_floats * (int64_t)sizeof(float);
+  // A part is cut where it has one and a half shares: into at most four thirds of them.
+  a.piece_bytes = a.whole ? 0 : ((int64_t)a.workgroups * 4 / 3 + 1) * a.piece_floats * (int64_t)sizeof(float);
 }
 
 hipError_t launch_kv4_tree(const Kv4Tree &a, bool f16, int dim, hipStream_t stream) {
   auto launch = [&](auto type, auto dims) {
     constexpr bool kF16 = decltype(type)::value;
     constexpr int kDim = decltype(dims)::value;
-    hipLaunchKernelGGL((kv4_tree_kernel<kF16, kDim>), dim3((unsigned)a.workgroups), dim3(kThreads), 0, stream, a);
-    if (a.whole) return;
-    const int64_t parts = (int64_t)a.pool.sequences * a.pool.kv_heads * a.most_passes;
+    const int64_t parts = most_parts(a);
     const unsigned in_pass = (unsigned)(most_blocks(a) < kPass ? most_blocks(a) : kPass);
+    hipLaunchKernelGGL((kv4_tree_kernel<kF16, kDim>), dim3((unsigned)(parts + (a.whole ? 0 : a.workgroups))), dim3(kThreads), 0, stream, a);
+    if (a.whole) return;
     if (parts <= 128)
-      hipLaunchKernelGGL((kv4_tree_combine_kernel<kF16, kDim, false>), dim3((unsigned)parts, in_pass, kDim / 8), dim3(kThreads), 0, stream, a);
-    else if (a.workgroups > 1)
-      hipLaunchKernelGGL((kv4_tree_combine_kernel<kF16, kDim, true>), dim3((unsigned)a.workgroups - 1, in_pass), dim3(kThreads), 0, stream, a);
+      hipLaunchKernelGGL((kv4_tree_combine_kernel<kF16, kDim, true>), dim3((unsigned)parts, in_pass, kDim / 8), dim3(kThreads), 0, stream, a);
+    else
+      hipLaunchKernelGGL((kv4_tree_combine_kernel<kF16, kDim, false>), dim3((unsigned)parts, in_pass), dim3(kThreads), 0, stream, a);
   };
   using std::integral_constant;
   if (f16 && dim == 128) launch(integral_constant<bool, true>{}, integral_constant<int, 128>{});
