@@ -1713,7 +1713,8 @@ int tx_kv4_append_rope(const void *q, int64_t q_token, int64_t q_head, const voi
   a.cu = cu;
   a.heads = heads, a.rotary = rotary, a.tokens = (int)tokens;
   DeviceGuard guard(device);
-  TX_HIP(tx::launch_kv4_append_rope(a, interleaved != 0, dtype == TX_DTYPE_F16, head_dim, pool, reinterpret_cast<hipStream_t>(stream)));
+  TX_HIP(tx::launch_kv4_append_rope(a, interleaved != 0, dtype == TX_DTYPE_F16, head_dim, pool, multiprocessors(device),
+                                    reinterpret_cast<hipStream_t>(stream)));
   return TX_OK;
 }
 

@@ -248,7 +248,7 @@ hipError_t launch_kv4_read(uint16_t *k, int64_t k_token, int64_t k_head, uint16_
                            int tokens, bool f16, int dim, const int *cu, const Kv4Pool &pool, hipStream_t stream);
 // The same with keys (and queries) rotated on the way, and the accepted rows of drafts moved together, in `layers` pools.
 struct Kv4Rope;
-hipError_t launch_kv4_append_rope(Kv4Rope a, bool interleaved, bool f16, int dim, const Kv4Pool &pool, hipStream_t stream);
+hipError_t launch_kv4_append_rope(Kv4Rope a, bool interleaved, bool f16, int dim, const Kv4Pool &pool, int cus, hipStream_t stream);
 hipError_t launch_kv4_keep_path(const Kv4Pool &pool, int dim, int layers, int64_t layer_bytes, const int *cu, int tokens,
                                 const int *path, const int *accepted, int *lengths_out, hipStream_t stream);
 constexpr int kKv4Pairs = 448;  // page pairs of one copy launch: 3.5 KiB of kernel arguments

@@ -59,7 +59,9 @@ struct Kv4Rope {
   const int *positions;  // [tokens], or null: every token's place in the cache
   const int *cu;
   int heads, rotary, tokens;
-  int per;  // heads of a workgroup, filled in by the launch
+  // Filled in by the launch: heads of a workgroup; whether four entries of the tables are 16-byte aligned.
+  int per;
+  bool wide;
 };
 
 // Attention of drafted rows; sl2, q_and and q_xor as above.
