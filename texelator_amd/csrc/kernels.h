@@ -279,11 +279,12 @@ struct Verify {
   int tokens, sequences, vocab;
   int *accepted, *path;  // [sequences], [tokens]
   int64_t *next;         // [tokens]
-  // Filled in by verify_plan: spans of a row's statistics, workgroups, parts and tokens a part of a last row; the workspace.
-  int spans, groups, parts, part;
-  int64_t closings_at, sums_at, workspace_bytes;
+  // Filled in by verify_plan: spans of a row's statistics, workgroups and chunks of a last row; the workspace.
+  int spans, groups, chunks;
+  int64_t counters_at, sums_at, workspace_bytes;
   float2 *partials;
-  void *closings, *sums;
+  int *counters;
+  void *sums;
 };
 constexpr int kVerifyF16 = 0, kVerifyBf16 = 1, kVerifyF32 = 2;
 void verify_plan(Verify &a, int dtype_bytes, int cus);

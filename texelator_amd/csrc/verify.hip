@@ -11,13 +11,18 @@
 //   * T = 0: accepted where the token is the largest logit's (of equal ones the first), which is the closing token too.
 // A token is drawn as the first whose running sum in the vocabulary's order exceeds u_0 times the whole sum.
 //
-// Three launches. The first reads all logits once, a wave 64 * kLoads * 16 bytes of a row, and leaves the maximum and the sum
-// of exponentials of each such span, in 32 bits: enough for the tests (off by some 1e-7). The second finds every sequence's path: a
-// lane has a row, all drafts are tested at once and a row is reached where all rows that lead to it are taken. Its
-// workgroups then share the last row reached and sum its weights in 64 bits, a wave a span: a draw is as exact as those
-// sums are, and 150 thousand borders lie close. The third finds the span, then the token in it. For the residual max(p - q, 0) the
-// sums of p and q are only known after the second launch: it sums p's and q's weights over the tokens where p > q by the
-// first launch's sums; a token that those put on the wrong side adds at most 1e-7 of its own probability.
+// Two launches. The first reads all logits once, a wave 64 * kLoads * 16 bytes of a row, and leaves the maximum and the sum
+// of exponentials of each such span, in 32 bits: enough for the tests (off by some 1e-7). In the second every workgroup of a sequence
+// finds its path: a lane has a row, all drafts are tested at once and a row is reached where all rows that lead to it are taken. The
+// workgroups then share the last row reached and sum its weights in 64 bits, a wave 512 tokens: a draw is as exact as those
+// sums are, and 150 thousand borders lie close. The one that ends last finds the 512 tokens, then the token in them; who that is
+// changes no result. For the residual max(p - q, 0) the sums of p and q are only known then: the weights of p and q are summed over the
+// tokens where p > q by the first launch's sums; a token that those put on the wrong side adds at most 1e-7 of its own probability.
+//
+// Measured, first and second launch: 16 chains of up to 8 rows sampled from a draft's logits of 151,936 bf16 tokens 15 us (the
+// logits' 81 MB at 5.4 TB/s) and 26 us, 24 trees of up to 64 rows of 32,003 fp32 tokens 26 us (5.5 TB/s) and 17 us, one
+// tree of 6 rows 4 us and 15 us. The second is bound by its steps' latency: 6 us to the path, 5 to 13 for the sums, 5 to 7 for the token.
+// With a launch of its own for the token and a wave for each row's statistics they took 64, 69 and 26 us in all.
 #include <math.h>
 
 #include "elementwise.h"
@@ -67,7 +72,7 @@ constexpr double power_of_ln2(int k) { return k == 0 ? 1.0 : power_of_ln2(k - 1)
 
 // 2^y of y <= 0 in 64 bits: the Taylor sum of 2^f, |f| <= 1/2, to the twelfth power (off by 2e-16). NaN stays.
 __device__ __forceinline__ double exp2_64(double y) {
-  if (!(y >= -1100.0)) return y != y ? y : 0.0;
+  y = y < -1100.0 ? -1100.0 : y;  // 2^-1100 is zero
   constexpr double kTerm[13] = {power_of_ln2(0), power_of_ln2(1), power_of_ln2(2),  power_of_ln2(3),  power_of_ln2(4),
                                 power_of_ln2(5), power_of_ln2(6), power_of_ln2(7),  power_of_ln2(8),  power_of_ln2(9),
                                 power_of_ln2(10), power_of_ln2(11), power_of_ln2(12)};
@@ -99,6 +104,8 @@ template <typename T>
 __global__ __launch_bounds__(kThreads) void verify_stats_kernel(Verify a) {
   const int lane = threadIdx.x & 63, span = blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int row = blockIdx.y;
+  if (blockIdx.x == 0 && blockIdx.z == 0)  // the second launch counts in them
+    for (int64_t s = (int64_t)row * kThreads + threadIdx.x; s < a.sequences; s += (int64_t)a.tokens * kThreads) a.counters[s] = 0;
   if (span >= a.spans) return;
   const bool draft = blockIdx.z != 0;
   const T *logits = reinterpret_cast<const T *>(draft ? a.draft : a.target) + row * (draft ? a.draft_row : a.target_row);
@@ -160,19 +167,19 @@ __global__ __launch_bounds__(kThreads) void verify_stats_kernel(Verify a) {
   if (lane == 0) *partial = make_float2(top, sum);
 }
 
-// What the second launch leaves of a sequence for the third.
+// How a sequence's last token is drawn.
 struct Closing {
-  int row;        // the last row reached, in the packed rows; -1: nothing to draw
-  int first;      // the sequence's first row
-  int slot;       // where the token goes
-  int residual;   // drawn from max(p - q, 0)
-  float temperature;
+  int row;       // the last row reached, in the packed rows; -1: nothing to draw
+  int first;     // the sequence's first row
+  int slot;      // where the token goes
+  int residual;  // drawn from max(p - q, 0)
   float top, draft_top;
-  int removed;  // tokens that are left out
+  double scale_p, scale_q;  // 1 / sums of the row's p and q, by the first launch
+  int removed;              // tokens that are left out
   int64_t tokens[kMostDrafts];
 };
 
-// Sums of a span of the last row: all weights of p and of q; of the tokens that may be drawn, those of p and of q.
+// Sums of a chunk of the last row: all weights of p and of q; of the tokens that may be drawn, those of p and of q.
 struct Sums {
   double p, q, rest_p, rest_q;
 };
@@ -188,79 +195,212 @@ __device__ __forceinline__ double wave_sum64(double v) {
   return v;
 }
 
-// The weights of one token of the last row: of p, of q, and whether it may be drawn.
+// Tokens that a wave sums at once, eight neighbours a lane.
+constexpr int kEight = 8, kChunk = 64 * kEight;
+constexpr int kWalkWaves = 16;  // waves of a workgroup of the second launch
+
+// The eight logits from `at` on, -infinity behind the last.
 template <typename T>
-struct Weights {
-  const Verify &a;
-  const Closing &c;
-  double rate;
-  double scale_p, scale_q;  // 1 / sums of p and of q, as well as they are known
-  __device__ __forceinline__ void at(int token, double &p, double &q, bool &rest) const {
-    const float x = logit<T>(a.target, a.target_row, c.row, token);
-    p = x == -INFINITY ? 0.0 : exp2_64(((double)x - (double)c.top) * rate);
-    q = 0.0;
-    rest = true;
-    if (c.residual) {
-      const float y = logit<T>(a.draft, a.draft_row, c.row, token);
-      q = y == -INFINITY ? 0.0 : exp2_64(((double)y - (double)c.draft_top) * rate);
-      rest = p * scale_p > q * scale_q;
-    }
-    for (int i = 0; i < c.removed; ++i) rest &= c.tokens[i] != token;
+__device__ __forceinline__ void eight_logits(const void *logits, int64_t row_stride, int64_t row, int at, int vocab, float *x) {
+  const T *from = reinterpret_cast<const T *>(logits) + row * row_stride + at;
+  if (at + kEight <= vocab) {
+#pragma unroll
+    for (int i = 0; i < kEight; i += kVector<T>) widen_all<T>(*reinterpret_cast<const u32x4_any *>(from + i), x + i);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kEight; ++i) x[i] = at + i < vocab ? widen(from[i]) : -INFINITY;
   }
-};
+}
+
+// exp((x - top) / T) in 64 bits.
+__device__ __forceinline__ double weight_of(float x, float top, double rate) {
+  const double w = exp2_64(((double)x - (double)top) * rate);
+  return x == -INFINITY ? 0.0 : w;
+}
+
+// Eight tokens of the last row: take(i, weight of p, weight of q, whether it may be drawn); scale_p and scale_q say where p > q.
+template <typename T, typename Take>
+__device__ __forceinline__ void eight_weights(const Verify &a, const Closing &c, double rate, int at, double scale_p, double scale_q, Take take) {
+  float x[kEight], y[kEight];
+  eight_logits<T>(a.target, a.target_row, c.row, at, a.vocab, x);
+  const bool residual = __builtin_amdgcn_readfirstlane(c.residual);
+  if (residual) eight_logits<T>(a.draft, a.draft_row, c.row, at, a.vocab, y);
+  uint32_t out = 0;
+  for (int i = 0; i < c.removed; ++i) {
+    const int64_t distance = c.tokens[i] - at;
+    out |= (uint64_t)distance < kEight ? 1u << distance : 0u;
+  }
+  // Without branches: the eight are then under way together.
+  double p[kEight], q[kEight];
+#pragma unroll
+  for (int i = 0; i < kEight; ++i) p[i] = weight_of(x[i], c.top, rate), q[i] = 0.0;
+  if (residual) {
+#pragma unroll
+    for (int i = 0; i < kEight; ++i) q[i] = weight_of(y[i], c.draft_top, rate);
+  }
+#pragma unroll
+  for (int i = 0; i < kEight; ++i) {
+    const bool some = !residual | (p[i] * scale_p > q[i] * scale_q);
+    take(i, p[i], q[i], !(out >> i & 1) & some);
+  }
+}
+
+// Inclusive sum over the lanes of a wave.
+__device__ __forceinline__ double wave_scan64(double v, int lane) {
+#pragma unroll
+  for (int w = 1; w < 64; w *= 2) {
+    const double other = __shfl_up(v, w);
+    v += lane >= w ? other : 0.0;
+  }
+  return v;
+}
+
+// The first lane whose running sum exceeds `target`, the sums before it added to `before`; else the last lane with a weight, else -1.
+__device__ __forceinline__ int crossing(double v, double target, double &before, int lane) {
+  const double sum = before + wave_scan64(v, lane);
+  const uint64_t past = __builtin_amdgcn_ballot_w64(sum > target && v > 0.0), some = __builtin_amdgcn_ballot_w64(v > 0.0);
+  if (some == 0) return -1;
+  const int at = past ? __builtin_ctzll(past) : 63 - __builtin_clzll(some);
+  before = __shfl(sum - v, at);
+  return at;
+}
+
+// Lanes that have this lane's `bits` low bits of v.
+__device__ __forceinline__ uint64_t same_lanes(int v, int bits) {
+  uint64_t same = ~(uint64_t)0;
+  for (int b = 0; b < bits; ++b) {
+    const bool mine = v >> b & 1;
+    const uint64_t set = __builtin_amdgcn_ballot_w64(mine);
+    same &= mine ? set : ~set;
+  }
+  return same;
+}
+
+// Draws the closing token by one wave: the 512 tokens of the last row in which the running sum passes, then the token in them.
+template <typename T>
+__device__ __forceinline__ int64_t closing_token(const Verify &a, const Closing &closing, double rate, const Sums *sums, float uniform) {
+  const int lane = threadIdx.x & 63;
+  // Lane l has the chunks l * each .. of the row.
+  const int each = (a.chunks + 63) / 64, first = lane * each, last = min(first + each, a.chunks);
+  Sums mine = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll 4
+  for (int i = first; i < last; ++i) {
+    mine.p += sums[i].p;
+    mine.q += sums[i].q;
+    mine.rest_p += sums[i].rest_p;
+    mine.rest_q += sums[i].rest_q;
+  }
+  const bool residual = __builtin_amdgcn_readfirstlane(closing.residual);
+  const double all_p = wave_sum64(mine.p), all_q = residual ? wave_sum64(mine.q) : 0.0;
+  const double scale_p = 1.0 / all_p, scale_q = residual ? 1.0 / all_q : 0.0;
+  // What counts of a sum, and whether anything does: else it is drawn from all of p.
+  auto rest_of = [&](const Sums &s) { return residual ? fmax(s.rest_p * scale_p - s.rest_q * scale_q, 0.0) : s.rest_p; };
+  const bool all = !(wave_sum64(rest_of(mine)) > 0.0);
+  auto value_of = [&](const Sums &s) { return all ? s.p : rest_of(s); };
+  double value = 0.0;
+#pragma unroll 4
+  for (int i = first; i < last; ++i) value += value_of(sums[i]);
+  const double total = wave_sum64(value);
+  if (!(total > 0.0) || (residual && !(all_q > 0.0))) return -1;
+  const double target = (double)uniform * total;
+  double before = 0.0;
+  const int l = crossing(value, target, before, lane);
+  const int base = l * each, count = min(base + each, a.chunks) - base;
+  const int chunk = base + crossing(lane < count ? value_of(sums[base + lane]) : 0.0, target, before, lane);
+  int64_t token = -1;
+  // Once more with all of p where a chunk's rest was nothing but rounding.
+  for (int turn = 0; turn < 2 && token < 0; ++turn) {
+    double weight[kEight], held = 0.0;
+    eight_weights<T>(a, closing, rate, chunk * kChunk + lane * kEight, scale_p, scale_q, [&](int i, double p, double q, bool rest) {
+      weight[i] = all || turn ? p : !rest ? 0.0 : residual ? p * scale_p - q * scale_q : p;
+      held += weight[i];
+    });
+    double sum = before;
+    const int at = crossing(held, target, sum, lane);
+    bool past = false;
+#pragma unroll
+    for (int i = 0; i < kEight; ++i) {
+      sum += weight[i];
+      if (weight[i] > 0.0 && !past) {
+        token = chunk * kChunk + lane * kEight + i;
+        past = sum > target;
+      }
+    }
+    token = at >= 0 ? __shfl(token, max(at, 0)) : -1;
+  }
+  return token;
+}
 
 // Grid: x workgroups of a sequence, y sequences.
 template <typename T>
-__global__ __launch_bounds__(kThreads) void verify_walk_kernel(Verify a) {
-  __shared__ float tops[2][kMostDrafts];    // maxima of the rows; of the draft's
-  __shared__ double sums[2][kMostDrafts];   // sums of their weights; at T = 0 the target's first largest token
+__global__ __launch_bounds__(64 * kWalkWaves) void verify_walk_kernel(Verify a) {
+  __shared__ float tops[2][kMostDrafts];   // maxima of the rows; of the draft's
+  __shared__ double sums[2][kMostDrafts];  // sums of their weights; at T = 0 the target's first largest token
   __shared__ Closing closing;
   __shared__ int order[kMostDrafts];  // the path's rows
+  __shared__ bool ends;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), sequence = blockIdx.y;
   const Rows rows = rows_of(a, sequence);
-  Closing *kept = reinterpret_cast<Closing *>(a.closings) + sequence;
   const bool writes = blockIdx.x == 0;
   if (rows.count <= 0) {
-    if (writes && threadIdx.x == 0) {
-      a.accepted[sequence] = -1;
-      kept->row = -1;
-    }
+    if (writes && threadIdx.x == 0) a.accepted[sequence] = -1;
     return;
   }
   const float temperature = temperature_of(a, sequence);
   const bool greedy = !(temperature > 0.f);
   const double rate = greedy ? 0.0 : rate_of(temperature);
-  // The rows' statistics from their spans'.
-  const int kinds = a.draft && !greedy ? 2 : 1;
-  for (int i = wave; i < rows.count * kinds; i += kWaves) {
-    const int kind = i / rows.count, local = i % rows.count;
+  // The first wave's lane i is row i; its logits are under way while the statistics are joined.
+  const bool row = wave == 0 && lane < rows.count;
+  int parent = -1;
+  int64_t token = -1;
+  float u = 0.f, x = -INFINITY, y = -INFINITY;
+  if (row) {
+    parent = a.parents ? a.parents[rows.begin + lane] : lane - 1;
+    token = a.ids[rows.begin + lane];
+    u = a.uniforms[rows.begin + lane];
+  }
+  if (lane == 0 || (uint32_t)parent >= (uint32_t)rows.count) parent = -1;
+  const bool child = row && parent >= 0, known = child && token >= 0 && token < a.vocab;
+  if (known && !greedy) {
+    x = logit<T>(a.target, a.target_row, rows.begin + parent, token);
+    if (a.draft) y = logit<T>(a.draft, a.draft_row, rows.begin + parent, token);
+  }
+  // The rows' statistics from their spans', by 16, 32 or 64 lanes a row.
+  const int kinds = a.draft && !greedy ? 2 : 1, width = a.spans <= 16 ? 16 : a.spans <= 32 ? 32 : 64;
+  for (int i = threadIdx.x / width; i < rows.count * kinds; i += 64 * kWalkWaves / width) {
+    const int kind = i >= rows.count, local = i - kind * rows.count, mine = lane & (width - 1);
     if (kind == 1 && local + 1 >= rows.count) continue;
     const float2 *partial = a.partials + ((int64_t)(kind ? a.tokens : 0) + rows.begin + local) * a.spans;
+    constexpr int kHeld = 4;
+    float2 held[kHeld];
+#pragma unroll
+    for (int s = 0; s < kHeld; ++s) held[s] = mine + s * width < a.spans ? partial[mine + s * width] : make_float2(-INFINITY, 0.f);
+    // The rest of a vocabulary of more spans is read twice.
+    auto each = [&](auto take) __attribute__((always_inline)) {
+#pragma unroll
+      for (int s = 0; s < kHeld; ++s) take(held[s]);
+      for (int s = mine + kHeld * width; s < a.spans; s += width) take(partial[s]);
+    };
     float top = -INFINITY;
-    bool odd = false;
-    for (int s = lane; s < a.spans; s += 64) {
-      const float2 v = partial[s];
+    int odd = 0;
+    each([&](float2 v) {
       odd |= v.x != v.x;
       top = fmaxf(top, v.x);
+    });
+    for (int w = 1; w < width; w *= 2) {
+      top = fmaxf(top, __shfl_xor(top, w));
+      odd |= __shfl_xor(odd, w);
     }
-    top = wave_max(top);
-    odd = __builtin_amdgcn_ballot_w64(odd) != 0;
     if (greedy) {
       int index = 0x7FFFFFFF;
-      for (int s = lane; s < a.spans; s += 64) {
-        const float2 v = partial[s];
-        if (v.x == top) index = min(index, __float_as_int(v.y));
-      }
-      index = wave_min_int(index);
-      if (lane == 0) sums[0][local] = odd || top == -INFINITY ? -1.0 : (double)index;
+      each([&](float2 v) { index = v.x == top ? min(index, __float_as_int(v.y)) : index; });
+      for (int w = 1; w < width; w *= 2) index = min(index, __shfl_xor(index, w));
+      if (mine == 0) sums[0][local] = odd || top == -INFINITY ? -1.0 : (double)index;
     } else {
       double sum = 0.0;
-      for (int s = lane; s < a.spans; s += 64) {
-        const float2 v = partial[s];
-        sum += v.x == -INFINITY ? (double)v.y : (double)v.y * exp2_64(((double)v.x - (double)top) * rate);
-      }
-      sum = wave_sum64(sum);
-      if (lane == 0) {
+      each([&](float2 v) { sum += v.x == -INFINITY ? (double)v.y : (double)v.y * exp2_64(((double)v.x - (double)top) * rate); });
+      for (int w = 1; w < width; w *= 2) sum += __shfl_xor(sum, w);
+      if (mine == 0) {
         tops[kind][local] = top;
         sums[kind][local] = sum;
       }
@@ -268,51 +408,30 @@ __global__ __launch_bounds__(kThreads) void verify_walk_kernel(Verify a) {
   }
   __syncthreads();
   if (wave == 0) {
-    // Lane i is row i.
-    const bool row = lane < rows.count;
-    int parent = -1;
-    int64_t token = -1;
-    float u = 0.f;
-    if (row) {
-      parent = a.parents ? a.parents[rows.begin + lane] : lane - 1;
-      token = a.ids[rows.begin + lane];
-      u = a.uniforms[rows.begin + lane];
-    }
-    if (lane == 0 || (uint32_t)parent >= (uint32_t)rows.count) parent = -1;
-    const bool child = row && parent >= 0, known = child && token >= 0 && token < a.vocab;
     double p = 0.0, q = 0.0;
     if (known) {
       if (greedy) {
         p = sums[0][parent] == (double)token ? 1.0 : 0.0;
       } else {
-        const float x = logit<T>(a.target, a.target_row, rows.begin + parent, token);
-        p = x == -INFINITY ? 0.0 : exp2_64(((double)x - (double)tops[0][parent]) * rate) / sums[0][parent];
-        if (a.draft) {
-          const float y = logit<T>(a.draft, a.draft_row, rows.begin + parent, token);
-          q = y == -INFINITY ? 0.0 : exp2_64(((double)y - (double)tops[1][parent]) * rate) / sums[1][parent];
-        }
+        p = weight_of(x, tops[0][parent], rate) / sums[0][parent];
+        if (a.draft) q = weight_of(y, tops[1][parent], rate) / sums[1][parent];
       }
     }
-    // Earlier drafts behind the same row: their tokens and probabilities.
+    // Earlier drafts behind the same row: whether one has this token, and their probabilities' sum.
+    const uint64_t earlier = child ? same_lanes(parent, 7) & __builtin_amdgcn_ballot_w64(child) & (((uint64_t)1 << lane) - 1) : 0;
+    const uint64_t twins = same_lanes((int)token, 31) & __builtin_amdgcn_ballot_w64(known);
+    const bool again = known && (earlier & twins) != 0;
     double before = 0.0;
-    bool again = false;
-    for (int j = 1; j < rows.count; ++j) {
-      const int theirs = __shfl(parent, j);
-      const int64_t their_token = __shfl(token, j);
-      const double their_p = __shfl(again ? 0.0 : p, j);
-      const bool earlier = child && j < lane && theirs == parent;
-      again |= earlier && their_token == token;
-      before += earlier ? their_p : 0.0;
+    uint64_t left = earlier & __builtin_amdgcn_ballot_w64(known && !again);
+    while (__builtin_amdgcn_ballot_w64(left != 0) != 0) {
+      const double theirs = __shfl(p, left ? __builtin_ctzll(left) : 0);
+      before += left ? theirs : 0.0;
+      left &= left - 1;
     }
     bool accept = p > 0.0 && !again;
     if (!greedy) accept = accept && (a.draft ? (double)u * q < p : (double)u * (1.0 - before) < p);
-    const uint64_t accepts = __builtin_amdgcn_ballot_w64(accept);
     // The first accepted draft behind a row is taken.
-    bool taken = accept;
-    for (int j = 1; j < rows.count; ++j) {
-      const int theirs = __shfl(parent, j);
-      taken &= !(j < lane && theirs == parent && (accepts >> j & 1));
-    }
+    const bool taken = accept && (earlier & __builtin_amdgcn_ballot_w64(accept)) == 0;
     const uint64_t fine = __builtin_amdgcn_ballot_w64(taken) | 1;
     // The rows that lead to each, by doubled pointers; reached: row 0 is among them and all are taken.
     uint64_t leads = (uint64_t)1 << lane;
@@ -346,129 +465,47 @@ __global__ __launch_bounds__(kThreads) void verify_walk_kernel(Verify a) {
       closing.first = rows.begin;
       closing.slot = rows.begin + count;
       closing.residual = a.draft && followers != 0;
-      closing.temperature = temperature;
       closing.removed = a.draft ? 0 : __builtin_popcountll(followers);
       if (!greedy) {
         closing.top = tops[0][last];
+        closing.scale_p = 1.0 / sums[0][last];
         closing.draft_top = closing.residual ? tops[1][last] : 0.f;
+        closing.scale_q = closing.residual ? 1.0 / sums[1][last] : 0.0;
       } else if (writes) {
         a.next[rows.begin + count] = (int64_t)sums[0][last];
       }
     }
     if (!a.draft && (followers >> lane & 1)) closing.tokens[__builtin_popcountll(followers & (((uint64_t)1 << lane) - 1))] = token;
-    if (lane == 0 && !greedy) {  // as well as they are known
-      sums[0][0] = 1.0 / sums[0][last];
-      sums[1][0] = closing.residual ? 1.0 / sums[1][last] : 0.0;
-    }
   }
   __syncthreads();
-  if (writes)
-    for (int i = threadIdx.x; i * sizeof(int) < sizeof(Closing); i += kThreads)
-      reinterpret_cast<int *>(kept)[i] = reinterpret_cast<const int *>(&closing)[i];
   if (closing.row < 0) return;
-  const Weights<T> weights = {a, closing, rate, sums[0][0], sums[1][0]};
-  const int part = blockIdx.x * kWaves + wave, begin = part * a.part, end = min(begin + a.part, a.vocab);
-  Sums mine = {0.0, 0.0, 0.0, 0.0};
-  for (int token = begin + lane; token < end; token += 64) {
-    double p, q;
-    bool rest;
-    weights.at(token, p, q, rest);
-    mine.p += p;
-    mine.q += q;
-    mine.rest_p += rest ? p : 0.0;
-    mine.rest_q += rest ? q : 0.0;
-  }
-  mine.p = wave_sum64(mine.p);
-  mine.q = wave_sum64(mine.q);
-  mine.rest_p = wave_sum64(mine.rest_p);
-  mine.rest_q = wave_sum64(mine.rest_q);
-  if (lane == 0) reinterpret_cast<Sums *>(a.sums)[(int64_t)sequence * a.parts + part] = mine;
-}
-
-// Inclusive sum over the lanes of a wave.
-__device__ __forceinline__ double wave_scan64(double v, int lane) {
-#pragma unroll
-  for (int w = 1; w < 64; w *= 2) {
-    const double other = __shfl_up(v, w);
-    v += lane >= w ? other : 0.0;
-  }
-  return v;
-}
-
-// The first lane whose running sum exceeds `target`, the sums before it added to `before`; else the last lane with a weight, else -1.
-__device__ __forceinline__ int crossing(double v, double target, double &before, int lane) {
-  const double sum = before + wave_scan64(v, lane);
-  const uint64_t past = __builtin_amdgcn_ballot_w64(sum > target && v > 0.0), some = __builtin_amdgcn_ballot_w64(v > 0.0);
-  if (some == 0) return -1;
-  const int at = past ? __builtin_ctzll(past) : 63 - __builtin_clzll(some);
-  before = __shfl(sum - v, at);
-  return at;
-}
-
-// The closing token: the part of the last row in which the running sum passes, then the token in it. One wave a sequence.
-template <typename T>
-__global__ __launch_bounds__(64) void verify_pick_kernel(Verify a) {
-  const int lane = threadIdx.x, sequence = blockIdx.x;
-  const Closing &closing = reinterpret_cast<const Closing *>(a.closings)[sequence];
-  if (closing.row < 0) return;
-  const Sums *sums = reinterpret_cast<const Sums *>(a.sums) + (int64_t)sequence * a.parts;
-  // Lane l has the parts l * each .. of the row.
-  const int each = (a.parts + 63) / 64, first = lane * each, last = min(first + each, a.parts);
-  Sums mine = {0.0, 0.0, 0.0, 0.0};
-  for (int i = first; i < last; ++i) {
-    mine.p += sums[i].p;
-    mine.q += sums[i].q;
-    mine.rest_p += sums[i].rest_p;
-    mine.rest_q += sums[i].rest_q;
-  }
-  const double all_p = wave_sum64(mine.p), all_q = wave_sum64(mine.q);
-  const double scale_p = 1.0 / all_p, scale_q = closing.residual ? 1.0 / all_q : 0.0;
-  const bool residual = closing.residual;
-  // What counts of a sum, and whether anything does: else it is drawn from all of p.
-  auto rest_of = [&](const Sums &s) { return residual ? fmax(s.rest_p * scale_p - s.rest_q * scale_q, 0.0) : s.rest_p; };
-  const bool all = !(wave_sum64(rest_of(mine)) > 0.0);
-  auto value_of = [&](const Sums &s) { return all ? s.p : rest_of(s); };
-  double value = 0.0;
-  for (int i = first; i < last; ++i) value += value_of(sums[i]);
-  const double total = wave_sum64(value);
-  int64_t token = -1;
-  if (total > 0.0 && !(residual && !(all_q > 0.0))) {
-    const double target = (double)a.uniforms[closing.first] * total;
-    double before = 0.0;
-    // The lane, its part, the part's tokens: 64 runs of them a lane each, and the token.
-    const int l = crossing(value, target, before, lane);
-    const int base = l * each, count = min(base + each, a.parts) - base;
-    double held = lane < count ? value_of(sums[base + lane]) : 0.0;
-    const int part = base + crossing(held, target, before, lane);
-    const Weights<T> weights = {a, closing, rate_of(closing.temperature), scale_p, scale_q};
-    const int begin = part * a.part, end = min(begin + a.part, a.vocab), run = (end - begin + 63) / 64;
-    const int from = min(begin + lane * run, end), to = min(from + run, end);
-    // Once more with all of p where a part's rest was nothing but rounding.
-    for (int turn = 0; turn < 2 && token < 0; ++turn) {
-      auto weight_of = [&](int t) {
-        double p, q;
-        bool rest;
-        weights.at(t, p, q, rest);
-        return all || turn ? p : !rest ? 0.0 : residual ? p * scale_p - q * scale_q : p;
-      };
-      held = 0.0;
-      for (int t = from; t < to; ++t) held += weight_of(t);
-      double sum = before;
-      const int at = crossing(held, target, sum, lane);
-      if (at == lane) {
-        for (int t = from; t < to; ++t) {
-          const double w = weight_of(t);
-          sum += w;
-          if (w > 0.0) {
-            token = t;
-            if (sum > target) break;
-          }
-        }
-      }
-      token = __shfl(token, max(at, 0));
+  Sums *kept = reinterpret_cast<Sums *>(a.sums) + (int64_t)sequence * a.chunks;
+  for (int chunk = blockIdx.x * kWalkWaves + wave; chunk < a.chunks; chunk += a.groups * kWalkWaves) {
+    Sums mine = {0.0, 0.0, 0.0, 0.0};
+    eight_weights<T>(a, closing, rate, chunk * kChunk + lane * kEight, closing.scale_p, closing.scale_q, [&](int, double p, double q, bool rest) {
+      mine.p += p;
+      mine.q += q;
+      mine.rest_p += rest ? p : 0.0;
+      mine.rest_q += rest ? q : 0.0;
+    });
+    mine.p = wave_sum64(mine.p);
+    mine.rest_p = wave_sum64(mine.rest_p);
+    if (closing.residual) {
+      mine.q = wave_sum64(mine.q);
+      mine.rest_q = wave_sum64(mine.rest_q);
     }
+    if (lane == 0) kept[chunk] = mine;
   }
-  if (lane == 0) a.next[closing.slot] = token;
+  __syncthreads();  // the workgroup's sums are in its cache: one thread's fence makes them visible to all
+  if (threadIdx.x == 0) {
+    __threadfence();
+    ends = atomicAdd(a.counters + sequence, 1) == a.groups - 1;
+  }
+  __syncthreads();
+  if (!ends || wave != 0) return;
+  __threadfence();
+  const int64_t drawn = closing_token<T>(a, closing, rate, kept, a.uniforms[closing.first]);
+  if (lane == 0) a.next[closing.slot] = drawn;
 }
 
 }  // namespace
@@ -476,30 +513,25 @@ __global__ __launch_bounds__(64) void verify_pick_kernel(Verify a) {
 void verify_plan(Verify &a, int dtype_bytes, int cus) {
   const int span = 64 * kLoads * 16 / dtype_bytes;
   a.spans = (a.vocab + span - 1) / span;
-  // Workgroups that share a sequence's last row: two a CU in all, of at least 512 tokens each.
-  int64_t groups = 2 * (int64_t)cus / (a.sequences > 0 ? a.sequences : 1);
-  if (groups > a.vocab / 512) groups = a.vocab / 512;
-  if (groups > 64) groups = 64;
-  if (groups < 1) groups = 1;
-  a.groups = (int)groups;
-  a.parts = a.groups * kWaves;
-  a.part = (a.vocab + a.parts - 1) / a.parts;
+  // Workgroups that share a sequence's last row: one a CU in all, with work for every wave.
+  a.chunks = (a.vocab + kChunk - 1) / kChunk;
+  const int64_t full = (int64_t)cus / (a.sequences > 0 ? a.sequences : 1), most = (a.chunks + kWalkWaves - 1) / kWalkWaves;
+  a.groups = (int)(full < 1 ? 1 : full < most ? full : most);
   auto whole = [](int64_t bytes) { return (bytes + 15) & ~(int64_t)15; };
-  a.closings_at = whole((int64_t)a.tokens * (a.draft ? 2 : 1) * a.spans * sizeof(float2));
-  a.sums_at = a.closings_at + whole((int64_t)a.sequences * sizeof(Closing));
-  a.workspace_bytes = a.sums_at + (int64_t)a.sequences * a.parts * sizeof(Sums);
+  a.counters_at = whole((int64_t)a.tokens * (a.draft ? 2 : 1) * a.spans * sizeof(float2));
+  a.sums_at = a.counters_at + whole((int64_t)a.sequences * sizeof(int));
+  a.workspace_bytes = a.sums_at + (int64_t)a.sequences * a.chunks * sizeof(Sums);
 }
 
 hipError_t launch_verify(Verify a, int dtype, char *workspace, hipStream_t stream) {
   a.partials = reinterpret_cast<float2 *>(workspace);
-  a.closings = workspace + a.closings_at;
+  a.counters = reinterpret_cast<int *>(workspace + a.counters_at);
   a.sums = workspace + a.sums_at;
   const dim3 stats((unsigned)((a.spans + kWaves - 1) / kWaves), (unsigned)a.tokens, a.draft ? 2 : 1);
   auto launch = [&](auto type) {
     using T = decltype(type);
     if (a.tokens > 0) hipLaunchKernelGGL(verify_stats_kernel<T>, stats, dim3(kThreads), 0, stream, a);
-    hipLaunchKernelGGL(verify_walk_kernel<T>, dim3((unsigned)a.groups, (unsigned)a.sequences), dim3(kThreads), 0, stream, a);
-    hipLaunchKernelGGL(verify_pick_kernel<T>, dim3((unsigned)a.sequences), dim3(64), 0, stream, a);
+    hipLaunchKernelGGL(verify_walk_kernel<T>, dim3((unsigned)a.groups, (unsigned)a.sequences), dim3(64 * kWalkWaves), 0, stream, a);
   };
   if (dtype == kVerifyF32) launch(0.f);
   else if (dtype == kVerifyF16) launch(Fp16{});
