@@ -1738,7 +1738,7 @@ int tx_kv4_keep_path(void *pages, int layers, int64_t num_pages, int kv_heads, i
   DeviceGuard guard(device);
   const int64_t layer_bytes = num_pages * kv_heads * 2 * tx::kv4_half_bytes(pool.page_shift, head_dim);
   TX_HIP(tx::launch_kv4_keep_path(pool, head_dim, layers, layer_bytes, cu, (int)tokens, path, accepted, lengths_out,
-                                  reinterpret_cast<hipStream_t>(stream)));
+                                  multiprocessors(device), reinterpret_cast<hipStream_t>(stream)));
   return TX_OK;
 }
 

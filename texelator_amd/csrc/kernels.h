@@ -250,7 +250,7 @@ hipError_t launch_kv4_read(uint16_t *k, int64_t k_token, int64_t k_head, uint16_
 struct Kv4Rope;
 hipError_t launch_kv4_append_rope(Kv4Rope a, bool interleaved, bool f16, int dim, const Kv4Pool &pool, int cus, hipStream_t stream);
 hipError_t launch_kv4_keep_path(const Kv4Pool &pool, int dim, int layers, int64_t layer_bytes, const int *cu, int tokens,
-                                const int *path, const int *accepted, int *lengths_out, hipStream_t stream);
+                                const int *path, const int *accepted, int *lengths_out, int cus, hipStream_t stream);
 constexpr int kKv4Pairs = 448;  // page pairs of one copy launch: 3.5 KiB of kernel arguments
 hipError_t launch_kv4_copy_pages(uint8_t *pool, int layers, int64_t layer_bytes, int64_t page_bytes, const int64_t *src,
                                  const int64_t *dst, int64_t count, hipStream_t stream);

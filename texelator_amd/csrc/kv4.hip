@@ -297,14 +297,14 @@ __global__ __launch_bounds__(kThreads) void kv4_append_rope_kernel(Kv4Rope a, Kv
 }
 
 // The rows of an accepted path moved together: of sequence s, whose last cu[s + 1] - cu[s] positions are drafted rows, row path[cu[s] + j]
-// moves to the place of row j, j = 1 .. accepted[s]. A wave has one head's keys or values of one sequence and layer: it holds
-// every piece that moves before it stores the first, so paths may run in any order. Grid: x sequences, y heads and halves by
-// kKeepWaves, z layers.
+// moves to the place of row j, j = 1 .. accepted[s]. A wave has one head's keys or values of one sequence, in `per` layers: it holds
+// every piece of a layer that moves before it stores the first, so paths may run in any order, and finds their places once for all
+// layers. Bound by the latency of its dependent loads. Grid: x sequences, y heads and halves by kKeepWaves, z layers by `per`.
 constexpr int kKeepWaves = 4;
 template <int DIM>
-__global__ __launch_bounds__(64 * kKeepWaves) void kv4_keep_path_kernel(Kv4Pool pool, int64_t layer_bytes, const int *cu,
-                                                                        int tokens, const int *path, const int *accepted,
-                                                                        int *lengths_out) {
+__global__ __launch_bounds__(64 * kKeepWaves) void kv4_keep_path_kernel(Kv4Pool pool, int layers, int per, int64_t layer_bytes,
+                                                                        const int *cu, int tokens, const int *path,
+                                                                        const int *accepted, int *lengths_out) {
   constexpr int kGroups = DIM / 32, kHeld = kMostDrafts * kGroups / 64;
   const int sequence = blockIdx.x, lane = threadIdx.x & 63, half = blockIdx.y * kKeepWaves + (threadIdx.x >> 6);
   const int begin = min(max(cu[sequence], 0), tokens), count = min(max(cu[sequence + 1], begin), tokens) - begin;
@@ -314,39 +314,58 @@ __global__ __launch_bounds__(64 * kKeepWaves) void kv4_keep_path_kernel(Kv4Pool 
   if (half == 0 && lane == 0 && blockIdx.z == 0) lengths_out[sequence] = context + kept + 1;
   if (half >= 2 * pool.kv_heads || kept < 1) return;
   const int64_t half_bytes = kv4_half_bytes(pool.page_shift, DIM), scales_at = (int64_t)(DIM / 2) << pool.page_shift;
-  uint8_t *layer = pool.pages + blockIdx.z * layer_bytes;
   const int group = lane % kGroups;
-  auto at = [&](int position) -> uint8_t * {  // this group's codes; null where there is none
+  // A group's place: of its codes in a layer (below 0: none), and how far behind them its scale is.
+  struct Group {
+    int64_t codes;
+    int scale;
+  };
+  auto group_at = [&](int position) -> Group {
     const Row row = row_at(pool, {sequence, position});
-    if (row.page < 0) return nullptr;
-    return layer + (row.page * pool.kv_heads * 2 + half) * half_bytes + row.offset * (DIM / 2) + 16 * group;
+    if (row.page < 0) return {-1, 0};
+    const int codes = row.offset * (DIM / 2) + 16 * group;
+    return {(row.page * pool.kv_heads * 2 + half) * half_bytes + codes, (int)scales_at + row.offset * kGroups + group - codes};
   };
-  auto scale_of = [&](uint8_t *codes, int position) {  // beside the codes at `at(position)`
-    const int offset = position & ((1 << pool.page_shift) - 1);
-    return codes - offset * (DIM / 2) - 16 * group + scales_at + offset * kGroups + group;
-  };
-  u32x4 codes[kHeld];
-  uint8_t scale[kHeld];
-  uint8_t *to[kHeld];
+  Group from[kHeld], to[kHeld];
 #pragma unroll
   for (int i = 0; i < kHeld; ++i) {
     const int j = 1 + (64 * i + lane) / kGroups;
-    to[i] = nullptr;
+    from[i] = to[i] = {-1, 0};
     if (j > kept) continue;
-    const int from = path[begin + j];
-    if (from < 0 || from >= rows || from == j) continue;
-    uint8_t *source = at(context + from);
-    to[i] = source ? at(context + j) : nullptr;
-    if (!to[i]) continue;
-    codes[i] = *reinterpret_cast<const u32x4 *>(source);
-    scale[i] = *scale_of(source, context + from);
+    const int row = path[begin + j];
+    if (row < 0 || row >= rows || row == j) continue;
+    from[i] = group_at(context + row);
+    to[i] = group_at(context + j);
+    if (to[i].codes < 0) from[i].codes = -1;
   }
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // everything is held
+  struct Held {
+    u32x4 codes[kHeld];
+    uint8_t scale[kHeld];
+  };
+  auto load = [&](int layer, Held &held) __attribute__((always_inline)) {
+    const uint8_t *pages = pool.pages + layer * layer_bytes;
 #pragma unroll
-  for (int i = 0; i < kHeld; ++i) {
-    if (!to[i]) continue;
-    *reinterpret_cast<u32x4 *>(to[i]) = codes[i];
-    *scale_of(to[i], context + 1 + (64 * i + lane) / kGroups) = scale[i];
+    for (int i = 0; i < kHeld; ++i)
+      if (from[i].codes >= 0) {
+        held.codes[i] = *reinterpret_cast<const u32x4 *>(pages + from[i].codes);
+        held.scale[i] = pages[from[i].codes + from[i].scale];
+      }
+  };
+  const int first = blockIdx.z * per, end = min(first + per, layers);
+  Held held;
+  load(first, held);
+#pragma unroll 1
+  for (int layer = first; layer < end; ++layer) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // everything of this layer is held
+    const Held now = held;
+    if (layer + 1 < end) load(layer + 1, held);
+    uint8_t *pages = pool.pages + layer * layer_bytes;
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i)
+      if (from[i].codes >= 0) {
+        *reinterpret_cast<u32x4 *>(pages + to[i].codes) = now.codes[i];
+        pages[to[i].codes + to[i].scale] = now.scale[i];
+      }
   }
 }
 
@@ -430,12 +449,16 @@ hipError_t launch_kv4_append_rope(Kv4Rope a, bool interleaved, bool f16, int dim
 }
 
 hipError_t launch_kv4_keep_path(const Kv4Pool &pool, int dim, int layers, int64_t layer_bytes, const int *cu, int tokens,
-                                const int *path, const int *accepted, int *lengths_out, hipStream_t stream) {
-  const dim3 grid((unsigned)pool.sequences, (unsigned)((2 * pool.kv_heads + kKeepWaves - 1) / kKeepWaves), (unsigned)layers);
-  if (dim == 128) hipLaunchKernelGGL(kv4_keep_path_kernel<128>, grid, dim3(64 * kKeepWaves), 0, stream, pool, layer_bytes, cu, tokens, path,
-                                   accepted, lengths_out);
-  else hipLaunchKernelGGL(kv4_keep_path_kernel<64>, grid, dim3(64 * kKeepWaves), 0, stream, pool, layer_bytes, cu, tokens, path,
-                                   accepted, lengths_out);
+                                const int *path, const int *accepted, int *lengths_out, int cus, hipStream_t stream) {
+  // Layers of a wave: as many as leave four workgroups a CU. 32 sequences of up to 33 rows, 16 heads and halves, 64 layers: 8.3 us with
+  // 8 layers (14.4 with one, 10.8 with 2, 9.4 with 4, 11.0 with 16).
+  const int64_t quads = (2 * pool.kv_heads + kKeepWaves - 1) / kKeepWaves, most = (int64_t)pool.sequences * quads * layers / (4 * cus);
+  const int per = (int)(most < 1 ? 1 : most > layers ? layers : most);
+  const dim3 grid((unsigned)pool.sequences, (unsigned)quads, (unsigned)((layers + per - 1) / per));
+  if (dim == 128) hipLaunchKernelGGL(kv4_keep_path_kernel<128>, grid, dim3(64 * kKeepWaves), 0, stream, pool, layers, per, layer_bytes, cu,
+                                     tokens, path, accepted, lengths_out);
+  else hipLaunchKernelGGL(kv4_keep_path_kernel<64>, grid, dim3(64 * kKeepWaves), 0, stream, pool, layers, per, layer_bytes, cu, tokens, path,
+                                     accepted, lengths_out);
   return hipGetLastError();
 }
 

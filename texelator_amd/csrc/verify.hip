@@ -20,7 +20,7 @@
 // tokens where p > q by the first launch's sums; a token that those put on the wrong side adds at most 1e-7 of its own probability.
 //
 // Measured, first and second launch: 16 chains of up to 8 rows sampled from a draft's logits of 151,936 bf16 tokens 15 us (the
-// logits' 81 MB at 5.4 TB/s) and 26 us, 24 trees of up to 64 rows of 32,003 fp32 tokens 26 us (5.5 TB/s) and 17 us, one
+// logits' 55 MB at 3.7 TB/s) and 26 us, 24 trees of up to 64 rows of 32,003 fp32 tokens 26 us (5.5 TB/s) and 17 us, one
 // tree of 6 rows 4 us and 15 us. The second is bound by its steps' latency: 6 us to the path, 5 to 13 for the sums, 5 to 7 for the token.
 // With a launch of its own for the token and a wave for each row's statistics they took 64, 69 and 26 us in all.
 #include <math.h>
@@ -162,7 +162,7 @@ __global__ __launch_bounds__(kThreads) void verify_stats_kernel(Verify a) {
 #pragma unroll
   for (int i = 0; i < kLoads; ++i)
 #pragma unroll
-    for (int j = 0; j < kVector; ++j) sum += x[i][j] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((x[i][j] - base) * rate);
+    for (int j = 0; j < kVector; ++j) sum += __builtin_amdgcn_exp2f((x[i][j] - base) * rate);
   sum = wave_sum(sum);
   if (lane == 0) *partial = make_float2(top, sum);
 }
