@@ -450,7 +450,7 @@ hipError_t launch_kv4_append_rope(Kv4Rope a, bool interleaved, bool f16, int dim
 
 hipError_t launch_kv4_keep_path(const Kv4Pool &pool, int dim, int layers, int64_t layer_bytes, const int *cu, int tokens,
                                 const int *path, const int *accepted, int *lengths_out, int cus, hipStream_t stream) {
-  // Layers of a wave: as many as leave four workgroups a CU. 32 sequences of up to 33 rows, 16 heads and halves, 64 layers: 8.3 us with
+  // Layers of a wave: as many as leave four workgroups a CU. 32 sequences of up to 26 rows, 16 heads and halves, 64 layers: 8.3 us with
   // 8 layers (14.4 with one, 10.8 with 2, 9.4 with 4, 11.0 with 16).
   const int64_t quads = (2 * pool.kv_heads + kKeepWaves - 1) / kKeepWaves, most = (int64_t)pool.sequences * quads * layers / (4 * cus);
   const int per = (int)(most < 1 ? 1 : most > layers ? layers : most);
