@@ -634,9 +634,10 @@ def _kv4_page_size(shape: torch.Size, head_dim: int) -> int:
     return page_size
 
 
-def _kv4_args(pages: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor, head_dim: int, device: torch.device) -> tuple:
-    """The cache's arguments of a C call, from pages to sequences."""
-    shape, table = pages.shape, block_table.shape
+def _kv4_args(pages: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor, head_dim: int, device: torch.device,
+              shape: torch.Size | None = None) -> tuple:
+    """The cache's arguments of a C call, from pages to sequences. ``shape``: one pool's, where ``pages`` are all layers'."""
+    shape, table = pages.shape if shape is None else shape, block_table.shape
     if pages.dtype != torch.uint8 or not pages.is_cuda or pages.device != device or not pages.is_contiguous():
         raise TexelatorError("pages must be contiguous CUDA uint8 [num_pages, kv_heads, 2, page bytes] on the rows' device")
     page_size = _kv4_page_size(shape, head_dim)
@@ -811,8 +812,9 @@ def kv4_append_rope(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torc
         _expect(tokens == sequences, "without cu there is one token for each sequence")
     else:
         _expect_ints("cu", cu, sequences + 1, device)
-    if (cos.dtype != torch.float32 or sin.dtype != torch.float32 or len(cos.shape) != 2 or cos.shape != sin.shape or cos.device != device
-            or sin.device != device or (cos.stride(1) != 1 and cos.shape[1] != 1) or (sin.stride(1) != 1 and sin.shape[1] != 1)):
+    table, cos_strides, sin_strides = cos.shape, cos.stride(), sin.stride()
+    if (cos.dtype != torch.float32 or sin.dtype != torch.float32 or len(table) != 2 or table != sin.shape or cos.device != device
+            or sin.device != device or (table[1] != 1 and (cos_strides[1] != 1 or sin_strides[1] != 1))):
         raise TexelatorError("cos and sin must be float32 [rows, rotary / 2] on the pages' device, rows contiguous")
     if positions is not None:
         _expect_ints("positions", positions, tokens, device)
@@ -828,8 +830,8 @@ def kv4_append_rope(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torc
         return out
     q_strides, out_strides, k_out_strides = q.stride(), out.stride(), (0, 0) if k_out is None else k_out.stride()
     check(_lib.load().tx_kv4_append_rope(
-        q.data_ptr(), q_strides[0], q_strides[1], *rows, heads, cos.data_ptr(), cos.stride(0), sin.data_ptr(), sin.stride(0),
-        cos.shape[0], 2 * cos.shape[1], bool(interleaved), _ptr(positions), _ptr(cu), *cache, out.data_ptr(), out_strides[0],
+        q.data_ptr(), q_strides[0], q_strides[1], *rows, heads, cos.data_ptr(), cos_strides[0], sin.data_ptr(), sin_strides[0],
+        table[0], 2 * table[1], bool(interleaved), _ptr(positions), _ptr(cu), *cache, out.data_ptr(), out_strides[0],
         out_strides[1], _ptr(k_out), k_out_strides[0], k_out_strides[1], device.index, _stream_address(device)))
     return out
 
@@ -984,14 +986,11 @@ def kv4_keep_path(pages: torch.Tensor, block_table: torch.Tensor, lengths: torch
     layers' pools ``[layers, ...]`` at once: the row of step j to the place of row j. Returns the lengths that are left, int32
     ``[sequences]``, ``lengths - rows + accepted + 1`` (into ``out`` where given, which is not ``lengths`` itself). What rows lie
     behind is stale, as any position past a length."""
-    _expect(pages.is_cuda and pages.dtype == torch.uint8 and pages.dim() in (4, 5) and pages.is_contiguous(),
-            "pages must be contiguous CUDA uint8 [num_pages, kv_heads, 2, page bytes], layers before it or not")
-    layered = pages.dim() == 5
-    _expect(not layered or pages.shape[0] > 0, "pages must have layers")
-    device = pages.device
-    cache = _kv4_args(pages[0] if layered else pages, block_table, lengths, head_dim, device)
-    sequences = cache[-1]
-    tokens = path.numel()
+    shape, device = pages.shape, pages.device
+    layers = 1 if len(shape) == 4 else shape[0] if len(shape) == 5 else 0
+    _expect(layers > 0, "pages must be [num_pages, kv_heads, 2, page bytes], layers before it or not")
+    cache = _kv4_args(pages, block_table, lengths, head_dim, device, shape[-4:])
+    sequences, tokens = cache[-1], path.numel()
     _expect_ints("cu", cu, sequences + 1, device)
     _expect_ints("path", path, tokens, device)
     _expect_ints("accepted", accepted, sequences, device)
@@ -1000,6 +999,6 @@ def kv4_keep_path(pages: torch.Tensor, block_table: torch.Tensor, lengths: torch
     else:
         _expect_ints("out", out, sequences, device)
     if sequences:
-        check(_lib.load().tx_kv4_keep_path(cache[0], pages.shape[0] if layered else 1, *cache[1:], cu.data_ptr(), tokens,
+        check(_lib.load().tx_kv4_keep_path(cache[0], layers, *cache[1:], cu.data_ptr(), tokens,
                                            path.data_ptr(), accepted.data_ptr(), out.data_ptr(), device.index, _stream_address(device)))
     return out
