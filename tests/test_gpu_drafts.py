@@ -189,6 +189,11 @@ TREES = [
     ([4 + (37 * i) % 301 for i in range(150)], [1 + i % 4 for i in range(150)], 4, 2, 128, 16, False),  # more sequences than lanes
     ([70 + (53 * i) % 1500 for i in range(70)], [i % 65 for i in range(70)], 12, 12, 64, 32, False),
     ([3, 2, 1], [5, 2, 7], 8, 2, 128, 16, False),     # fewer positions than rows
+    # as many short (sequence, head)s as fill the grid by themselves
+    ([20 + (37 * i) % 300 for i in range(80)], [1 + i % 20 for i in range(80)], 24, 8, 128, 16, False),
+    ([64 + (41 * i) % 200 for i in range(40)], [64 - i % 7 for i in range(40)], 32, 16, 64, 32, True),
+    # long sequences among and behind the 64th
+    ([30 + i for i in range(63)] + [20000, 40, 6000, 9], [1 + i % 3 for i in range(63)] + [40, 2, 7, 9], 4, 2, 128, 64, False),
 ]
 
 

@@ -696,9 +696,11 @@ bool kv4_tree_fits(const Kv4Tree &a) {
 void kv4_tree_plan(Kv4Tree &a, int dim, int cus) {
   const int64_t room = (int64_t)a.pool.max_pages << a.pool.page_shift;
   a.most_passes = (int)most_passes(a);
-  a.whole = room <= 512;
   const int64_t shares = most_ticks(a, dim == 128 ? kTile<128> : kTile<64>) / kLeast + 1;
   const int64_t fill = (dim == 128 ? kResident<128> : kResident<64>) * (int64_t)cus;
+  // Short parts that fill the grid by themselves are not cut: 32 sequences of up to 400 positions and 8 heads of 16 * 5 rows take 15 us,
+  // cut and combined 20; one such sequence 18 and 13, eight 17.6 and 16.2; 32 of up to 1,000 26 and 22.
+  a.whole = room <= 512 && most_parts(a) >= fill;
   a.workgroups = (int)(shares < fill ? shares : fill);
   const int64_t blocks = most_blocks(a) < kPass ? most_blocks(a) : kPass;
   a.piece_floats = (int)blocks * (dim == 128 ? kPieceFloats<128> : kPieceFloats<64>);
@@ -714,6 +716,7 @@ hipError_t launch_kv4_tree(const Kv4Tree &a, bool f16, int dim, hipStream_t stre
     const unsigned in_pass = (unsigned)(most_blocks(a) < kPass ? most_blocks(a) : kPass);
     hipLaunchKernelGGL((kv4_tree_kernel<kF16, kDim>), dim3((unsigned)(parts + (a.whole ? 0 : a.workgroups))), dim3(kThreads), 0, stream, a);
     if (a.whole) return;
+    // Few parts have many pieces. 24 parts: 8.7 us shared, 21 not; 96: 11.6 and 14.3; 192: 13.0 and 7.5; 576: 35 and 14.
     if (parts <= 128)
       hipLaunchKernelGGL((kv4_tree_combine_kernel<kF16, kDim, true>), dim3((unsigned)parts, in_pass, kDim / 8), dim3(kThreads), 0, stream, a);
     else
