@@ -185,7 +185,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 // group's scale. Queries and rotated key rows (k_out, where given) are rounded once, from 32 bits (a value next to a rounding
 // border of 16 bits is off by 2^-24 of itself more); what is stored is quantized from the exact value (turned_to_odd): a
 // slowly turning key stays so near the 16-bit value that it was that 32 bits put it midway between two codes. Bound by memory:
-// 136 us for 21,456 tokens of 40 + 2 * 8 heads of 128, 4.05 TB/s.
+// 136 us for 21,447 tokens of 40 + 2 * 8 heads of 128, 4.05 TB/s.
 template <bool F16, int DIM, bool INTERLEAVED>
 __global__ __launch_bounds__(kThreads) void kv4_append_rope_kernel(Kv4Rope a, Kv4Pool pool) {
   constexpr int kChunks = DIM / 8, kGroups = DIM / 32;
@@ -431,7 +431,7 @@ hipError_t launch_kv4_read(uint16_t *k, int64_t k_token, int64_t k_head, uint16_
 hipError_t launch_kv4_append_rope(Kv4Rope a, bool interleaved, bool f16, int dim, const Kv4Pool &pool, int cus, hipStream_t stream) {
   const int heads = a.heads + 2 * pool.kv_heads, rows = kThreads / (dim / 8);
   const int64_t blocks = (a.tokens + (int64_t)rows - 1) / rows;
-  // Heads of a workgroup, which loads their angles once: as many as leave eight workgroups a CU, up to 16 in even shares. For 21,456
+  // Heads of a workgroup, which loads their angles once: as many as leave eight workgroups a CU, up to 16 in even shares. For 21,447
   // tokens of 56 heads: 432 us with one, 165 with 4, 141 with 8, 137 with 14.
   const int64_t full = blocks * heads / (8 * cus), most = full < 1 ? 1 : full > 16 ? 16 : full, shares = (heads + most - 1) / most;
   a.per = (int)((heads + shares - 1) / shares);
