@@ -121,20 +121,22 @@ def verify64(logits, ids, uniforms, trees, temperatures, draft_logits=None):
                 p = torch.zeros(vocab, dtype=torch.float64)
                 p[int((x == x.max()).nonzero()[0])] = 1.0
                 return p
-            p = torch.exp((x - x.max()) / float(torch.tensor(temperature, dtype=torch.float32)))
-            return p / p.sum()
+            p = torch.exp(((x - x.max()) / float(torch.tensor(temperature, dtype=torch.float32))).masked_fill(x == float("-inf"), float("-inf")))
+            return p
 
         row, steps, closing = 0, [0], -1
         while n:
-            p = weights(logits, row)
+            raw = weights(logits, row)
+            p = None if raw is None else raw / raw.sum()
             children = [i for i in range(1, n) if tree[i] == row]
             if p is None:
                 break
-            rest, taken = p.clone(), None
+            rest, taken = raw.clone(), None  # the closing token is drawn from weights as they are: their sums round least
             if draft_logits is not None and temperature > 0:
                 q = weights(draft_logits, row) if children else None
                 if children and q is None:
                     break
+                q = q / q.sum() if children else None
                 for i in children:
                     x = token[i]
                     if 0 <= x < vocab and p[x] > 0 and u[i] * q[x] < p[x]:
@@ -157,7 +159,7 @@ def verify64(logits, ids, uniforms, trees, temperatures, draft_logits=None):
                 steps.append(row)
                 continue
             if temperature <= 0 or not rest.sum() > 0:
-                rest = p
+                rest = raw
             summed = rest.cumsum(0)
             closing = min(int((summed <= u[0] * summed[-1]).sum()), int(rest.nonzero().max()))
             break

@@ -571,6 +571,18 @@ def test_temperatures_of_all_sizes(ext):
     check_verified(rows, trees, logits, None, ids, uniforms, temperatures, "tree")
 
 
+@pytest.mark.parametrize("temperature", [float("inf"), 3e38])
+@pytest.mark.parametrize("kind", ["tree", "sampled"])
+def test_masked_tokens_at_the_largest_temperatures(ext, kind, temperature):
+    """Every token above -infinity weighs the same, the others nothing: drafts are accepted at that share."""
+    rows, vocab = [6, 3], 11
+    trees, logits, draft, ids, uniforms = drafted(rows, vocab, FP32, 8, kind)
+    logits[:, 4:9] = -np.inf
+    ids[:] = torch.tensor([0, 1, 2, 3, 9, 10, 4, 0, 1])
+    uniforms[:] = torch.tensor([0.9, 0.05, 0.1, 0.16, 0.05, 0.1, 0.5, 0.0, 0.1])
+    check_verified(rows, trees, logits, draft, ids, uniforms, [temperature] * 2, kind)
+
+
 def test_identical_models_and_the_largest_numbers(ext):
     """Draft and target alike: every draft is accepted, for numbers of 1 too (where q(x) is not below p(x)) nothing breaks."""
     rows, vocab = [5, 7], 3001

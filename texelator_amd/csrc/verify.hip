@@ -159,10 +159,17 @@ __global__ __launch_bounds__(kThreads) void verify_stats_kernel(Verify a) {
   }
   const float rate = (float)fmin(rate_of(temperature), 1e30), base = top == -INFINITY ? 0.f : top;
   float sum = 0.f;
+  if (rate > 0.f) {
 #pragma unroll
-  for (int i = 0; i < kLoads; ++i)
+    for (int i = 0; i < kLoads; ++i)
 #pragma unroll
-    for (int j = 0; j < kVector; ++j) sum += __builtin_amdgcn_exp2f((x[i][j] - base) * rate);
+      for (int j = 0; j < kVector; ++j) sum += __builtin_amdgcn_exp2f((x[i][j] - base) * rate);
+  } else {  // at an infinite temperature everything above -infinity weighs the same
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i)
+#pragma unroll
+      for (int j = 0; j < kVector; ++j) sum += x[i][j] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((x[i][j] - base) * rate);
+  }
   sum = wave_sum(sum);
   if (lane == 0) *partial = make_float2(top, sum);
 }
