@@ -583,6 +583,18 @@ def test_masked_tokens_at_the_largest_temperatures(ext, kind, temperature):
     check_verified(rows, trees, logits, draft, ids, uniforms, [temperature] * 2, kind)
 
 
+@pytest.mark.parametrize("temperature", [0.0, 1.3])
+@pytest.mark.parametrize("kind", ["tree", "sampled"])
+def test_the_largest_vocabulary(ext, kind, temperature):
+    rows, vocab = [3, 2], 1 << 24
+    trees, logits, draft, ids, uniforms = drafted(rows, vocab, FP16, 3, "tree")
+    if kind == "sampled":
+        trees, draft = [list(range(-1, n - 1)) for n in rows], torch.cat([logits[:, 5:], logits[:, :5]], dim=1)
+    logits[0, -1] = 30.0  # the last token is drawn or drafted
+    ids[1] = vocab - 1
+    check_verified(rows, trees, logits, draft, ids, uniforms, [temperature] * 2, kind)
+
+
 def test_identical_models_and_the_largest_numbers(ext):
     """Draft and target alike: every draft is accepted, for numbers of 1 too (where q(x) is not below p(x)) nothing breaks."""
     rows, vocab = [5, 7], 3001

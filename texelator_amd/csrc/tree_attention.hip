@@ -699,7 +699,7 @@ int64_t most_ticks(const Kv4Tree &a, int tile) {
 
 // Ticks are 32-bit; a launch has fewer than 2^32 threads, 256 for each (head, pass).
 bool kv4_tree_fits(const Kv4Tree &a) {
-  return most_ticks(a, kTile<128>) <= (int64_t)1 << 30 && most_parts(a) < (int64_t)1 << 24;
+  return most_ticks(a, kTile<128>) <= (int64_t)1 << 30 && most_parts(a) < (int64_t)1 << 23;
 }
 
 void kv4_tree_plan(Kv4Tree &a, int dim, int cus) {

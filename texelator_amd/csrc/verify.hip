@@ -304,16 +304,27 @@ __device__ __forceinline__ int64_t closing_token(const Verify &a, const Closing 
   auto rest_of = [&](const Sums &s) { return residual ? fmax(s.rest_p * scale_p - s.rest_q * scale_q, 0.0) : s.rest_p; };
   const bool all = !(wave_sum64(rest_of(mine)) > 0.0);
   auto value_of = [&](const Sums &s) { return all ? s.p : rest_of(s); };
-  double value = 0.0;
+  // A lane's sum of the chunks from `at` on, of `run` that end before `stop`.
+  auto value_from = [&](int at, int run, int stop) {
+    double value = 0.0;
 #pragma unroll 4
-  for (int i = first; i < last; ++i) value += value_of(sums[i]);
+    for (int i = at; i < min(at + run, stop); ++i) value += value_of(sums[i]);
+    return value;
+  };
+  double value = value_from(first, each, a.chunks);
   const double total = wave_sum64(value);
   if (!(total > 0.0) || (residual && !(all_q > 0.0))) return -1;
   const double target = (double)uniform * total;
+  // The run of chunks in which the sum passes, then 64 runs of that, down to one chunk.
   double before = 0.0;
-  const int l = crossing(value, target, before, lane);
-  const int base = l * each, count = min(base + each, a.chunks) - base;
-  const int chunk = base + crossing(lane < count ? value_of(sums[base + lane]) : 0.0, target, before, lane);
+  int chunk = 0, run = each, stop = a.chunks;
+  while (true) {
+    chunk += run * max(crossing(value, target, before, lane), 0);
+    if (run == 1) break;
+    stop = min(chunk + run, stop);
+    run = (run + 63) / 64;
+    value = value_from(chunk + lane * run, run, stop);
+  }
   int64_t token = -1;
   // Once more with all of p where a chunk's rest was nothing but rounding.
   for (int turn = 0; turn < 2 && token < 0; ++turn) {
