@@ -498,7 +498,8 @@ __global__ __launch_bounds__(64 * kWalkWaves) void verify_walk_kernel(Verify a) 
   __syncthreads();
   if (closing.row < 0) return;
   Sums *kept = reinterpret_cast<Sums *>(a.sums) + (int64_t)sequence * a.chunks;
-  for (int chunk = blockIdx.x * kWalkWaves + wave; chunk < a.chunks; chunk += a.groups * kWalkWaves) {
+  // Neighbouring chunks go to different workgroups: what is left for a second round is spread over all of them.
+  for (int chunk = wave * a.groups + blockIdx.x; chunk < a.chunks; chunk += a.groups * kWalkWaves) {
     Sums mine = {0.0, 0.0, 0.0, 0.0};
     eight_weights<T>(a, closing, rate, chunk * kChunk + lane * kEight, closing.scale_p, closing.scale_q, [&](int, double p, double q, bool rest) {
       mine.p += p;
