@@ -149,6 +149,7 @@ __device__ __forceinline__ int part_ticks(const Drafts &d) { return kStart + wei
 // How the parts are cut: into as many pieces as they have even shares of the grid, rounded; the pieces of cut parts are at most
 // four thirds of the grid's even shares.
 struct Cut {
+  Drafts d;  // in scalar registers
   int sequence, part, piece, pieces;  // part: head * passes + pass
   int before;                         // pieces of cut parts before this part
 };
@@ -156,11 +157,14 @@ struct Cut {
 template <int TILE>
 __device__ __forceinline__ Cut cut_at(const Kv4Tree &a, int wanted) {
   const int lane = threadIdx.x & 63, sequences = a.pool.sequences;
-  int parts = 0, ticks = 0, tiles = 0;  // of the lane's sequence
+  int parts = 0, ticks = 0, tiles = 0, begin = 0, end = 0, length = 0;  // of the lane's sequence
   auto load = [&](int first) {
     parts = ticks = tiles = 0;
     if (first + lane < sequences) {
-      const Drafts d = drafts_of(a, first + lane);
+      begin = a.cu[first + lane];
+      end = a.cu[first + lane + 1];
+      length = kv4_length(a.pool, first + lane);
+      const Drafts d = drafts_of(a, begin, end, length);
       parts = a.pool.kv_heads * d.passes;
       tiles = tiles_of<TILE>(d.length);
       ticks = part_ticks<TILE>(d);
@@ -188,12 +192,13 @@ __device__ __forceinline__ Cut cut_at(const Kv4Tree &a, int wanted) {
         const int at = __builtin_ctzll(past), each = __builtin_amdgcn_readlane(pieces, at);
         const int start = before + __builtin_amdgcn_readlane(sum - n, at), local = scalar(max(wanted, start)) - start;
         const int part = scalar(local / each);
-        return {first + at, part, local - part * each, each, start + part * each};
+        const Drafts d = drafts_of(a, __builtin_amdgcn_readlane(begin, at), __builtin_amdgcn_readlane(end, at), __builtin_amdgcn_readlane(length, at));
+        return {d, first + at, part, local - part * each, each, start + part * each};
       }
       before += __builtin_amdgcn_readlane(sum, 63);
     }
   }
-  return {-1, 0, 0, 1, 0};
+  return {{}, -1, 0, 0, 1, 0};
 }
 
 // The row of a column, and its query head in the KV head's group: column / a.group by the host's ceil(2^32 / group), exact for
@@ -276,7 +281,7 @@ __global__ __launch_bounds__(kThreads, kResident<DIM>) void kv4_tree_kernel(Kv4T
     const Cut cut = cut_at<kTile>(a, blockIdx.x);
     if (cut.sequence < 0) return;
     sequence = cut.sequence;
-    d = scalar_drafts(a, sequence);
+    d = cut.d;
     head = scalar(cut.part / d.passes);
     pass = cut.part - head * d.passes;
     piece = cut.piece;
@@ -616,10 +621,10 @@ __global__ __launch_bounds__(kThreads) void kv4_tree_combine_kernel(Kv4Tree a) {
   const int lane = threadIdx.x & 63, wave = scalar(threadIdx.x >> 6);
   const int pass = blockIdx.x % a.most_passes, head = blockIdx.x / a.most_passes % pool.kv_heads;
   const int sequence = blockIdx.x / a.most_passes / pool.kv_heads, block = blockIdx.y;
-  const Drafts d = scalar_drafts(a, sequence);
+  const Cut cut = cut_at<kTile>(a, ~sequence);
+  const Drafts &d = cut.d;
   const int col0 = (pass * d.blocks + block) * kCols;
   if (pass >= d.passes || block >= d.blocks || col0 >= d.columns) return;
-  const Cut cut = cut_at<kTile>(a, ~sequence);
   const int w1 = cut.pieces - 1, slice0 = SHARED ? blockIdx.z : wave * kSlices;
   if (w1 == 0) return;  // one workgroup had it all and wrote the output
   const float *pieces = a.pieces + (int64_t)(cut.before + (head * d.passes + pass) * cut.pieces) * a.piece_floats + block * kPieceFloats<DIM>;
