@@ -27,13 +27,13 @@
 // Statistics and sums in fp32; sums run over the probabilities as rounded. In fp16 they are held times 2^11, in bf16 times a power
 // of two below 1 / (2^4 length), so that sums of the largest values stay finite.
 //
-// Bound by instruction issue where contexts are long: 80 columns over 262,144 positions of 8 heads of 128 take 168 us and 9 to combine
-// (1.7 TB/s of codes, 510 TFLOP/s); the same loop takes 76 without its products and exponentials, a wave and tile having some 110
-// vector instructions to convert with, 200 for the scores and 32 products, of which two waves a SIMD overlap a part. Short contexts are
-// a chain of dependent steps: 24 trees of 130 columns over up to 8,191 positions 29 us and 14, of which 5 find the place, 6 fetch and
+// Bound by instruction issue where contexts are long: 80 columns over 262,144 positions of 8 heads of 128 take 150 us and 8.5 to combine
+// (1.9 TB/s of codes, 570 TFLOP/s), a tile as long as the two 32-position steps of its busiest wave: scores, maximum, exponentials and
+// value products one behind the other, beside one wave of another workgroup. Short contexts are
+// a chain of dependent steps: 24 trees of 130 columns over up to 8,191 positions 29 us and 13, of which 5 find the place, 6 fetch and
 // convert the first tile and 1 to 2 are each tile behind.
 // Columns in units of 16 (v_mfma_f32_16x16x32), each wave converting for itself, took 145 us for the one and 54 for the other;
-// 64 positions a step with joined maxima 174 and 34; one buffer, two barriers a tile 174 and 28.
+// 64 positions a step with joined maxima (spills) 174 and 34; one buffer, two barriers a tile 174 and 28.
 
 #include <math.h>
 
@@ -291,14 +291,14 @@ __global__ __launch_bounds__(kThreads, kResident<DIM>) void kv4_tree_kernel(Kv4T
   // Products pass 32 bits.
   const int first = (int)((uint64_t)tiles * piece / pieces), until = (int)((uint64_t)tiles * (piece + 1) / pieces);
 
-  // This thread's part of a conversion: position p of the tile, elements 32 g .. 32 g + 31.
-  const int p = threadIdx.x / kGroups, g = threadIdx.x % kGroups;
+  // This thread's part of a conversion: position `row` of its wave's kTile / kWaves, elements 32 g .. 32 g + 31.
+  const int row = lane / kGroups, g = lane % kGroups;
   const int64_t half_bytes = kv4_half_bytes(pool.page_shift, DIM), scales_at = (int64_t)(DIM / 2) << pool.page_shift;
   const int64_t head_bytes = 2 * half_bytes, page_bytes = head_bytes * pool.kv_heads;
   const int page_mask = (1 << pool.page_shift) - 1;
   // 16-byte chunk c of row r lies at chunk c ^ turn: operand reads and these stores hit distinct banks.
-  const int k_turn = DIM == 128 ? p & 15 : (p >> 1) & 7;
-  const int v_turn = DIM == 128 ? 5 * (p & 3) : 4 * ((p >> 1) & 1) ^ ((p >> 1) & 3);
+  const int k_turn = DIM == 128 ? row & 15 : (row >> 1) & 7;
+  const int v_turn = DIM == 128 ? 5 * (row & 3) : 4 * ((row >> 1) & 1) ^ ((row >> 1) & 3);
   // Operands: key row n, dimensions 16 st + 8 h at k_at ^ 32 st; by the transposing reads key 4 h + (lane % 16) / 4,
   // dimensions 32 t + 16 ((lane / 16) % 2) + 4 (lane % 4) at v_at ^ 64 t.
   const uint32_t k_at = (uint32_t)n * kRow + 16u * (uint32_t)(h ^ (DIM == 128 ? n & 15 : (n >> 1) & 7));
@@ -308,31 +308,40 @@ __global__ __launch_bounds__(kThreads, kResident<DIM>) void kv4_tree_kernel(Kv4T
 
   const int col0 = pass * d.blocks * kCols;
   const int blocks = min(d.blocks, pieces_of(d.columns - col0, kCols));
-  // Waves that share a block's positions: all of them for one block (at dim 128 two), pairs for two.
-  const int shares = blocks >= 3 ? 1 : blocks == 2 ? 2 : min(kWaves, kSubs);
-  const int block = blocks >= 3 ? wave : blocks == 2 ? wave & 1 : 0, share = blocks >= 3 ? 0 : blocks == 2 ? wave >> 1 : wave;
+  // Waves that share a block's positions: all of them for one block (at dim 128 two), pairs for two. Of three blocks two waves have one
+  // each and two share the third.
+  const int shares = blocks >= 4 ? 1 : blocks == 3 ? (wave >= 2 ? 2 : 1) : blocks == 2 ? 2 : min(kWaves, kSubs);
+  const int block = blocks >= 4 ? wave : blocks == 3 ? min(wave, 2) : blocks == 2 ? wave & 1 : 0;
+  const int share = blocks >= 4 ? 0 : blocks == 3 ? (wave == 3 ? 1 : 0) : blocks == 2 ? wave >> 1 : wave;
   const bool works = block < blocks && share < shares;
   const int stop = min(until * kTile, d.length);
 
-  // Page ids of this wave's positions of a tile (at dim 64 twice 16 of them), a tile before its codes.
+  // Quarters of a tile that this wave converts: its own; where two waves have less to multiply, or nothing, they convert for all. 80
+  // columns and 262,144 positions 150 us (165 where all convert), 32 columns and 100,000 positions of 2 heads 17.1 (19.2), of 16 heads
+  // in 8 sequences of up to as many 18.7 (21.6).
+  const bool apart = blocks == 3 || (blocks == 1 && kSubs < kWaves);
+  const int quarters = !apart ? 1 : wave >= 2 ? 2 : 0, quarter = !apart ? wave : 2 * (wave & 1);
+  // Page ids of a quarter's positions (at dim 64 twice 16 of them), a tile before its codes.
   constexpr int kIds = kTile / kWaves / 16;
   struct Ids {
     int page[kIds];
   };
-  auto ids_of = [&](int tile) __attribute__((always_inline)) {
+  auto ids_of = [&](int tile, int k) __attribute__((always_inline)) {
     // Constant for the whole launch: scalar loads.
     const auto *table = (const __attribute__((address_space(4))) int *)(pool.table + sequence * pool.table_stride);
     Ids ids;
 #pragma unroll
     for (int i = 0; i < kIds; ++i)
-      ids.page[i] = table[min(tile * kTile + wave * (kTile / kWaves) + 16 * i, max(d.length - 1, 0)) >> pool.page_shift];
+      ids.page[i] = table[min(tile * kTile + (quarter + k) * (kTile / kWaves) + 16 * i, max(d.length - 1, 0)) >> pool.page_shift];
     return ids;
   };
-  u32x4 k_codes, v_codes;
-  uint32_t k_scale, v_scale;
-  int there;  // of this thread's position: whether its page is known
-  auto load = [&](int tile, const Ids &ids) __attribute__((always_inline)) {
-    const int position = tile * kTile + p, at = position & page_mask;
+  struct Codes {
+    u32x4 k, v;
+    uint32_t k_scale, v_scale;
+    int there;  // whether the position's page is known
+  };
+  auto codes_of = [&](int tile, int k, const Ids &ids) __attribute__((always_inline)) {
+    const int position = tile * kTile + (quarter + k) * (kTile / kWaves) + row, at = position & page_mask;
     const uint8_t *half[kIds];
     int known_page[kIds];
 #pragma unroll
@@ -342,15 +351,29 @@ __global__ __launch_bounds__(kThreads, kResident<DIM>) void kv4_tree_kernel(Kv4T
     }
     const bool second = kIds == 2 && lane >= 32;
     const uint8_t *mine = second ? half[kIds - 1] : half[0];
-    there = second ? known_page[kIds - 1] : known_page[0];
-    k_codes = *reinterpret_cast<const u32x4 *>(mine + at * (DIM / 2) + 16 * g);
-    v_codes = *reinterpret_cast<const u32x4 *>(mine + half_bytes + at * (DIM / 2) + 16 * g);
-    k_scale = mine[scales_at + at * kGroups + g];
-    v_scale = mine[half_bytes + scales_at + at * kGroups + g];
+    Codes c;
+    c.there = second ? known_page[kIds - 1] : known_page[0];
+    c.k = *reinterpret_cast<const u32x4 *>(mine + at * (DIM / 2) + 16 * g);
+    c.v = *reinterpret_cast<const u32x4 *>(mine + half_bytes + at * (DIM / 2) + 16 * g);
+    c.k_scale = mine[scales_at + at * kGroups + g];
+    c.v_scale = mine[half_bytes + scales_at + at * kGroups + g];
+    return c;
   };
-  Ids ids = ids_of(first);
-  load(first, ids);
-  ids = ids_of(first + 1);
+  Codes codes[2] = {};
+  Ids ids[2] = {};
+  // The codes of `tile`, whose ids are here, and the ids of the one behind.
+  auto load = [&](int tile) __attribute__((always_inline)) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      if (k < quarters) {
+        codes[k] = codes_of(tile, k, ids[k]);
+        ids[k] = ids_of(tile + 1, k);
+      }
+  };
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+    if (k < quarters) ids[k] = ids_of(first, k);
+  load(first);
 
   const int column = col0 + block * kCols + n;  // this lane's query
   const Query query = query_of(a, min(column, d.columns - 1));
@@ -389,43 +412,43 @@ __global__ __launch_bounds__(kThreads, kResident<DIM>) void kv4_tree_kernel(Kv4T
   for (int t = 0; t < kOut; ++t) o[t] = f32x16{};
 
   // The codes in registers, converted into the buffers of their tile.
-  auto convert = [&](int tile) __attribute__((always_inline)) {
+  auto convert_one = [&](int tile, int k, Codes c) __attribute__((always_inline)) {
+    const int p = (quarter + k) * (kTile / kWaves) + row, position = tile * kTile + p;
     char *const kb = keys[tile & 1] + p * kRow, *const vb = values[tile & 1] + p * kRow;
-    const int position = tile * kTile + p;
-    const bool counts = there && position < d.length;
-    uint32_t ks = k_scale, vs = v_scale;
+    const bool counts = c.there && position < d.length;
     if (tile * kTile + kTile > min(d.context, d.length)) {
       asm volatile("" ::: "memory");  // stays a branch: the last tiles of a sequence
       bool odd = false;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const u32x4 x = kv4_octet<F16>(v_codes[i], __uint_as_float(vs << 23));
+        const u32x4 x = kv4_octet<F16>(c.v[i], __uint_as_float(c.v_scale << 23));
 #pragma unroll
         for (int j = 0; j < 4; ++j) odd |= not_finite<F16>(x[j]);
       }
       odd = odd && counts && position >= d.context;
-      const int row = position - d.context;
-      if (odd && row < kMostDrafts) atomicOr((unsigned long long *)&mads, 1ull << row);
-      vs = odd ? 127u : vs;
+      const int draft = position - d.context;
+      if (odd && draft < kMostDrafts) atomicOr((unsigned long long *)&mads, 1ull << draft);
+      c.v_scale = odd ? 127u : c.v_scale;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v_codes[i] = odd ? 0u : v_codes[i];
+      for (int i = 0; i < 4; ++i) c.v[i] = odd ? 0u : c.v[i];
     }
-    ks = counts ? ks : 127u;
-    vs = counts ? vs : 127u;
+    const uint32_t ks = counts ? c.k_scale : 127u, vs = counts ? c.v_scale : 127u;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint32_t kc = counts ? k_codes[i] : 0u, vc = counts ? v_codes[i] : 0u;
+      const uint32_t kc = counts ? c.k[i] : 0u, vc = counts ? c.v[i] : 0u;
       *reinterpret_cast<u32x4 *>(kb + 16 * ((4 * g + i) ^ k_turn)) = kv4_octet<F16>(kc, __uint_as_float(ks << 23));
       *reinterpret_cast<u32x4 *>(vb + 16 * ((4 * g + i) ^ v_turn)) = kv4_octet<F16>(vc, __uint_as_float(vs << 23));
     }
-    if (g == 0 && p % 16 == 0) known[tile & 1][p / 16] = (uint8_t)there;
+    if (g == 0 && p % 16 == 0) known[tile & 1][p / 16] = (uint8_t)c.there;
+  };
+  auto convert = [&](int tile) __attribute__((always_inline)) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      if (k < quarters) convert_one(tile, k, codes[k]);
   };
   lds_barrier();  // `mads` is clear
   convert(first);
-  if (first + 1 < until) {
-    load(first + 1, ids);
-    ids = ids_of(first + 2);
-  }
+  if (first + 1 < until) load(first + 1);
 
 #pragma unroll 1
   for (int tile = first; tile < until; ++tile) {
@@ -433,10 +456,7 @@ __global__ __launch_bounds__(kThreads, kResident<DIM>) void kv4_tree_kernel(Kv4T
     lds_barrier();  // this tile is converted, the last one read
     if (tile + 1 < until) {
       convert(tile + 1);
-      if (tile + 2 < until) {
-        load(tile + 2, ids);
-        ids = ids_of(tile + 3);
-      }
+      if (tile + 2 < until) load(tile + 2);
     }
     if (!works) continue;
 #pragma unroll 1
@@ -522,9 +542,9 @@ __global__ __launch_bounds__(kThreads, kResident<DIM>) void kv4_tree_kernel(Kv4T
   if (m == -INFINITY && any) l += kNoScore;
   lds_barrier();  // the last tile is read
   const uint64_t lost = mads;
-  if (shares > 1) {
+  if (blocks < 4) {
     // Share s of a block: 4 KiB for each 32 dimensions, of which the keys' place has 8.
-    auto region = [&](int s) { return reinterpret_cast<f32x4 *>(keys[0] + ((s - 1) * blocks + block) * kOut * 4096) + lane; };
+    auto region = [&](int s) { return reinterpret_cast<f32x4 *>(keys[0] + (blocks == 3 ? 0 : (s - 1) * blocks + block) * kOut * 4096) + lane; };
     if (works && share > 0) {
       stats[wave][0][lane] = m;
       stats[wave][1][lane] = l;
@@ -538,7 +558,7 @@ __global__ __launch_bounds__(kThreads, kResident<DIM>) void kv4_tree_kernel(Kv4T
     if (works && share == 0) {
 #pragma unroll 1
       for (int s = 1; s < shares; ++s) {
-        const int theirs = blocks == 2 ? 2 * s + block : s;
+        const int theirs = blocks == 3 ? 3 : blocks == 2 ? 2 * s + block : s;
         const float m2 = stats[theirs][0][lane], l2 = stats[theirs][1][lane], top = fmaxf(m, m2);
         const float w1 = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - top) * a.sl2);
         const float w2 = m2 == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m2 - top) * a.sl2);
