@@ -27,8 +27,8 @@
 // Statistics and sums in fp32; sums run over the probabilities as rounded. In fp16 they are held times 2^11, in bf16 times a power
 // of two below 1 / (2^4 length), so that sums of the largest values stay finite.
 //
-// Bound by instruction issue where contexts are long: 80 columns over 262,144 positions of 8 heads of 128 take 150 us and 8.5 to combine
-// (1.9 TB/s of codes, 570 TFLOP/s), a tile as long as the two 32-position steps of its busiest wave: scores, maximum, exponentials and
+// Bound by instruction issue where contexts are long: 80 columns over 262,144 positions of 8 heads of 128 take 150 to 156 us and 9 to combine
+// (1.9 TB/s of codes, 560 TFLOP/s), a tile as long as the two 32-position steps of its busiest wave: scores, maximum, exponentials and
 // value products one behind the other, beside one wave of another workgroup. Short contexts are
 // a chain of dependent steps: 24 trees of 130 columns over up to 8,191 positions 29 us and 13, of which 5 find the place, 6 fetch and
 // convert the first tile and 1 to 2 are each tile behind.
