@@ -36,6 +36,9 @@ ROPE = [
     ([64, 300], [64, 3], 7, 7, 128, 64, 112, False, True),
     (list(range(1, 101)), [1 + n // 3 for n in range(1, 101)], 2, 2, 128, 16, 64, True, False),
     ([2] * 2500, [n % 3 for n in range(2500)], 2, 1, 64, 16, 64, False, False),  # more sequences than the search holds in LDS
+    # several heads a workgroup, queries, keys and values among them
+    ([2000, 1300], [1999, 1200], 30, 5, 128, 64, 128, False, True),
+    ([3000, 900, 2500], [2999, 800, 2400], 40, 8, 64, 256, 48, True, False),
 ]
 
 
@@ -189,6 +192,9 @@ TREES = [
     ([4 + (37 * i) % 301 for i in range(150)], [1 + i % 4 for i in range(150)], 4, 2, 128, 16, False),  # more sequences than lanes
     ([70 + (53 * i) % 1500 for i in range(70)], [i % 65 for i in range(70)], 12, 12, 64, 32, False),
     ([3, 2, 1], [5, 2, 7], 8, 2, 128, 16, False),     # fewer positions than rows
+    # hundreds of queries a row
+    ([90, 40], [3, 1], 300, 1, 64, 16, False),
+    ([2000], [2], 601, 1, 128, 64, False),
     # as many short (sequence, head)s as fill the grid by themselves
     ([20 + (37 * i) % 300 for i in range(80)], [1 + i % 20 for i in range(80)], 24, 8, 128, 16, False),
     ([64 + (41 * i) % 200 for i in range(40)], [64 - i % 7 for i in range(40)], 32, 16, 64, 32, True),
@@ -644,7 +650,8 @@ def test_rows_past_the_64th_take_no_part_in_a_path(ext):
 # the accepted rows
 
 
-@pytest.mark.parametrize("layer_count,kv_heads,dim,page", [(None, 1, 64, 16), (3, 2, 128, 16), (2, 5, 64, 32), (1, 3, 128, 1024)])
+@pytest.mark.parametrize("layer_count,kv_heads,dim,page", [(None, 1, 64, 16), (3, 2, 128, 16), (2, 5, 64, 32), (1, 3, 128, 1024),
+                                                          (100, 8, 64, 16), (101, 5, 128, 16)])
 def test_accepted_rows_move_together(ext, layer_count, kv_heads, dim, page):
     """Every byte of every pool: the path's rows at their places, nothing else changed; paths in any order, whole, empty."""
     rng = np.random.default_rng(dim + kv_heads)
