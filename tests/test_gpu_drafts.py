@@ -601,6 +601,23 @@ def test_the_largest_vocabulary(ext, kind, temperature):
     check_verified(rows, trees, logits, draft, ids, uniforms, [temperature] * 2, kind)
 
 
+def test_the_same_tokens_whichever_workgroup_ends_last(ext):
+    """Other numbers for the last draw between two calls that are alike: their sums lie in the same workspace."""
+    rows, vocab = [5] * 12, 70001
+    trees, logits, draft, ids, uniforms = drafted(rows, vocab, BF16, 9, "sampled")
+    scratch = torch.empty(layers.verify_drafts_workspace_bytes(logits.cuda(), 12, sampled=True), dtype=torch.uint8, device="cuda")
+    logits, draft, ids, cu = logits.cuda(), draft.cuda(), ids.cuda(), cumulative(rows)
+    numbers = [uniforms.cuda(), (uniforms * 0.37).cuda()]
+
+    def call(i, temperature):
+        return layers.verify_drafts(logits, ids, numbers[i], cu, draft_logits=draft, temperature=temperature, workspace=scratch)
+
+    want = [[t.tolist() for t in call(i, 1.0 + i)] for i in range(2)]
+    for _ in range(60):
+        for i in range(2):
+            assert [t.tolist() for t in call(i, 1.0 + i)] == want[i]
+
+
 def test_identical_models_and_the_largest_numbers(ext):
     """Draft and target alike: every draft is accepted, for numbers of 1 too (where q(x) is not below p(x)) nothing breaks."""
     rows, vocab = [5, 7], 3001

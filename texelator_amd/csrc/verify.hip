@@ -515,7 +515,10 @@ __global__ __launch_bounds__(64 * kWalkWaves) void verify_walk_kernel(Verify a) 
     }
     if (lane == 0) kept[chunk] = mine;
   }
-  __syncthreads();  // the workgroup's sums are in its cache: one thread's fence makes them visible to all
+  // Every wave's sums have reached the cache of its die before the barrier, which does not wait for stores by itself; one thread's fence
+  // behind it makes them visible to the other dies.
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
   if (threadIdx.x == 0) {
     __threadfence();
     ends = atomicAdd(a.counters + sequence, 1) == a.groups - 1;
