@@ -132,10 +132,7 @@ __device__ __forceinline__ Drafts drafts_of(const Kv4Tree &a, int first, int end
   d.blocks = d.passes <= 1 ? blocks : pieces_of(blocks, d.passes);
   return d;
 }
-__device__ __forceinline__ Drafts drafts_of(const Kv4Tree &a, int sequence) {
-  return drafts_of(a, a.cu[sequence], a.cu[sequence + 1], kv4_length(a.pool, sequence));
-}
-// The same of a sequence that all lanes ask for, in scalar registers: page ids then stay scalar.
+// Of a sequence that all lanes ask for, in scalar registers: page ids then stay scalar.
 __device__ __forceinline__ Drafts scalar_drafts(const Kv4Tree &a, int sequence) {
   return drafts_of(a, scalar(a.cu[sequence]), scalar(a.cu[sequence + 1]), scalar(kv4_length(a.pool, sequence)));
 }
