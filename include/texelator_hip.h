@@ -527,7 +527,7 @@ int tx_kv4_append_rope(const void *q, int64_t q_token, int64_t q_head, const voi
  * all of its rows, itself and the rows that its parents lead to. out the same shape: zeros for a row that sees no position in the
  * pool, NaN where all scores are -infinity. Positions that a row does not see, and their values, may hold anything. out must not
  * overlap q; queries 16-byte aligned, output rows 8-byte. Arithmetic, workspace rules and limits as tx_kv4_attention, at most
- * 2^22 rows and 4,096 query heads for each KV head. */
+ * 2^22 rows, 4,096 query heads for each KV head (a group), and fewer than 2^23 sequences x kv_heads x ceil(min(tokens, 64) group / 128). */
 int tx_kv4_tree_attention_workspace(int sequences, int64_t tokens, int heads, int kv_heads, int head_dim, int page_size, int max_pages,
                                     int device, int64_t *bytes);
 int tx_kv4_tree_attention(const void *q, int64_t q_token, int64_t q_head, int dtype, int64_t tokens, int heads, const int *cu,

@@ -118,6 +118,16 @@ def test_sizes_of_workspaces():
     assert lib.tx_verify_drafts_workspace(1, 20, 1000, 3, 0, 0, None) == _lib.TX_ERR_INVALID
 
 
+@pytest.mark.parametrize("sequences,tokens,heads,kv_heads,dim,page_size,max_pages", [
+    (1024, 6144, 64, 8, 128, 1024, 1024), (4096, 20000, 32, 8, 64, 256, 2048), (6, 157, 128, 2, 128, 1024, 1 << 20), (1, 64, 4096, 1, 128, 1024, 1 << 20)])
+def test_tables_with_room_for_long_sequences(sequences, tokens, heads, kv_heads, dim, page_size, max_pages):
+    """What single tokens' attention takes, a drafted step takes: how many rows a sequence could have is no reason to refuse the few it has."""
+    lib, out = _lib.load(), ctypes.c_int64()
+    assert lib.tx_kv4_attention_workspace(sequences, heads, kv_heads, dim, page_size, max_pages, 0, out) == _lib.TX_OK
+    assert lib.tx_kv4_tree_attention_workspace(sequences, tokens, heads, kv_heads, dim, page_size, max_pages, 0, out) == _lib.TX_OK
+    assert 0 < out.value < 1 << 30
+
+
 def test_tensors_are_checked(monkeypatch):
     """Wrong types, shapes and strides never reach the native call."""
     monkeypatch.setattr(_lib, "load", lambda: pytest.fail("reached the native call"))

@@ -217,6 +217,23 @@ def test_trees_against_64_bits(ext, lengths, rows, heads, kv_heads, dim, page_si
     assert torch.equal(run(), got)  # the same bits again
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+def test_tables_with_room_for_a_billion_positions(ext, dim):
+    """Room for far more work than there is: a table of 2^20 pages of 1,024 positions, 64 queries a row and KV head."""
+    lengths, rows = [20011, 900, 64, 1, 5000, 33], [16, 64, 3, 1, 40, 33]
+    trees = Trees(lengths, rows, 2, dim, 1024, 11)
+    table = torch.full((len(rows), 1 << 20), -1, dtype=torch.int32, device="cuda")
+    table[:, :trees.table.shape[1]] = trees.table
+    q = torch.randn(sum(rows), 128, dim, generator=torch.Generator().manual_seed(1)).to(BF16).cuda()
+
+    def run():
+        return layers.kv4_tree_attention(q, trees.pages, table, trees.lengths, trees.cu, dim ** -0.5, parents=trees.parents)
+
+    got = run()
+    assert_within(got, *trees.tree_attention(q, dim ** -0.5))
+    assert torch.equal(run(), got)
+
+
 def test_a_row_alone_is_single_token_attention(ext):
     """One row a sequence: within both calls' roundings of kv4_attention."""
     cache = Cache([700, 1, 9000, 33], 2, 128, 64, 3)

@@ -263,7 +263,7 @@ hipError_t launch_kv4_attention(const Kv4Attention &a, bool f16, int dim, hipStr
 // Attention of drafted rows over the cache (tree_attention.hip).
 struct Kv4Tree;
 bool kv4_tree_fits(const Kv4Tree &a);
-// Fills in workgroups, passes, whole and piece_bytes (the workspace's size).
+// Fills in workgroups, passes, shift, whole and piece_bytes (the workspace's size).
 void kv4_tree_plan(Kv4Tree &a, int dim, int cus);
 hipError_t launch_kv4_tree(const Kv4Tree &a, bool f16, int dim, hipStream_t stream);
 

@@ -80,6 +80,7 @@ struct Kv4Tree {
   float *pieces;  // results of heads that several workgroups share
   int64_t piece_bytes;
   int piece_floats, workgroups, most_passes;
+  int shift;   // work is counted in units of 2^shift ticks
   bool whole;  // a workgroup for each sequence, head and pass: no pieces
 };
 

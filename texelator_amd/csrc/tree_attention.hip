@@ -139,9 +139,11 @@ __device__ __forceinline__ Drafts scalar_drafts(const Kv4Tree &a, int sequence) 
 
 template <int TILE>
 __device__ __forceinline__ int tiles_of(int length) { return max(1, (length + TILE - 1) / TILE); }
-// Ticks of a part, the start among them: passes count alike, whatever their blocks.
+// Ticks of a part, the start among them, in units of 2^shift: passes count alike, whatever their blocks.
 template <int TILE>
-__device__ __forceinline__ int part_ticks(const Drafts &d) { return kStart + weight_of(d.blocks) * tiles_of<TILE>(d.length); }
+__device__ __forceinline__ int part_ticks(const Kv4Tree &a, const Drafts &d) {
+  return ((kStart + weight_of(d.blocks) * tiles_of<TILE>(d.length)) >> a.shift) + (a.shift > 0);
+}
 
 // How the parts are cut: into as many pieces as they have even shares of the grid, rounded; the pieces of cut parts are at most
 // four thirds of the grid's even shares.
@@ -164,7 +166,7 @@ __device__ __forceinline__ Cut cut_at(const Kv4Tree &a, int wanted) {
       const Drafts d = drafts_of(a, begin, end, length);
       parts = a.pool.kv_heads * d.passes;
       tiles = tiles_of<TILE>(d.length);
-      ticks = part_ticks<TILE>(d);
+      ticks = part_ticks<TILE>(a, d);
     }
   };
   int total = 0;
@@ -172,7 +174,7 @@ __device__ __forceinline__ Cut cut_at(const Kv4Tree &a, int wanted) {
     load(first);
     total += __builtin_amdgcn_readlane(wave_scan(parts * ticks), 63);
   }
-  const int share = max((total + a.workgroups - 1) / a.workgroups, kLeast);
+  const int share = max((total + a.workgroups - 1) / a.workgroups, max(kLeast >> a.shift, 1));
   auto pieces_now = [&] { return max(min((int)((2u * ticks + share) / (2u * share)), tiles), 1); };
   int before = 0;
 #pragma unroll 1
@@ -719,14 +721,16 @@ int64_t most_ticks(const Kv4Tree &a, int tile) {
 
 }  // namespace
 
-// Ticks are 32-bit; a launch has fewer than 2^32 threads, 256 for each (head, pass).
-bool kv4_tree_fits(const Kv4Tree &a) {
-  return most_ticks(a, kTile<128>) <= (int64_t)1 << 30 && most_parts(a) < (int64_t)1 << 23;
-}
+// What single tokens' attention takes; a launch has fewer than 2^32 threads, 256 for each (head, pass).
+bool kv4_tree_fits(const Kv4Tree &a) { return kv4_attention_fits(a.pool) && most_parts(a) < (int64_t)1 << 23; }
 
 void kv4_tree_plan(Kv4Tree &a, int dim, int cus) {
   const int64_t room = (int64_t)a.pool.max_pages << a.pool.page_shift;
   a.most_passes = (int)most_passes(a);
+  // Ticks are 32-bit: where tables have room for more of them than 2^30 (64 rows a sequence, all as long as the table), in coarser units, so
+  // that their sum holds whatever cu and the lengths are. Cuts are then as fine as 2^-30 of that most.
+  a.shift = 0;
+  while (most_ticks(a, dim == 128 ? kTile<128> : kTile<64>) >> a.shift > (int64_t)1 << 30) ++a.shift;
   const int64_t shares = most_ticks(a, dim == 128 ? kTile<128> : kTile<64>) / kLeast + 1;
   const int64_t fill = (dim == 128 ? kResident<128> : kResident<64>) * (int64_t)cus;
   // Short parts that fill the grid by themselves are not cut: 32 sequences of up to 400 positions and 8 heads of 16 * 5 rows take 15 us,
