@@ -545,8 +545,8 @@ int tx_kv4_tree_attention(const void *q, int64_t q_token, int64_t q_head, int dt
  *   with draft_logits [tokens][vocab] (chains alone: parents must be NULL; x was drawn from q_v = softmax(draft_logits[v] /
  *     temperature)) where u q_v(x) < p_v(x); else the closing token is drawn from max(p_v - q_v, 0).
  * Where that leaves nothing, it is drawn from p_v. A token is drawn as the first whose running sum in the vocabulary's order
- * exceeds u times the whole sum, in 64 bits; the tests use sums of 32-bit terms (off by some 1e-7). temperatures [sequences], or
- * NULL: `temperature` for all. A temperature that is not above 0: the largest logit's token is accepted and closes, of equal ones
+ * exceeds u times the whole sum, in 64 bits; the tests use sums of 32-bit terms (off by some 1e-8; where few terms count,
+ * by up to 1e-7). temperatures [sequences], or NULL: `temperature` for all. A temperature that is not above 0: the largest logit's token is accepted and closes, of equal ones
  * the first. Logits of -infinity have no weight; where a row that is reached holds a NaN, at temperatures above 0 an infinity, or
  * nothing above -infinity, no draft behind it is accepted and the closing token is -1.
  * accepted [sequences]: accepted drafts, -1 for a sequence without rows. path [tokens]: path[cu[s] + j] is the row at step j, 0 to

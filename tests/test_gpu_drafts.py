@@ -527,6 +527,29 @@ def test_every_token_is_drawn_at_its_share(ext):
     assert torch.equal(closing, expected.clamp(max=vocab - 1))
 
 
+@pytest.mark.parametrize("temperature", [0.9, 1.3, 2.5])
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+def test_drafts_next_to_their_border(ext, dtype, temperature):
+    """Numbers 9e-8 of a draft's probability below it accept, as far above it they do not. Terms in 32 bits are off by half of an
+    exponential's last bit in common at most (2^-24 = 6e-8); their other roundings are each its own, and 2^-24 (2 + exponent) of thousands of
+    terms that count make less than 1e-8 of the sum."""
+    vocab, drafts, off = 151936, 200, 9e-8
+    g = torch.Generator().manual_seed(3)
+    logits = (2.5 * torch.randn(1, vocab, generator=g)).to(dtype)
+    p = torch.softmax(logits[0].double() / float(torch.tensor(temperature, dtype=FP32)), 0)
+    ids = torch.randint(0, vocab, (drafts,), generator=g)
+    borders = p[ids].numpy()
+    below, above = (borders * (1 - off)).astype(np.float32), (borders * (1 + off)).astype(np.float32)
+    below = np.where(below.astype(np.float64) > borders * (1 - off), np.nextafter(below, np.float32(0)), below)
+    above = np.where(above.astype(np.float64) < borders * (1 + off), np.nextafter(above, np.float32(1)), above)
+    tokens, uniforms = torch.zeros(4 * drafts, dtype=torch.int64), torch.full((4 * drafts,), 0.5)
+    tokens[1::2] = ids.repeat_interleave(2)
+    uniforms[1::4], uniforms[3::4] = torch.from_numpy(below), torch.from_numpy(above)
+    accepted, _, _ = layers.verify_drafts(logits.cuda().expand(4 * drafts, -1), tokens.cuda(), uniforms.cuda(), i32(range(0, 4 * drafts + 1, 2)),
+                                          temperature=temperature)
+    assert accepted[0::2].all() and not accepted[1::2].any()
+
+
 def test_repeated_unknown_and_impossible_drafts(ext):
     """A token that a sibling had already, tokens outside the vocabulary, tokens without weight: never accepted, and not counted."""
     vocab = 50
@@ -604,6 +627,22 @@ def test_masked_tokens_at_the_largest_temperatures(ext, kind, temperature):
     ids[:] = torch.tensor([0, 1, 2, 3, 9, 10, 4, 0, 1])
     uniforms[:] = torch.tensor([0.9, 0.05, 0.1, 0.16, 0.05, 0.1, 0.5, 0.0, 0.1])
     check_verified(rows, trees, logits, draft, ids, uniforms, [temperature] * 2, kind)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("kind", ["tree", "sampled"])
+def test_lowest_values_as_masks_and_the_widest_rows(ext, kind, dtype):
+    """The type's lowest value in place of most logits, or of all; logits further apart than fp32's largest value; exponents far from zero."""
+    rows, vocab, info = [3] * 5, 2500, torch.finfo(dtype)
+    temperatures = [1.0, 1e-3, float("inf"), 2e-38, 0.9]
+    trees, logits, draft, ids, uniforms = drafted(rows, vocab, dtype, 12, kind)
+    logits[:, 100:2400] = info.min
+    logits[3:6, ::2] = info.min  # spans with a maximum of their own
+    logits[7] = info.min
+    logits[8, ::3] = info.max
+    logits[13:, :90] += 900.0 if dtype == FP16 else 1e5
+    uniforms = uniforms * 0.02
+    check_verified(rows, trees, logits, draft, ids, uniforms, temperatures, kind)
 
 
 @pytest.mark.parametrize("temperature", [0.0, 1.3])

@@ -12,12 +12,14 @@
 // A token is drawn as the first whose running sum in the vocabulary's order exceeds u_0 times the whole sum.
 //
 // Two launches. The first reads all logits once, a wave 64 * kLoads * 16 bytes of a row, and leaves the maximum and the sum
-// of exponentials of each such span, in 32 bits: enough for the tests (off by some 1e-7). In the second every workgroup of a sequence
+// of exponentials of each such span, in 32 bits: enough for the tests (sums of thousands of terms that count are off by some 1e-8, of a
+// few by up to 1e-7, half a unit of the last bit of each). In the second every workgroup of a sequence
 // finds its path: a lane has a row, all drafts are tested at once and a row is reached where all rows that lead to it are taken. The
 // workgroups then share the last row reached and sum its weights in 64 bits, a wave 512 tokens: a draw is as exact as those
 // sums are, and 150 thousand borders lie close. The one that ends last finds the 512 tokens, then the token in them; who that is
 // changes no result. For the residual max(p - q, 0) the sums of p and q are only known then: the weights of p and q are summed over the
-// tokens where p > q by the first launch's sums; a token that those put on the wrong side adds at most 1e-7 of its own probability.
+// tokens where p > q by the first launch's sums; a token that those put on the wrong side adds at most what they are off by, of its own
+// probability.
 //
 // Measured, first and second launch: 16 chains of up to 8 rows sampled from a draft's logits of 151,936 bf16 tokens 14 us (the
 // logits' 55 MB at 3.9 TB/s) and 23 us, 24 trees of up to 64 rows of 32,003 fp32 tokens 26 us (5.5 TB/s) and 17 us, one
@@ -70,7 +72,7 @@ __device__ __forceinline__ void widen_all(u32x4 raw, float *x) {
 // ln(2)^k / k!: 2^f is the sum of these times f^k.
 constexpr double power_of_ln2(int k) { return k == 0 ? 1.0 : power_of_ln2(k - 1) * 0.693147180559945309417232121458 / k; }
 
-// 2^y of y <= 0 in 64 bits: the Taylor sum of 2^f, |f| <= 1/2, to the twelfth power (off by 2e-16). NaN stays.
+// 2^y of y <= 1 in 64 bits: the Taylor sum of 2^f, |f| <= 1/2, to the twelfth power (off by 2e-16). NaN stays.
 __device__ __forceinline__ double exp2_64(double y) {
   y = y < -1100.0 ? -1100.0 : y;  // 2^-1100 is zero
   constexpr double kTerm[13] = {power_of_ln2(0), power_of_ln2(1), power_of_ln2(2),  power_of_ln2(3),  power_of_ln2(4),
@@ -83,8 +85,24 @@ __device__ __forceinline__ double exp2_64(double y) {
   return ldexp(sum, (int)whole);
 }
 
-// log2(e) / T; above zero and finite for every T above zero.
-__device__ __forceinline__ double rate_of(float temperature) { return fmin(1.44269504088896340736 / (double)temperature, 1e300); }
+// log2(e) / T; finite for every T above zero, of which those that fp32 holds with fewer bits count as the least that it holds with all.
+__device__ __forceinline__ double rate_of(float temperature) { return 1.44269504088896340736 / fmax((double)temperature, 0x1p-126); }
+
+// The exponents of a span's terms, x * rate - shift. The rate is the sum of two floats: rounded to one it would put all terms of a row off
+// alike, the more the farther they are below the maximum (sums of 151,936 tokens at a temperature of 2.5 by 1.3e-7, so by 1e-8). The
+// larger has 12 bits, or the smaller's products would be lost behind its products' last bits, again all one way. The shift is the
+// largest exponent, rounded, so that no subtraction comes before the products; where that rounding would tell, or a part of the rate
+// is zero (no factor for -infinity), it is (x - maximum) * rate. Neither part is below zero.
+struct Exponents {
+  float high, low, shift;
+  bool shifted;
+};
+__device__ __forceinline__ Exponents exponents_of(float top, double rate) {
+  const float near = (float)rate;
+  const float high = __uint_as_float((__float_as_uint(near) - ((double)near > rate)) & 0xFFFFF000u), low = (float)(rate - (double)high);
+  const float shift = (float)((double)top * rate);
+  return {high, low, shift, high > 0.f && low > 0.f && fabsf(shift) < 1024.f};
+}
 
 struct Rows {
   int begin, count;  // a sequence's rows: at most kMostDrafts
@@ -98,8 +116,8 @@ __device__ __forceinline__ float temperature_of(const Verify &a, int sequence) {
 }
 __device__ __forceinline__ int wave_min_int(int v) { return -wave_max_int(-v); }
 
-// Grid: x spans by kWaves, y rows, z target and draft logits. Partial of a span: (maximum, sum of exp((x - maximum) / T)), or at
-// T = 0 (maximum, its first index); a NaN among the logits makes the sum (at T = 0 the maximum) NaN.
+// Grid: x spans by kWaves, y rows, z target and draft logits. Partial of a span: (maximum, sum of 2^(x / T * log2(e) - shift)), or
+// at T = 0 (maximum, its first index); a NaN among the logits makes the sum (at T = 0 the maximum) NaN.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void verify_stats_kernel(Verify a) {
   const int lane = threadIdx.x & 63, span = blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -157,18 +175,22 @@ __global__ __launch_bounds__(kThreads) void verify_stats_kernel(Verify a) {
     if (lane == 0) *partial = make_float2(top, __int_as_float(index));
     return;
   }
-  const float rate = (float)fmin(rate_of(temperature), 1e30), base = top == -INFINITY ? 0.f : top;
+  const float base = top == -INFINITY ? 0.f : top;
+  const Exponents e = exponents_of(base, rate_of(temperature));
   float sum = 0.f;
-  if (rate > 0.f) {
+  if (e.shifted) {
 #pragma unroll
     for (int i = 0; i < kLoads; ++i)
 #pragma unroll
-      for (int j = 0; j < kVector; ++j) sum += __builtin_amdgcn_exp2f((x[i][j] - base) * rate);
-  } else {  // at an infinite temperature everything above -infinity weighs the same
+      for (int j = 0; j < kVector; ++j) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(x[i][j], e.low, __builtin_fmaf(x[i][j], e.high, -e.shift)));
+  } else {
 #pragma unroll
     for (int i = 0; i < kLoads; ++i)
 #pragma unroll
-      for (int j = 0; j < kVector; ++j) sum += x[i][j] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((x[i][j] - base) * rate);
+      for (int j = 0; j < kVector; ++j) {
+        const float below = 0.5f * x[i][j] - 0.5f * base;  // halves: finite for all that are
+        sum += x[i][j] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(2.f * __builtin_fmaf(below, e.high, below * e.low));
+      }
   }
   sum = wave_sum(sum);
   if (lane == 0) *partial = make_float2(top, sum);
@@ -416,7 +438,11 @@ __global__ __launch_bounds__(64 * kWalkWaves) void verify_walk_kernel(Verify a) 
       if (mine == 0) sums[0][local] = odd || top == -INFINITY ? -1.0 : (double)index;
     } else {
       double sum = 0.0;
-      each([&](float2 v) { sum += v.x == -INFINITY ? (double)v.y : (double)v.y * exp2_64(((double)v.x - (double)top) * rate); });
+      each([&](float2 v) {
+        const Exponents e = exponents_of(v.x, rate);
+        const double exponent = (e.shifted ? (double)e.shift : (double)v.x * rate) - (double)top * rate;
+        sum += v.x == -INFINITY ? (double)v.y : (double)v.y * exp2_64(exponent);
+      });
       for (int w = 1; w < width; w *= 2) sum += __shfl_xor(sum, w);
       if (mine == 0) {
         tops[kind][local] = top;
