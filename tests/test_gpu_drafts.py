@@ -527,6 +527,40 @@ def test_every_token_is_drawn_at_its_share(ext):
     assert torch.equal(closing, expected.clamp(max=vocab - 1))
 
 
+@pytest.mark.parametrize("temperature", [0.6, 1.0, 2.0])
+def test_sampled_drafts_leave_the_targets_distribution(ext, temperature):
+    """A draft x drawn from q, then the call: the first new token is p's. Numbers on a grid: for each x the share a(x) of them that accept, then
+    with x rejected the shares r(y | x) of the closing tokens. q(y) a(y) + sum over x of q(x) (1 - a(x)) r(y | x) is p(y) but for the grid,
+    which is off by 1 / grid at most in each a and 1 / grid in each r (a token's numbers are an interval): 3 / grid in all."""
+    vocab, grid = 11, 2048
+    g = torch.Generator().manual_seed(4)
+    logits, draft = (1.5 * torch.randn(1, vocab, generator=g) for _ in range(2))
+    t = float(torch.tensor(temperature, dtype=FP32))
+    p, q = (torch.softmax(x[0].double() / t, 0) for x in (logits, draft))
+    u = ((torch.arange(grid) + 0.5) / grid).repeat(vocab)
+    n = vocab * grid
+    ids = torch.arange(vocab).repeat_interleave(grid).repeat_interleave(2).cuda()
+    cu = i32(range(0, 2 * n + 1, 2))
+    rows = [x.cuda().expand(2 * n, -1) for x in (logits, draft)]
+
+    def call(tests, closing):
+        accepted, _, tokens = layers.verify_drafts(rows[0], ids, torch.stack([closing, tests], 1).flatten().cuda(), cu, draft_logits=rows[1],
+                                                   temperature=temperature)
+        return accepted.cpu().view(vocab, grid), tokens.cpu().view(vocab, grid, 2)
+
+    accepted, tokens = call(u, u.flip(0))
+    assert torch.equal(tokens[accepted == 1][:, 0], torch.arange(vocab)[:, None].expand(-1, grid)[accepted == 1])
+    share = accepted.double().mean(1)
+    total = q * share
+    rejected, tokens = call(torch.full((n,), 1 - 2.0 ** -24), u)
+    for x in range(vocab):
+        if share[x] == 1:
+            continue
+        assert p[x] < q[x] and not rejected[x].any()
+        total += q[x] * (1 - share[x]) * torch.bincount(tokens[x, :, 0], minlength=vocab) / grid
+    assert (share < 1).any() and ((total - p).abs() <= 3 / grid).all()
+
+
 @pytest.mark.parametrize("temperature", [0.9, 1.3, 2.5])
 @pytest.mark.parametrize("dtype", [BF16, FP32])
 def test_drafts_next_to_their_border(ext, dtype, temperature):
