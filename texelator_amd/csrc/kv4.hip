@@ -182,10 +182,10 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 // row of the token's position has for pair i; the others pass. Grid: x token blocks, y blocks of `per` heads of [q | k | v]. A
 // thread has eight elements of one token, loads their cosines and sines once for all its heads and has the next head's elements
 // under way while it turns one's; a pair's other element comes from another lane where it is not its own; four neighbours share a
-// group's scale. Queries and rotated key rows (k_out, where given) are rounded once, from 32 bits (a value next to a rounding
-// border of 16 bits is off by 2^-24 of itself more); what is stored is quantized from the exact value (turned_to_odd): a
-// slowly turning key stays so near the 16-bit value that it was that 32 bits put it midway between two codes. Bound by memory:
-// 136 us for 21,447 tokens of 40 + 2 * 8 heads of 128, 4.05 TB/s.
+// group's scale. Queries are computed in 32 bits, two products and their sum (off by 2^-23 (|a cos| + |b sin|) at most, which may be
+// much of a result that cancels), then rounded. Keys are stored and returned (k_out, where given) from the exact value
+// (turned_to_odd), rounded once: a slowly turning key stays so near the 16-bit value that it was that 32 bits put it midway
+// between two codes. Bound by memory: 136 us for 21,447 tokens of 40 + 2 * 8 heads of 128, 4.05 TB/s.
 template <bool F16, int DIM, bool INTERLEAVED>
 __global__ __launch_bounds__(kThreads) void kv4_append_rope_kernel(Kv4Rope a, Kv4Pool pool) {
   constexpr int kChunks = DIM / 8, kGroups = DIM / 32;
