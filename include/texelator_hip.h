@@ -512,9 +512,9 @@ int tx_kv4_copy_pages(void *pages, int layers, int64_t num_pages, int64_t page_b
  * pairs (i, i + rotary / 2), with `interleaved` (2 i, 2 i + 1): a cos - b sin, b cos + a sin, pair i's cosine and sine at
  * cos[position * cos_row + i] and sin[position * sin_row + i] (fp32 [table_rows][rotary / 2]; a scaling for long contexts lies
  * in the tables). positions [tokens], or NULL: every token's place in its sequence; a position outside the tables turns into NaN.
- * q_out is computed in 32 bits (off by 2^-23 (|a cos| + |b sin|) at most) and rounded; what is stored is the nearest code to the exact
- * value, a value beyond fp32's largest counts as infinite. k_out [tokens][kv_heads][head_dim], or NULL: the turned keys, the exact
- * values rounded once. q_out and k_out must not overlap q, k, v or each other. Rows of tokens outside cu are left as they are.
+ * q_out is computed in 32 bits (off by 2^-23 (|a cos| + |b sin|) at most) and rounded; what is stored is the nearest code to the value
+ * in 64 bits, a value beyond fp32's largest counts as infinite. k_out [tokens][kv_heads][head_dim], or NULL: the turned keys, the
+ * values in 64 bits rounded once. q_out and k_out must not overlap q, k, v or each other. Rows of tokens outside cu are left as they are.
  * Rows 16-byte aligned. */
 int tx_kv4_append_rope(const void *q, int64_t q_token, int64_t q_head, const void *k, int64_t k_token, int64_t k_head, const void *v,
                        int64_t v_token, int64_t v_head, int dtype, int64_t tokens, int heads, const float *cos, int64_t cos_row,

@@ -162,9 +162,10 @@ __global__ __launch_bounds__(kThreads) void kv4_read_kernel(uint16_t *k, int64_t
   }
 }
 
-// A value of two 16-bit numbers turned: a cos - b sin, rounded to 32 bits so that no comparison of the quantizer comes out
-// otherwise than for the exact value: towards an odd last bit where it is not exact (borders of codes and scales are even by
-// many bits). The products are exact in 64 bits.
+// A value of two 16-bit numbers turned: a cos - b sin in 64 bits, rounded to 32 so that no comparison of the quantizer comes out
+// otherwise: towards an odd last bit where it does not fit (borders of codes and scales are even by many bits). The products are exact in
+// 64 bits, and so is their difference but where one is below 2^-18 of the other. One below 2^-53 of the other is not seen, though on
+// a border it would decide: to bring back what the sum leaves out took 141 us instead of 137 for 21,447 tokens of 56 heads.
 __device__ __forceinline__ float turned_to_odd(float a, float cos, float b, float sin) {
   const double exact = __builtin_fma((double)a, (double)cos, -((double)b * (double)sin));
   const float near = (float)exact;
@@ -183,7 +184,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 // thread has eight elements of one token, loads their cosines and sines once for all its heads and has the next head's elements
 // under way while it turns one's; a pair's other element comes from another lane where it is not its own; four neighbours share a
 // group's scale. Queries are computed in 32 bits, two products and their sum (off by 2^-23 (|a cos| + |b sin|) at most, which may be
-// much of a result that cancels), then rounded. Keys are stored and returned (k_out, where given) from the exact value
+// much of a result that cancels), then rounded. Keys are stored and returned (k_out, where given) from the value in 64 bits
 // (turned_to_odd), rounded once: a slowly turning key stays so near the 16-bit value that it was that 32 bits put it midway
 // between two codes. Bound by memory: 136 us for 21,447 tokens of 40 + 2 * 8 heads of 128, 4.05 TB/s.
 template <bool F16, int DIM, bool INTERLEAVED>

@@ -798,8 +798,8 @@ def kv4_append_rope(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torc
     that a scaling for long contexts lies in the tables. Pairs are (i, i + rotary / 2), or (2 i, 2 i + 1) with ``interleaved``.
     ``positions`` (int32 ``[tokens]``): each token's row of the tables, its place in the sequence where not given (the rows of a tree
     of drafts are placed one behind the other, but their positions follow their depth); one outside the tables turns to NaN.
-    Queries are computed in 32 bits and rounded; a key is stored as the nearest code to its exact value. ``k_out`` ``[tokens, kv_heads,
-    dim]`` receives the turned keys, their exact values rounded once, where a prompt's attention needs them. ``out`` and ``k_out``
+    Queries are computed in 32 bits and rounded; a key is stored as the nearest code to its value in 64 bits. ``k_out`` ``[tokens,
+    kv_heads, dim]`` receives the turned keys, those values rounded once, where a prompt's attention needs them. ``out`` and ``k_out``
     share no element with q, k and v."""
     shape, device, code = q.shape, pages.device, _ROW_CODE.get(q.dtype)
     if code is None or len(shape) != 3 or not q.is_cuda or q.device != device or q.stride(2) != 1 or q.dtype != k.dtype:
