@@ -528,7 +528,9 @@ int tx_kv4_append_rope(const void *q, int64_t q_token, int64_t q_head, const voi
  * all of its rows, itself and the rows that its parents lead to. out the same shape: zeros for a row that sees no position in the
  * pool, NaN where all scores are -infinity. Positions that a row does not see, and their values, may hold anything. out must not
  * overlap q; queries 16-byte aligned, output rows 8-byte. Arithmetic, workspace rules and limits as tx_kv4_attention, at most
- * 2^22 rows, 4,096 query heads for each KV head (a group), and fewer than 2^23 sequences x kv_heads x ceil(min(tokens, 64) group / 128). */
+ * 2^22 rows, 4,096 query heads for each KV head (a group), and fewer than 2^23 sequences x kv_heads x ceil(min(tokens, 64) group / 128).
+ * Every workgroup looks through all sequences' lengths, twice or more above 64 of them: the time of large batches grows faster than the
+ * batch (16/2 heads of 128, 6 rows behind up to 600 positions: 38 us for 128 sequences, 614 for 1,024, in calls of 128 282). */
 int tx_kv4_tree_attention_workspace(int sequences, int64_t tokens, int heads, int kv_heads, int head_dim, int page_size, int max_pages,
                                     int device, int64_t *bytes);
 int tx_kv4_tree_attention(const void *q, int64_t q_token, int64_t q_head, int dtype, int64_t tokens, int heads, const int *cu,
@@ -547,9 +549,9 @@ int tx_kv4_tree_attention(const void *q, int64_t q_token, int64_t q_head, int dt
  *     temperature)) where u q_v(x) < p_v(x); else the closing token is drawn from max(p_v - q_v, 0).
  * Where that leaves nothing, it is drawn from p_v. A token is drawn as the first whose running sum in the vocabulary's order
  * exceeds u times the whole sum, in 64 bits; the tests use sums of 32-bit terms (off by some 1e-8; where few terms count,
- * by up to 1e-7). temperatures [sequences], or NULL: `temperature` for all. A temperature that is not above 0: the largest logit's token is accepted and closes, of equal ones
- * the first. Logits of -infinity have no weight; where a row that is reached holds a NaN, at temperatures above 0 an infinity, or
- * nothing above -infinity, no draft behind it is accepted and the closing token is -1.
+ * by up to 1e-7). temperatures [sequences], or NULL: `temperature` for all. A temperature that is not above 0: the largest
+ * logit's token is accepted and closes, of equal ones the first. Logits of -infinity have no weight; where a row that is reached holds
+ * a NaN, at temperatures above 0 an infinity, or nothing above -infinity, no draft behind it is accepted and the closing token is -1.
  * accepted [sequences]: accepted drafts, -1 for a sequence without rows. path [tokens]: path[cu[s] + j] is the row at step j, 0 to
  * accepted[s] (0 first). next [tokens]: next[cu[s] + j] the new tokens, accepted[s] drafts and the closing one. Both -1 behind.
  * At most 65535 rows and 2^24 tokens of vocabulary. The outputs must not overlap the inputs, each other or the workspace, which is

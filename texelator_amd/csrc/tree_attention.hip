@@ -27,10 +27,10 @@
 // Statistics and sums in fp32; sums run over the probabilities as rounded. In fp16 they are held times 2^11, in bf16 times a power
 // of two below 1 / (2^4 length), so that sums of the largest values stay finite.
 //
-// Bound by instruction issue where contexts are long: 80 columns over 262,144 positions of 8 heads of 128 take 150 to 156 us and 9 to combine
+// Bound by instruction issue where contexts are long: 80 columns over 262,144 positions of 8 heads of 128 take 150 us and 9 to combine
 // (1.9 TB/s of codes, 560 TFLOP/s), a tile as long as the two 32-position steps of its busiest wave: scores, maximum, exponentials and
 // value products one behind the other, beside one wave of another workgroup. Short contexts are
-// a chain of dependent steps: 24 trees of 130 columns over up to 8,191 positions 29 us and 13, of which 5 find the place, 6 fetch and
+// a chain of dependent steps: 24 trees of 130 columns over up to 8,191 positions 30 us and 13, of which 5 find the place, 6 fetch and
 // convert the first tile and 1 to 2 are each tile behind.
 // Columns in units of 16 (v_mfma_f32_16x16x32), each wave converting for itself, took 145 us for the one and 54 for the other;
 // 64 positions a step with joined maxima (spills) 174 and 34; one buffer, two barriers a tile 174 and 28.
@@ -733,8 +733,12 @@ void kv4_tree_plan(Kv4Tree &a, int dim, int cus) {
   while (most_ticks(a, dim == 128 ? kTile<128> : kTile<64>) >> a.shift > (int64_t)1 << 30) ++a.shift;
   const int64_t shares = most_ticks(a, dim == 128 ? kTile<128> : kTile<64>) / kLeast + 1;
   const int64_t fill = (dim == 128 ? kResident<128> : kResident<64>) * (int64_t)cus;
-  // Short parts that fill the grid by themselves are not cut: 32 sequences of up to 400 positions and 8 heads of 16 * 5 rows take 15 us,
-  // cut and combined 20; one such sequence 18 and 13, eight 17.6 and 16.2; 32 of up to 1,000 26 and 22.
+  // Where tables hold at most 512 positions and the parts, were all sequences as wide as they may be, fill the grid, none is cut. That
+  // many are seldom there, but a second launch costs more than uneven workgroups: up to 400 positions, 8 heads of 16 * 5
+  // rows, 32 sequences take 20.6 us, cut and combined 27.5; up to 512, 64 of 6 rows and 16/2 heads 21.5 and 23.6, 90 of 4 rows
+  // and 12/1 heads 16.6 and 23.5. Others lose: 26 of 3 rows and 40/1 heads 20.9 and 19.7; where half the workgroups have no part
+  // (64 of 5 rows and 32/8 heads) 31.5 and 24.3. Below the bound 1 sequence of 16 * 5 rows takes 15.7 whole and 12.9 cut, 2 11.0 and
+  // 15.3, 4 14.1 and 21.4, 8 17.4 and 18.6. 32 of up to 1,000 positions: 26 and 22.
   a.whole = room <= 512 && most_parts(a) >= fill;
   a.workgroups = (int)(shares < fill ? shares : fill);
   const int64_t blocks = most_blocks(a) < kPass ? most_blocks(a) : kPass;

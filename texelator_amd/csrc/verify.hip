@@ -24,7 +24,8 @@
 // Measured, first and second launch: 16 chains of up to 8 rows sampled from a draft's logits of 151,936 bf16 tokens 14 us (the
 // logits' 55 MB at 3.9 TB/s) and 23 us, 24 trees of up to 64 rows of 32,003 fp32 tokens 26 us (5.5 TB/s) and 17 us, one
 // tree of 6 rows 4 us and 15 us. The second is bound by its steps' latency: 6 us to the path, 5 to 10 for the sums, 5 to 7 for the token.
-// With a launch of its own for the token and a wave for each row's statistics they took 64, 69 and 26 us in all.
+// With a launch of its own for the token and a wave for each row's statistics they took 64, 69 and 26 us in all; with a fence by every
+// thread behind the sums, not one, the second launch takes 84, 32 and 19 us.
 #include <math.h>
 
 #include "elementwise.h"
